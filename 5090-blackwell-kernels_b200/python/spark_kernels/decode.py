@@ -5,10 +5,11 @@ of the path, in the order the reference's engine runs it (python/spark_kernels/e
     residual add + rmsnorm -> gate|up projection -> SwiGLU -> down projection -> residual add
 and its replay from a CUDA graph (engine.py:870-899). The four projections are `quant.make_linear`
 objects (int4, fp8, mxfp8, nvfp4 ...), or, for int4 with `fuse_swiglu`, the fused gate|up + SwiGLU GEMM
-of this library. The row operations between them (RMSNorm, RoPE, attention, residual adds) are outside
-the quantized-GEMM path; plain torch stands in for the reference's row kernels here, so this module is
-about the data flow through the projections (every GEMM consumes the previous one's output, unlike a
-benchmark over fixed buffers), not about those kernels' speed.
+of this library. What lies between them comes in two forms. With the default bf16 cache, plain torch stands in for the
+reference's row kernels, and the module is about the data flow through the projections (every GEMM consumes
+the previous one's output, unlike a benchmark over fixed buffers). With kv="int4" the step runs on this library's
+operators from end to end: `add_rmsnorm` (residual and norm in one launch), `kv4_append` (rotation and a 4-bit
+paged cache) and `kv4_attention`; `extend` then also takes several tokens of a sequence at once, e.g. its prompt.
 
 `TorchDecoder` is the same arithmetic on the dequantized weights in bf16 torch matmuls, which is what the
 reference checks its engine against (tests/test_quant.py:94-105).
@@ -20,8 +21,11 @@ from dataclasses import dataclass
 
 import torch
 
+from . import kv4
 from . import ops as sk
 from . import quant
+
+KV_PAGE = 64  # tokens of a page of the 4-bit cache
 
 
 @dataclass(frozen=True)
@@ -102,17 +106,28 @@ class _Dense:
 class QuantizedDecoder:
     """Decoder whose projections run on this library. `decode(x, pos)` advances every sequence of the batch by
     one token: x [B, hidden] bf16 are the embedded tokens, pos [B] int64 their positions; the KV cache holds
-    `max_len` positions per sequence."""
+    `max_len` positions per sequence, in bf16, or with kv="int4" in 4 bits (head_dim 64 or 128)."""
 
     def __init__(self, cfg: DecoderConfig, weights: list[dict], fmt: str = "int4", fuse_swiglu: bool = True,
-                 batch: int = 1, max_len: int = 64):
+                 batch: int = 1, max_len: int = 64, kv: str = "bf16"):
+        if kv not in ("bf16", "int4"):
+            raise ValueError(f"unknown cache format {kv!r}; expected 'bf16' or 'int4'")
         self.cfg, self.fmt = cfg, fmt
         dev = weights[0]["wqkv"].device
         self.layers = [self._projections(w, fmt, fuse_swiglu) for w in weights]
         self.norms = [(w["norm1"], w["norm2"]) for w in weights]
-        shape = (cfg.layers, batch, cfg.kv_heads, max_len, cfg.head_dim)
-        self.k_cache = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
-        self.v_cache = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+        self.kv = kv
+        if kv == "int4":
+            # every sequence has the pages for max_len tokens; a serving engine would hand them out as sequences grow
+            per = -(-max_len // KV_PAGE)
+            self.cache = [kv4.KV4Cache(batch * per, cfg.kv_heads, cfg.head_dim, KV_PAGE, min(64, cfg.head_dim), device=dev) for _ in weights]
+            self.page_table = torch.arange(batch * per, dtype=torch.int32, device=dev).reshape(batch, per)
+            self.cos_sin = kv4.rotation_table(max_len, cfg.head_dim, cfg.rope_theta, device=dev)
+        else:
+            shape = (cfg.layers, batch, cfg.kv_heads, max_len, cfg.head_dim)
+            self.k_cache = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+            self.v_cache = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+        self.device = dev
         self.max_len = max_len
         self._graph = None
 
@@ -136,6 +151,8 @@ class QuantizedDecoder:
 
     def decode(self, x: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         cfg = self.cfg
+        if self.kv == "int4":
+            return self.extend(x, (pos + 1).to(torch.int32))
         B = x.shape[0]
         rows = torch.arange(B, device=x.device)
         # keys at positions <= pos are visible; the mask is computed from pos on the device (graph safe)
@@ -157,9 +174,24 @@ class QuantizedDecoder:
             x = x + lay.down(lay.mlp_in(rmsnorm(x, n2, cfg.eps)))
         return x
 
+    def extend(self, x: torch.Tensor, lens: torch.Tensor, q_offsets: torch.Tensor | None = None) -> torch.Tensor:
+        """kv="int4" only: the hidden states after the last layer for the new tokens x [rows, hidden] of the sequences.
+        lens int32 [batch]: tokens of every sequence after this call (0: an empty slot); q_offsets int32 [batch + 1]: rows
+        q_offsets[b] .. q_offsets[b + 1] - 1 are the new tokens of sequence b, its last ones; None: one each."""
+        if self.kv != "int4":
+            raise ValueError("extend needs kv='int4'")
+        r, h = sk.add_rmsnorm(x, gain=self.norms[0][0], eps=self.cfg.eps)
+        for li, lay in enumerate(self.layers):
+            q = kv4.kv4_append(lay.qkv(h), self.cache[li], self.page_table, lens, self.cos_sin, q_offsets)
+            att = kv4.kv4_attention(q, self.cache[li], self.page_table, lens, q_offsets)
+            r, h = sk.add_rmsnorm(r, lay.o(att.reshape(x.shape[0], -1)), gain=self.norms[li][1], eps=self.cfg.eps)
+            nxt = self.norms[li + 1][0] if li + 1 < len(self.layers) else None
+            r, h = sk.add_rmsnorm(r, lay.down(lay.mlp_in(h)), gain=nxt, eps=self.cfg.eps)
+        return r
+
     # ---- CUDA-graph replay of the step (fixed buffers, as the reference's engine does) ----
     def capture(self, batch: int) -> None:
-        dev = self.k_cache.device
+        dev = self.device
         self._x = torch.zeros(batch, self.cfg.hidden, dtype=torch.bfloat16, device=dev)
         self._pos = torch.zeros(batch, dtype=torch.int64, device=dev)
         side = torch.cuda.Stream()
@@ -168,8 +200,12 @@ class QuantizedDecoder:
             self.decode(self._x, self._pos)
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
-        self.k_cache.zero_()
-        self.v_cache.zero_()
+        if self.kv == "int4":
+            for c in self.cache:
+                c.pool.zero_()
+        else:
+            self.k_cache.zero_()
+            self.v_cache.zero_()
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
             self._y = self.decode(self._x, self._pos)

@@ -138,3 +138,13 @@ def fp8_quantize_block128(x, block_rows: int):
 
 def fp8gemm_block128(a, b_t, scale_a_blocks, scale_b_blocks):
     return _C.fp8gemm_block128(a, b_t, scale_a_blocks, scale_b_blocks)
+
+
+def add_rmsnorm(x, y=None, gain=None, eps: float = 1e-5, post_gain=None, gate=None, residual_scale: float = 1.0):
+    """What a decoder does between two blocks, in one launch: x [rows, hidden] bf16 the residual stream, y [rows, hidden]
+    bf16 the output of the block before. Returns (r, h) with z = y, or rmsnorm(y) * post_gain;
+    r = bf16(residual_scale * x + gate * z); h = bf16(rmsnorm(r) * gain); rmsnorm(v) = v / sqrt(mean(v^2) + eps).
+    gate is [hidden], or [rows, hidden] (a row stride of 0 is fine). Without y, r is x; without gain, h is None.
+    hidden a multiple of 8, up to 65536; rows of x, y and gate 16-byte aligned. Forward only. The reference runs
+    the two halves as separate kernels (python/spark_kernels/engine.py:441-456)."""
+    return _C.add_rmsnorm(x, y, gain, eps, post_gain, gate, residual_scale)

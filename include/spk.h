@@ -29,7 +29,8 @@ enum {
     SPK_INVALID = 1,     /* host-side validation failed (reference: std::invalid_argument) */
     SPK_CUDA_ERROR = 2,  /* a CUDA call failed (reference: std::runtime_error) */
     SPK_TIMEOUT = 3,     /* a bounded device-side wait gave up (read by spk_device_status) */
-    SPK_UNSUPPORTED = 4  /* the device is not an sm_100 part */
+    SPK_UNSUPPORTED = 4, /* the device is not an sm_100 part */
+    SPK_BAD_INDEX = 5    /* a page, slot, length or position outside its table (read by spk_device_status) */
 };
 
 /* Message of the last failure on the calling thread ("" if none). */
@@ -46,6 +47,9 @@ SPK_API int spk_init(void);
  * the outputs of the GEMMs launched since the last clean status are not to be trusted: run them
  * again. Does not cover spk_w4gemm_bf16_noalloc, which has its own status call below. */
 SPK_API int spk_device_status(void* stream, int* code);
+/* The same word also reports SPK_BAD_INDEX, from the kernels over the 4-bit KV cache: they never follow a
+ * bad index (the token is left out), so the scratch needs no repair then, but the call's output is not what
+ * was asked for. */
 /* Test hook, no counterpart in the reference: launches a one-block kernel that leaves `dirty` words of
  * the split-K scratch non-zero, waits a tenth of a millisecond for a barrier phase nothing completes and
  * records SPK_TIMEOUT, i.e. the state a broken pipeline would leave. No fault, no trap; the context
@@ -159,6 +163,51 @@ SPK_API int spk_grouped_gemm_fp8(const void* A, const void* W, const int32_t* of
                                  const float* scale_a, const float* scale_b, void* stream);
 SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int32_t* offsets, void* C, int T, int E, int N,
                                         int K, const float* scale_a, const float* scale_b, void* stream);
+
+/* ---- 4-bit KV cache and the row operations of a decode step ------------------------------------
+ * No counterpart in the reference for the 4-bit cache (its own is bf16). A pool is bytes
+ * [pages][kv_heads][page_size / 16][spk_kv4_tile_bytes(head_dim, group)], 16-byte aligned; a tile is 16 tokens of
+ * one head: K codes, V codes, then per token and group of `group` channels a word (minimum in the low
+ * half, scale in the high half, bf16), K's and V's. A code c stands for c * scale + minimum; the order of the codes
+ * inside a tile is the kernels' (csrc/kv4_layout.cuh). head_dim 64 or 128; group 32, 64 or 128, at most
+ * head_dim; page_size a multiple of 16 up to 1024.
+ * A call's sequences: lens int32 [seqs] on the device, tokens in the cache INCLUDING this call's; page_table int32
+ * [seqs][table_width] on the device, the pages of a sequence in order; q_offsets int32 [seqs + 1] on the device, the call's
+ * rows of sequence b are q_offsets[b] .. q_offsets[b + 1] - 1 and they are its last tokens; NULL: one row per
+ * sequence (rows == seqs). Row i of n of a sequence thus has position lens - n + i; a row of negative position is
+ * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest. A page outside the pool, a
+ * length outside the table and a position outside the rotation's table are skipped and reported as SPK_BAD_INDEX by
+ * spk_device_status. seqs <= 4096. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
+SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported pair */
+/* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
+ * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16
+ * [rows][q_heads][head_dim] (zeros for padding) and quantizes k and v into the pool: per group m = bf16(min), s = bf16((max - m) / 15),
+ * c = clamp(rint((x - m) / s), 0, 15); a group with an infinity or a NaN reads back as NaN. */
+SPK_API int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool, int pages, int page_size, int q_heads, int kv_heads,
+                           int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,
+                           const int32_t* q_offsets, int seqs, int rows, const float* cos_sin, int positions, int rot_dim,
+                           void* q_out, int zero_rest, void* stream);
+/* k, v bf16 [n][kv_heads][head_dim]: the values of the tokens in slots[n] (int64: page * page_size + place in the page);
+ * zeros for a negative slot. */
+SPK_API int spk_kv4_read(const void* pool, int pages, int page_size, int kv_heads, int head_dim, int group, const int64_t* slots, int n,
+                         void* k, void* v, void* stream);
+/* out bf16 [rows][q_heads][head_dim] = softmax(scale q k^T) v over the tokens at positions <= the row's own (window > 0:
+ * only the last `window` of them), fp32 sums; zeros where there are none. q bf16, rows q_stride elements apart; q_heads a
+ * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads). workspace: spk_kv4_attention_workspace(...) bytes of
+ * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter. */
+SPK_API long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim);
+SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
+                              int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,
+                              const int32_t* q_offsets, int seqs, int rows, float scale, int window, void* out, int zero_rest,
+                              void* workspace, long long workspace_bytes, void* stream);
+/* The step between two blocks (reference python/spark_kernels/engine.py:441-456: residual add, then rmsnorm), with the
+ * forms that other blocks have. z = y, or with post_gain rmsnorm(y) * post_gain; r = bf16(residual_scale * x + gate * z);
+ * h = bf16(rmsnorm(r) * gain), rmsnorm(v) = v / sqrt(mean(v^2) + eps), all in fp32. y NULL: r is x (and not written).
+ * gain NULL: no h. gate bf16, rows gate_stride elements apart (0: one row for all). x, y, r, h bf16 [rows][hidden], x and y with row
+ * strides; r may be x. hidden a multiple of 8, at most 65536; 16-byte aligned pointers, strides multiples of 8. */
+SPK_API int spk_add_rmsnorm(const void* x, long long x_stride, const void* y, long long y_stride, const void* gain, const void* post_gain,
+                            const void* gate, long long gate_stride, float residual_scale, float eps, void* r, void* h, int rows,
+                            int hidden, void* stream);
 
 /* ---- fp4 e2m1 (NVFP4, MXFP4) -------------------------------------------------------------- */
 

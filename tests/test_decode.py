@@ -64,3 +64,80 @@ def test_graph_replay_equals_eager(sk):
         x = torch.randn(2, cfg.hidden, device="cuda", generator=g).to(torch.bfloat16)
         pos = torch.full((2,), step, dtype=torch.int64, device="cuda")
         assert torch.equal(graphed.replay(x, pos), eager.decode(x, pos)), step
+
+
+def _reference_step(decode, ref, cfg, weights, state, x, where):
+    """A step over the 4-bit cache in plain torch: x [rows, hidden], where[row] = (sequence, position). Keys and values are
+    rounded to what their 4-bit codes stand for; `state[layer][sequence]` is the list of (k, v) so far."""
+    cs = torch.cat([f(torch.arange(64)[:, None] * cfg.rope_theta ** (-torch.arange(0, cfg.head_dim, 2, dtype=torch.float64) / cfg.head_dim)) for f in (torch.cos, torch.sin)], 1)
+    pos = torch.tensor([p for _, p in where])
+    for li, w in enumerate(weights):
+        qkv = (decode.rmsnorm(x, w["norm1"], cfg.eps) @ w["wqkv"]).cpu().double().reshape(len(where), -1, cfg.head_dim)
+        turned = ref.rotate(qkv[:, : cfg.q_heads + cfg.kv_heads], cs[pos])
+        k = ref.quantize(turned[:, cfg.q_heads:], 64)[0]
+        v = ref.quantize(qkv[:, cfg.q_heads + cfg.kv_heads:], 64)[0]
+        for row, (b, _) in enumerate(where):
+            state[li][b].append((k[row], v[row]))
+        att = torch.zeros(len(where), cfg.q_heads, cfg.head_dim, dtype=torch.float64)
+        for row, (b, p) in enumerate(where):
+            kk, vv = (torch.stack([t[i] for t in state[li][b][: p + 1]]) for i in (0, 1))
+            for h in range(cfg.q_heads):
+                kv = h * cfg.kv_heads // cfg.q_heads
+                att[row, h] = torch.softmax(kk[:, kv] @ turned[row, h] / cfg.head_dim ** 0.5, -1) @ vv[:, kv]
+        x = x + att.reshape(len(where), -1).to(torch.bfloat16).to(x.device) @ w["wo"]
+        gu = decode.rmsnorm(x, w["norm2"], cfg.eps) @ w["w_gate_up"]
+        inter = gu.shape[1] // 2
+        x = x + (torch.nn.functional.silu(gu[:, :inter].float()) * gu[:, inter:].float()).to(torch.bfloat16) @ w["w_down"]
+    return x
+
+
+@pytest.mark.parametrize("fmt", ["int4", "int4-asym", "fp8-tok"])
+def test_four_bit_cache_prompt_then_steps(sk, fmt):
+    """Prompts of different lengths (one slot empty) in one call, then single tokens, over the 4-bit cache: the
+    whole step on this library's operators against plain torch. The same bound as with the bf16 cache, doubled
+    for codes that fall on the other side of a border when their input moves by a rounding."""
+    from spark_kernels import decode
+    from tests import kv4_reference as ref
+
+    cfg = _cfg(sk)
+    w = decode.random_weights(cfg, "cuda", seed=15)
+    m = decode.QuantizedDecoder(cfg, w, fmt=fmt, batch=3, max_len=40, kv="int4")
+    deq = m.dequantized_weights()
+    state = [[[] for _ in range(3)] for _ in deq]
+    g = torch.Generator(device="cuda").manual_seed(16)
+    lens, news = [17, 0, 5], [17, 0, 5]
+    for step in range(4):
+        off = [0] + torch.tensor(news).cumsum(0).tolist()
+        x = torch.randn(off[-1], cfg.hidden, device="cuda", generator=g).to(torch.bfloat16)
+        got = m.extend(x, torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(off, dtype=torch.int32).cuda()).float()
+        want = _reference_step(decode, ref, cfg, deq, state, x, ref.rows_of(lens, off)).float()
+        assert ((got - want).norm() / want.norm()).item() < 2 * TOL[fmt], step
+        news = [1, 0, 1] if step else [3, 0, 1]
+        lens = [a + n for a, n in zip(lens, news)]
+    assert sk._C.device_status() == 0
+
+
+def test_four_bit_cache_graph_replay_equals_eager(sk):
+    from spark_kernels import decode
+
+    cfg = _cfg(sk)
+    w = decode.random_weights(cfg, "cuda", seed=18)
+    eager = decode.QuantizedDecoder(cfg, w, fmt="int4", batch=2, max_len=80, kv="int4")
+    graphed = decode.QuantizedDecoder(cfg, w, fmt="int4", batch=2, max_len=80, kv="int4")
+    graphed.capture(2)
+    g = torch.Generator(device="cuda").manual_seed(19)
+    for step in range(70):
+        x = torch.randn(2, cfg.hidden, device="cuda", generator=g).to(torch.bfloat16)
+        pos = torch.full((2,), step, dtype=torch.int64, device="cuda")
+        assert torch.equal(graphed.replay(x, pos), eager.decode(x, pos)), step
+
+
+def test_cache_formats_are_checked(sk):
+    from spark_kernels import decode
+
+    cfg = _cfg(sk)
+    w = decode.random_weights(cfg, "cuda", seed=20)
+    with pytest.raises(ValueError):
+        decode.QuantizedDecoder(cfg, w, kv="int8")
+    with pytest.raises(ValueError):
+        decode.QuantizedDecoder(cfg, w, batch=1).extend(torch.zeros(1, cfg.hidden, dtype=torch.bfloat16).cuda(), torch.ones(1, dtype=torch.int32).cuda())
