@@ -1,13 +1,40 @@
 // Attention over the 4-bit paged KV cache (its bytes: kv4_layout.cuh): for a row (token at position p, query head)
 //     out = sum_j softmax_j(scale q . k_j) v_j   over the positions j <= p, with a window only p - window < j,
-// k_j and v_j being c s + m. One pass over the keys with the running maximum and sum of the softmax, in fp32.
+// k_j and v_j being c s + m, the codes and words of the cache.
+//
+// One pass over the keys with the running maximum and sum of the softmax, everything between the loads and the output in
+// registers. The rows that read one KV head (its query heads times the call's tokens of the sequence) are taken 8 NQ at a
+// time as the n side of warp-level MMAs whose 16-row side is the cache:
+//     S^T [16 tokens x rows] = K codes [16 x d] . Q^T,        O^T [channels x rows] += V codes^T [channels x 16 tokens] . P^T
+// The codes go into the MMA as small integers in fp16, built by one LOP3 per pair (a nibble or-ed into the mantissa of
+// 1024 reads 1024 + c, one nibble higher into that of 64 reads 64 + c); the words are applied outside it:
+//     K  q . k = sum over groups of s (sum (c + o) q' - sum o q') + m sum q'   with the o-sums of q as the accumulator's start;
+//        q' = q 2^-e fits fp16 exactly (bf16 has fewer bits; e the exponent of the row's largest |q|), the products are exact
+//        in fp32, and four to eight MMAs a group leave the offset no room to cost precision
+//     V  sum p v = sum (p s)(c - 8) + sum p (8 s + m): here the offsets are taken out before the MMA (a sum over the whole
+//        sequence of values with a large common offset would drift), p s is rounded to fp16 against a power of two
+//        that follows the largest s so far (2^-11 each, unbiased; bf16 would lose another half step of the output), and the
+//        second sum is fp32.
+// P^T comes out of S^T's accumulator layout by movmatrix (one 8 x 8 transpose per register).
+//
+// Work is cut into equal contiguous ranges of (sequence, block of rows, KV head, 16-token tile) units over the resident
+// CTAs, whatever the lengths are; every CTA finds its range itself from the lengths on the device. A warp takes every
+// eighth step of a range through a ring of its own, filled by bulk copies (a tile is one copy); a CTA merges its
+// warps in shared memory. What a CTA holds of a piece that is cut across CTAs goes to the workspace, and a second, chained
+// launch adds such pieces in the order of the CTAs: the same bits every run.
 #include "kv4_layout.cuh"
+#include "ptx_sm100.cuh"
 
 namespace spk {
 namespace {
 
 using kv4::Batch;
 using kv4::Pool;
+
+constexpr int kWarps = 8, kSteps = 2;  // warps of a CTA; 16-token tiles of a ring stage
+constexpr int kMinUnits = kWarps;      // a CTA gets at least this many tiles: one per warp
+
+constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
 
 struct AttendParams {
     const __nv_bfloat16* q;
@@ -17,99 +44,646 @@ struct AttendParams {
     int q_heads, window, zero_rest;
     float scale;
     __nv_bfloat16* out;
+    int4* pieces;     // [grid] (CTAs that share the piece begun in this CTA, or 0; sequence; row block; KV head)
+    float* partials;  // [grid][2][rows][D + 2]: a piece continued from the CTA before, a piece begun here
     int* status;
 };
 
-// The simplest right form: a warp per row and head, a lane per key for the scores, four channels a lane for the output.
-template <int D, int G>
-__global__ void __launch_bounds__(256) kv4_attend_rows_kernel(const AttendParams p) {
-    __shared__ float qs[8][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_release();
-    pdl_wait();
-    const long long id = static_cast<long long>(blockIdx.x) * 8 + warp;
-    const int h = static_cast<int>(id % p.q_heads), t = static_cast<int>(id / p.q_heads);
-    if (t >= p.batch.rows) return;
-    int b = t;
-    if (p.batch.offsets != nullptr) {
-        int passed = 0;
-        for (int i = lane; i < p.batch.seqs; i += 32) passed += p.batch.offsets[i + 1] <= t;
-        b = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(passed)));
-    }
-    int pos = -1;
-    if (b < p.batch.seqs) {
-        int first, count;
-        kv4::rows_of(p.batch, b, first, count);
-        if (t >= first && t < first + count) pos = kv4::length_of(p.batch, p.pool.page_size, b, p.status) - count + (t - first);
-    } else if (!p.zero_rest) {
-        return;
-    }
-    const __nv_bfloat16* q = p.q + t * p.stride + static_cast<long long>(h) * D;
-    for (int i = lane; i < D; i += 32) qs[warp][i] = __bfloat162float(q[i]) * p.scale * 1.4426950408889634f;
-    __syncwarp();
-    const int tiles = p.pool.page_size / kv4::kTile, kv = h / (p.q_heads / p.pool.heads);
-    auto tile_of = [&](int j) -> const unsigned char* {
-        const int page = p.batch.table[static_cast<size_t>(b) * p.batch.width + j / p.pool.page_size];
-        if (page < 0 || page >= p.pool.pages) {
-            atomicCAS(p.status, 0, SPK_BAD_INDEX);
-            return nullptr;
-        }
-        return p.pool.data + ((static_cast<size_t>(page) * p.pool.heads + kv) * tiles + j % p.pool.page_size / kv4::kTile) * p.pool.tile_bytes;
-    };
-    float top = -INFINITY, sum = 0.0f, acc[4] = {};
-    const int ch = 4 * lane;
-    for (int j0 = p.window > 0 ? max(0, pos - p.window + 1) : 0; j0 <= pos; j0 += 32) {
-        const int j = j0 + lane;
-        const unsigned char* tile = j <= pos ? tile_of(j) : nullptr;
-        float s = -INFINITY;
-        if (tile != nullptr) {
-            s = 0.0f;
-            const int in = j % kv4::kTile;
-            for (int c = 0; c < D; c += 8) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + kv4::k_word_at(D, in, c));
-                const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + (in * (D / G) + c / G) * 4);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s = fmaf(fmaf(static_cast<float>(w >> (4 * i) & 15u), kv4::word_scale(word), kv4::word_min(word)), qs[warp][c + i], s);
-            }
-        }
-        float most = s;
-        for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        most = fmaxf(most, top);
-        const float base = most == -INFINITY ? 0.0f : most, keep = exp2f(top - base);
-        const float e = tile != nullptr ? exp2f(s - base) : 0.0f;
-        top = most;
-        sum = sum * keep + e;
-        for (int i = 0; i < 4; ++i) acc[i] *= keep;
-        const unsigned seen = __ballot_sync(0xffffffffu, tile != nullptr);
-        for (int o = 0; o < 32; ++o) {
-            if (!(seen >> o & 1u)) continue;
-            const float w = __shfl_sync(0xffffffffu, e, o);
-            const unsigned char* from = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(tile), o));
-            if (ch >= D) continue;
-            const int in = (j0 + o) % kv4::kTile;
-            const uint32_t codes = *reinterpret_cast<const uint16_t*>(from + kv4::v_codes_at(D) + kv4::v_piece_at(D, in, ch % 32 / 4) + ch / 32 * 2);
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(from + kv4::v_words_at(D, G) + (in * (D / G) + ch / G) * 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, fmaf(static_cast<float>(codes >> (4 * i) & 15u), kv4::word_scale(word), kv4::word_min(word)), acc[i]);
-        }
-    }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (ch < D)
-        for (int i = 0; i < 4; ++i)
-            p.out[(static_cast<size_t>(t) * p.q_heads + h) * D + ch + i] = __float2bfloat16_rn(top == -INFINITY ? 0.0f : acc[i] / sum);
+template <int D, int G, int NQ>
+struct SplitCfg {
+    static constexpr int kRows = 8 * NQ, kGroups = D / G, kWords = D / 32;
+    static constexpr int kTileBytes = kv4::tile_bytes(D, G), kStageBytes = kSteps * kTileBytes;
+    static constexpr int kCtas = NQ == 1 ? 2 : 1;  // per SM: what the registers allow
+    static constexpr int kORow = D * 4 + 32;       // a row's pitch in the merge buffer: the lanes of a store hit every bank once
+    static constexpr int kMerge = kWarps / 2 * kRows * kORow;
+    // maxima and sums [2][warps][rows], chunk starts [threads + 1], barriers and valid flags of six stages
+    static constexpr int kSmall = 2 * 2 * kWarps * kRows * 4 + (32 * kWarps + 1) * 8 + kWarps * 6 * 12 + 64;
+    static constexpr int kFit = ((227 * 1024 - 1024 * kCtas) / kCtas - kMerge - kSmall) / (kWarps * kStageBytes);
+    static constexpr int kStages = kFit < 6 ? kFit : 6;
+    static constexpr int kRing = kWarps * kStages * kStageBytes, kSmem = kRing + kMerge + kSmall;
+    static constexpr int kPartial = kRows * (D + 2);  // floats
+    static_assert(kStages >= 2, "the ring needs two stages");
+};
+
+// A sequence and its place in the order of units.
+struct Seq {
+    int b, first, count, len;  // its rows of q, its tokens
+    int lo, hi;                // tiles of 16 tokens that any of its rows sees
+    long long begin, units;    // units before it, its own: row blocks x KV heads x tiles
+};
+
+__device__ __forceinline__ void load_seq(const AttendParams& p, int rows, Seq& s) {
+    kv4::rows_of(p.batch, s.b, s.first, s.count);
+    s.len = kv4::length_of(p.batch, p.pool.page_size, s.b, p.status);
+    s.hi = s.count > 0 ? (s.len + kv4::kTile - 1) / kv4::kTile : 0;
+    s.lo = p.window > 0 && s.count > 0 ? max(0, s.len - s.count - p.window + 1) / kv4::kTile : 0;
+    const int group = p.q_heads / p.pool.heads;
+    s.units = static_cast<long long>((s.count * group + rows - 1) / rows) * p.pool.heads * (s.hi - s.lo);
 }
 
-template <int D, int G>
-int attend(const AttendParams& p, cudaStream_t stream) {
-    const int64_t warps = int64_t{p.batch.rows} * p.q_heads;
-    SPK_CUDA(launch_chained(kv4_attend_rows_kernel<D, G>, dim3(static_cast<unsigned>(cdiv64(warps, 8))), dim3(256), 0, stream, p));
+// What a CTA's range holds of one (sequence, block of rows, KV head).
+struct Piece {
+    int block, head;
+    int tile0, tiles;    // tiles from the sequence's start
+    bool begins, ends;   // whether the range holds the piece's first and last tile
+};
+
+// The piece at unit u; s is the sequence that holds an earlier unit, and becomes the one that holds u.
+__device__ __forceinline__ Piece piece_at(const AttendParams& p, int rows, long long u, long long end, Seq& s) {
+    while (s.begin + s.units <= u) {
+        s.begin += s.units;
+        ++s.b;
+        load_seq(p, rows, s);
+    }
+    const int n = s.hi - s.lo;
+    const long long local = u - s.begin;
+    const int which = static_cast<int>(local / n), skip = static_cast<int>(local - static_cast<long long>(which) * n);
+    Piece x;
+    x.block = which / p.pool.heads, x.head = which - x.block * p.pool.heads;
+    x.tile0 = s.lo + skip;
+    x.tiles = static_cast<int>(min(static_cast<long long>(n - skip), end - u));
+    x.begins = skip == 0, x.ends = skip + x.tiles == n;
+    return x;
+}
+
+// A token's words, one per group, in one load.
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *at;
+    }
+}
+
+template <int D, int G, int NQ>
+__global__ void __launch_bounds__(32 * kWarps, (SplitCfg<D, G, NQ>::kCtas))
+kv4_attend_split_kernel(const AttendParams p) {
+    using Cfg = SplitCfg<D, G, NQ>;
+    constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages;
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char* merge = smem + Cfg::kRing;
+    float* m_max = reinterpret_cast<float*>(merge + Cfg::kMerge);  // [2][warps][rows]
+    float* m_sum = m_max + 2 * kWarps * R;
+    long long* chunk_start = reinterpret_cast<long long*>(m_sum + 2 * kWarps * R);  // [threads + 1]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(chunk_start + 32 * kWarps + 1);
+    int* valid_all = reinterpret_cast<int*>(bars + kWarps * S);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    unsigned char* ring = smem + warp * S * Cfg::kStageBytes;
+    uint64_t* full = bars + warp * S;
+    int* valid = valid_all + warp * S;
+    if (lane == 0) {
+        for (int s = 0; s < S; ++s) ptx::mbar_init(&full[s], 1);
+        ptx::fence_mbar_init();
+    }
+    pdl_release();
+    pdl_wait();
+
+    const int group = p.q_heads / p.pool.heads, tiles_per_page = p.pool.page_size / kv4::kTile;
+    // rows of a sequence with nothing in sight, and rows that belong to no sequence
+    auto zero_rows = [&](int from, int to) {
+        const long long pieces = static_cast<long long>(max(0, to - from)) * p.q_heads * (D / 8);
+        uint4* at = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(from) * p.q_heads * D);
+        for (long long i = threadIdx.x; i < pieces; i += 32 * kWarps) at[i] = make_uint4(0, 0, 0, 0);
+    };
+    // units before every chunk of sequences, one chunk a thread
+    const int chunk = (p.batch.seqs + 32 * kWarps - 1) / (32 * kWarps);
+    long long total;
+    {
+        __shared__ long long warp_sum[kWarps];
+        __shared__ int empties, empty_seqs[kv4::kMaxSeqs / kMinGrid];  // of the ones that fall to this CTA
+        if (threadIdx.x == 0) empties = 0;
+        __syncthreads();
+        long long units = 0;
+        for (int i = 0; i < chunk; ++i) {
+            Seq s;
+            s.b = threadIdx.x * chunk + i;
+            if (s.b >= p.batch.seqs) break;
+            load_seq(p, R, s);
+            units += s.units;
+            if (s.units == 0 && s.count > 0 && s.b % gridDim.x == blockIdx.x) empty_seqs[atomicAdd(&empties, 1)] = s.b;
+        }
+        long long run = units;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long up = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += up;
+        }
+        if (lane == 31) warp_sum[warp] = run;
+        __syncthreads();
+        long long before = 0;
+        total = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += warp_sum[w];
+            total += warp_sum[w];
+        }
+        chunk_start[threadIdx.x] = before + run - units;
+        __syncthreads();
+        for (int i = 0; i < empties; ++i) {
+            int first, count;
+            kv4::rows_of(p.batch, empty_seqs[i], first, count);
+            zero_rows(first, first + count);
+        }
+    }
+    if (p.zero_rest && blockIdx.x == gridDim.x - 1) {
+        const int head = p.batch.seqs > 0 ? min(max(p.batch.offsets[0], 0), p.batch.rows) : 0;
+        const int tail = p.batch.seqs > 0 ? min(max(p.batch.offsets[p.batch.seqs], 0), p.batch.rows) : 0;
+        zero_rows(0, head);
+        zero_rows(tail, p.batch.rows);
+    }
+    const long long active = max(1ll, min(static_cast<long long>(gridDim.x), (total + kMinUnits - 1) / kMinUnits));
+    const long long start = blockIdx.x < active ? blockIdx.x * total / active : total;
+    const long long end = blockIdx.x < active ? (blockIdx.x + 1) * total / active : total;
+    if (start >= end) {
+        if (threadIdx.x == 0) p.pieces[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    auto cta_of = [&](long long unit) { return static_cast<int>(((unit + 1) * active - 1) / total); };
+
+    Seq seq;
+    {
+        int at = 0;
+        for (int hi = 32 * kWarps - 1; at < hi;) {
+            const int mid = (at + hi + 1) >> 1;
+            if (chunk_start[mid] <= start) at = mid; else hi = mid - 1;
+        }
+        seq.b = min(at * chunk, p.batch.seqs - 1);
+        seq.begin = chunk_start[at];
+        load_seq(p, R, seq);
+    }
+
+    // the filling side of the ring walks the same steps ahead of the consuming side; page numbers are read a step early
+    long long fill_u = start;
+    Seq fill_seq = seq;
+    Piece fill = piece_at(p, R, fill_u, end, fill_seq);
+    int fill_step = warp, issued = 0, page[kSteps];
+    auto fill_settle = [&]() {  // to the next step of this warp at or after fill_step; false at the end of the range
+        while (fill_step * kSteps >= fill.tiles) {
+            fill_u += fill.tiles;
+            if (fill_u >= end) return false;
+            fill = piece_at(p, R, fill_u, end, fill_seq);
+            fill_step = warp;
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            if (fill_step * kSteps + i < fill.tiles)
+                page[i] = __ldg(p.batch.table + static_cast<size_t>(fill_seq.b) * p.batch.width + (fill.tile0 + fill_step * kSteps + i) / tiles_per_page);
+        return true;
+    };
+    bool filling = fill_settle();
+    auto fill_one = [&](int slot) {
+        if (!filling) return;
+        if (lane == 0) {
+            int ok = 0, n = 0;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (fill_step * kSteps + i < fill.tiles) {
+                    if (page[i] >= 0 && page[i] < p.pool.pages) ok |= 1 << i, ++n;
+                    else atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                }
+            valid[slot] = ok;
+            ptx::mbar_arrive_expect_tx(&full[slot], n * Cfg::kTileBytes);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (ok >> i & 1) {
+                    const int tile = fill.tile0 + fill_step * kSteps + i;
+                    const unsigned char* from = p.pool.data + ((static_cast<size_t>(page[i]) * p.pool.heads + fill.head) * tiles_per_page + tile % tiles_per_page) * Cfg::kTileBytes;
+                    ptx::bulk_g2s(ring + slot * Cfg::kStageBytes + i * Cfg::kTileBytes, from, Cfg::kTileBytes, &full[slot]);
+                }
+        }
+        ++issued;
+        fill_step += kWarps;
+        filling = fill_settle();
+    };
+    for (int s = 0; s < S; ++s) fill_one(s);
+
+    int slot = 0, used = 0, merges = 0;
+    unsigned phase = 0;
+    bool alive = true;
+    Piece s;
+    for (long long u = start; u < end; u += s.tiles) {
+        s = piece_at(p, R, u, end, seq);
+        // ---- the rows of this piece: Q fragments, their sums per group, what each row sees -----------
+        uint32_t qf[NQ][NW][4];  // [word][(step A: b0, b1), (step B: b0, b1)]
+        float start_acc[NQ][NG][2], q_sum[NQ][NG][2], mult[NQ][2];
+        int lo[NQ][2], hi[NQ][2], all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const int row = s.block * R + 8 * n + g;  // B fragments: this lane's column is row g
+            const bool there = row < seq.count * group;
+            uint4 raw[NW] = {};
+            if (there) {
+                const __nv_bfloat16* q = p.q + static_cast<long long>(seq.first + row / group) * p.stride + static_cast<long long>(s.head * group + row % group) * D + 8 * c;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 32 * i);
+            }
+            uint32_t top = 0;
+            float v[NW][8];
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[i][2 * j] = __uint_as_float(w[j] << 16), v[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
+                }
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = static_cast<int>(top >> 23);  // biased exponent of the row's largest |q|
+            const bool finite = e < 255;
+            const float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, min(254, 254 - e))) << 23) : 0.0f;
+            const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
+            float even[NG] = {}, odd[NG] = {};
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                float h[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = finite ? v[i][j] * down : 0.0f;
+                qf[n][i][0] = ptx::f16x2_pack(h[0], h[4]), qf[n][i][1] = ptx::f16x2_pack(h[2], h[6]);
+                qf[n][i][2] = ptx::f16x2_pack(h[1], h[5]), qf[n][i][3] = ptx::f16x2_pack(h[3], h[7]);
+                // sums of what the MMA will really multiply by
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][i][j]));
+                    (j < 2 ? even : odd)[32 * i / G] += f.x + f.y;
+                }
+            }
+            const float m = p.scale * 1.4426950408889634f * up;
+            const int pos = seq.len - seq.count + row / group;
+            const int row_hi = there ? max(0, pos + 1) : 0, row_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                even[k] += __shfl_xor_sync(0xffffffffu, even[k], 1), even[k] += __shfl_xor_sync(0xffffffffu, even[k], 2);
+                odd[k] += __shfl_xor_sync(0xffffffffu, odd[k], 1), odd[k] += __shfl_xor_sync(0xffffffffu, odd[k], 2);
+            }
+            // accumulator fragments: this lane's columns are rows 2 c and 2 c + 1
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int from = 4 * (2 * c + x);
+                mult[n][x] = __shfl_sync(0xffffffffu, m, from);
+                lo[n][x] = __shfl_sync(0xffffffffu, row_lo, from);
+                hi[n][x] = __shfl_sync(0xffffffffu, row_hi, from);
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    const float a = __shfl_sync(0xffffffffu, even[k], from), b = __shfl_sync(0xffffffffu, odd[k], from);
+                    start_acc[n][k][x] = -fmaf(1024.0f, a, 64.0f * b), q_sum[n][k][x] = a + b;
+                }
+            }
+            if (there) all_lo = max(all_lo, row_lo), all_hi = min(all_hi, row_hi), any_lo = min(any_lo, row_lo), any_hi = max(any_hi, row_hi);
+        }
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo), all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+
+        float o[NQ][D / 16][4] = {}, z[NQ][NG][2] = {}, top[NQ][2], sum[NQ][2] = {};
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) top[n][0] = top[n][1] = -INFINITY;
+        int ref = 8;  // biased exponent that p s is scaled against: follows the largest s
+
+        for (int step = warp; step * kSteps < s.tiles; step += kWarps) {
+            if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
+            __syncwarp();
+            const int ok = valid[slot];
+            const int base = (s.tile0 + step * kSteps) * kv4::kTile;
+            const int here = min(kSteps, s.tiles - step * kSteps);
+            const bool masked = here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi;
+            float sc[NQ][kSteps][4];
+            uint32_t vw[kSteps][2][NG], most = 0;
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                const unsigned char* tile = ring + slot * Cfg::kStageBytes + t * Cfg::kTileBytes;
+                uint32_t kw[2][NG];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    load_words(reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D)) + (g + 8 * x) * NG, kw[x]);
+                    load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_words_at(D, G)) + (g + 8 * x) * NG, vw[t][x]);
+                    if (masked) {  // what lies outside every row's sight may be anything, NaN among it
+                        const int j = base + t * kv4::kTile + g + 8 * x;
+                        const bool seen = t < here && (ok >> t & 1) && j >= any_lo && j < any_hi;
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k]);
+                }
+                uint32_t code[2][NW];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const unsigned char* at = tile + (g + 8 * x) * (D / 2) + c * (D / 8);
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at);
+                        code[x][0] = w.x, code[x][1] = w.y, code[x][NW - 2] = w.z, code[x][NW - 1] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(at);
+                        code[x][0] = w.x, code[x][1] = w.y;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sc[n][t][x] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    float acc[NQ][4];
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][2] = start_acc[n][k][0], acc[n][1] = acc[n][3] = start_acc[n][k][1];
+#pragma unroll
+                    for (int i = k * G / 32; i < (k + 1) * G / 32; ++i) {
+                        const uint32_t a0 = code[0][i], a1 = code[1][i], b0 = a0 >> 8, b1 = a1 >> 8;
+                        const uint32_t fa[4] = {ptx::lop3_and_or(a0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(a1, 0x000f000fu, 0x64006400u),
+                                                ptx::lop3_and_or(b0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(b1, 0x000f000fu, 0x64006400u)};
+                        const uint32_t fb[4] = {ptx::lop3_and_or(a0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(a1, 0x00f000f0u, 0x54005400u),
+                                                ptx::lop3_and_or(b0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(b1, 0x00f000f0u, 0x54005400u)};
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) {
+                            ptx::mma_f16_16816(acc[n], fa, qf[n][i][0], qf[n][i][1]);
+                            ptx::mma_f16_16816(acc[n], fb, qf[n][i][2], qf[n][i][3]);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t w = kw[x >> 1][k];
+                            sc[n][t][x] = fmaf(kv4::word_scale(w), acc[n][x], fmaf(kv4::word_min(w), q_sum[n][k][x & 1], sc[n][t][x]));
+                        }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        sc[n][t][x] *= mult[n][x & 1];
+                        if (masked) {
+                            const int j = base + t * kv4::kTile + g + 8 * (x >> 1);
+                            const bool seen = t < here && (ok >> t & 1) && j >= lo[n][x & 1] && j < hi[n][x & 1];
+                            sc[n][t][x] = seen ? sc[n][t][x] : -INFINITY;
+                        }
+                    }
+            }
+            // ---- running maximum, reference exponent -------------------------------------------------
+            most = __reduce_max_sync(0xffffffffu, most);
+            const int ref_new = max(ref, static_cast<int>(most >> 23));
+            float now[NQ][2];
+            bool moved = ref_new != ref;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float m = top[n][x];
+#pragma unroll
+                    for (int t = 0; t < kSteps; ++t) m = fmaxf(m, fmaxf(sc[n][t][x], sc[n][t][x + 2]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    now[n][x] = m;
+                    moved |= m != top[n][x];
+                }
+            if (__any_sync(0xffffffffu, moved)) {
+                const float fall = ref_new - ref > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - ref_new + ref) << 23);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float keep = top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(top[n][x] - now[n][x]);
+                        const float both = keep * fall;
+                        sum[n][x] *= keep;
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) z[n][k][x] *= keep;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) o[n][i][x] *= both, o[n][i][x + 2] *= both;
+                        top[n][x] = now[n][x];
+                    }
+                ref = ref_new;
+            }
+            const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - ref) << 23);  // p s scale_s < 2^8
+            // ---- weights and values ------------------------------------------------------------------
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                const unsigned char* tile = ring + slot * Cfg::kStageBytes + t * Cfg::kTileBytes;
+                uint32_t pf[NQ][NG][2];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    float pr[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float m = top[n][x & 1];
+                        pr[x] = ptx::exp2_fast(sc[n][t][x] - (m == -INFINITY ? 0.0f : m));
+                        sum[n][x & 1] += pr[x];
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) {
+                        float ps[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t w = vw[t][x >> 1][k];
+                            const bool skip = masked && pr[x] == 0.0f;  // a row that does not see the token: it may be a NaN
+                            const float sv = skip ? 0.0f : kv4::word_scale(w), mid = skip ? 0.0f : fmaf(8.0f, sv, kv4::word_min(w));
+                            ps[x] = pr[x] * (sv * scale_s);
+                            z[n][k][x & 1] = fmaf(pr[x], mid, z[n][k][x & 1]);
+                        }
+                        pf[n][k][0] = ptx::transpose_8x8(ptx::f16x2_pack(ps[0], ps[1]));
+                        pf[n][k][1] = ptx::transpose_8x8(ptx::f16x2_pack(ps[2], ps[3]));
+                    }
+                }
+                uint32_t w0[2][NW / 2], w1[2][NW / 2];  // [half of the tile][word]: tokens 2 c and 2 c + 1
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const unsigned char* at = tile + kv4::v_codes_at(D) + x * 4 * D + g * (D / 2) + c * (D / 8);
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at);
+                        w0[x][0] = w.x, w0[x][NW / 2 - 1] = w.y, w1[x][0] = w.z, w1[x][NW / 2 - 1] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(at);
+                        w0[x][0] = w.x, w1[x][0] = w.y;
+                    }
+                }
+#pragma unroll
+                for (int unit = 0; unit < NW; ++unit) {  // channels 32 unit .. + 31
+                    const uint32_t pick = unit & 1 ? 0x7632u : 0x5410u;
+                    const uint32_t a = __byte_perm(w0[0][unit / 2], w1[0][unit / 2], pick), b = __byte_perm(w0[1][unit / 2], w1[1][unit / 2], pick);
+                    const uint32_t a8 = a >> 8, b8 = b >> 8;
+                    auto low = [](uint32_t w) { return ptx::f16x2_sub(ptx::lop3_and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u); };   // 1024 + c - 1032
+                    auto high = [](uint32_t w) { return ptx::f16x2_sub(ptx::lop3_and_or(w, 0x00f000f0u, 0x54005400u), 0x54805480u); };  // 64 + c - 72
+                    const uint32_t fa[4] = {low(a), low(a8), low(b), low(b8)}, fb[4] = {high(a), high(a8), high(b), high(b8)};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        ptx::mma_f16_16816(o[n][2 * unit], fa, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
+                        ptx::mma_f16_16816(o[n][2 * unit + 1], fb, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (alive) fill_one(slot);
+            ++used;
+            if (++slot == S) slot = 0, phase ^= 1u;
+        }
+
+        // ---- the CTA's warps together ------------------------------------------------------------------
+        float* mx = m_max + (merges & 1) * kWarps * R;
+        float* sm = m_sum + (merges & 1) * kWarps * R;
+        ++merges;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {
+                    sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], d);
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) z[n][k][x] += __shfl_xor_sync(0xffffffffu, z[n][k][x], d);
+                }
+                if (g == 0) mx[warp * R + 8 * n + 2 * c + x] = top[n][x], sm[warp * R + 8 * n + 2 * c + x] = sum[n][x];
+            }
+        __syncthreads();
+        // what each warp holds, on the common maximum; the upper half of the warps hands its part to the lower half
+        const float unscale = __uint_as_float(static_cast<uint32_t>(ref - 7) << 23);
+        float part[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float m = -INFINITY;
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + 8 * n + 2 * c + x]);
+                part[n][x] = top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(top[n][x] - m);
+            }
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+            if (warp / (kWarps / 2) == half) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float* at = reinterpret_cast<float*>(merge + (warp % (kWarps / 2) * R + 8 * n + 2 * c + x) * Cfg::kORow);
+#pragma unroll
+                        for (int unit = 0; unit < NW; ++unit) {
+                            const float zz = z[n][32 * unit / G][x], k = part[n][x];
+                            float4* to = reinterpret_cast<float4*>(at + 32 * unit + 4 * g);
+                            float4 v = make_float4(fmaf(o[n][2 * unit][x], unscale, zz) * k, fmaf(o[n][2 * unit + 1][x], unscale, zz) * k,
+                                                   fmaf(o[n][2 * unit][x + 2], unscale, zz) * k, fmaf(o[n][2 * unit + 1][x + 2], unscale, zz) * k);
+                            if (half == 0) {
+                                const float4 other = *to;
+                                v.x += other.x, v.y += other.y, v.z += other.z, v.w += other.w;
+                            }
+                            *to = v;
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        const bool whole = s.begins && s.ends;
+        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (s.begins ? 1 : 0)) * Cfg::kPartial;
+        for (int i = threadIdx.x; i < R * (D / 4); i += 32 * kWarps) {
+            const int row = i / (D / 4), ch = i % (D / 4) * 4;
+            float m = -INFINITY, l = 0.0f;
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + row]);
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps / 2; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(merge + (w * R + row) * Cfg::kORow + ch * 4);
+                a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+            }
+            for (int w = 0; w < kWarps; ++w) {
+                const float t = mx[w * R + row];
+                l += t == -INFINITY ? sm[w * R + row] * 0.0f : sm[w * R + row] * ptx::exp2_fast(t - m);
+            }
+            if (whole) {
+                const int r = s.block * R + row;
+                if (r >= seq.count * group) continue;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(seq.first + r / group) * p.q_heads + s.head * group + r % group) * D + ch) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            } else {
+                *reinterpret_cast<float4*>(partial + row * D + ch) = a;
+                if (ch == 0) partial[R * D + 2 * row] = m, partial[R * D + 2 * row + 1] = l;
+            }
+        }
+        if (threadIdx.x == 0 && u + s.tiles >= end) {
+            // the last piece of the range: if it began here and goes on, this CTA's entry tells the adding launch of it
+            int4 entry = make_int4(0, 0, 0, 0);
+            if (s.begins && !s.ends)
+                entry = make_int4(cta_of(u + (seq.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1, seq.b, s.block, s.head);
+            p.pieces[blockIdx.x] = entry;
+        }
+    }
+    while (used < issued) {  // only after a wait that gave up: copies still in flight, each waited for once
+        ptx::mbar_wait(&full[slot], phase, p.status);
+        ++used;
+        if (++slot == S) slot = 0, phase ^= 1u;
+    }
+}
+
+// Adds the parts of the pieces that were cut across CTAs: block i those of the piece that began in CTA i of the launch before.
+template <int D, int R>
+__global__ void __launch_bounds__(256) kv4_attend_add_kernel(const AttendParams p) {
+    pdl_release();
+    pdl_wait();
+    const int4 piece = p.pieces[blockIdx.x];
+    if (piece.x == 0) return;
+    constexpr int kPartial = R * (D + 2);
+    const int group = p.q_heads / p.pool.heads;
+    int first, count;
+    kv4::rows_of(p.batch, piece.y, first, count);
+    const float* mine = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + 1) * kPartial;  // then every second slot
+    auto part = [&](int i) { return i == 0 ? mine : mine + (2 * static_cast<size_t>(i) - 1) * kPartial; };
+    for (int i = threadIdx.x; i < R * (D / 4); i += 256) {
+        const int row = i / (D / 4), ch = i % (D / 4) * 4, r = piece.z * R + row;
+        if (r >= count * group) break;
+        float m = -INFINITY;
+        for (int k = 0; k < piece.x; ++k) m = fmaxf(m, part(k)[R * D + 2 * row]);
+        float l = 0.0f;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < piece.x; ++k) {
+            const float* from = part(k);
+            const float t = from[R * D + 2 * row], w = t == -INFINITY ? 0.0f : ptx::exp2_fast(t - m);
+            const float4 v = *reinterpret_cast<const float4*>(from + row * D + ch);
+            a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
+            l = fmaf(from[R * D + 2 * row + 1], w, l);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(first + r / group) * p.q_heads + piece.w * group + r % group) * D + ch) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+}
+
+int rows_per_block(int rows, int seqs, int group) { return (static_cast<int64_t>(rows) * group > int64_t{8} * seqs) ? 16 : 8; }
+
+
+template <int D, int G, int NQ>
+int attend(AttendParams p, DeviceState* dev, cudaStream_t stream) {
+    using Cfg = SplitCfg<D, G, NQ>;
+    auto kernel = kv4_attend_split_kernel<D, G, NQ>;
+    static bool configured[kMaxDevices] = {};
+    if (!configured[dev->device]) {
+        SPK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+        configured[dev->device] = true;
+    }
+    const int grid = dev->sm_count * Cfg::kCtas < kMaxGrid ? dev->sm_count * Cfg::kCtas : kMaxGrid;
+    if (grid < kMinGrid) return fail(SPK_UNSUPPORTED, "kv4_attention: needs at least %d SMs, the device has %d", kMinGrid, dev->sm_count);
+    SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(32 * kWarps), Cfg::kSmem, stream, p));
+    SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows>, dim3(grid), dim3(256), 0, stream, p));
     return SPK_OK;
+}
+template <int D, int G>
+int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStream_t stream) {
+    return per_block == 8 ? attend<D, G, 1>(p, dev, stream) : attend<D, G, 2>(p, dev, stream);
 }
 
 }  // namespace
 }  // namespace spk
 
-extern "C" long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim) { return 16; }
+extern "C" long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim) {
+    using namespace spk;
+    if (rows < 0 || seqs < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
+    const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads);
+    return kMaxGrid * (16ll + 2ll * per_block * (head_dim + 2) * 4);
+}
 
 extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
                                  int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,
@@ -126,6 +700,7 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     if (rows == 0) return SPK_OK;
     SPK_REQUIRE(q && out && aligned16(q) && aligned16(out), "kv4_attention: q and out must be 16-byte aligned device pointers");
     SPK_REQUIRE(q_stride >= static_cast<long long>(q_heads) * head_dim && q_stride % 8 == 0, "kv4_attention: rows of q must be at least q_heads head_dim apart and a multiple of 8, got %lld", q_stride);
+    SPK_REQUIRE(static_cast<long long>(rows) * (q_heads / kv_heads) <= INT32_MAX / 2, "kv4_attention: rows x query heads per KV head must stay below 2^30");
     SPK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= spk_kv4_attention_workspace(rows, seqs, q_heads, kv_heads, head_dim),
                 "kv4_attention: the workspace must be 16-byte aligned and hold spk_kv4_attention_workspace() bytes, got %lld", workspace_bytes);
     DeviceState* dev = nullptr;
@@ -134,7 +709,10 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     p.pool = {static_cast<unsigned char*>(const_cast<void*>(pool)), pages, page_size, kv_heads, kv4::tile_bytes(head_dim, group)};
     p.q_heads = q_heads, p.window = window, p.zero_rest = zero_rest, p.scale = scale;
     p.out = static_cast<__nv_bfloat16*>(out), p.status = dev->status;
+    p.pieces = static_cast<int4*>(workspace);
+    p.partials = reinterpret_cast<float*>(p.pieces + kMaxGrid);
     auto stream = static_cast<cudaStream_t>(stream_);
-    if (head_dim == 64) return group == 32 ? attend<64, 32>(p, stream) : attend<64, 64>(p, stream);
-    return group == 32 ? attend<128, 32>(p, stream) : group == 64 ? attend<128, 64>(p, stream) : attend<128, 128>(p, stream);
+    const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads);
+    if (head_dim == 64) return group == 32 ? attend_rows<64, 32>(p, per_block, dev, stream) : attend_rows<64, 64>(p, per_block, dev, stream);
+    return group == 32 ? attend_rows<128, 32>(p, per_block, dev, stream) : group == 64 ? attend_rows<128, 64>(p, per_block, dev, stream) : attend_rows<128, 128>(p, per_block, dev, stream);
 }

@@ -4,7 +4,7 @@
 //             the cache as 4-bit codes, in one launch. The definition, in fp32 except where said:
 //               y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin   (x1, x2 the halves of the first rot channels; products and
 //                                                            sums rounded one by one; q rounded once more, to bf16)
-//               per group: m = bf16(min y), s = bf16((max y - m) / 15), 0 where that is below 2^-126,
+//               per group: m = bf16(min y), s = bf16((max y - m) * fp32(1 / 15)), 0 where that is below 2^-126,
 //                          c = clamp(rint((y - m) / s), 0, 15), 0 where s is 0
 //             A group that holds an infinity or a NaN, or whose range is past fp32, reads back as NaN (s = 0, m = NaN).
 //             The division is a true one: bf16 inputs often lie exactly on the border between two codes.
@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t quantize4(const Four& x, uint32_t& word) {
     }
     const __nv_bfloat16 mb = __float2bfloat16_rn(lo);
     const float m = __bfloat162float(mb);
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, m), 15.0f));
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, m), 1.0f / 15.0f));
     float s = __bfloat162float(sb);
     if (!finite || !(s <= FLT_MAX) || !(fabsf(m) <= FLT_MAX)) {
         word = 0x7fc0u;

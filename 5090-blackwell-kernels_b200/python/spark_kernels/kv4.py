@@ -72,7 +72,7 @@ def kv4_append(qkv: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, len
     positions, k and v quantized into the cache, q returned as bf16 [rows, Hq, head_dim]. cos_sin float32
     [positions, rot]: cosines then sines of the rotation of the first rot channels, whose halves are the pairs
     (rot a multiple of 8; None: no rotation). Per group of the (unrounded) channels y: m = bf16(min y),
-    s = bf16((max y - m) / 15), code = clamp(rint((y - m) / s), 0, 15), value = code * s + m; a group that holds an
+    s = bf16((max y - m) * (1 / 15)) in fp32, code = clamp(rint((y - m) / s), 0, 15), value = code * s + m; a group that holds an
     infinity or a NaN reads back as NaN. Rows of a given q_out behind the last sequence are left as they were (zeros
     in one that the call allocates)."""
     return _C.kv4_append(qkv, cache.pool, page_table, lens, cos_sin, q_offsets, cache.head_dim, cache.group, q_out)

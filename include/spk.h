@@ -181,7 +181,7 @@ SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int3
 SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported pair */
 /* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
  * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16
- * [rows][q_heads][head_dim] (zeros for padding) and quantizes k and v into the pool: per group m = bf16(min), s = bf16((max - m) / 15),
+ * [rows][q_heads][head_dim] (zeros for padding) and quantizes k and v into the pool: per group m = bf16(min), s = bf16((max - m) * fp32(1 / 15)),
  * c = clamp(rint((x - m) / s), 0, 15); a group with an infinity or a NaN reads back as NaN. */
 SPK_API int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool, int pages, int page_size, int q_heads, int kv_heads,
                            int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,

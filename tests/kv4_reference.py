@@ -40,7 +40,7 @@ def quantize(x: torch.Tensor, group: int):
     """x [..., d] float64 -> (values, scales, minima) of its codes, [..., d] each."""
     g = x.unflatten(-1, (-1, group))
     m = g.amin(-1, keepdim=True).to(torch.bfloat16).to(F64)
-    s = ((g.amax(-1, keepdim=True) - m) / 15).clamp(min=0).to(torch.bfloat16).to(F64)
+    s = ((g.amax(-1, keepdim=True) - m).float() * (1 / 15)).clamp(min=0).to(torch.bfloat16).to(F64)  # in fp32, as defined
     s = torch.where(s < 2.0 ** -126, torch.zeros_like(s), s)
     c = torch.where(s > 0, ((g - m) / s).round().clamp(0, 15), torch.zeros_like(g))
     return (c * s + m).flatten(-2), s.expand_as(g).flatten(-2), m.expand_as(g).flatten(-2)
