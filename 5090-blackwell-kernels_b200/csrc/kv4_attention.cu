@@ -19,7 +19,7 @@
 //
 // Work is cut into equal contiguous ranges of (sequence, block of rows, KV head, 16-token tile) units over the resident
 // CTAs, whatever the lengths are; every CTA finds its range itself from the lengths on the device. A warp takes every
-// eighth step of a range through a ring of its own, filled by bulk copies (a tile is one copy); a CTA merges its
+// seventh step of a range through a ring of its own, filled by bulk copies (a tile is one copy); a CTA merges its
 // warps in shared memory. What a CTA holds of a piece that is cut across CTAs goes to the workspace, and a second, chained
 // launch adds such pieces in the order of the CTAs: the same bits every run.
 #include "kv4_layout.cuh"
@@ -31,7 +31,10 @@ namespace {
 using kv4::Batch;
 using kv4::Pool;
 
-constexpr int kWarps = 8, kSteps = 2;  // warps of a CTA; 16-token tiles of a ring stage
+// Seven consuming warps and one that fills their rings: a ninth would cost every thread a quarter of its registers.
+constexpr int kWarps = 7, kThreads = 32 * (kWarps + 1);
+constexpr int kSteps = 2;                // 16-token tiles of a ring stage
+constexpr int kFold = (kWarps + 1) / 2;  // in a merge warp w takes the part of warp w + kFold
 constexpr int kMinUnits = kWarps;      // a CTA gets at least this many tiles: one per warp
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
@@ -55,9 +58,9 @@ struct SplitCfg {
     static constexpr int kTileBytes = kv4::tile_bytes(D, G), kStageBytes = kSteps * kTileBytes;
     static constexpr int kCtas = NQ == 1 ? 2 : 1;  // per SM: what the registers allow
     static constexpr int kORow = D * 4 + 32;       // a row's pitch in the merge buffer: the lanes of a store hit every bank once
-    static constexpr int kMerge = kWarps / 2 * kRows * kORow;
-    // maxima and sums [2][warps][rows], chunk starts [threads + 1], barriers and valid flags of six stages
-    static constexpr int kSmall = 2 * 2 * kWarps * kRows * 4 + (32 * kWarps + 1) * 8 + kWarps * 6 * 12 + 64;
+    static constexpr int kMerge = kFold * kRows * kORow;
+    // maxima and sums [2][warps][rows], chunk starts, barriers and valid flags of six stages
+    static constexpr int kSmall = 2 * 2 * kWarps * kRows * 4 + kThreads * 8 + kWarps * 6 * 20 + 64;
     static constexpr int kFit = ((227 * 1024 - 1024 * kCtas) / kCtas - kMerge - kSmall) / (kWarps * kStageBytes);
     static constexpr int kStages = kFit < 6 ? kFit : 6;
     static constexpr int kRing = kWarps * kStages * kStageBytes, kSmem = kRing + kMerge + kSmall;
@@ -120,8 +123,171 @@ __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N])
     }
 }
 
+// A barrier of the consuming warps.
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+// What a warp carries through the tiles of a piece.
 template <int D, int G, int NQ>
-__global__ void __launch_bounds__(32 * kWarps, (SplitCfg<D, G, NQ>::kCtas))
+struct State {
+    static constexpr int kGroups = D / G, kWords = D / 32;
+    // of the piece's rows, as B fragments (column: row g): word i's step A (even channels) b0, b1, step B (odd ones) b0, b1
+    uint32_t q[NQ][kWords][4];
+    // as accumulator columns (rows 2 c and 2 c + 1): the offsets' start value, the sum of q', the score's factor, the tokens seen
+    float start[NQ][kGroups][2], q_sum[NQ][kGroups][2], mult[NQ][2];
+    int lo[NQ][2], hi[NQ][2], any_lo, any_hi;
+    // the running softmax: maxima (in powers of two), sums, values (channels 32 u + 4 g + {0, 2} in o[2 u], {1, 3} in o[2 u + 1]), sum p (8 s + m)
+    float top[NQ][2], sum[NQ][2], o[NQ][D / 16][4], z[NQ][kGroups][2];
+    int ref;  // biased exponent of the largest s so far: what p s is scaled against
+};
+
+// kSteps tiles of 16 tokens. Masked: some token is out of some row's sight, or a tile is missing (ok: the tiles that are there).
+template <int D, int G, int NQ, bool Masked>
+__device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned char* tiles, int lane, int ok, int base) {
+    constexpr int NG = D / G, NW = D / 32, kTileBytes = kv4::tile_bytes(D, G);
+    const int g = lane >> 2, c = lane & 3;
+    float sc[NQ][kSteps][4];
+    uint32_t vw[kSteps][2][NG], most = 0;
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+        const unsigned char* tile = tiles + t * kTileBytes;
+        uint32_t kw[2][NG], code[2][NW];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D)) + (g + 8 * x) * NG, kw[x]);
+            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_words_at(D, G)) + (g + 8 * x) * NG, vw[t][x]);
+            load_words(reinterpret_cast<const uint32_t*>(tile + (g + 8 * x) * (D / 2) + c * (D / 8)), code[x]);
+            if (Masked) {  // what lies outside every row's sight may be anything, NaN among it
+                const int j = base + t * kv4::kTile + g + 8 * x;
+                const bool seen = (ok >> t & 1) && j >= st.any_lo && j < st.any_hi;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            float acc[NQ][4];
+#pragma unroll
+            for (int i = k * G / 32; i < (k + 1) * G / 32; ++i) {
+                const uint32_t a0 = code[0][i], a1 = code[1][i], b0 = a0 >> 8, b1 = a1 >> 8;
+                const uint32_t fa[4] = {ptx::lop3_and_or(a0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(a1, 0x000f000fu, 0x64006400u),
+                                        ptx::lop3_and_or(b0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(b1, 0x000f000fu, 0x64006400u)};
+                const uint32_t fb[4] = {ptx::lop3_and_or(a0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(a1, 0x00f000f0u, 0x54005400u),
+                                        ptx::lop3_and_or(b0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(b1, 0x00f000f0u, 0x54005400u)};
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    if (i == k * G / 32) ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1], st.start[n][k][0], st.start[n][k][1]);
+                    else ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1]);
+                    ptx::mma_f16_16816(acc[n], fb, st.q[n][i][2], st.q[n][i][3]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float s = kv4::word_scale(kw[x >> 1][k]), m = kv4::word_min(kw[x >> 1][k]), qs = st.q_sum[n][k][x & 1];
+                    sc[n][t][x] = fmaf(s, acc[n][x], k == 0 ? m * qs : fmaf(m, qs, sc[n][t][x]));
+                }
+        }
+        if (Masked) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int j = base + t * kv4::kTile + g + 8 * (x >> 1);
+                    const bool seen = (ok >> t & 1) && j >= st.lo[n][x & 1] && j < st.hi[n][x & 1];
+                    sc[n][t][x] = seen ? sc[n][t][x] : -INFINITY;
+                }
+        }
+    }
+    // ---- running maximum, reference exponent
+    most = __reduce_max_sync(0xffffffffu, most);
+    const int ref = max(st.ref, static_cast<int>(most >> 23));
+    float now[NQ][2];
+    bool moved = ref != st.ref;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float m = fmaxf(sc[n][0][x], sc[n][0][x + 2]);
+#pragma unroll
+            for (int t = 1; t < kSteps; ++t) m = fmaxf(m, fmaxf(sc[n][t][x], sc[n][t][x + 2]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            now[n][x] = fmaxf(st.top[n][x], m * st.mult[n][x]);
+            moved |= now[n][x] != st.top[n][x];
+        }
+    if (__any_sync(0xffffffffu, moved)) {
+        const float fall = ref - st.ref > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - ref + st.ref) << 23);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float keep = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - now[n][x]);
+                const float both = keep * fall;
+                st.sum[n][x] *= keep;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) st.z[n][k][x] *= keep;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) st.o[n][i][x] *= both, st.o[n][i][x + 2] *= both;
+                st.top[n][x] = now[n][x];
+            }
+        st.ref = ref;
+    }
+    const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - ref) << 23);  // p s scale_s < 2^8
+    // ---- weights and values
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+        const unsigned char* tile = tiles + t * kTileBytes;
+        uint32_t pf[NQ][NG][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float pr[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float m = Masked && st.top[n][x & 1] == -INFINITY ? 0.0f : st.top[n][x & 1];
+                pr[x] = ptx::exp2_fast(fmaf(sc[n][t][x], st.mult[n][x & 1], -m));
+                st.sum[n][x & 1] += pr[x];
+            }
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                float ps[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t w = vw[t][x >> 1][k];
+                    float sv = kv4::word_scale(w), mid = fmaf(8.0f, sv, kv4::word_min(w));
+                    if (Masked && pr[x] == 0.0f) sv = mid = 0.0f;  // a row that does not see the token: it may be a NaN
+                    ps[x] = pr[x] * (sv * scale_s);
+                    st.z[n][k][x & 1] = fmaf(pr[x], mid, st.z[n][k][x & 1]);
+                }
+                pf[n][k][0] = ptx::transpose_8x8(ptx::f16x2_pack(ps[0], ps[1]));
+                pf[n][k][1] = ptx::transpose_8x8(ptx::f16x2_pack(ps[2], ps[3]));
+            }
+        }
+        uint32_t w[2][NW];  // [half of the tile]: words of tokens 2 c, then of 2 c + 1
+#pragma unroll
+        for (int x = 0; x < 2; ++x) load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_codes_at(D) + x * 4 * D + g * (D / 2) + c * (D / 8)), w[x]);
+#pragma unroll
+        for (int unit = 0; unit < NW; ++unit) {  // channels 32 unit .. + 31
+            const uint32_t pick = unit & 1 ? 0x7632u : 0x5410u;
+            const uint32_t a = __byte_perm(w[0][unit / 2], w[0][unit / 2 + NW / 2], pick), b = __byte_perm(w[1][unit / 2], w[1][unit / 2 + NW / 2], pick);
+            const uint32_t a8 = a >> 8, b8 = b >> 8;
+            auto low = [](uint32_t v) { return ptx::f16x2_sub(ptx::lop3_and_or(v, 0x000f000fu, 0x64006400u), 0x64086408u); };   // 1024 + c - 1032
+            auto high = [](uint32_t v) { return ptx::f16x2_sub(ptx::lop3_and_or(v, 0x00f000f0u, 0x54005400u), 0x54805480u); };  // 64 + c - 72
+            const uint32_t fa[4] = {low(a), low(a8), low(b), low(b8)}, fb[4] = {high(a), high(a8), high(b), high(b8)};
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                ptx::mma_f16_16816(st.o[n][2 * unit], fa, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
+                ptx::mma_f16_16816(st.o[n][2 * unit + 1], fb, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
+            }
+        }
+    }
+}
+
+template <int D, int G, int NQ>
+__global__ void __launch_bounds__(kThreads, (SplitCfg<D, G, NQ>::kCtas))
 kv4_attend_split_kernel(const AttendParams p) {
     using Cfg = SplitCfg<D, G, NQ>;
     constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages;
@@ -129,16 +295,18 @@ kv4_attend_split_kernel(const AttendParams p) {
     unsigned char* merge = smem + Cfg::kRing;
     float* m_max = reinterpret_cast<float*>(merge + Cfg::kMerge);  // [2][warps][rows]
     float* m_sum = m_max + 2 * kWarps * R;
-    long long* chunk_start = reinterpret_cast<long long*>(m_sum + 2 * kWarps * R);  // [threads + 1]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(chunk_start + 32 * kWarps + 1);
-    int* valid_all = reinterpret_cast<int*>(bars + kWarps * S);
+    long long* chunk_start = reinterpret_cast<long long*>(m_sum + 2 * kWarps * R);  // [threads]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(chunk_start + kThreads);
+    int* valid_all = reinterpret_cast<int*>(bars + 2 * kWarps * S);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    unsigned char* ring = smem + warp * S * Cfg::kStageBytes;
-    uint64_t* full = bars + warp * S;
-    int* valid = valid_all + warp * S;
-    if (lane == 0) {
-        for (int s = 0; s < S; ++s) ptx::mbar_init(&full[s], 1);
+    // a ring per consuming warp; the last warp's lane w fills that of warp w
+    const int mine = warp < kWarps ? warp : min(lane, kWarps - 1);
+    unsigned char* ring = smem + mine * S * Cfg::kStageBytes;
+    uint64_t *full = bars + mine * 2 * S, *empty = full + S;
+    int* valid = valid_all + mine * S;
+    if (warp == kWarps && lane < kWarps) {
+        for (int s = 0; s < 2 * S; ++s) ptx::mbar_init(&full[s], 1);
         ptx::fence_mbar_init();
     }
     pdl_release();
@@ -149,13 +317,13 @@ kv4_attend_split_kernel(const AttendParams p) {
     auto zero_rows = [&](int from, int to) {
         const long long pieces = static_cast<long long>(max(0, to - from)) * p.q_heads * (D / 8);
         uint4* at = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(from) * p.q_heads * D);
-        for (long long i = threadIdx.x; i < pieces; i += 32 * kWarps) at[i] = make_uint4(0, 0, 0, 0);
+        for (long long i = threadIdx.x; i < pieces; i += kThreads) at[i] = make_uint4(0, 0, 0, 0);
     };
     // units before every chunk of sequences, one chunk a thread
-    const int chunk = (p.batch.seqs + 32 * kWarps - 1) / (32 * kWarps);
+    const int chunk = (p.batch.seqs + kThreads - 1) / kThreads;
     long long total;
     {
-        __shared__ long long warp_sum[kWarps];
+        __shared__ long long warp_sum[kWarps + 1];
         __shared__ int empties, empty_seqs[kv4::kMaxSeqs / kMinGrid];  // of the ones that fall to this CTA
         if (threadIdx.x == 0) empties = 0;
         __syncthreads();
@@ -178,7 +346,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         __syncthreads();
         long long before = 0;
         total = 0;
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w <= kWarps; ++w) {
             if (w < warp) before += warp_sum[w];
             total += warp_sum[w];
         }
@@ -208,7 +376,7 @@ kv4_attend_split_kernel(const AttendParams p) {
     Seq seq;
     {
         int at = 0;
-        for (int hi = 32 * kWarps - 1; at < hi;) {
+        for (int hi = kThreads - 1; at < hi;) {
             const int mid = (at + hi + 1) >> 1;
             if (chunk_start[mid] <= start) at = mid; else hi = mid - 1;
         }
@@ -217,61 +385,72 @@ kv4_attend_split_kernel(const AttendParams p) {
         load_seq(p, R, seq);
     }
 
-    // the filling side of the ring walks the same steps ahead of the consuming side; page numbers are read a step early
-    long long fill_u = start;
-    Seq fill_seq = seq;
-    Piece fill = piece_at(p, R, fill_u, end, fill_seq);
-    int fill_step = warp, issued = 0, page[kSteps];
-    auto fill_settle = [&]() {  // to the next step of this warp at or after fill_step; false at the end of the range
-        while (fill_step * kSteps >= fill.tiles) {
-            fill_u += fill.tiles;
-            if (fill_u >= end) return false;
-            fill = piece_at(p, R, fill_u, end, fill_seq);
-            fill_step = warp;
-        }
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (fill_step * kSteps + i < fill.tiles)
-                page[i] = __ldg(p.batch.table + static_cast<size_t>(fill_seq.b) * p.batch.width + (fill.tile0 + fill_step * kSteps + i) / tiles_per_page);
-        return true;
-    };
-    bool filling = fill_settle();
-    auto fill_one = [&](int slot) {
-        if (!filling) return;
-        if (lane == 0) {
-            int ok = 0, n = 0;
+    if (warp == kWarps) {
+        // ---- the filling warp: each lane walks the steps of its consuming warp, page numbers a step early ----------
+        long long u = start;
+        Piece s = piece_at(p, R, u, end, seq);
+        int step = lane, slot = 0, page[kSteps];
+        unsigned phase = 1;  // the first round of a ring is free
+        auto settle = [&]() {  // to the next step of this lane's warp at or after `step`; false at the end of the range
+            while (step * kSteps >= s.tiles) {
+                u += s.tiles;
+                if (u >= end) return false;
+                s = piece_at(p, R, u, end, seq);
+                step = lane;
+            }
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
-                if (fill_step * kSteps + i < fill.tiles) {
-                    if (page[i] >= 0 && page[i] < p.pool.pages) ok |= 1 << i, ++n;
-                    else atomicCAS(p.status, 0, SPK_BAD_INDEX);
-                }
-            valid[slot] = ok;
-            ptx::mbar_arrive_expect_tx(&full[slot], n * Cfg::kTileBytes);
+                if (step * kSteps + i < s.tiles)
+                    page[i] = __ldg(p.batch.table + static_cast<size_t>(seq.b) * p.batch.width + (s.tile0 + step * kSteps + i) / tiles_per_page);
+            return true;
+        };
+        bool filling = lane < kWarps && settle();
+        long long since = clock64();
+        while (__any_sync(0xffffffffu, filling)) {
+            bool went = false;
+            if (filling && ptx::mbar_test_wait(&empty[slot], phase)) {
+                went = true;
+                int ok = 0, n = 0;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                if (ok >> i & 1) {
-                    const int tile = fill.tile0 + fill_step * kSteps + i;
-                    const unsigned char* from = p.pool.data + ((static_cast<size_t>(page[i]) * p.pool.heads + fill.head) * tiles_per_page + tile % tiles_per_page) * Cfg::kTileBytes;
-                    ptx::bulk_g2s(ring + slot * Cfg::kStageBytes + i * Cfg::kTileBytes, from, Cfg::kTileBytes, &full[slot]);
+                for (int i = 0; i < kSteps; ++i)
+                    if (step * kSteps + i < s.tiles) {
+                        if (page[i] >= 0 && page[i] < p.pool.pages) ok |= 1 << i, ++n;
+                        else atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                    }
+                valid[slot] = ok;
+                ptx::mbar_arrive_expect_tx(&full[slot], n * Cfg::kTileBytes);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+                    if (ok >> i & 1) {
+                        const int tile = s.tile0 + step * kSteps + i;
+                        const unsigned char* from = p.pool.data + ((static_cast<size_t>(page[i]) * p.pool.heads + s.head) * tiles_per_page + tile % tiles_per_page) * Cfg::kTileBytes;
+                        ptx::bulk_g2s(ring + slot * Cfg::kStageBytes + i * Cfg::kTileBytes, from, Cfg::kTileBytes, &full[slot]);
+                    }
+                step += kWarps;
+                if (++slot == S) slot = 0, phase ^= 1u;
+                filling = settle();
+            }
+            if (__any_sync(0xffffffffu, went)) {
+                since = clock64();
+            } else {
+                if (clock64() - since > 2 * ptx::kWaitCycles) {  // the consumers gave up; what is in flight has long landed
+                    if (lane == 0) atomicCAS(p.status, 0, SPK_TIMEOUT);
+                    break;
                 }
+                __nanosleep(40);
+            }
         }
-        ++issued;
-        fill_step += kWarps;
-        filling = fill_settle();
-    };
-    for (int s = 0; s < S; ++s) fill_one(s);
+    }
 
-    int slot = 0, used = 0, merges = 0;
+    int slot = 0, merges = 0;
     unsigned phase = 0;
     bool alive = true;
     Piece s;
-    for (long long u = start; u < end; u += s.tiles) {
+    State<D, G, NQ> st;
+    for (long long u = start; warp < kWarps && u < end; u += s.tiles) {
         s = piece_at(p, R, u, end, seq);
         // ---- the rows of this piece: Q fragments, their sums per group, what each row sees -----------
-        uint32_t qf[NQ][NW][4];  // [word][(step A: b0, b1), (step B: b0, b1)]
-        float start_acc[NQ][NG][2], q_sum[NQ][NG][2], mult[NQ][2];
-        int lo[NQ][2], hi[NQ][2], all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
+        int all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const int row = s.block * R + 8 * n + g;  // B fragments: this lane's column is row g
@@ -304,17 +483,17 @@ kv4_attend_split_kernel(const AttendParams p) {
             for (int i = 0; i < NW; ++i) {
                 float h[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = finite ? v[i][j] * down : 0.0f;
-                qf[n][i][0] = ptx::f16x2_pack(h[0], h[4]), qf[n][i][1] = ptx::f16x2_pack(h[2], h[6]);
-                qf[n][i][2] = ptx::f16x2_pack(h[1], h[5]), qf[n][i][3] = ptx::f16x2_pack(h[3], h[7]);
+                for (int j = 0; j < 8; ++j) h[j] = finite ? v[i][j] * (p.scale < 0.0f ? -down : down) : 0.0f;
+                st.q[n][i][0] = ptx::f16x2_pack(h[0], h[4]), st.q[n][i][1] = ptx::f16x2_pack(h[2], h[6]);
+                st.q[n][i][2] = ptx::f16x2_pack(h[1], h[5]), st.q[n][i][3] = ptx::f16x2_pack(h[3], h[7]);
                 // sums of what the MMA will really multiply by
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][i][j]));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&st.q[n][i][j]));
                     (j < 2 ? even : odd)[32 * i / G] += f.x + f.y;
                 }
             }
-            const float m = p.scale * 1.4426950408889634f * up;
+            const float m = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
             const int pos = seq.len - seq.count + row / group;
             const int row_hi = there ? max(0, pos + 1) : 0, row_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
 #pragma unroll
@@ -326,200 +505,42 @@ kv4_attend_split_kernel(const AttendParams p) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int from = 4 * (2 * c + x);
-                mult[n][x] = __shfl_sync(0xffffffffu, m, from);
-                lo[n][x] = __shfl_sync(0xffffffffu, row_lo, from);
-                hi[n][x] = __shfl_sync(0xffffffffu, row_hi, from);
+                st.mult[n][x] = __shfl_sync(0xffffffffu, m, from);
+                st.lo[n][x] = __shfl_sync(0xffffffffu, row_lo, from);
+                st.hi[n][x] = __shfl_sync(0xffffffffu, row_hi, from);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     const float a = __shfl_sync(0xffffffffu, even[k], from), b = __shfl_sync(0xffffffffu, odd[k], from);
-                    start_acc[n][k][x] = -fmaf(1024.0f, a, 64.0f * b), q_sum[n][k][x] = a + b;
+                    st.start[n][k][x] = -fmaf(1024.0f, a, 64.0f * b), st.q_sum[n][k][x] = a + b;
                 }
             }
             if (there) all_lo = max(all_lo, row_lo), all_hi = min(all_hi, row_hi), any_lo = min(any_lo, row_lo), any_hi = max(any_hi, row_hi);
         }
         all_lo = __reduce_max_sync(0xffffffffu, all_lo), all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-        any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
-
-        float o[NQ][D / 16][4] = {}, z[NQ][NG][2] = {}, top[NQ][2], sum[NQ][2] = {};
+        st.any_lo = __reduce_min_sync(0xffffffffu, any_lo), st.any_hi = __reduce_max_sync(0xffffffffu, any_hi);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) top[n][0] = top[n][1] = -INFINITY;
-        int ref = 8;  // biased exponent that p s is scaled against: follows the largest s
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                st.top[n][x] = -INFINITY, st.sum[n][x] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) st.z[n][k][x] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) st.o[n][i][x] = st.o[n][i][x + 2] = 0.0f;
+            }
+        st.ref = 8;
 
         for (int step = warp; step * kSteps < s.tiles; step += kWarps) {
             if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
-            __syncwarp();
-            const int ok = valid[slot];
-            const int base = (s.tile0 + step * kSteps) * kv4::kTile;
+            const int ok = valid[slot], base = (s.tile0 + step * kSteps) * kv4::kTile;
             const int here = min(kSteps, s.tiles - step * kSteps);
-            const bool masked = here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi;
-            float sc[NQ][kSteps][4];
-            uint32_t vw[kSteps][2][NG], most = 0;
-#pragma unroll
-            for (int t = 0; t < kSteps; ++t) {
-                const unsigned char* tile = ring + slot * Cfg::kStageBytes + t * Cfg::kTileBytes;
-                uint32_t kw[2][NG];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    load_words(reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D)) + (g + 8 * x) * NG, kw[x]);
-                    load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_words_at(D, G)) + (g + 8 * x) * NG, vw[t][x]);
-                    if (masked) {  // what lies outside every row's sight may be anything, NaN among it
-                        const int j = base + t * kv4::kTile + g + 8 * x;
-                        const bool seen = t < here && (ok >> t & 1) && j >= any_lo && j < any_hi;
-#pragma unroll
-                        for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
-                    }
-#pragma unroll
-                    for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k]);
-                }
-                uint32_t code[2][NW];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const unsigned char* at = tile + (g + 8 * x) * (D / 2) + c * (D / 8);
-                    if constexpr (D == 128) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(at);
-                        code[x][0] = w.x, code[x][1] = w.y, code[x][NW - 2] = w.z, code[x][NW - 1] = w.w;
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(at);
-                        code[x][0] = w.x, code[x][1] = w.y;
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) sc[n][t][x] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    float acc[NQ][4];
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][2] = start_acc[n][k][0], acc[n][1] = acc[n][3] = start_acc[n][k][1];
-#pragma unroll
-                    for (int i = k * G / 32; i < (k + 1) * G / 32; ++i) {
-                        const uint32_t a0 = code[0][i], a1 = code[1][i], b0 = a0 >> 8, b1 = a1 >> 8;
-                        const uint32_t fa[4] = {ptx::lop3_and_or(a0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(a1, 0x000f000fu, 0x64006400u),
-                                                ptx::lop3_and_or(b0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(b1, 0x000f000fu, 0x64006400u)};
-                        const uint32_t fb[4] = {ptx::lop3_and_or(a0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(a1, 0x00f000f0u, 0x54005400u),
-                                                ptx::lop3_and_or(b0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(b1, 0x00f000f0u, 0x54005400u)};
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n) {
-                            ptx::mma_f16_16816(acc[n], fa, qf[n][i][0], qf[n][i][1]);
-                            ptx::mma_f16_16816(acc[n], fb, qf[n][i][2], qf[n][i][3]);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t w = kw[x >> 1][k];
-                            sc[n][t][x] = fmaf(kv4::word_scale(w), acc[n][x], fmaf(kv4::word_min(w), q_sum[n][k][x & 1], sc[n][t][x]));
-                        }
-                }
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        sc[n][t][x] *= mult[n][x & 1];
-                        if (masked) {
-                            const int j = base + t * kv4::kTile + g + 8 * (x >> 1);
-                            const bool seen = t < here && (ok >> t & 1) && j >= lo[n][x & 1] && j < hi[n][x & 1];
-                            sc[n][t][x] = seen ? sc[n][t][x] : -INFINITY;
-                        }
-                    }
-            }
-            // ---- running maximum, reference exponent -------------------------------------------------
-            most = __reduce_max_sync(0xffffffffu, most);
-            const int ref_new = max(ref, static_cast<int>(most >> 23));
-            float now[NQ][2];
-            bool moved = ref_new != ref;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float m = top[n][x];
-#pragma unroll
-                    for (int t = 0; t < kSteps; ++t) m = fmaxf(m, fmaxf(sc[n][t][x], sc[n][t][x + 2]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    now[n][x] = m;
-                    moved |= m != top[n][x];
-                }
-            if (__any_sync(0xffffffffu, moved)) {
-                const float fall = ref_new - ref > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - ref_new + ref) << 23);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float keep = top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(top[n][x] - now[n][x]);
-                        const float both = keep * fall;
-                        sum[n][x] *= keep;
-#pragma unroll
-                        for (int k = 0; k < NG; ++k) z[n][k][x] *= keep;
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) o[n][i][x] *= both, o[n][i][x + 2] *= both;
-                        top[n][x] = now[n][x];
-                    }
-                ref = ref_new;
-            }
-            const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - ref) << 23);  // p s scale_s < 2^8
-            // ---- weights and values ------------------------------------------------------------------
-#pragma unroll
-            for (int t = 0; t < kSteps; ++t) {
-                const unsigned char* tile = ring + slot * Cfg::kStageBytes + t * Cfg::kTileBytes;
-                uint32_t pf[NQ][NG][2];
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    float pr[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float m = top[n][x & 1];
-                        pr[x] = ptx::exp2_fast(sc[n][t][x] - (m == -INFINITY ? 0.0f : m));
-                        sum[n][x & 1] += pr[x];
-                    }
-#pragma unroll
-                    for (int k = 0; k < NG; ++k) {
-                        float ps[4];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t w = vw[t][x >> 1][k];
-                            const bool skip = masked && pr[x] == 0.0f;  // a row that does not see the token: it may be a NaN
-                            const float sv = skip ? 0.0f : kv4::word_scale(w), mid = skip ? 0.0f : fmaf(8.0f, sv, kv4::word_min(w));
-                            ps[x] = pr[x] * (sv * scale_s);
-                            z[n][k][x & 1] = fmaf(pr[x], mid, z[n][k][x & 1]);
-                        }
-                        pf[n][k][0] = ptx::transpose_8x8(ptx::f16x2_pack(ps[0], ps[1]));
-                        pf[n][k][1] = ptx::transpose_8x8(ptx::f16x2_pack(ps[2], ps[3]));
-                    }
-                }
-                uint32_t w0[2][NW / 2], w1[2][NW / 2];  // [half of the tile][word]: tokens 2 c and 2 c + 1
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const unsigned char* at = tile + kv4::v_codes_at(D) + x * 4 * D + g * (D / 2) + c * (D / 8);
-                    if constexpr (D == 128) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(at);
-                        w0[x][0] = w.x, w0[x][NW / 2 - 1] = w.y, w1[x][0] = w.z, w1[x][NW / 2 - 1] = w.w;
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(at);
-                        w0[x][0] = w.x, w1[x][0] = w.y;
-                    }
-                }
-#pragma unroll
-                for (int unit = 0; unit < NW; ++unit) {  // channels 32 unit .. + 31
-                    const uint32_t pick = unit & 1 ? 0x7632u : 0x5410u;
-                    const uint32_t a = __byte_perm(w0[0][unit / 2], w1[0][unit / 2], pick), b = __byte_perm(w0[1][unit / 2], w1[1][unit / 2], pick);
-                    const uint32_t a8 = a >> 8, b8 = b >> 8;
-                    auto low = [](uint32_t w) { return ptx::f16x2_sub(ptx::lop3_and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u); };   // 1024 + c - 1032
-                    auto high = [](uint32_t w) { return ptx::f16x2_sub(ptx::lop3_and_or(w, 0x00f000f0u, 0x54005400u), 0x54805480u); };  // 64 + c - 72
-                    const uint32_t fa[4] = {low(a), low(a8), low(b), low(b8)}, fb[4] = {high(a), high(a8), high(b), high(b8)};
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        ptx::mma_f16_16816(o[n][2 * unit], fa, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
-                        ptx::mma_f16_16816(o[n][2 * unit + 1], fb, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
-                    }
-                }
-            }
+            const unsigned char* tiles = ring + slot * Cfg::kStageBytes;
+            if (here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi)
+                attend_step<D, G, NQ, true>(st, tiles, lane, ok & ((1 << here) - 1), base);
+            else
+                attend_step<D, G, NQ, false>(st, tiles, lane, ok, base);
             __syncwarp();
-            if (alive) fill_one(slot);
-            ++used;
+            if (lane == 0) ptx::mbar_arrive(&empty[slot]);
             if (++slot == S) slot = 0, phase ^= 1u;
         }
 
@@ -533,15 +554,15 @@ kv4_attend_split_kernel(const AttendParams p) {
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) {
-                    sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], d);
+                    st.sum[n][x] += __shfl_xor_sync(0xffffffffu, st.sum[n][x], d);
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) z[n][k][x] += __shfl_xor_sync(0xffffffffu, z[n][k][x], d);
+                    for (int k = 0; k < NG; ++k) st.z[n][k][x] += __shfl_xor_sync(0xffffffffu, st.z[n][k][x], d);
                 }
-                if (g == 0) mx[warp * R + 8 * n + 2 * c + x] = top[n][x], sm[warp * R + 8 * n + 2 * c + x] = sum[n][x];
+                if (g == 0) mx[warp * R + 8 * n + 2 * c + x] = st.top[n][x], sm[warp * R + 8 * n + 2 * c + x] = st.sum[n][x];
             }
-        __syncthreads();
+        consumers_sync();
         // what each warp holds, on the common maximum; the upper half of the warps hands its part to the lower half
-        const float unscale = __uint_as_float(static_cast<uint32_t>(ref - 7) << 23);
+        const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
         float part[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -549,23 +570,23 @@ kv4_attend_split_kernel(const AttendParams p) {
             for (int x = 0; x < 2; ++x) {
                 float m = -INFINITY;
                 for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + 8 * n + 2 * c + x]);
-                part[n][x] = top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(top[n][x] - m);
+                part[n][x] = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m);
             }
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
-            if (warp / (kWarps / 2) == half) {
+            if (warp / kFold == half) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float* at = reinterpret_cast<float*>(merge + (warp % (kWarps / 2) * R + 8 * n + 2 * c + x) * Cfg::kORow);
+                        float* at = reinterpret_cast<float*>(merge + (warp % kFold * R + 8 * n + 2 * c + x) * Cfg::kORow);
 #pragma unroll
                         for (int unit = 0; unit < NW; ++unit) {
-                            const float zz = z[n][32 * unit / G][x], k = part[n][x];
+                            const float zz = st.z[n][32 * unit / G][x], k = part[n][x];
                             float4* to = reinterpret_cast<float4*>(at + 32 * unit + 4 * g);
-                            float4 v = make_float4(fmaf(o[n][2 * unit][x], unscale, zz) * k, fmaf(o[n][2 * unit + 1][x], unscale, zz) * k,
-                                                   fmaf(o[n][2 * unit][x + 2], unscale, zz) * k, fmaf(o[n][2 * unit + 1][x + 2], unscale, zz) * k);
-                            if (half == 0) {
+                            float4 v = make_float4(fmaf(st.o[n][2 * unit][x], unscale, zz) * k, fmaf(st.o[n][2 * unit + 1][x], unscale, zz) * k,
+                                                   fmaf(st.o[n][2 * unit][x + 2], unscale, zz) * k, fmaf(st.o[n][2 * unit + 1][x + 2], unscale, zz) * k);
+                            if (half == 0 && warp + kFold < kWarps) {
                                 const float4 other = *to;
                                 v.x += other.x, v.y += other.y, v.z += other.z, v.w += other.w;
                             }
@@ -573,7 +594,7 @@ kv4_attend_split_kernel(const AttendParams p) {
                         }
                     }
             }
-            __syncthreads();
+            consumers_sync();
         }
         const bool whole = s.begins && s.ends;
         float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (s.begins ? 1 : 0)) * Cfg::kPartial;
@@ -583,7 +604,7 @@ kv4_attend_split_kernel(const AttendParams p) {
             for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + row]);
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kWarps / 2; ++w) {
+            for (int w = 0; w < kFold; ++w) {
                 const float4 v = *reinterpret_cast<const float4*>(merge + (w * R + row) * Cfg::kORow + ch * 4);
                 a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
             }
@@ -610,11 +631,6 @@ kv4_attend_split_kernel(const AttendParams p) {
                 entry = make_int4(cta_of(u + (seq.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1, seq.b, s.block, s.head);
             p.pieces[blockIdx.x] = entry;
         }
-    }
-    while (used < issued) {  // only after a wait that gave up: copies still in flight, each waited for once
-        ptx::mbar_wait(&full[slot], phase, p.status);
-        ++used;
-        if (++slot == S) slot = 0, phase ^= 1u;
     }
 }
 
@@ -666,7 +682,7 @@ int attend(AttendParams p, DeviceState* dev, cudaStream_t stream) {
     }
     const int grid = dev->sm_count * Cfg::kCtas < kMaxGrid ? dev->sm_count * Cfg::kCtas : kMaxGrid;
     if (grid < kMinGrid) return fail(SPK_UNSUPPORTED, "kv4_attention: needs at least %d SMs, the device has %d", kMinGrid, dev->sm_count);
-    SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(32 * kWarps), Cfg::kSmem, stream, p));
+    SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(kThreads), Cfg::kSmem, stream, p));
     SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows>, dim3(grid), dim3(256), 0, stream, p));
     return SPK_OK;
 }
