@@ -52,12 +52,14 @@ struct AttendParams {
     int* status;
 };
 
-template <int D, int G, int NQ>
+// H = 2 is the form for at most four rows a KV head (NQ = 1): a row has two of the eight columns, each for half of the
+// groups, so that the scales of one group are all a column ever meets.
+template <int D, int G, int NQ, int H>
 struct SplitCfg {
-    static constexpr int kRows = 8 * NQ, kGroups = D / G, kWords = D / 32;
+    static constexpr int kRows = 8 * NQ / H, kGroups = D / G / H, kWords = D / 32;
     static constexpr int kTileBytes = kv4::tile_bytes(D, G), kStageBytes = kSteps * kTileBytes;
     static constexpr int kCtas = NQ == 1 ? 2 : 1;  // per SM: what the registers allow
-    static constexpr int kORow = D * 4 + 32;       // a row's pitch in the merge buffer: the lanes of a store hit every bank once
+    static constexpr int kORow = D * 4 + 32;       // a row's pitch in the merge buffer: the lanes of a store spread over the banks
     static constexpr int kMerge = kFold * kRows * kORow;
     // maxima and sums [2][warps][rows], chunk starts, barriers and valid flags of six stages
     static constexpr int kSmall = 2 * 2 * kWarps * kRows * 4 + kThreads * 8 + kWarps * 6 * 20 + 64;
@@ -100,7 +102,8 @@ __device__ __forceinline__ Piece piece_at(const AttendParams& p, int rows, long 
     }
     const int n = s.hi - s.lo;
     const long long local = u - s.begin;
-    const int which = static_cast<int>(local / n), skip = static_cast<int>(local - static_cast<long long>(which) * n);
+    const int which = local >> 32 ? static_cast<int>(local / n) : static_cast<int>(static_cast<uint32_t>(local) / n);  // a 64-bit division is long
+    const int skip = static_cast<int>(local - static_cast<long long>(which) * n);
     Piece x;
     x.block = which / p.pool.heads, x.head = which - x.block * p.pool.heads;
     x.tile0 = s.lo + skip;
@@ -123,14 +126,23 @@ __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N])
     }
 }
 
+// The piece as the consuming warps need it, in shared memory: written while they work on the one before.
+struct Task {
+    int tile0, tiles, block, head;
+    int first, count, len;
+    int whole, slot;  // whether the range holds all of it; else where its part goes in the workspace
+    int4 entry;       // what to tell the adding launch of the range, once its last piece is done
+    bool last;
+};
+
 // A barrier of the consuming warps.
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
 
 // What a warp carries through the tiles of a piece.
-template <int D, int G, int NQ>
+template <int D, int G, int NQ, int H>
 struct State {
-    static constexpr int kGroups = D / G, kWords = D / 32;
-    // of the piece's rows, as B fragments (column: row g): word i's step A (even channels) b0, b1, step B (odd ones) b0, b1
+    static constexpr int kGroups = D / G / H, kWords = D / 32;  // groups a column meets
+    // of the piece's rows, as B fragments (column g: row g, or row g % 4 in the channels of half g / 4): word i's step A (even channels) b0, b1, step B (odd ones) b0, b1
     uint32_t q[NQ][kWords][4];
     // as accumulator columns (rows 2 c and 2 c + 1): the offsets' start value, the sum of q', the score's factor, the tokens seen
     float start[NQ][kGroups][2], q_sum[NQ][kGroups][2], mult[NQ][2];
@@ -141,10 +153,11 @@ struct State {
 };
 
 // kSteps tiles of 16 tokens. Masked: some token is out of some row's sight, or a tile is missing (ok: the tiles that are there).
-template <int D, int G, int NQ, bool Masked>
-__device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned char* tiles, int lane, int ok, int base) {
-    constexpr int NG = D / G, NW = D / 32, kTileBytes = kv4::tile_bytes(D, G);
+template <int D, int G, int NQ, int H, bool Masked>
+__device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsigned char* tiles, int lane, int ok, int base) {
+    constexpr int NG = D / G / H, NW = D / 32, kTileBytes = kv4::tile_bytes(D, G);
     const int g = lane >> 2, c = lane & 3;
+    const int my_words = H == 2 ? (c >> 1) * NG * 4 : 0;  // where the words of this lane's columns begin in a token's
     float sc[NQ][kSteps][4];
     uint32_t vw[kSteps][2][NG], most = 0;
 #pragma unroll
@@ -153,8 +166,8 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
         uint32_t kw[2][NG], code[2][NW];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D)) + (g + 8 * x) * NG, kw[x]);
-            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_words_at(D, G)) + (g + 8 * x) * NG, vw[t][x]);
+            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + (g + 8 * x) * (D / G) * 4 + my_words), kw[x]);
+            load_words(reinterpret_cast<const uint32_t*>(tile + kv4::v_words_at(D, G) + (g + 8 * x) * (D / G) * 4 + my_words), vw[t][x]);
             load_words(reinterpret_cast<const uint32_t*>(tile + (g + 8 * x) * (D / 2) + c * (D / 8)), code[x]);
             if (Masked) {  // what lies outside every row's sight may be anything, NaN among it
                 const int j = base + t * kv4::kTile + g + 8 * x;
@@ -168,8 +181,10 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
             float acc[NQ][4];
+            bool fresh = true;
 #pragma unroll
-            for (int i = k * G / 32; i < (k + 1) * G / 32; ++i) {
+            for (int i = 0; i < NW; ++i) {
+                if (32 * i / G % NG != k) continue;
                 const uint32_t a0 = code[0][i], a1 = code[1][i], b0 = a0 >> 8, b1 = a1 >> 8;
                 const uint32_t fa[4] = {ptx::lop3_and_or(a0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(a1, 0x000f000fu, 0x64006400u),
                                         ptx::lop3_and_or(b0, 0x000f000fu, 0x64006400u), ptx::lop3_and_or(b1, 0x000f000fu, 0x64006400u)};
@@ -177,10 +192,11 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
                                         ptx::lop3_and_or(b0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(b1, 0x00f000f0u, 0x54005400u)};
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    if (i == k * G / 32) ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1], st.start[n][k][0], st.start[n][k][1]);
+                    if (fresh) ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1], st.start[n][k][0], st.start[n][k][1]);
                     else ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1]);
                     ptx::mma_f16_16816(acc[n], fb, st.q[n][i][2], st.q[n][i][3]);
                 }
+                fresh = false;
             }
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
@@ -189,6 +205,12 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
                     const float s = kv4::word_scale(kw[x >> 1][k]), m = kv4::word_min(kw[x >> 1][k]), qs = st.q_sum[n][k][x & 1];
                     sc[n][t][x] = fmaf(s, acc[n][x], k == 0 ? m * qs : fmaf(m, qs, sc[n][t][x]));
                 }
+        }
+        if (H == 2) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sc[n][t][x] += __shfl_xor_sync(0xffffffffu, sc[n][t][x], 2);
         }
         if (Masked) {
 #pragma unroll
@@ -201,11 +223,11 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
                 }
         }
     }
-    // ---- running maximum, reference exponent
-    most = __reduce_max_sync(0xffffffffu, most);
-    const int ref = max(st.ref, static_cast<int>(most >> 23));
-    float now[NQ][2];
-    bool moved = ref != st.ref;
+    // ---- running maximum, reference exponent: moved only when some score is 2^kSlack over the maximum or some s over
+    // the reference (p is then at most 2^kSlack, p s scale_s below 2^(8 + kSlack)), so most steps need no shuffle
+    constexpr float kSlack = 6.0f;
+    float high[NQ][2];
+    bool over = static_cast<int>(most >> 23) > st.ref;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -213,30 +235,32 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
             float m = fmaxf(sc[n][0][x], sc[n][0][x + 2]);
 #pragma unroll
             for (int t = 1; t < kSteps; ++t) m = fmaxf(m, fmaxf(sc[n][t][x], sc[n][t][x + 2]));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            now[n][x] = fmaxf(st.top[n][x], m * st.mult[n][x]);
-            moved |= now[n][x] != st.top[n][x];
+            high[n][x] = m * st.mult[n][x];
+            over |= high[n][x] > st.top[n][x] + kSlack;
         }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, over)) {
+        const int ref = max(st.ref, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 23));
         const float fall = ref - st.ref > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - ref + st.ref) << 23);
+        st.ref = ref;
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const float keep = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - now[n][x]);
-                const float both = keep * fall;
+                float m = high[n][x];
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                m = fmaxf(m, st.top[n][x]);
+                const float keep = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m), both = keep * fall;
                 st.sum[n][x] *= keep;
 #pragma unroll
                 for (int k = 0; k < NG; ++k) st.z[n][k][x] *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) st.o[n][i][x] *= both, st.o[n][i][x + 2] *= both;
-                st.top[n][x] = now[n][x];
+                st.top[n][x] = m;
             }
-        st.ref = ref;
     }
-    const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - ref) << 23);  // p s scale_s < 2^8
+    const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - st.ref) << 23);  // s scale_s < 2^8
     // ---- weights and values
 #pragma unroll
     for (int t = 0; t < kSteps; ++t) {
@@ -279,17 +303,17 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ>& st, const unsigned 
             const uint32_t fa[4] = {low(a), low(a8), low(b), low(b8)}, fb[4] = {high(a), high(a8), high(b), high(b8)};
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                ptx::mma_f16_16816(st.o[n][2 * unit], fa, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
-                ptx::mma_f16_16816(st.o[n][2 * unit + 1], fb, pf[n][32 * unit / G][0], pf[n][32 * unit / G][1]);
+                ptx::mma_f16_16816(st.o[n][2 * unit], fa, pf[n][32 * unit / G % NG][0], pf[n][32 * unit / G % NG][1]);
+                ptx::mma_f16_16816(st.o[n][2 * unit + 1], fb, pf[n][32 * unit / G % NG][0], pf[n][32 * unit / G % NG][1]);
             }
         }
     }
 }
 
-template <int D, int G, int NQ>
-__global__ void __launch_bounds__(kThreads, (SplitCfg<D, G, NQ>::kCtas))
+template <int D, int G, int NQ, int H>
+__global__ void __launch_bounds__(kThreads, (SplitCfg<D, G, NQ, H>::kCtas))
 kv4_attend_split_kernel(const AttendParams p) {
-    using Cfg = SplitCfg<D, G, NQ>;
+    using Cfg = SplitCfg<D, G, NQ, H>;
     constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* merge = smem + Cfg::kRing;
@@ -388,45 +412,52 @@ kv4_attend_split_kernel(const AttendParams p) {
     if (warp == kWarps) {
         // ---- the filling warp: each lane walks the steps of its consuming warp, page numbers a step early ----------
         long long u = start;
-        Piece s = piece_at(p, R, u, end, seq);
-        int step = lane, slot = 0, page[kSteps];
+        int left = 0, at = 0, in_page = 0, page = 0, next_page = 0, slot = 0;  // tiles left from this step on; the step's place in the table
+        const int32_t* row = nullptr;
+        const unsigned char* base = nullptr;
+        const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTileBytes;
+        const int hop = kWarps * kSteps / tiles_per_page, hop_rest = kWarps * kSteps % tiles_per_page;
         unsigned phase = 1;  // the first round of a ring is free
-        auto settle = [&]() {  // to the next step of this lane's warp at or after `step`; false at the end of the range
-            while (step * kSteps >= s.tiles) {
-                u += s.tiles;
+        auto settle = [&]() {  // to this lane's next step; false at the end of the range
+            while (left <= 0) {
                 if (u >= end) return false;
-                s = piece_at(p, R, u, end, seq);
-                step = lane;
+                const Piece s = piece_at(p, R, u, end, seq);
+                u += s.tiles;
+                left = s.tiles - lane * kSteps;
+                const int tile = s.tile0 + lane * kSteps;
+                at = tile / tiles_per_page, in_page = tile - at * tiles_per_page;
+                row = p.batch.table + static_cast<size_t>(seq.b) * p.batch.width;
+                base = p.pool.data + static_cast<size_t>(s.head) * tiles_per_page * Cfg::kTileBytes;
             }
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                if (step * kSteps + i < s.tiles)
-                    page[i] = __ldg(p.batch.table + static_cast<size_t>(seq.b) * p.batch.width + (s.tile0 + step * kSteps + i) / tiles_per_page);
+            page = __ldg(row + at);
+            next_page = left > 1 && in_page + 1 == tiles_per_page ? __ldg(row + at + 1) : page;
             return true;
         };
+        static_assert(kSteps == 2, "a step spans at most two pages");
         bool filling = lane < kWarps && settle();
         long long since = clock64();
         while (__any_sync(0xffffffffu, filling)) {
             bool went = false;
             if (filling && ptx::mbar_test_wait(&empty[slot], phase)) {
                 went = true;
-                int ok = 0, n = 0;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i)
-                    if (step * kSteps + i < s.tiles) {
-                        if (page[i] >= 0 && page[i] < p.pool.pages) ok |= 1 << i, ++n;
-                        else atomicCAS(p.status, 0, SPK_BAD_INDEX);
-                    }
+                const int n = min(left, kSteps);
+                int ok = (page >= 0 && page < p.pool.pages ? 1 : 0) | (next_page >= 0 && next_page < p.pool.pages ? 2 : 0);
+                if (ok != 3) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                ok &= (1 << n) - 1;
                 valid[slot] = ok;
-                ptx::mbar_arrive_expect_tx(&full[slot], n * Cfg::kTileBytes);
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i)
-                    if (ok >> i & 1) {
-                        const int tile = s.tile0 + step * kSteps + i;
-                        const unsigned char* from = p.pool.data + ((static_cast<size_t>(page[i]) * p.pool.heads + s.head) * tiles_per_page + tile % tiles_per_page) * Cfg::kTileBytes;
-                        ptx::bulk_g2s(ring + slot * Cfg::kStageBytes + i * Cfg::kTileBytes, from, Cfg::kTileBytes, &full[slot]);
-                    }
-                step += kWarps;
+                unsigned char* to = ring + slot * Cfg::kStageBytes;
+                const unsigned char* from = base + page * page_bytes + in_page * Cfg::kTileBytes;
+                if (ok == 3 && in_page + 1 < tiles_per_page) {  // both tiles in one page: one copy
+                    ptx::mbar_arrive_expect_tx(&full[slot], 2 * Cfg::kTileBytes);
+                    ptx::bulk_g2s(to, from, 2 * Cfg::kTileBytes, &full[slot]);
+                } else {
+                    ptx::mbar_arrive_expect_tx(&full[slot], ((ok & 1) + (ok >> 1)) * Cfg::kTileBytes);
+                    if (ok & 1) ptx::bulk_g2s(to, from, Cfg::kTileBytes, &full[slot]);
+                    if (ok & 2) ptx::bulk_g2s(to + Cfg::kTileBytes, base + next_page * page_bytes, Cfg::kTileBytes, &full[slot]);
+                }
+                left -= kWarps * kSteps;
+                at += hop, in_page += hop_rest;
+                if (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
                 if (++slot == S) slot = 0, phase ^= 1u;
                 filling = settle();
             }
@@ -437,82 +468,106 @@ kv4_attend_split_kernel(const AttendParams p) {
                     if (lane == 0) atomicCAS(p.status, 0, SPK_TIMEOUT);
                     break;
                 }
-                __nanosleep(40);
+                __nanosleep(20);
             }
         }
+        return;
     }
 
+    // ---- the consuming warps ---------------------------------------------------------------------------------
+    __shared__ Task tasks[2];
+    long long next_u = start;  // of warp 0: what the next task begins at
+    auto prepare_task = [&](int which) {  // by warp 0; nothing at the end of the range
+        if (next_u >= end) return;
+        const Piece s = piece_at(p, R, next_u, end, seq);
+        next_u += s.tiles;
+        if (lane == 0) {
+            Task& t = tasks[which];
+            t.tile0 = s.tile0, t.tiles = s.tiles, t.block = s.block, t.head = s.head;
+            t.first = seq.first, t.count = seq.count, t.len = seq.len;
+            t.whole = s.begins && s.ends, t.slot = s.begins ? 1 : 0;
+            t.last = next_u >= end;
+            t.entry = make_int4(0, 0, 0, 0);
+            // the last piece of the range: if it began here and goes on, its parts are in this CTA and the ones after it
+            if (t.last && s.begins && !s.ends) t.entry = make_int4(cta_of(next_u - s.tiles + (seq.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1, seq.b, s.block, s.head);
+        }
+        // its rows of q into the first-level cache
+        const int row = s.block * R + lane % R, rows = min(seq.count * group - s.block * R, R);
+        if (lane % R < rows)
+            for (int i = lane / R; i < D / 64; i += 32 / R)
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + static_cast<long long>(seq.first + row / group) * p.stride + static_cast<long long>(s.head * group + row % group) * D + 64 * i));
+    };
+    if (warp == 0) prepare_task(0);
+    consumers_sync();
     int slot = 0, merges = 0;
     unsigned phase = 0;
     bool alive = true;
-    Piece s;
-    State<D, G, NQ> st;
-    for (long long u = start; warp < kWarps && u < end; u += s.tiles) {
-        s = piece_at(p, R, u, end, seq);
+    State<D, G, NQ, H> st;
+    for (bool last = false; !last; ++merges) {
+        const Task& task = tasks[merges & 1];
+        last = task.last;
+        if (warp == 0) prepare_task((merges & 1) ^ 1);
         // ---- the rows of this piece: Q fragments, their sums per group, what each row sees -----------
         int all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            const int row = s.block * R + 8 * n + g;  // B fragments: this lane's column is row g
-            const bool there = row < seq.count * group;
-            uint4 raw[NW] = {};
+            const int row = task.block * R + 8 * n + (H == 2 ? g & 3 : g);  // B fragments: this lane's column
+            const bool there = row < task.count * group;
+            const int token = row / group;
+            uint32_t raw[NW][4] = {}, most = 0;
             if (there) {
-                const __nv_bfloat16* q = p.q + static_cast<long long>(seq.first + row / group) * p.stride + static_cast<long long>(s.head * group + row % group) * D + 8 * c;
+                const __nv_bfloat16* q = p.q + static_cast<long long>(task.first + token) * p.stride + static_cast<long long>(task.head * group + row - token * group) * D + 8 * c;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 32 * i);
+                for (int i = 0; i < NW; ++i) load_words(reinterpret_cast<const uint32_t*>(q + 32 * i), raw[i]);
             }
-            uint32_t top = 0;
-            float v[NW][8];
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            for (int i = 0; i < NW; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[i][2 * j] = __uint_as_float(w[j] << 16), v[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                    top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
-                }
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = static_cast<int>(top >> 23);  // biased exponent of the row's largest |q|
+                for (int j = 0; j < 4; ++j) most = __vmaxu2(most, raw[i][j] & 0x7fff7fffu);
+            most = max(most >> 16, most & 0xffffu);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = static_cast<int>(most >> 7);  // biased exponent of the row's largest |q|
             const bool finite = e < 255;
-            const float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, min(254, 254 - e))) << 23) : 0.0f;
+            float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23) : 0.0f;
             const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
-            float even[NG] = {}, odd[NG] = {};
+            if (p.scale < 0.0f) down = -down;
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
+                const bool mine = H == 1 || g / 4 == 32 * i / G / NG;
                 float h[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = finite ? v[i][j] * (p.scale < 0.0f ? -down : down) : 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = finite && mine ? raw[i][j] : 0;
+                    h[2 * j] = __uint_as_float(w << 16) * down, h[2 * j + 1] = __uint_as_float(w & 0xffff0000u) * down;
+                }
                 st.q[n][i][0] = ptx::f16x2_pack(h[0], h[4]), st.q[n][i][1] = ptx::f16x2_pack(h[2], h[6]);
                 st.q[n][i][2] = ptx::f16x2_pack(h[1], h[5]), st.q[n][i][3] = ptx::f16x2_pack(h[3], h[7]);
-                // sums of what the MMA will really multiply by
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&st.q[n][i][j]));
-                    (j < 2 ? even : odd)[32 * i / G] += f.x + f.y;
-                }
             }
             const float m = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
-            const int pos = seq.len - seq.count + row / group;
+            const int pos = task.len - task.count + token;
             const int row_hi = there ? max(0, pos + 1) : 0, row_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                even[k] += __shfl_xor_sync(0xffffffffu, even[k], 1), even[k] += __shfl_xor_sync(0xffffffffu, even[k], 2);
-                odd[k] += __shfl_xor_sync(0xffffffffu, odd[k], 1), odd[k] += __shfl_xor_sync(0xffffffffu, odd[k], 2);
-            }
-            // accumulator fragments: this lane's columns are rows 2 c and 2 c + 1
+            // accumulator fragments: this lane's columns are 2 c and 2 c + 1
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int from = 4 * (2 * c + x);
                 st.mult[n][x] = __shfl_sync(0xffffffffu, m, from);
                 st.lo[n][x] = __shfl_sync(0xffffffffu, row_lo, from);
                 st.hi[n][x] = __shfl_sync(0xffffffffu, row_hi, from);
+            }
+            // the sums over a group of what the codes' offsets multiply: 1024 the even channels, 64 the odd ones
+            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    const float a = __shfl_sync(0xffffffffu, even[k], from), b = __shfl_sync(0xffffffffu, odd[k], from);
-                    st.start[n][k][x] = -fmaf(1024.0f, a, 64.0f * b), st.q_sum[n][k][x] = a + b;
+            for (int k = 0; k < NG; ++k) {
+                float even[4] = {}, odd[4] = {};
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    if (32 * i / G % NG != k) continue;
+                    ptx::mma_f16_16816(even, ones, st.q[n][i][0], st.q[n][i][1]);
+                    ptx::mma_f16_16816(odd, ones, st.q[n][i][2], st.q[n][i][3]);
                 }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) st.start[n][k][x] = -fmaf(1024.0f, even[x], 64.0f * odd[x]), st.q_sum[n][k][x] = even[x] + odd[x];
             }
             if (there) all_lo = max(all_lo, row_lo), all_hi = min(all_hi, row_hi), any_lo = min(any_lo, row_lo), any_hi = max(any_hi, row_hi);
         }
@@ -530,24 +585,26 @@ kv4_attend_split_kernel(const AttendParams p) {
             }
         st.ref = 8;
 
-        for (int step = warp; step * kSteps < s.tiles; step += kWarps) {
+        const int tile0 = task.tile0, tiles_here = task.tiles;
+        for (int step = warp; step * kSteps < tiles_here; step += kWarps) {
             if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
-            const int ok = valid[slot], base = (s.tile0 + step * kSteps) * kv4::kTile;
-            const int here = min(kSteps, s.tiles - step * kSteps);
+            const int ok = valid[slot], base = (tile0 + step * kSteps) * kv4::kTile;
+            const int here = min(kSteps, tiles_here - step * kSteps);
             const unsigned char* tiles = ring + slot * Cfg::kStageBytes;
             if (here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi)
-                attend_step<D, G, NQ, true>(st, tiles, lane, ok & ((1 << here) - 1), base);
+                attend_step<D, G, NQ, H, true>(st, tiles, lane, ok & ((1 << here) - 1), base);
             else
-                attend_step<D, G, NQ, false>(st, tiles, lane, ok, base);
+                attend_step<D, G, NQ, H, false>(st, tiles, lane, ok, base);
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&empty[slot]);
             if (++slot == S) slot = 0, phase ^= 1u;
         }
 
-        // ---- the CTA's warps together ------------------------------------------------------------------
+        // ---- the CTA's warps together, on the common maximum ----------------------------------------------
+        const Task done = task;  // its place is written again once this merge's barriers are passed
         float* mx = m_max + (merges & 1) * kWarps * R;
         float* sm = m_sum + (merges & 1) * kWarps * R;
-        ++merges;
+        auto row_of = [&](int n, int x) { return 8 * n + (H == 2 ? 2 * c + x & 3 : 2 * c + x); };
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -558,10 +615,9 @@ kv4_attend_split_kernel(const AttendParams p) {
 #pragma unroll
                     for (int k = 0; k < NG; ++k) st.z[n][k][x] += __shfl_xor_sync(0xffffffffu, st.z[n][k][x], d);
                 }
-                if (g == 0) mx[warp * R + 8 * n + 2 * c + x] = st.top[n][x], sm[warp * R + 8 * n + 2 * c + x] = st.sum[n][x];
+                if (lane < 4 / H) mx[warp * R + row_of(n, x)] = st.top[n][x], sm[warp * R + row_of(n, x)] = st.sum[n][x];
             }
         consumers_sync();
-        // what each warp holds, on the common maximum; the upper half of the warps hands its part to the lower half
         const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
         float part[NQ][2];
 #pragma unroll
@@ -569,9 +625,11 @@ kv4_attend_split_kernel(const AttendParams p) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 float m = -INFINITY;
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + 8 * n + 2 * c + x]);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + row_of(n, x)]);
                 part[n][x] = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m);
             }
+        // the upper warps hand their part to the lower ones
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
             if (warp / kFold == half) {
@@ -579,13 +637,20 @@ kv4_attend_split_kernel(const AttendParams p) {
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float* at = reinterpret_cast<float*>(merge + (warp % kFold * R + 8 * n + 2 * c + x) * Cfg::kORow);
+                        float* at = reinterpret_cast<float*>(merge + (warp % kFold * R + row_of(n, x)) * Cfg::kORow);
+                        const float k = part[n][x], ku = k * unscale;
 #pragma unroll
-                        for (int unit = 0; unit < NW; ++unit) {
-                            const float zz = st.z[n][32 * unit / G][x], k = part[n][x];
+                        for (int u = 0; u < NW / H; ++u) {  // H = 2: a lane's columns hold one half of the channels
+                            const bool second = H == 2 && c >= 2;
+                            const int unit = second ? u + NW / 2 : u;
+                            float f[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float a = st.o[n][2 * u + (j & 1)][x + (j & 2)], b = st.o[n][(2 * u + (j & 1) + (H - 1) * NW) % (D / 16)][x + (j & 2)];
+                                f[j] = fmaf(second ? b : a, ku, st.z[n][32 * u / G % NG][x] * k);
+                            }
                             float4* to = reinterpret_cast<float4*>(at + 32 * unit + 4 * g);
-                            float4 v = make_float4(fmaf(st.o[n][2 * unit][x], unscale, zz) * k, fmaf(st.o[n][2 * unit + 1][x], unscale, zz) * k,
-                                                   fmaf(st.o[n][2 * unit][x + 2], unscale, zz) * k, fmaf(st.o[n][2 * unit + 1][x + 2], unscale, zz) * k);
+                            float4 v = make_float4(f[0], f[1], f[2], f[3]);
                             if (half == 0 && warp + kFold < kWarps) {
                                 const float4 other = *to;
                                 v.x += other.x, v.y += other.y, v.z += other.z, v.w += other.w;
@@ -596,8 +661,7 @@ kv4_attend_split_kernel(const AttendParams p) {
             }
             consumers_sync();
         }
-        const bool whole = s.begins && s.ends;
-        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + (s.begins ? 1 : 0)) * Cfg::kPartial;
+        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + done.slot) * Cfg::kPartial;
         for (int i = threadIdx.x; i < R * (D / 4); i += 32 * kWarps) {
             const int row = i / (D / 4), ch = i % (D / 4) * 4;
             float m = -INFINITY, l = 0.0f;
@@ -612,25 +676,19 @@ kv4_attend_split_kernel(const AttendParams p) {
                 const float t = mx[w * R + row];
                 l += t == -INFINITY ? sm[w * R + row] * 0.0f : sm[w * R + row] * ptx::exp2_fast(t - m);
             }
-            if (whole) {
-                const int r = s.block * R + row;
-                if (r >= seq.count * group) continue;
+            if (done.whole) {
+                const int r = done.block * R + row;
+                if (r >= done.count * group) continue;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(seq.first + r / group) * p.q_heads + s.head * group + r % group) * D + ch) =
+                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(done.first + r / group) * p.q_heads + done.head * group + r % group) * D + ch) =
                     make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
             } else {
                 *reinterpret_cast<float4*>(partial + row * D + ch) = a;
                 if (ch == 0) partial[R * D + 2 * row] = m, partial[R * D + 2 * row + 1] = l;
             }
         }
-        if (threadIdx.x == 0 && u + s.tiles >= end) {
-            // the last piece of the range: if it began here and goes on, this CTA's entry tells the adding launch of it
-            int4 entry = make_int4(0, 0, 0, 0);
-            if (s.begins && !s.ends)
-                entry = make_int4(cta_of(u + (seq.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1, seq.b, s.block, s.head);
-            p.pieces[blockIdx.x] = entry;
-        }
+        if (threadIdx.x == 0 && last) p.pieces[blockIdx.x] = done.entry;
     }
 }
 
@@ -668,13 +726,17 @@ __global__ void __launch_bounds__(256) kv4_attend_add_kernel(const AttendParams 
     }
 }
 
-int rows_per_block(int rows, int seqs, int group) { return (static_cast<int64_t>(rows) * group > int64_t{8} * seqs) ? 16 : 8; }
+// Rows of a block. Up to four rows a KV head and sequence, and two groups or more: the form in which a row has two columns.
+// Up to eight: one column each. More: sixteen at a time.
+int rows_per_block(int rows, int seqs, int q_per_kv, int groups) {
+    const int64_t r = static_cast<int64_t>(rows) * q_per_kv;
+    return r <= int64_t{4} * seqs && groups > 1 ? 4 : r <= int64_t{8} * seqs ? 8 : 16;
+}
 
-
-template <int D, int G, int NQ>
+template <int D, int G, int NQ, int H>
 int attend(AttendParams p, DeviceState* dev, cudaStream_t stream) {
-    using Cfg = SplitCfg<D, G, NQ>;
-    auto kernel = kv4_attend_split_kernel<D, G, NQ>;
+    using Cfg = SplitCfg<D, G, NQ, H>;
+    auto kernel = kv4_attend_split_kernel<D, G, NQ, H>;
     static bool configured[kMaxDevices] = {};
     if (!configured[dev->device]) {
         SPK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
@@ -688,7 +750,10 @@ int attend(AttendParams p, DeviceState* dev, cudaStream_t stream) {
 }
 template <int D, int G>
 int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStream_t stream) {
-    return per_block == 8 ? attend<D, G, 1>(p, dev, stream) : attend<D, G, 2>(p, dev, stream);
+    if constexpr (D / G > 1) {
+        if (per_block == 4) return attend<D, G, 1, 2>(p, dev, stream);
+    }
+    return per_block == 8 ? attend<D, G, 1, 1>(p, dev, stream) : attend<D, G, 2, 1>(p, dev, stream);
 }
 
 }  // namespace
@@ -697,8 +762,7 @@ int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStre
 extern "C" long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim) {
     using namespace spk;
     if (rows < 0 || seqs < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-    const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads);
-    return kMaxGrid * (16ll + 2ll * per_block * (head_dim + 2) * 4);
+    return kMaxGrid * (16ll + 2ll * rows_per_block(rows, seqs, q_heads / kv_heads, 1) * (head_dim + 2) * 4);
 }
 
 extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
@@ -728,7 +792,7 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     p.pieces = static_cast<int4*>(workspace);
     p.partials = reinterpret_cast<float*>(p.pieces + kMaxGrid);
     auto stream = static_cast<cudaStream_t>(stream_);
-    const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads);
+    const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads, head_dim / group);
     if (head_dim == 64) return group == 32 ? attend_rows<64, 32>(p, per_block, dev, stream) : attend_rows<64, 64>(p, per_block, dev, stream);
     return group == 32 ? attend_rows<128, 32>(p, per_block, dev, stream) : group == 64 ? attend_rows<128, 64>(p, per_block, dev, stream) : attend_rows<128, 128>(p, per_block, dev, stream);
 }
