@@ -31,11 +31,8 @@ namespace {
 using kv4::Batch;
 using kv4::Pool;
 
-// Seven consuming warps and one that fills their rings: a ninth would cost every thread a quarter of its registers.
-constexpr int kWarps = 7, kThreads = 32 * (kWarps + 1);
-constexpr int kSteps = 2;                // 16-token tiles of a ring stage
-constexpr int kFold = (kWarps + 1) / 2;  // in a merge warp w takes the part of warp w + kFold
-constexpr int kMinUnits = kWarps;      // a CTA gets at least this many tiles: one per warp
+constexpr int kSteps = 2;     // 16-token tiles of a ring stage
+constexpr int kMinUnits = 8;  // a CTA gets at least this many tiles
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
 
@@ -54,20 +51,24 @@ struct AttendParams {
 
 // H = 2 is the form for at most four rows a KV head (NQ = 1): a row has two of the eight columns, each for half of the
 // groups, so that the scales of one group are all a column ever meets.
-template <int D, int G, int NQ, int H>
+//
+// W consuming warps and one that fills their rings; kCtas such blocks on an SM. The accumulators (D NQ / 4 registers) decide:
+// the more warps, the better the latencies of their long dependent chains are covered.
+template <int D, int G, int NQ, int H, int W, int C>
 struct SplitCfg {
     static constexpr int kRows = 8 * NQ / H, kGroups = D / G / H, kWords = D / 32;
+    static constexpr int kThreads = 32 * (W + 1);
+    static constexpr int kFold = (W + 1) / 2;  // in a merge warp w takes the part of warp w + kFold
     static constexpr int kTileBytes = kv4::tile_bytes(D, G), kStageBytes = kSteps * kTileBytes;
-    static constexpr int kCtas = NQ == 1 ? 2 : 1;  // per SM: what the registers allow
-    static constexpr int kORow = D * 4 + 32;       // a row's pitch in the merge buffer: the lanes of a store spread over the banks
+    static constexpr int kORow = D * 4 + 32;  // a row's pitch in the merge buffer: the lanes of a store spread over the banks
     static constexpr int kMerge = kFold * kRows * kORow;
-    // maxima and sums [2][warps][rows], chunk starts, barriers and valid flags of six stages
-    static constexpr int kSmall = 2 * 2 * kWarps * kRows * 4 + kThreads * 8 + kWarps * 6 * 20 + 64;
-    static constexpr int kFit = ((227 * 1024 - 1024 * kCtas) / kCtas - kMerge - kSmall) / (kWarps * kStageBytes);
+    // two tasks; maxima and sums [2][warps][rows]; barriers and valid flags of six stages
+    static constexpr int kTask = (NQ * kWords * 512 + (NQ * kGroups * 2 + NQ * 3) * 32 + 128 + 127) / 128 * 128;
+    static constexpr int kSmall = 2 * kTask + 2 * 2 * W * kRows * 4 + W * 6 * 20 + 64;
+    static constexpr int kFit = ((227 * 1024 - 1024 * C) / C - 1024 - kMerge - kSmall) / (W * kStageBytes);
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kRing = kWarps * kStages * kStageBytes, kSmem = kRing + kMerge + kSmall;
+    static constexpr int kRing = W * kStages * kStageBytes, kSmem = kRing + kMerge + kSmall;
     static constexpr int kPartial = kRows * (D + 2);  // floats
-    static_assert(kStages >= 2, "the ring needs two stages");
 };
 
 // A sequence and its place in the order of units.
@@ -126,27 +127,32 @@ __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N])
     }
 }
 
-// The piece as the consuming warps need it, in shared memory: written while they work on the one before.
+// The piece as the consuming warps need it, in shared memory: one of them writes it while they work on the piece before.
+template <int D, int G, int NQ, int H>
 struct Task {
-    int tile0, tiles, block, head;
-    int first, count, len;
-    int whole, slot;  // whether the range holds all of it; else where its part goes in the workspace
-    int4 entry;       // what to tell the adding launch of the range, once its last piece is done
-    bool last;
+    static constexpr int kGroups = D / G / H, kWords = D / 32;  // groups a column meets
+    // the rows' q as B fragments (column g: row g, or row g % 4 in the channels of half g / 4), one 16-byte piece a lane:
+    // word i's step A (even channels) b0, b1, step B (odd ones) b0, b1
+    uint4 q[NQ][kWords][32];
+    // by column: the offsets' start value and the sum of q' per group, the score's factor, the tokens its row sees
+    float start[NQ][kGroups][8], q_sum[NQ][kGroups][8], mult[NQ][8];
+    int lo[NQ][8], hi[NQ][8];
+    int all_lo, all_hi, any_lo, any_hi;  // tokens that every row sees, that any row sees
+    int tile0, tiles, block, head, first, count;
+    int whole, slot;  // whether the range holds all of the piece; else where its part goes in the workspace
+    int last, sharers, seq;  // the range's last piece; then the CTAs that share it from this one on (0: not ours to name)
 };
 
 // A barrier of the consuming warps.
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+template <int W>
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory"); }
 
 // What a warp carries through the tiles of a piece.
 template <int D, int G, int NQ, int H>
 struct State {
-    static constexpr int kGroups = D / G / H, kWords = D / 32;  // groups a column meets
-    // of the piece's rows, as B fragments (column g: row g, or row g % 4 in the channels of half g / 4): word i's step A (even channels) b0, b1, step B (odd ones) b0, b1
-    uint32_t q[NQ][kWords][4];
-    // as accumulator columns (rows 2 c and 2 c + 1): the offsets' start value, the sum of q', the score's factor, the tokens seen
+    static constexpr int kGroups = D / G / H;  // groups a column meets
+    // of the task, for this lane's accumulator columns 2 c and 2 c + 1
     float start[NQ][kGroups][2], q_sum[NQ][kGroups][2], mult[NQ][2];
-    int lo[NQ][2], hi[NQ][2], any_lo, any_hi;
     // the running softmax: maxima (in powers of two), sums, values (channels 32 u + 4 g + {0, 2} in o[2 u], {1, 3} in o[2 u + 1]), sum p (8 s + m)
     float top[NQ][2], sum[NQ][2], o[NQ][D / 16][4], z[NQ][kGroups][2];
     int ref;  // biased exponent of the largest s so far: what p s is scaled against
@@ -154,7 +160,7 @@ struct State {
 
 // kSteps tiles of 16 tokens. Masked: some token is out of some row's sight, or a tile is missing (ok: the tiles that are there).
 template <int D, int G, int NQ, int H, bool Masked>
-__device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsigned char* tiles, int lane, int ok, int base) {
+__device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D, G, NQ, H>& task, const unsigned char* tiles, int lane, int ok, int base) {
     constexpr int NG = D / G / H, NW = D / 32, kTileBytes = kv4::tile_bytes(D, G);
     const int g = lane >> 2, c = lane & 3;
     const int my_words = H == 2 ? (c >> 1) * NG * 4 : 0;  // where the words of this lane's columns begin in a token's
@@ -171,7 +177,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsign
             load_words(reinterpret_cast<const uint32_t*>(tile + (g + 8 * x) * (D / 2) + c * (D / 8)), code[x]);
             if (Masked) {  // what lies outside every row's sight may be anything, NaN among it
                 const int j = base + t * kv4::kTile + g + 8 * x;
-                const bool seen = (ok >> t & 1) && j >= st.any_lo && j < st.any_hi;
+                const bool seen = (ok >> t & 1) && j >= task.any_lo && j < task.any_hi;
 #pragma unroll
                 for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
             }
@@ -192,9 +198,10 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsign
                                         ptx::lop3_and_or(b0, 0x00f000f0u, 0x54005400u), ptx::lop3_and_or(b1, 0x00f000f0u, 0x54005400u)};
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    if (fresh) ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1], st.start[n][k][0], st.start[n][k][1]);
-                    else ptx::mma_f16_16816(acc[n], fa, st.q[n][i][0], st.q[n][i][1]);
-                    ptx::mma_f16_16816(acc[n], fb, st.q[n][i][2], st.q[n][i][3]);
+                    const uint4 q = task.q[n][i][lane];
+                    if (fresh) ptx::mma_f16_16816(acc[n], fa, q.x, q.y, st.start[n][k][0], st.start[n][k][1]);
+                    else ptx::mma_f16_16816(acc[n], fa, q.x, q.y);
+                    ptx::mma_f16_16816(acc[n], fb, q.z, q.w);
                 }
                 fresh = false;
             }
@@ -218,7 +225,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsign
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const int j = base + t * kv4::kTile + g + 8 * (x >> 1);
-                    const bool seen = (ok >> t & 1) && j >= st.lo[n][x & 1] && j < st.hi[n][x & 1];
+                    const bool seen = (ok >> t & 1) && j >= task.lo[n][2 * c + (x & 1)] && j < task.hi[n][2 * c + (x & 1)];
                     sc[n][t][x] = seen ? sc[n][t][x] : -INFINITY;
                 }
         }
@@ -310,17 +317,100 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const unsign
     }
 }
 
+// Writes a task: the rows of the piece, scaled to fp16 and laid out as fragments, and what the columns need. One warp.
 template <int D, int G, int NQ, int H>
-__global__ void __launch_bounds__(kThreads, (SplitCfg<D, G, NQ, H>::kCtas))
+__device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq, const Piece& s, Task<D, G, NQ, H>& task, int lane) {
+    constexpr int NG = D / G / H, NW = D / 32, R = 8 * NQ / H;
+    const int g = lane >> 2, c = lane & 3, group = p.q_heads / p.pool.heads;
+    int all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int row = s.block * R + 8 * n + (H == 2 ? g & 3 : g);  // this lane's column
+        const bool there = row < seq.count * group;
+        const int token = row / group;
+        uint32_t raw[NW][4] = {}, most = 0;
+        if (there) {
+            const __nv_bfloat16* q = p.q + static_cast<long long>(seq.first + token) * p.stride + static_cast<long long>(s.head * group + row - token * group) * D + 8 * c;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) load_words(reinterpret_cast<const uint32_t*>(q + 32 * i), raw[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = __vmaxu2(most, raw[i][j] & 0x7fff7fffu);
+        most = max(most >> 16, most & 0xffffu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = static_cast<int>(most >> 7);  // biased exponent of the row's largest |q|
+        const bool finite = e < 255;
+        float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23) : 0.0f;
+        const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
+        if (p.scale < 0.0f) down = -down;
+        uint4 q[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const bool mine = H == 1 || g / 4 == 32 * i / G / NG;
+            float h[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = finite && mine ? raw[i][j] : 0;
+                h[2 * j] = __uint_as_float(w << 16) * down, h[2 * j + 1] = __uint_as_float(w & 0xffff0000u) * down;
+            }
+            q[i] = make_uint4(ptx::f16x2_pack(h[0], h[4]), ptx::f16x2_pack(h[2], h[6]), ptx::f16x2_pack(h[1], h[5]), ptx::f16x2_pack(h[3], h[7]));
+            task.q[n][i][lane] = q[i];
+        }
+        const int pos = seq.len - seq.count + token;
+        const int hi = there ? max(0, pos + 1) : 0, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        if (c == 0) {
+            // never 0: masked scores are -inf times it
+            task.mult[n][g] = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);
+            task.lo[n][g] = lo, task.hi[n][g] = hi;
+        }
+        // the sums over a group of what the codes' offsets multiply: 1024 the even channels, 64 the odd ones
+        const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            float even[4] = {}, odd[4] = {};
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                if (32 * i / G % NG != k) continue;
+                ptx::mma_f16_16816(even, ones, q[i].x, q[i].y);
+                ptx::mma_f16_16816(odd, ones, q[i].z, q[i].w);
+            }
+            if (g == 0) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) task.start[n][k][2 * c + x] = -fmaf(1024.0f, even[x], 64.0f * odd[x]), task.q_sum[n][k][2 * c + x] = even[x] + odd[x];
+            }
+        }
+        if (there) all_lo = max(all_lo, lo), all_hi = min(all_hi, hi), any_lo = min(any_lo, lo), any_hi = max(any_hi, hi);
+    }
+    all_lo = __reduce_max_sync(0xffffffffu, all_lo), all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+    any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+    if (lane == 0) {
+        task.all_lo = all_lo, task.all_hi = all_hi, task.any_lo = any_lo, task.any_hi = any_hi;
+        task.tile0 = s.tile0, task.tiles = s.tiles, task.block = s.block, task.head = s.head;
+        task.first = seq.first, task.count = seq.count, task.seq = seq.b;
+        task.whole = s.begins && s.ends, task.slot = s.begins ? 1 : 0;
+    }
+}
+
+template <int D, int G, int NQ, int H, int W, int C>
+__global__ void __launch_bounds__(32 * (W + 1), C)
 kv4_attend_split_kernel(const AttendParams p) {
-    using Cfg = SplitCfg<D, G, NQ, H>;
+    using Cfg = SplitCfg<D, G, NQ, H, W, C>;
+    static_assert(Cfg::kStages >= 2, "the ring needs two stages");
+    constexpr int kWarps = W, kThreads = Cfg::kThreads, kFold = Cfg::kFold;
     constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* merge = smem + Cfg::kRing;
-    float* m_max = reinterpret_cast<float*>(merge + Cfg::kMerge);  // [2][warps][rows]
+    using Task_ = Task<D, G, NQ, H>;
+    static_assert(sizeof(Task_) <= Cfg::kTask && Cfg::kRing % 16 == 0 && Cfg::kMerge % 16 == 0, "the tasks' place in shared memory");
+    Task_* tasks = reinterpret_cast<Task_*>(merge + Cfg::kMerge);  // [2]
+    float* m_max = reinterpret_cast<float*>(merge + Cfg::kMerge + 2 * Cfg::kTask);  // [2][warps][rows]
     float* m_sum = m_max + 2 * kWarps * R;
-    long long* chunk_start = reinterpret_cast<long long*>(m_sum + 2 * kWarps * R);  // [threads]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(chunk_start + kThreads);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(m_sum + 2 * kWarps * R);
+    long long* chunk_start = reinterpret_cast<long long*>(merge);  // [threads], of the set-up alone
+    static_assert(kThreads * 8 <= Cfg::kMerge, "the set-up's sums fit the merge buffer");
     int* valid_all = reinterpret_cast<int*>(bars + 2 * kWarps * S);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -408,6 +498,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         seq.begin = chunk_start[at];
         load_seq(p, R, seq);
     }
+    __syncthreads();  // chunk_start has been read
 
     if (warp == kWarps) {
         // ---- the filling warp: each lane walks the steps of its consuming warp, page numbers a step early ----------
@@ -475,104 +566,49 @@ kv4_attend_split_kernel(const AttendParams p) {
     }
 
     // ---- the consuming warps ---------------------------------------------------------------------------------
-    __shared__ Task tasks[2];
-    long long next_u = start;  // of warp 0: what the next task begins at
-    auto prepare_task = [&](int which) {  // by warp 0; nothing at the end of the range
-        if (next_u >= end) return;
-        const Piece s = piece_at(p, R, next_u, end, seq);
-        next_u += s.tiles;
-        if (lane == 0) {
-            Task& t = tasks[which];
-            t.tile0 = s.tile0, t.tiles = s.tiles, t.block = s.block, t.head = s.head;
-            t.first = seq.first, t.count = seq.count, t.len = seq.len;
-            t.whole = s.begins && s.ends, t.slot = s.begins ? 1 : 0;
-            t.last = next_u >= end;
-            t.entry = make_int4(0, 0, 0, 0);
-            // the last piece of the range: if it began here and goes on, its parts are in this CTA and the ones after it
-            if (t.last && s.begins && !s.ends) t.entry = make_int4(cta_of(next_u - s.tiles + (seq.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1, seq.b, s.block, s.head);
+    auto task_of = [&](int i) -> Task_& { return *reinterpret_cast<Task_*>(reinterpret_cast<unsigned char*>(tasks) + (i & 1) * Cfg::kTask); };
+    // the task after task i is written by warp i % W; the walk through the range goes from warp to warp in shared memory
+    __shared__ Seq walk_seq;
+    __shared__ long long walk_u;
+    auto write_next = [&](int i) {
+        const long long u = walk_u;
+        Seq at = walk_seq;
+        if (u < end) {
+            const Piece s = piece_at(p, R, u, end, at);
+            Task_& t = task_of(i);
+            write_task<D, G, NQ, H>(p, at, s, t, lane);
+            __syncwarp();
+            if (lane == 0) {
+                t.last = u + s.tiles >= end;
+                // a last piece that began here and goes on has its parts in this CTA and the ones after it
+                t.sharers = t.last && s.begins && !s.ends ? cta_of(u + (at.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
+                walk_u = u + s.tiles, walk_seq = at;
+            }
         }
-        // its rows of q into the first-level cache
-        const int row = s.block * R + lane % R, rows = min(seq.count * group - s.block * R, R);
-        if (lane % R < rows)
-            for (int i = lane / R; i < D / 64; i += 32 / R)
-                asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + static_cast<long long>(seq.first + row / group) * p.stride + static_cast<long long>(s.head * group + row % group) * D + 64 * i));
     };
-    if (warp == 0) prepare_task(0);
-    consumers_sync();
+    if (warp == 0) {
+        if (lane == 0) walk_u = start, walk_seq = seq;
+        __syncwarp();
+        write_next(0);
+    }
+    consumers_sync<W>();
     int slot = 0, merges = 0;
     unsigned phase = 0;
     bool alive = true;
     State<D, G, NQ, H> st;
     for (bool last = false; !last; ++merges) {
-        const Task& task = tasks[merges & 1];
+        const Task_& task = task_of(merges);
         last = task.last;
-        if (warp == 0) prepare_task((merges & 1) ^ 1);
-        // ---- the rows of this piece: Q fragments, their sums per group, what each row sees -----------
-        int all_lo = 0, all_hi = INT32_MAX, any_lo = INT32_MAX, any_hi = 0;
+        if (merges % W == warp) write_next(merges + 1);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const int row = task.block * R + 8 * n + (H == 2 ? g & 3 : g);  // B fragments: this lane's column
-            const bool there = row < task.count * group;
-            const int token = row / group;
-            uint32_t raw[NW][4] = {}, most = 0;
-            if (there) {
-                const __nv_bfloat16* q = p.q + static_cast<long long>(task.first + token) * p.stride + static_cast<long long>(task.head * group + row - token * group) * D + 8 * c;
-#pragma unroll
-                for (int i = 0; i < NW; ++i) load_words(reinterpret_cast<const uint32_t*>(q + 32 * i), raw[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < NW; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) most = __vmaxu2(most, raw[i][j] & 0x7fff7fffu);
-            most = max(most >> 16, most & 0xffffu);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = static_cast<int>(most >> 7);  // biased exponent of the row's largest |q|
-            const bool finite = e < 255;
-            float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23) : 0.0f;
-            const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
-            if (p.scale < 0.0f) down = -down;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                const bool mine = H == 1 || g / 4 == 32 * i / G / NG;
-                float h[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t w = finite && mine ? raw[i][j] : 0;
-                    h[2 * j] = __uint_as_float(w << 16) * down, h[2 * j + 1] = __uint_as_float(w & 0xffff0000u) * down;
-                }
-                st.q[n][i][0] = ptx::f16x2_pack(h[0], h[4]), st.q[n][i][1] = ptx::f16x2_pack(h[2], h[6]);
-                st.q[n][i][2] = ptx::f16x2_pack(h[1], h[5]), st.q[n][i][3] = ptx::f16x2_pack(h[3], h[7]);
-            }
-            const float m = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
-            const int pos = task.len - task.count + token;
-            const int row_hi = there ? max(0, pos + 1) : 0, row_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-            // accumulator fragments: this lane's columns are 2 c and 2 c + 1
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const int from = 4 * (2 * c + x);
-                st.mult[n][x] = __shfl_sync(0xffffffffu, m, from);
-                st.lo[n][x] = __shfl_sync(0xffffffffu, row_lo, from);
-                st.hi[n][x] = __shfl_sync(0xffffffffu, row_hi, from);
+                st.mult[n][x] = task.mult[n][2 * c + x];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) st.start[n][k][x] = task.start[n][k][2 * c + x], st.q_sum[n][k][x] = task.q_sum[n][k][2 * c + x];
             }
-            // the sums over a group of what the codes' offsets multiply: 1024 the even channels, 64 the odd ones
-            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                float even[4] = {}, odd[4] = {};
-#pragma unroll
-                for (int i = 0; i < NW; ++i) {
-                    if (32 * i / G % NG != k) continue;
-                    ptx::mma_f16_16816(even, ones, st.q[n][i][0], st.q[n][i][1]);
-                    ptx::mma_f16_16816(odd, ones, st.q[n][i][2], st.q[n][i][3]);
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) st.start[n][k][x] = -fmaf(1024.0f, even[x], 64.0f * odd[x]), st.q_sum[n][k][x] = even[x] + odd[x];
-            }
-            if (there) all_lo = max(all_lo, row_lo), all_hi = min(all_hi, row_hi), any_lo = min(any_lo, row_lo), any_hi = max(any_hi, row_hi);
-        }
-        all_lo = __reduce_max_sync(0xffffffffu, all_lo), all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-        st.any_lo = __reduce_min_sync(0xffffffffu, any_lo), st.any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+        const int all_lo = task.all_lo, all_hi = task.all_hi;
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -592,16 +628,18 @@ kv4_attend_split_kernel(const AttendParams p) {
             const int here = min(kSteps, tiles_here - step * kSteps);
             const unsigned char* tiles = ring + slot * Cfg::kStageBytes;
             if (here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi)
-                attend_step<D, G, NQ, H, true>(st, tiles, lane, ok & ((1 << here) - 1), base);
+                attend_step<D, G, NQ, H, true>(st, task, tiles, lane, ok & ((1 << here) - 1), base);
             else
-                attend_step<D, G, NQ, H, false>(st, tiles, lane, ok, base);
+                attend_step<D, G, NQ, H, false>(st, task, tiles, lane, ok, base);
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&empty[slot]);
             if (++slot == S) slot = 0, phase ^= 1u;
         }
 
         // ---- the CTA's warps together, on the common maximum ----------------------------------------------
-        const Task done = task;  // its place is written again once this merge's barriers are passed
+        // the task's place is written again once this merge's barriers are passed
+        const int block = task.block, head = task.head, first = task.first, count = task.count, whole = task.whole, slot_of = task.slot;
+        const int4 entry = make_int4(task.sharers, task.seq, block, head);
         float* mx = m_max + (merges & 1) * kWarps * R;
         float* sm = m_sum + (merges & 1) * kWarps * R;
         auto row_of = [&](int n, int x) { return 8 * n + (H == 2 ? 2 * c + x & 3 : 2 * c + x); };
@@ -617,7 +655,7 @@ kv4_attend_split_kernel(const AttendParams p) {
                 }
                 if (lane < 4 / H) mx[warp * R + row_of(n, x)] = st.top[n][x], sm[warp * R + row_of(n, x)] = st.sum[n][x];
             }
-        consumers_sync();
+        consumers_sync<W>();
         const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
         float part[NQ][2];
 #pragma unroll
@@ -659,9 +697,9 @@ kv4_attend_split_kernel(const AttendParams p) {
                         }
                     }
             }
-            consumers_sync();
+            consumers_sync<W>();
         }
-        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + done.slot) * Cfg::kPartial;
+        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + slot_of) * Cfg::kPartial;
         for (int i = threadIdx.x; i < R * (D / 4); i += 32 * kWarps) {
             const int row = i / (D / 4), ch = i % (D / 4) * 4;
             float m = -INFINITY, l = 0.0f;
@@ -676,19 +714,19 @@ kv4_attend_split_kernel(const AttendParams p) {
                 const float t = mx[w * R + row];
                 l += t == -INFINITY ? sm[w * R + row] * 0.0f : sm[w * R + row] * ptx::exp2_fast(t - m);
             }
-            if (done.whole) {
-                const int r = done.block * R + row;
-                if (r >= done.count * group) continue;
+            if (whole) {
+                const int r = block * R + row;
+                if (r >= count * group) continue;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(done.first + r / group) * p.q_heads + done.head * group + r % group) * D + ch) =
+                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(first + r / group) * p.q_heads + head * group + r % group) * D + ch) =
                     make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
             } else {
                 *reinterpret_cast<float4*>(partial + row * D + ch) = a;
                 if (ch == 0) partial[R * D + 2 * row] = m, partial[R * D + 2 * row + 1] = l;
             }
         }
-        if (threadIdx.x == 0 && last) p.pieces[blockIdx.x] = done.entry;
+        if (threadIdx.x == 0 && last) p.pieces[blockIdx.x] = entry;
     }
 }
 
@@ -733,27 +771,31 @@ int rows_per_block(int rows, int seqs, int q_per_kv, int groups) {
     return r <= int64_t{4} * seqs && groups > 1 ? 4 : r <= int64_t{8} * seqs ? 8 : 16;
 }
 
-template <int D, int G, int NQ, int H>
-int attend(AttendParams p, DeviceState* dev, cudaStream_t stream) {
-    using Cfg = SplitCfg<D, G, NQ, H>;
-    auto kernel = kv4_attend_split_kernel<D, G, NQ, H>;
+template <int D, int G, int NQ, int H, int W, int C>
+int attend(const AttendParams& p, DeviceState* dev, cudaStream_t stream) {
+    using Cfg = SplitCfg<D, G, NQ, H, W, C>;
+    auto kernel = kv4_attend_split_kernel<D, G, NQ, H, W, C>;
     static bool configured[kMaxDevices] = {};
     if (!configured[dev->device]) {
         SPK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
         configured[dev->device] = true;
     }
-    const int grid = dev->sm_count * Cfg::kCtas < kMaxGrid ? dev->sm_count * Cfg::kCtas : kMaxGrid;
+    const int grid = dev->sm_count * C < kMaxGrid ? dev->sm_count * C : kMaxGrid;
     if (grid < kMinGrid) return fail(SPK_UNSUPPORTED, "kv4_attention: needs at least %d SMs, the device has %d", kMinGrid, dev->sm_count);
-    SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(kThreads), Cfg::kSmem, stream, p));
+    SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, p));
     SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows>, dim3(grid), dim3(256), 0, stream, p));
     return SPK_OK;
 }
 template <int D, int G>
 int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStream_t stream) {
+    // warps and blocks an SM by the accumulators: 16, 32 and 64 registers a thread
+    constexpr int kFew = D == 64 ? 7 : 7;
     if constexpr (D / G > 1) {
-        if (per_block == 4) return attend<D, G, 1, 2>(p, dev, stream);
+        if (per_block == 4) return attend<D, G, 1, 2, 7, 2>(p, dev, stream);
     }
-    return per_block == 8 ? attend<D, G, 1, 1>(p, dev, stream) : attend<D, G, 2, 1>(p, dev, stream);
+    if (per_block == 8) return attend<D, G, 1, 1, kFew, 2>(p, dev, stream);
+    if constexpr (D == 64) return attend<D, G, 2, 1, 7, 2>(p, dev, stream);
+    else return attend<D, G, 2, 1, 7, 1>(p, dev, stream);
 }
 
 }  // namespace
