@@ -18,10 +18,10 @@
 // P^T comes out of S^T's accumulator layout by movmatrix (one 8 x 8 transpose per register).
 //
 // Work is cut into equal contiguous ranges of (sequence, block of rows, KV head, 16-token tile) units over the resident
-// CTAs, whatever the lengths are; every CTA finds its range itself from the lengths on the device. A warp takes every
-// seventh step of a range through a ring of its own, filled by bulk copies (a tile is one copy); a CTA merges its
-// warps in shared memory. What a CTA holds of a piece that is cut across CTAs goes to the workspace, and a second, chained
-// launch adds such pieces in the order of the CTAs: the same bits every run.
+// warps, whatever the lengths are; every warp finds its range itself from the lengths on the device and walks it alone,
+// through a ring of its own filled by bulk copies. What a warp holds of a piece that is cut across warps is added up in
+// the CTA at its end, what crosses CTAs goes through the workspace to a second, chained launch; always in the order of the
+// units: the same bits every run.
 #include "kv4_layout.cuh"
 #include "ptx_sm100.cuh"
 
@@ -32,7 +32,11 @@ using kv4::Batch;
 using kv4::Pool;
 
 constexpr int kSteps = 2;     // 16-token tiles of a ring stage
-constexpr int kMinUnits = 8;  // a CTA gets at least this many tiles
+constexpr int kMinUnits = 8;  // a CTA gets at least this many units
+// Units that stand in front of a piece's tiles for what its beginning costs (q, the lengths, the end's sums). Without them
+// a batch with short sequences waits for the warps that got many (64 x 4k, ragged: 60.1 us with 0, 56.6 / 47.7 / 45.4 with 1 / 3 / 6).
+constexpr int kLead = 6;
+constexpr int kMaxWarps = 11;  // consuming warps of a CTA, of any form
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
 
@@ -45,7 +49,7 @@ struct AttendParams {
     float scale;
     __nv_bfloat16* out;
     int4* pieces;     // [grid] (CTAs that share the piece begun in this CTA, or 0; sequence; row block; KV head)
-    float* partials;  // [grid][2][rows][D + 2]: a piece continued from the CTA before, a piece begun here
+    float* partials;  // [grid][2 + warps][rows][D + 2]: a piece continued from the CTA before, a piece begun here, the warps' own
     int* status;
 };
 
@@ -58,24 +62,21 @@ template <int D, int G, int NQ, int H, int W, int C>
 struct SplitCfg {
     static constexpr int kRows = 8 * NQ / H, kGroups = D / G / H, kWords = D / 32;
     static constexpr int kThreads = 32 * (W + 1);
-    static constexpr int kFold = (W + 1) / 2;  // in a merge warp w takes the part of warp w + kFold
     static constexpr int kTileBytes = kv4::tile_bytes(D, G), kStageBytes = kSteps * kTileBytes;
-    static constexpr int kORow = D * 4 + 32;  // a row's pitch in the merge buffer: the lanes of a store spread over the banks
-    static constexpr int kMerge = kFold * kRows * kORow;
-    // two tasks; maxima and sums [2][warps][rows]; barriers and valid flags of six stages
-    static constexpr int kTask = (NQ * kWords * 512 + (NQ * kGroups * 2 + NQ * 3) * 32 + 128 + 127) / 128 * 128;
-    static constexpr int kSmall = 2 * kTask + 2 * 2 * W * kRows * 4 + W * 6 * 20 + 64;
-    static constexpr int kFit = ((227 * 1024 - 1024 * C) / C - 1024 - kMerge - kSmall) / (W * kStageBytes);
+    // a task per warp; barriers and valid flags of six stages
+    static constexpr int kTask = (NQ * kWords * 512 + (NQ * kGroups * 2 + NQ * 3) * 32 + 64 + 127) / 128 * 128;
+    static constexpr int kSmall = W * kTask + W * 6 * 20 + 64;
+    static constexpr int kFit = ((227 * 1024 - 1024 * C) / C - 2048 - kSmall) / (W * kStageBytes);
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kRing = W * kStages * kStageBytes, kSmem = kRing + kMerge + kSmall;
-    static constexpr int kPartial = kRows * (D + 2);  // floats
+    static constexpr int kRing = W * kStages * kStageBytes, kSmem = kRing + kSmall;
+    static constexpr int kPart = kRows * (D + 2);  // floats: values, then maximum and sum of every row
 };
 
 // A sequence and its place in the order of units.
 struct Seq {
     int b, first, count, len;  // its rows of q, its tokens
     int lo, hi;                // tiles of 16 tokens that any of its rows sees
-    long long begin, units;    // units before it, its own: row blocks x KV heads x tiles
+    long long begin, units;    // units before it, its own: row blocks x KV heads x (lead + tiles)
 };
 
 __device__ __forceinline__ void load_seq(const AttendParams& p, int rows, Seq& s) {
@@ -84,13 +85,14 @@ __device__ __forceinline__ void load_seq(const AttendParams& p, int rows, Seq& s
     s.hi = s.count > 0 ? (s.len + kv4::kTile - 1) / kv4::kTile : 0;
     s.lo = p.window > 0 && s.count > 0 ? max(0, s.len - s.count - p.window + 1) / kv4::kTile : 0;
     const int group = p.q_heads / p.pool.heads;
-    s.units = static_cast<long long>((s.count * group + rows - 1) / rows) * p.pool.heads * (s.hi - s.lo);
+    s.units = static_cast<long long>((s.count * group + rows - 1) / rows) * p.pool.heads * (s.hi > s.lo ? s.hi - s.lo + kLead : 0);
 }
 
-// What a CTA's range holds of one (sequence, block of rows, KV head).
+// What a range holds of one (sequence, block of rows, KV head).
 struct Piece {
     int block, head;
-    int tile0, tiles;    // tiles from the sequence's start
+    int units;           // how far the range goes in it
+    int tile0, tiles;    // tiles from the sequence's start; none where the range ends in the lead
     bool begins, ends;   // whether the range holds the piece's first and last tile
 };
 
@@ -101,15 +103,16 @@ __device__ __forceinline__ Piece piece_at(const AttendParams& p, int rows, long 
         ++s.b;
         load_seq(p, rows, s);
     }
-    const int n = s.hi - s.lo;
+    const int n = s.hi - s.lo + kLead;
     const long long local = u - s.begin;
     const int which = local >> 32 ? static_cast<int>(local / n) : static_cast<int>(static_cast<uint32_t>(local) / n);  // a 64-bit division is long
     const int skip = static_cast<int>(local - static_cast<long long>(which) * n);
     Piece x;
     x.block = which / p.pool.heads, x.head = which - x.block * p.pool.heads;
-    x.tile0 = s.lo + skip;
-    x.tiles = static_cast<int>(min(static_cast<long long>(n - skip), end - u));
-    x.begins = skip == 0, x.ends = skip + x.tiles == n;
+    x.units = static_cast<int>(min(static_cast<long long>(n - skip), end - u));
+    const int from = max(0, skip - kLead), to = max(0, skip + x.units - kLead);
+    x.tile0 = s.lo + from, x.tiles = to - from;
+    x.begins = from == 0, x.ends = skip + x.units == n;
     return x;
 }
 
@@ -127,7 +130,7 @@ __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N])
     }
 }
 
-// The piece as the consuming warps need it, in shared memory: one of them writes it while they work on the piece before.
+// A piece as the warp that works on it needs it, in shared memory.
 template <int D, int G, int NQ, int H>
 struct Task {
     static constexpr int kGroups = D / G / H, kWords = D / 32;  // groups a column meets
@@ -139,13 +142,14 @@ struct Task {
     int lo[NQ][8], hi[NQ][8];
     int all_lo, all_hi, any_lo, any_hi;  // tokens that every row sees, that any row sees
     int tile0, tiles, block, head, first, count;
-    int whole, slot;  // whether the range holds all of the piece; else where its part goes in the workspace
-    int last, sharers, seq;  // the range's last piece; then the CTAs that share it from this one on (0: not ours to name)
 };
 
-// A barrier of the consuming warps.
-template <int W>
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory"); }
+// What a warp leaves of a piece it holds in part.
+struct Member {
+    int block, head, first, count, seq, begins, ends;
+    const float* at;  // values [rows][D], maxima and sums [rows][2]
+    long long end;    // the unit behind the piece
+};
 
 // What a warp carries through the tiles of a piece.
 template <int D, int G, int NQ, int H>
@@ -389,8 +393,7 @@ __device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq
     if (lane == 0) {
         task.all_lo = all_lo, task.all_hi = all_hi, task.any_lo = any_lo, task.any_hi = any_hi;
         task.tile0 = s.tile0, task.tiles = s.tiles, task.block = s.block, task.head = s.head;
-        task.first = seq.first, task.count = seq.count, task.seq = seq.b;
-        task.whole = s.begins && s.ends, task.slot = s.begins ? 1 : 0;
+        task.first = seq.first, task.count = seq.count;
     }
 }
 
@@ -398,30 +401,27 @@ template <int D, int G, int NQ, int H, int W, int C>
 __global__ void __launch_bounds__(32 * (W + 1), C)
 kv4_attend_split_kernel(const AttendParams p) {
     using Cfg = SplitCfg<D, G, NQ, H, W, C>;
-    static_assert(Cfg::kStages >= 2, "the ring needs two stages");
-    constexpr int kWarps = W, kThreads = Cfg::kThreads, kFold = Cfg::kFold;
-    constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages;
-    extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char* merge = smem + Cfg::kRing;
     using Task_ = Task<D, G, NQ, H>;
-    static_assert(sizeof(Task_) <= Cfg::kTask && Cfg::kRing % 16 == 0 && Cfg::kMerge % 16 == 0, "the tasks' place in shared memory");
-    Task_* tasks = reinterpret_cast<Task_*>(merge + Cfg::kMerge);  // [2]
-    float* m_max = reinterpret_cast<float*>(merge + Cfg::kMerge + 2 * Cfg::kTask);  // [2][warps][rows]
-    float* m_sum = m_max + 2 * kWarps * R;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(m_sum + 2 * kWarps * R);
-    long long* chunk_start = reinterpret_cast<long long*>(merge);  // [threads], of the set-up alone
-    static_assert(kThreads * 8 <= Cfg::kMerge, "the set-up's sums fit the merge buffer");
-    int* valid_all = reinterpret_cast<int*>(bars + 2 * kWarps * S);
+    constexpr int R = Cfg::kRows, NG = Cfg::kGroups, NW = Cfg::kWords, S = Cfg::kStages, kThreads = Cfg::kThreads;
+    static_assert(W <= kMaxWarps, "the workspace's size");
+    static_assert(S >= 2, "the ring needs two stages");
+    static_assert(sizeof(Task_) <= Cfg::kTask && Cfg::kRing % 16 == 0, "the tasks' place in shared memory");
+    static_assert(Cfg::kPart * 4 <= S * Cfg::kStageBytes && kThreads * 8 <= Cfg::kRing, "what the ring's memory is used for before and after");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ Member members[2 * W];  // in the order of the units: what warp w began before its last piece, its last piece
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kRing + W * Cfg::kTask);
+    int* valid_all = reinterpret_cast<int*>(bars + 2 * W * S);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     // a ring per consuming warp; the last warp's lane w fills that of warp w
-    const int mine = warp < kWarps ? warp : min(lane, kWarps - 1);
+    const int mine = warp < W ? warp : min(lane, W - 1);
     unsigned char* ring = smem + mine * S * Cfg::kStageBytes;
     uint64_t *full = bars + mine * 2 * S, *empty = full + S;
     int* valid = valid_all + mine * S;
-    if (warp == kWarps && lane < kWarps) {
+    if (warp == W && lane < W) {
         for (int s = 0; s < 2 * S; ++s) ptx::mbar_init(&full[s], 1);
         ptx::fence_mbar_init();
+        members[2 * lane].at = members[2 * lane + 1].at = nullptr;
     }
     pdl_release();
     pdl_wait();
@@ -435,9 +435,10 @@ kv4_attend_split_kernel(const AttendParams p) {
     };
     // units before every chunk of sequences, one chunk a thread
     const int chunk = (p.batch.seqs + kThreads - 1) / kThreads;
+    long long* chunk_start = reinterpret_cast<long long*>(smem);  // in the ring's memory, before it is used
     long long total;
     {
-        __shared__ long long warp_sum[kWarps + 1];
+        __shared__ long long warp_sum[W + 1];
         __shared__ int empties, empty_seqs[kv4::kMaxSeqs / kMinGrid];  // of the ones that fall to this CTA
         if (threadIdx.x == 0) empties = 0;
         __syncthreads();
@@ -460,7 +461,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         __syncthreads();
         long long before = 0;
         total = 0;
-        for (int w = 0; w <= kWarps; ++w) {
+        for (int w = 0; w <= W; ++w) {
             if (w < warp) before += warp_sum[w];
             total += warp_sum[w];
         }
@@ -478,17 +479,16 @@ kv4_attend_split_kernel(const AttendParams p) {
         zero_rows(0, head);
         zero_rows(tail, p.batch.rows);
     }
+    // the CTAs that work, and this warp's range (a filling lane: that of its warp)
     const long long active = max(1ll, min(static_cast<long long>(gridDim.x), (total + kMinUnits - 1) / kMinUnits));
-    const long long start = blockIdx.x < active ? blockIdx.x * total / active : total;
-    const long long end = blockIdx.x < active ? (blockIdx.x + 1) * total / active : total;
-    if (start >= end) {
+    if (blockIdx.x >= active || total == 0) {
         if (threadIdx.x == 0) p.pieces[blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
-    auto cta_of = [&](long long unit) { return static_cast<int>(((unit + 1) * active - 1) / total); };
-
+    const long long cta_start = blockIdx.x * total / active, cta_end = (blockIdx.x + 1) * total / active;
+    const long long start = cta_start + mine * (cta_end - cta_start) / W, end = cta_start + (mine + 1) * (cta_end - cta_start) / W;
     Seq seq;
-    {
+    if (start < end) {
         int at = 0;
         for (int hi = kThreads - 1; at < hi;) {
             const int mid = (at + hi + 1) >> 1;
@@ -498,25 +498,25 @@ kv4_attend_split_kernel(const AttendParams p) {
         seq.begin = chunk_start[at];
         load_seq(p, R, seq);
     }
-    __syncthreads();  // chunk_start has been read
+    ptx::fence_proxy_async();
+    __syncthreads();  // chunk_start has been read: its place is the copies' now
 
-    if (warp == kWarps) {
-        // ---- the filling warp: each lane walks the steps of its consuming warp, page numbers a step early ----------
+    float* const parts = p.partials + static_cast<size_t>(blockIdx.x) * (2 + W) * Cfg::kPart;
+    if (warp == W) {
+        // ---- the filling warp: each lane walks its consuming warp's range, page numbers a step early ------------------
         long long u = start;
-        int left = 0, at = 0, in_page = 0, page = 0, next_page = 0, slot = 0;  // tiles left from this step on; the step's place in the table
+        int left = 0, at = 0, in_page = 0, page = 0, next_page = 0, slot = 0;  // tiles left of the piece; the step's place in the table
         const int32_t* row = nullptr;
         const unsigned char* base = nullptr;
         const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTileBytes;
-        const int hop = kWarps * kSteps / tiles_per_page, hop_rest = kWarps * kSteps % tiles_per_page;
         unsigned phase = 1;  // the first round of a ring is free
         auto settle = [&]() {  // to this lane's next step; false at the end of the range
             while (left <= 0) {
                 if (u >= end) return false;
                 const Piece s = piece_at(p, R, u, end, seq);
-                u += s.tiles;
-                left = s.tiles - lane * kSteps;
-                const int tile = s.tile0 + lane * kSteps;
-                at = tile / tiles_per_page, in_page = tile - at * tiles_per_page;
+                u += s.units;
+                left = s.tiles;
+                at = s.tile0 / tiles_per_page, in_page = s.tile0 - at * tiles_per_page;
                 row = p.batch.table + static_cast<size_t>(seq.b) * p.batch.width;
                 base = p.pool.data + static_cast<size_t>(s.head) * tiles_per_page * Cfg::kTileBytes;
             }
@@ -525,7 +525,7 @@ kv4_attend_split_kernel(const AttendParams p) {
             return true;
         };
         static_assert(kSteps == 2, "a step spans at most two pages");
-        bool filling = lane < kWarps && settle();
+        bool filling = lane < W && settle();
         long long since = clock64();
         while (__any_sync(0xffffffffu, filling)) {
             bool went = false;
@@ -546,9 +546,9 @@ kv4_attend_split_kernel(const AttendParams p) {
                     if (ok & 1) ptx::bulk_g2s(to, from, Cfg::kTileBytes, &full[slot]);
                     if (ok & 2) ptx::bulk_g2s(to + Cfg::kTileBytes, base + next_page * page_bytes, Cfg::kTileBytes, &full[slot]);
                 }
-                left -= kWarps * kSteps;
-                at += hop, in_page += hop_rest;
-                if (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
+                left -= kSteps;
+                in_page += kSteps;
+                while (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
                 if (++slot == S) slot = 0, phase ^= 1u;
                 filling = settle();
             }
@@ -562,187 +562,156 @@ kv4_attend_split_kernel(const AttendParams p) {
                 __nanosleep(20);
             }
         }
-        return;
-    }
-
-    // ---- the consuming warps ---------------------------------------------------------------------------------
-    auto task_of = [&](int i) -> Task_& { return *reinterpret_cast<Task_*>(reinterpret_cast<unsigned char*>(tasks) + (i & 1) * Cfg::kTask); };
-    // the task after task i is written by warp i % W; the walk through the range goes from warp to warp in shared memory
-    __shared__ Seq walk_seq;
-    __shared__ long long walk_u;
-    auto write_next = [&](int i) {
-        const long long u = walk_u;
-        Seq at = walk_seq;
-        if (u < end) {
-            const Piece s = piece_at(p, R, u, end, at);
-            Task_& t = task_of(i);
-            write_task<D, G, NQ, H>(p, at, s, t, lane);
+    } else {
+        // ---- a consuming warp -----------------------------------------------------------------------------------------
+        Task_& task = *reinterpret_cast<Task_*>(smem + Cfg::kRing + warp * Cfg::kTask);
+        int slot = 0;
+        unsigned phase = 0;
+        bool alive = true;
+        State<D, G, NQ, H> st;
+        for (long long u = start; u < end;) {
+            const Piece s = piece_at(p, R, u, end, seq);
+            u += s.units;
+            if (s.tiles == 0) continue;
+            write_task<D, G, NQ, H>(p, seq, s, task, lane);
             __syncwarp();
-            if (lane == 0) {
-                t.last = u + s.tiles >= end;
-                // a last piece that began here and goes on has its parts in this CTA and the ones after it
-                t.sharers = t.last && s.begins && !s.ends ? cta_of(u + (at.hi - s.tile0) - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
-                walk_u = u + s.tiles, walk_seq = at;
-            }
-        }
-    };
-    if (warp == 0) {
-        if (lane == 0) walk_u = start, walk_seq = seq;
-        __syncwarp();
-        write_next(0);
-    }
-    consumers_sync<W>();
-    int slot = 0, merges = 0;
-    unsigned phase = 0;
-    bool alive = true;
-    State<D, G, NQ, H> st;
-    for (bool last = false; !last; ++merges) {
-        const Task_& task = task_of(merges);
-        last = task.last;
-        if (merges % W == warp) write_next(merges + 1);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                st.mult[n][x] = task.mult[n][2 * c + x];
+                for (int x = 0; x < 2; ++x) {
+                    st.mult[n][x] = task.mult[n][2 * c + x];
+                    st.top[n][x] = -INFINITY, st.sum[n][x] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < NG; ++k) st.start[n][k][x] = task.start[n][k][2 * c + x], st.q_sum[n][k][x] = task.q_sum[n][k][2 * c + x];
-            }
-        const int all_lo = task.all_lo, all_hi = task.all_hi;
+                    for (int k = 0; k < NG; ++k) {
+                        st.start[n][k][x] = task.start[n][k][2 * c + x], st.q_sum[n][k][x] = task.q_sum[n][k][2 * c + x];
+                        st.z[n][k][x] = 0.0f;
+                    }
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                st.top[n][x] = -INFINITY, st.sum[n][x] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) st.z[n][k][x] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) st.o[n][i][x] = st.o[n][i][x + 2] = 0.0f;
-            }
-        st.ref = 8;
-
-        const int tile0 = task.tile0, tiles_here = task.tiles;
-        for (int step = warp; step * kSteps < tiles_here; step += kWarps) {
-            if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
-            const int ok = valid[slot], base = (tile0 + step * kSteps) * kv4::kTile;
-            const int here = min(kSteps, tiles_here - step * kSteps);
-            const unsigned char* tiles = ring + slot * Cfg::kStageBytes;
-            if (here < kSteps || ok != (1 << kSteps) - 1 || base < all_lo || base + kSteps * kv4::kTile > all_hi)
-                attend_step<D, G, NQ, H, true>(st, task, tiles, lane, ok & ((1 << here) - 1), base);
-            else
-                attend_step<D, G, NQ, H, false>(st, task, tiles, lane, ok, base);
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&empty[slot]);
-            if (++slot == S) slot = 0, phase ^= 1u;
-        }
-
-        // ---- the CTA's warps together, on the common maximum ----------------------------------------------
-        // the task's place is written again once this merge's barriers are passed
-        const int block = task.block, head = task.head, first = task.first, count = task.count, whole = task.whole, slot_of = task.slot;
-        const int4 entry = make_int4(task.sharers, task.seq, block, head);
-        float* mx = m_max + (merges & 1) * kWarps * R;
-        float* sm = m_sum + (merges & 1) * kWarps * R;
-        auto row_of = [&](int n, int x) { return 8 * n + (H == 2 ? 2 * c + x & 3 : 2 * c + x); };
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) {
-                    st.sum[n][x] += __shfl_xor_sync(0xffffffffu, st.sum[n][x], d);
-#pragma unroll
-                    for (int k = 0; k < NG; ++k) st.z[n][k][x] += __shfl_xor_sync(0xffffffffu, st.z[n][k][x], d);
+                    for (int i = 0; i < D / 16; ++i) st.o[n][i][x] = st.o[n][i][x + 2] = 0.0f;
                 }
-                if (lane < 4 / H) mx[warp * R + row_of(n, x)] = st.top[n][x], sm[warp * R + row_of(n, x)] = st.sum[n][x];
+            st.ref = 8;
+            int base = s.tile0 * kv4::kTile;
+            for (int left = s.tiles; left > 0; left -= kSteps, base += kSteps * kv4::kTile) {
+                if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
+                const int ok = valid[slot];  // of the tiles that the step has
+                const unsigned char* tiles = ring + slot * Cfg::kStageBytes;
+                if (ok != (1 << kSteps) - 1 || base < task.all_lo || base + kSteps * kv4::kTile > task.all_hi)
+                    attend_step<D, G, NQ, H, true>(st, task, tiles, lane, left < kSteps ? ok & 1 : ok, base);
+                else
+                    attend_step<D, G, NQ, H, false>(st, task, tiles, lane, ok, base);
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&empty[slot]);
+                if (++slot == S) slot = 0, phase ^= 1u;
             }
-        consumers_sync<W>();
-        const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
-        float part[NQ][2];
+
+            // ---- what the warp has of the piece: to the output if that is all of it, else kept for the CTA's end
+            const bool whole = s.begins && s.ends, last = u >= end;
+            float* part = last ? reinterpret_cast<float*>(ring) : parts + (2 + warp) * Cfg::kPart;
+            const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
+            const int first = task.first, count = task.count, block = s.block, head = s.head;
+            if (last) __syncwarp();  // every lane is past the ring
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float m = -INFINITY;
+                for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + row_of(n, x)]);
-                part[n][x] = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m);
-            }
-        // the upper warps hand their part to the lower ones
+                    for (int d = 4; d < 32; d *= 2) {
+                        st.sum[n][x] += __shfl_xor_sync(0xffffffffu, st.sum[n][x], d);
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-            if (warp / kFold == half) {
+                        for (int k = 0; k < NG; ++k) st.z[n][k][x] += __shfl_xor_sync(0xffffffffu, st.z[n][k][x], d);
+                    }
+                    const bool second = H == 2 && c >= 2;  // H = 2: a lane's columns hold one half of the channels
+                    const int row = 8 * n + (H == 2 ? (2 * c + x) & 3 : 2 * c + x), r = block * R + row;
+                    const float l = st.sum[n][x], k = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l, ku = k * unscale;
+                    __nv_bfloat16* to = p.out + (static_cast<size_t>(first + r / group) * p.q_heads + head * group + r % group) * D + 4 * g;
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                    for (int i = 0; i < NW / H; ++i) {
+                        const int ch = 32 * (second ? i + NW / 2 : i);
+                        float f[4];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float* at = reinterpret_cast<float*>(merge + (warp % kFold * R + row_of(n, x)) * Cfg::kORow);
-                        const float k = part[n][x], ku = k * unscale;
-#pragma unroll
-                        for (int u = 0; u < NW / H; ++u) {  // H = 2: a lane's columns hold one half of the channels
-                            const bool second = H == 2 && c >= 2;
-                            const int unit = second ? u + NW / 2 : u;
-                            float f[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float a = st.o[n][2 * u + (j & 1)][x + (j & 2)], b = st.o[n][(2 * u + (j & 1) + (H - 1) * NW) % (D / 16)][x + (j & 2)];
-                                f[j] = fmaf(second ? b : a, ku, st.z[n][32 * u / G % NG][x] * k);
-                            }
-                            float4* to = reinterpret_cast<float4*>(at + 32 * unit + 4 * g);
-                            float4 v = make_float4(f[0], f[1], f[2], f[3]);
-                            if (half == 0 && warp + kFold < kWarps) {
-                                const float4 other = *to;
-                                v.x += other.x, v.y += other.y, v.z += other.z, v.w += other.w;
-                            }
-                            *to = v;
+                        for (int j = 0; j < 4; ++j) {
+                            const float a = st.o[n][2 * i + (j & 1)][x + (j & 2)], b = st.o[n][(2 * i + (j & 1) + (H - 1) * NW) % (D / 16)][x + (j & 2)];
+                            f[j] = whole ? fmaf(second ? b : a, ku, st.z[n][32 * i / G % NG][x] * k) : fmaf(second ? b : a, unscale, st.z[n][32 * i / G % NG][x]);
+                        }
+                        if (!whole) {
+                            *reinterpret_cast<float4*>(part + row * D + ch + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
+                        } else if (r < count * group) {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]), w = __floats2bfloat162_rn(f[2], f[3]);
+                            *reinterpret_cast<uint2*>(to + ch) = make_uint2(*reinterpret_cast<const uint32_t*>(&v), *reinterpret_cast<const uint32_t*>(&w));
                         }
                     }
+                    if (!whole && lane < 4 / H) part[R * D + 2 * row] = st.top[n][x], part[R * D + 2 * row + 1] = st.sum[n][x];
+                }
+            if (!whole && lane == 0) {
+                Member& m = members[2 * warp + (last ? 1 : 0)];
+                m.block = block, m.head = head, m.first = first, m.count = count, m.seq = seq.b, m.begins = s.begins, m.ends = s.ends;
+                m.at = part, m.end = u + (seq.hi - s.tile0 - s.tiles);
             }
-            consumers_sync<W>();
+            __syncwarp();  // the task's place is free
         }
-        float* partial = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + slot_of) * Cfg::kPartial;
-        for (int i = threadIdx.x; i < R * (D / 4); i += 32 * kWarps) {
-            const int row = i / (D / 4), ch = i % (D / 4) * 4;
-            float m = -INFINITY, l = 0.0f;
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mx[w * R + row]);
+    }
+
+    // ---- the CTA's members, chained: one begins a piece, the next ones go on with it ----------------------------------------
+    __syncthreads();
+    int4 entry = make_int4(0, 0, 0, 0);
+    for (int i = 0; i < 2 * W;) {
+        if (members[i].at == nullptr) {
+            ++i;
+            continue;
+        }
+        const Member& m = members[i];
+        int stop = i + 1, n = 1;
+        bool ends = m.ends;
+        for (; !ends && stop < 2 * W; ++stop)
+            if (members[stop].at != nullptr) ends = members[stop].ends, ++n;
+        const bool whole = m.begins && ends;
+        float* part = parts + (m.begins ? 1 : 0) * Cfg::kPart;
+        for (int e = threadIdx.x; e < R * (D / 4); e += kThreads) {
+            const int row = e / (D / 4), ch = e % (D / 4) * 4;
+            float top = -INFINITY, l = 0.0f;
+            for (int k = i; k < stop; ++k)
+                if (members[k].at != nullptr) top = fmaxf(top, members[k].at[R * D + 2 * row]);
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < kFold; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(merge + (w * R + row) * Cfg::kORow + ch * 4);
-                a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-            }
-            for (int w = 0; w < kWarps; ++w) {
-                const float t = mx[w * R + row];
-                l += t == -INFINITY ? sm[w * R + row] * 0.0f : sm[w * R + row] * ptx::exp2_fast(t - m);
+            for (int k = i; k < stop; ++k) {
+                const float* from = members[k].at;
+                if (from == nullptr) continue;
+                const float t = from[R * D + 2 * row], w = t == -INFINITY ? 0.0f : ptx::exp2_fast(t - top);
+                const float4 v = *reinterpret_cast<const float4*>(from + row * D + ch);
+                a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
+                l = fmaf(from[R * D + 2 * row + 1], w, l);
             }
             if (whole) {
-                const int r = block * R + row;
-                if (r >= count * group) continue;
+                const int r = m.block * R + row;
+                if (r >= m.count * group) break;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(first + r / group) * p.q_heads + head * group + r % group) * D + ch) =
+                *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(m.first + r / group) * p.q_heads + m.head * group + r % group) * D + ch) =
                     make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
             } else {
-                *reinterpret_cast<float4*>(partial + row * D + ch) = a;
-                if (ch == 0) partial[R * D + 2 * row] = m, partial[R * D + 2 * row + 1] = l;
+                *reinterpret_cast<float4*>(part + row * D + ch) = a;
+                if (ch == 0) part[R * D + 2 * row] = top, part[R * D + 2 * row + 1] = l;
             }
         }
-        if (threadIdx.x == 0 && last) p.pieces[blockIdx.x] = entry;
+        // a piece that begins here and goes on: its parts are in this CTA and the ones after it
+        if (m.begins && !ends) entry = make_int4(static_cast<int>((m.end * active - 1) / total) - static_cast<int>(blockIdx.x) + 1, m.seq, m.block, m.head);
+        i = stop;
     }
+    if (threadIdx.x == 0) p.pieces[blockIdx.x] = entry;
 }
 
 // Adds the parts of the pieces that were cut across CTAs: block i those of the piece that began in CTA i of the launch before.
-template <int D, int R>
+template <int D, int R, int W>
 __global__ void __launch_bounds__(256) kv4_attend_add_kernel(const AttendParams p) {
     pdl_release();
     pdl_wait();
     const int4 piece = p.pieces[blockIdx.x];
     if (piece.x == 0) return;
-    constexpr int kPartial = R * (D + 2);
+    constexpr int kPart = R * (D + 2), kPer = (2 + W) * kPart;  // a CTA's parts in the workspace
     const int group = p.q_heads / p.pool.heads;
     int first, count;
     kv4::rows_of(p.batch, piece.y, first, count);
-    const float* mine = p.partials + (static_cast<size_t>(blockIdx.x) * 2 + 1) * kPartial;  // then every second slot
-    auto part = [&](int i) { return i == 0 ? mine : mine + (2 * static_cast<size_t>(i) - 1) * kPartial; };
+    const float* mine = p.partials + static_cast<size_t>(blockIdx.x) * kPer;
+    auto part = [&](int i) { return i == 0 ? mine + kPart : mine + static_cast<size_t>(i) * kPer; };
     for (int i = threadIdx.x; i < R * (D / 4); i += 256) {
         const int row = i / (D / 4), ch = i % (D / 4) * 4, r = piece.z * R + row;
         if (r >= count * group) break;
@@ -783,7 +752,7 @@ int attend(const AttendParams& p, DeviceState* dev, cudaStream_t stream) {
     const int grid = dev->sm_count * C < kMaxGrid ? dev->sm_count * C : kMaxGrid;
     if (grid < kMinGrid) return fail(SPK_UNSUPPORTED, "kv4_attention: needs at least %d SMs, the device has %d", kMinGrid, dev->sm_count);
     SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, p));
-    SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows>, dim3(grid), dim3(256), 0, stream, p));
+    SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows, W>, dim3(grid), dim3(256), 0, stream, p));
     return SPK_OK;
 }
 template <int D, int G>
@@ -804,7 +773,7 @@ int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStre
 extern "C" long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim) {
     using namespace spk;
     if (rows < 0 || seqs < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-    return kMaxGrid * (16ll + 2ll * rows_per_block(rows, seqs, q_heads / kv_heads, 1) * (head_dim + 2) * 4);
+    return kMaxGrid * (16ll + (2ll + kMaxWarps) * rows_per_block(rows, seqs, q_heads / kv_heads, 1) * (head_dim + 2) * 4);
 }
 
 extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
