@@ -14,6 +14,7 @@ There is no CPU or eager fallback: if the shared library is missing this module 
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -587,154 +588,218 @@ _spk_kv4_attention = _sig("spk_kv4_attention", [_p, _i64, _p, _i, _i, _i, _i, _i
 _spk_add_rmsnorm = _sig("spk_add_rmsnorm", [_p, _i64, _p, _i64, _p, _p, _p, _i64, _f, _f, _p, _p, _i, _i, _p])
 
 
+# These operators run in a few microseconds, less than careful Python around them: what follows checks with plain
+# conditions and builds messages only for a failure, and enters a device's context only when another is current.
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_BF16, _I32 = torch.bfloat16, torch.int32
+_KV4_TILE = {(d, g): int(_spk_kv4_tile_bytes(d, g)) for d in (64, 128) for g in (32, 64, 128) if _spk_kv4_tile_bytes(d, g)}
+
+
 def kv4_tile_bytes(head_dim: int, group: int) -> int:
     """Bytes of 16 tokens of one KV head in the 4-bit cache, K and V; 0 for an unsupported pair."""
-    return int(_spk_kv4_tile_bytes(int(head_dim), int(group)))
+    return _KV4_TILE.get((head_dim, group), 0)
 
 
-def _check_pool(pool: torch.Tensor, head_dim: int, group: int, what: str) -> None:
-    _check_cuda_contig(pool, "pool")
-    nbytes = kv4_tile_bytes(head_dim, group)
-    _check(nbytes > 0, f"{what} supports head_dim 64 or 128 and group 32, 64 or 128 (at most head_dim), got head_dim={head_dim} group={group}")
-    _check(pool.dtype == torch.uint8 and pool.dim() == 4 and pool.shape[3] == nbytes and min(pool.shape) >= 1,
-           f"pool must be uint8 [pages, kv_heads, page_size / 16, {nbytes}], got {pool.dtype} {list(pool.shape)}")
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace_bytes(rows: int, seqs: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    return int(_spk_kv4_attention_workspace(rows, seqs, q_heads, kv_heads, head_dim))
 
 
-def _check_batch(what: str, rows: int, ref: torch.Tensor, page_table, lens, q_offsets) -> None:
-    """The arguments that say what a call's sequences are: int32, on the tensors' device."""
-    for t, name, dim in ((page_table, "page_table", 2), (lens, "lens", 1), (q_offsets, "q_offsets", 1)):
-        if t is None and name == "q_offsets":
-            continue
-        _check_cuda_contig(t, name)
-        _check(t.dtype == torch.int32 and t.dim() == dim, f"{name} must be int32 with {dim} dimension(s), got {t.dtype} {list(t.shape)}")
-        _check(t.device == ref.device, f"{name} must be on the device of the other tensors")
-    seqs = lens.shape[0]
-    _check(page_table.shape[0] == seqs, f"page_table has {page_table.shape[0]} rows for {seqs} sequences")
+def _fail(msg: str):
+    raise RuntimeError(msg)
+
+
+def _on_device(index: int, call):
+    """call() with device `index` current."""
+    if torch.cuda.current_device() == index:
+        return call()
+    with torch.cuda.device(index):
+        return call()
+
+
+def _check_pool(pool: torch.Tensor, head_dim: int, group: int, what: str):
+    """The pool's shape, checked."""
+    nbytes = _KV4_TILE.get((head_dim, group))
+    if nbytes is None:
+        _fail(f"{what} supports head_dim 64 or 128 and group 32, 64 or 128 (at most head_dim), got head_dim={head_dim} group={group}")
+    if not isinstance(pool, torch.Tensor) or not pool.is_cuda or not pool.is_contiguous():
+        _fail("pool must be a contiguous CUDA tensor")
+    shape = pool.shape
+    if pool.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != nbytes or pool.numel() == 0:
+        _fail(f"pool must be uint8 [pages, kv_heads, page_size / 16, {nbytes}], got {pool.dtype} {list(shape)}")
+    return shape
+
+
+def _check_int32(t, name: str, dim: int, index: int) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.dim() != dim or t.get_device() != index or not t.is_contiguous():
+        got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        _fail(f"{name} must be a contiguous int32 tensor with {dim} dimension(s) on the pool's device, got {got}")
+
+
+def _check_batch(what: str, rows: int, index: int, page_table, lens, q_offsets):
+    """The arguments that say what a call's sequences are; -> (sequences, pages in a row of the table)."""
+    _check_int32(page_table, "page_table", 2, index)
+    _check_int32(lens, "lens", 1, index)
+    seqs, width = page_table.shape
+    if lens.shape[0] != seqs:
+        _fail(f"page_table has {seqs} rows for {lens.shape[0]} sequences")
     if q_offsets is None:
-        _check(rows == seqs, f"{what} without q_offsets takes one row per sequence, got {rows} rows and {seqs} sequences")
+        if rows != seqs:
+            _fail(f"{what} without q_offsets takes one row per sequence, got {rows} rows and {seqs} sequences")
     else:
-        _check(q_offsets.shape[0] == seqs + 1, f"q_offsets must have {seqs + 1} entries for {seqs} sequences, got {q_offsets.shape[0]}")
+        _check_int32(q_offsets, "q_offsets", 1, index)
+        if q_offsets.shape[0] != seqs + 1:
+            _fail(f"q_offsets must have {seqs + 1} entries for {seqs} sequences, got {q_offsets.shape[0]}")
+    return seqs, width
 
 
-def _check_out(out, shape, ref: torch.Tensor, name: str) -> None:
-    _check_cuda_contig(out, name)
-    _check(out.dtype == torch.bfloat16 and tuple(out.shape) == tuple(shape) and out.device == ref.device and _aligned16(out),
-           f"{name} must be bfloat16 {list(shape)}, 16-byte aligned, on the inputs' device")
+def _check_out(out, shape: tuple, index: int, name: str) -> int:
+    if (not isinstance(out, torch.Tensor) or out.dtype is not _BF16 or tuple(out.shape) != shape or out.get_device() != index
+            or not out.is_contiguous() or out.data_ptr() & 15):
+        _fail(f"{name} must be a contiguous bfloat16 tensor {list(shape)}, 16-byte aligned, on the inputs' device")
+    return out.data_ptr()
 
 
-def _row_strided(t, name: str, cols: int, ref: torch.Tensor) -> int:
-    """The row stride of a bf16 matrix whose rows are contiguous."""
-    _check(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2, f"{name} must be a 2-D CUDA tensor")
-    _check(t.dtype == torch.bfloat16, f"{name} must be bfloat16")
-    _check(t.device == ref.device, f"{name} must be on the device of the other tensors")
-    _check(t.shape[1] == cols and (t.stride(1) == 1 or cols <= 1), f"{name} must have {cols} contiguous columns, got {list(t.shape)} with strides {list(t.stride())}")
-    stride = t.stride(0) if t.shape[0] > 1 else cols
-    _check(stride % 8 == 0 and _aligned16(t), f"{name} needs 16-byte aligned rows")
+def _row_strided(t, name: str, cols: int, index: int) -> int:
+    """The row stride of a bf16 matrix whose rows are contiguous and 16-byte aligned."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.dim() != 2 or t.get_device() != index:
+        _fail(f"{name} must be a 2-D bfloat16 CUDA tensor on the device of the other tensors")
+    stride, inner = t.stride()
+    if t.shape[1] != cols or inner != 1:
+        _fail(f"{name} must have {cols} contiguous columns, got {list(t.shape)} with strides {list(t.stride())}")
+    if t.shape[0] <= 1:
+        stride = cols
+    if stride & 7 or t.data_ptr() & 15:
+        _fail(f"{name} needs 16-byte aligned rows")
     return stride
 
 
 def kv4_append(qkv, pool, page_table, lens, cos_sin, q_offsets, head_dim: int, group: int, q_out=None) -> torch.Tensor:
     """Rotates q and k of qkv [rows, (Hq + 2 Hkv) head_dim] bf16, quantizes k and v into the pool, returns q [rows, Hq, head_dim]."""
-    _check_pool(pool, head_dim, group, "kv4_append")
-    _check(isinstance(qkv, torch.Tensor) and qkv.dim() == 2, "qkv must be a 2-D tensor")
+    pages, kv_heads, tiles, _ = _check_pool(pool, head_dim, group, "kv4_append")
+    index = pool.get_device()
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
+        _fail("qkv must be a 2-D tensor")
     rows, cols = qkv.shape
-    kv_heads = pool.shape[1]
     q_heads = cols // head_dim - 2 * kv_heads
-    _check(cols % head_dim == 0 and q_heads >= 0, f"qkv has {cols} columns, expected (Hq + 2 * {kv_heads}) * {head_dim}")
-    stride = _row_strided(qkv, "qkv", cols, pool)
-    _check(rows < 2 or stride >= cols, "rows of qkv must not overlap")
-    _check_batch("kv4_append", rows, pool, page_table, lens, q_offsets)
+    if cols % head_dim or q_heads < 0:
+        _fail(f"qkv has {cols} columns, expected (Hq + 2 * {kv_heads}) * {head_dim}")
+    stride = _row_strided(qkv, "qkv", cols, index)
+    if stride < cols:
+        _fail("rows of qkv must not overlap")
+    seqs, width = _check_batch("kv4_append", rows, index, page_table, lens, q_offsets)
     positions = rot = 0
     if cos_sin is not None:
-        _check_cuda_contig(cos_sin, "cos_sin")
-        _check(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.device == pool.device,
-               "cos_sin must be float32 [positions, rotated channels] on the pool's device")
+        if not isinstance(cos_sin, torch.Tensor) or cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.get_device() != index or not cos_sin.is_contiguous():
+            _fail("cos_sin must be a contiguous float32 tensor [positions, rotated channels] on the pool's device")
         positions, rot = cos_sin.shape
-        _check(8 <= rot <= head_dim and rot % 8 == 0 and positions >= 1 and _aligned16(cos_sin),
-               f"cos_sin must be [positions, a multiple of 8 up to {head_dim}] and 16-byte aligned, got {list(cos_sin.shape)}")
-    with torch.cuda.device(pool.device):
-        zero_rest = 0
-        if q_out is None:
-            q_out = torch.empty((rows, q_heads, head_dim), dtype=torch.bfloat16, device=pool.device)
-            zero_rest = int(q_offsets is not None)
-        else:
-            _check_out(q_out, (rows, q_heads, head_dim), pool, "q_out")
-        _status(_spk_kv4_append(qkv.data_ptr(), stride, pool.data_ptr(), pool.shape[0], pool.shape[2] * 16, q_heads, kv_heads, head_dim, group,
-                                page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), _ptr(q_offsets), lens.shape[0], rows,
-                                _ptr(cos_sin), positions, rot, q_out.data_ptr(), zero_rest, _stream(pool)))
+        if not 8 <= rot <= head_dim or rot & 7 or positions < 1 or cos_sin.data_ptr() & 15:
+            _fail(f"cos_sin must be [positions, a multiple of 8 up to {head_dim}] and 16-byte aligned, got {list(cos_sin.shape)}")
+    zero_rest = 0
+    if q_out is None:
+        q_out = torch.empty((rows, q_heads, head_dim), dtype=_BF16, device=pool.device)
+        zero_rest = int(q_offsets is not None)
+    else:
+        _check_out(q_out, (rows, q_heads, head_dim), index, "q_out")
+    args = (qkv.data_ptr(), stride, pool.data_ptr(), pages, tiles * 16, q_heads, kv_heads, head_dim, group, page_table.data_ptr(), width, lens.data_ptr(),
+            _ptr(q_offsets), seqs, rows, _ptr(cos_sin), positions, rot, q_out.data_ptr(), zero_rest, _raw_stream(index))
+    rc = _on_device(index, lambda: _spk_kv4_append(*args))
+    if rc:
+        _status(rc)
     return q_out
 
 
 def kv4_read(pool, slots, head_dim: int, group: int):
     """(k, v) bf16 [n, Hkv, head_dim] of the tokens in int64 slots [n] (page * page_size + place); zeros for negative slots."""
-    _check_pool(pool, head_dim, group, "kv4_read")
-    _check_cuda_contig(slots, "slots")
-    _check(slots.dtype == torch.int64 and slots.dim() == 1 and slots.device == pool.device, "slots must be int64 [n] on the pool's device")
-    n, kv_heads = slots.shape[0], pool.shape[1]
-    with torch.cuda.device(pool.device):
-        k, v = (torch.empty((n, kv_heads, head_dim), dtype=torch.bfloat16, device=pool.device) for _ in range(2))
-        _status(_spk_kv4_read(pool.data_ptr(), pool.shape[0], pool.shape[2] * 16, kv_heads, head_dim, group, slots.data_ptr(), n, k.data_ptr(),
-                              v.data_ptr(), _stream(pool)))
+    pages, kv_heads, tiles, _ = _check_pool(pool, head_dim, group, "kv4_read")
+    index = pool.get_device()
+    if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.dim() != 1 or slots.get_device() != index or not slots.is_contiguous():
+        _fail("slots must be a contiguous int64 tensor [n] on the pool's device")
+    n = slots.shape[0]
+    k, v = torch.empty((2, n, kv_heads, head_dim), dtype=_BF16, device=pool.device).unbind(0)
+    args = (pool.data_ptr(), pages, tiles * 16, kv_heads, head_dim, group, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _raw_stream(index))
+    rc = _on_device(index, lambda: _spk_kv4_read(*args))
+    if rc:
+        _status(rc)
     return k, v
 
 
 def kv4_attention(q, pool, page_table, lens, q_offsets, head_dim: int, group: int, scale: float, window: int, out=None) -> torch.Tensor:
     """Causal attention of q [rows, Hq, head_dim] bf16 over the pool -> [rows, Hq, head_dim] bf16."""
-    _check_pool(pool, head_dim, group, "kv4_attention")
-    _check(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.dtype == torch.bfloat16 and q.device == pool.device,
-           "q must be bfloat16 [rows, Hq, head_dim] on the pool's device")
-    rows, q_heads, kv_heads = q.shape[0], q.shape[1], pool.shape[1]
-    _check(q.shape[2] == head_dim, f"q has {q.shape[2]} channels a head, the cache {head_dim}")
-    _check(q_heads >= 1 and q_heads % kv_heads == 0, f"the query heads must be a multiple of the {kv_heads} KV heads, got {q_heads}")
-    _check(q.stride(2) == 1 and (q.stride(1) == head_dim or q_heads == 1), f"the heads of a row of q must be contiguous, got strides {list(q.stride())}")
-    stride = q.stride(0) if rows > 1 else q_heads * head_dim
-    _check(stride >= q_heads * head_dim and stride % 8 == 0 and _aligned16(q), "q needs 16-byte aligned rows that do not overlap")
-    _check_batch("kv4_attention", rows, pool, page_table, lens, q_offsets)
-    _check(int(window) >= 0, f"window must be 0 (none) or positive, got {window}")
-    with torch.cuda.device(pool.device):
-        zero_rest = 0
-        if out is None:
-            out = torch.empty((rows, q_heads, head_dim), dtype=torch.bfloat16, device=pool.device)
-            zero_rest = int(q_offsets is not None)
-        else:
-            _check_out(out, (rows, q_heads, head_dim), pool, "out")
-        nbytes = int(_spk_kv4_attention_workspace(rows, lens.shape[0], q_heads, kv_heads, head_dim))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
-        _status(_spk_kv4_attention(q.data_ptr(), stride, pool.data_ptr(), pool.shape[0], pool.shape[2] * 16, q_heads, kv_heads, head_dim, group,
-                                   page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), _ptr(q_offsets), lens.shape[0], rows, float(scale),
-                                   int(window), out.data_ptr(), zero_rest, ws.data_ptr(), nbytes, _stream(pool)))
+    pages, kv_heads, tiles, _ = _check_pool(pool, head_dim, group, "kv4_attention")
+    index = pool.get_device()
+    if not isinstance(q, torch.Tensor) or q.dtype is not _BF16 or q.dim() != 3 or q.get_device() != index:
+        _fail("q must be bfloat16 [rows, Hq, head_dim] on the pool's device")
+    rows, q_heads, channels = shape = tuple(q.shape)
+    if channels != head_dim:
+        _fail(f"q has {channels} channels a head, the cache {head_dim}")
+    if q_heads < 1 or q_heads % kv_heads:
+        _fail(f"the query heads must be a multiple of the {kv_heads} KV heads, got {q_heads}")
+    stride, head_stride, inner = q.stride()
+    if inner != 1 or (head_stride != head_dim and q_heads > 1):
+        _fail(f"the heads of a row of q must be contiguous, got strides {list(q.stride())}")
+    if rows <= 1:
+        stride = q_heads * head_dim
+    if stride < q_heads * head_dim or stride & 7 or q.data_ptr() & 15:
+        _fail("q needs 16-byte aligned rows that do not overlap")
+    seqs, width = _check_batch("kv4_attention", rows, index, page_table, lens, q_offsets)
+    window = int(window)
+    if window < 0:
+        _fail(f"window must be 0 (none) or positive, got {window}")
+    zero_rest = 0
+    if out is None:
+        out = torch.empty(shape, dtype=_BF16, device=pool.device)
+        zero_rest = int(q_offsets is not None)
+    else:
+        _check_out(out, shape, index, "out")
+    nbytes = _kv4_workspace_bytes(rows, seqs, q_heads, kv_heads, head_dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
+    args = (q.data_ptr(), stride, pool.data_ptr(), pages, tiles * 16, q_heads, kv_heads, head_dim, group, page_table.data_ptr(), width, lens.data_ptr(),
+            _ptr(q_offsets), seqs, rows, scale, window, out.data_ptr(), zero_rest, ws.data_ptr(), nbytes, _raw_stream(index))
+    rc = _on_device(index, lambda: _spk_kv4_attention(*args))
+    if rc:
+        _status(rc)
     return out
 
 
 def add_rmsnorm(x, y, gain, eps: float, post_gain, gate, residual_scale: float):
     """(r, h): r = bf16(residual_scale x + gate z), z = y or rmsnorm(y) post_gain; h = bf16(rmsnorm(r) gain). None for what is not asked for."""
-    _check(isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2, "x must be a 2-D CUDA tensor")
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
+        _fail("x must be a 2-D CUDA tensor")
     rows, hidden = x.shape
-    _check(hidden >= 8 and hidden % 8 == 0 and hidden <= 65536, f"add_rmsnorm needs hidden a multiple of 8 up to 65536, got {hidden}")
-    _check(y is not None or gain is not None, "add_rmsnorm needs y, gain or both")
-    _check(y is not None or (post_gain is None and gate is None and residual_scale == 1.0), "post_gain, gate and residual_scale need y")
-    x_stride = _row_strided(x, "x", hidden, x)
+    index = x.get_device()
+    if hidden < 8 or hidden & 7 or hidden > 65536:
+        _fail(f"add_rmsnorm needs hidden a multiple of 8 up to 65536, got {hidden}")
+    x_stride = _row_strided(x, "x", hidden, index)
     y_stride = gate_stride = 0
     if y is not None:
-        y_stride = _row_strided(y, "y", hidden, x)
-        _check(y.shape[0] == rows, f"y has {y.shape[0]} rows, x {rows}")
+        y_stride = _row_strided(y, "y", hidden, index)
+        if y.shape[0] != rows:
+            _fail(f"y has {y.shape[0]} rows, x {rows}")
+    elif gain is None or post_gain is not None or gate is not None or residual_scale != 1.0:
+        _fail("add_rmsnorm needs y, gain or both; post_gain, gate and residual_scale need y")
     for t, name in ((gain, "gain"), (post_gain, "post_gain")):
-        if t is not None:
-            _check_cuda_contig(t, name)
-            _check(t.dtype == torch.bfloat16 and tuple(t.shape) == (hidden,) and t.device == x.device and _aligned16(t),
-                   f"{name} must be bfloat16 [{hidden}], 16-byte aligned, on x's device")
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.dim() != 1 or t.shape[0] != hidden or t.get_device() != index
+                              or not t.is_contiguous() or t.data_ptr() & 15):
+            _fail(f"{name} must be a contiguous bfloat16 tensor [{hidden}], 16-byte aligned, on x's device")
     if gate is not None:
-        _check(isinstance(gate, torch.Tensor) and gate.dim() in (1, 2), f"gate must be [{hidden}] or [{rows}, {hidden}]")
+        if not isinstance(gate, torch.Tensor) or gate.dim() not in (1, 2):
+            _fail(f"gate must be [{hidden}] or [{rows}, {hidden}]")
         g = gate[None] if gate.dim() == 1 else gate
-        gate_stride = _row_strided(g, "gate", hidden, x)
-        _check(g.shape[0] in (1, rows), f"gate must be [{hidden}] or [{rows}, {hidden}], got {list(gate.shape)}")
+        gate_stride = _row_strided(g, "gate", hidden, index)
+        if g.shape[0] not in (1, rows):
+            _fail(f"gate must be [{hidden}] or [{rows}, {hidden}], got {list(gate.shape)}")
         if g.shape[0] == 1:
             gate_stride = 0
-    with torch.cuda.device(x.device):
-        r = x if y is None else torch.empty((rows, hidden), dtype=torch.bfloat16, device=x.device)
-        h = None if gain is None else torch.empty((rows, hidden), dtype=torch.bfloat16, device=x.device)
-        _status(_spk_add_rmsnorm(x.data_ptr(), x_stride, _ptr(y), y_stride, _ptr(gain), _ptr(post_gain), _ptr(gate), gate_stride,
-                                 float(residual_scale), float(eps), None if y is None else r.data_ptr(), _ptr(h), rows, hidden, _stream(x)))
+    dev = x.device
+    r = x if y is None else torch.empty((rows, hidden), dtype=_BF16, device=dev)
+    h = None if gain is None else torch.empty((rows, hidden), dtype=_BF16, device=dev)
+    args = (x.data_ptr(), x_stride, _ptr(y), y_stride, _ptr(gain), _ptr(post_gain), _ptr(gate), gate_stride, residual_scale, eps,
+            None if y is None else r.data_ptr(), _ptr(h), rows, hidden, _raw_stream(index))
+    rc = _on_device(index, lambda: _spk_add_rmsnorm(*args))
+    if rc:
+        _status(rc)
     return r, h
 
 
