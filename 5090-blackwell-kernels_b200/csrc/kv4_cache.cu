@@ -11,6 +11,7 @@
 // kv4_read    the values c s + m of named tokens, rounded once to bf16.
 //
 // Both are bound by memory: a token of Hq = 32, Hkv = 8, d = 128 is 12 KiB of qkv in, 8 KiB of q and 1.1 KiB of cache out.
+#include <algorithm>
 #include <cfloat>
 
 #include "kv4_layout.cuh"
@@ -36,73 +37,128 @@ struct Four {
     float v[4];
 };
 
-__device__ __forceinline__ Four load4(const __nv_bfloat16* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ Four unpack4(uint2 w) {
     return {{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)}};
 }
+__device__ __forceinline__ uint2 load4(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const Four& x) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(x.v[0], x.v[1]), b = __floats2bfloat162_rn(x.v[2], x.v[3]);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// A head vector belongs to D / 4 neighbouring lanes, lane l of them holding channels 4 l .. 4 l + 3: the rotation's
-// partner channels and a group's extremes are then shuffles inside the warp.
+// A head vector belongs to L = D / 8 neighbouring lanes; lane l holds channels 4 l .. + 3 and, half a vector on, D / 2 + 4 l .. + 3.
+// With all channels rotated these are each other's partners; with fewer the partner's channels are loaded beside them.
+struct Pair {
+    Four a, b;
+};
+
+// What a lane needs of the rotation of its token, the same for every head.
+struct Turn {
+    float4 ca, sa, cb, sb;  // of the channels in a and b
+    int pa, pb;             // channel of the partners of a and b, -1: not rotated
+    bool fa, fb;            // whether a and b lie in the first half of the rotated channels
+};
+
 template <int D>
-__device__ __forceinline__ void rotate(Four& x, int l, const float* cs, int rot) {
-    const int quads = rot >> 3;  // lanes of one half
-    const bool first = l < quads, in = l < 2 * quads;
-    const int partner = first ? l + quads : in ? l - quads : l;
-    Four other;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) other.v[i] = __shfl_sync(0xffffffffu, x.v[i], partner, D / 4);
-    if (!in) return;
-    const int at = 4 * (first ? l : l - quads);
-    const float4 c = *reinterpret_cast<const float4*>(cs + at), s = *reinterpret_cast<const float4*>(cs + rot / 2 + at);
+__device__ __forceinline__ void turn_of(Turn& t, int l, const float* cs, int rot) {
+    const int half = rot / 2;
+    auto one = [&](int ch, float4& c, float4& s, int& partner, bool& first) {
+        first = ch < half;
+        partner = ch < rot ? (first ? ch + half : ch - half) : -1;
+        c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (partner >= 0) {
+            const float* at = cs + (first ? ch : ch - half);
+            c = __ldg(reinterpret_cast<const float4*>(at)), s = __ldg(reinterpret_cast<const float4*>(at + half));
+        }
+    };
+    one(4 * l, t.ca, t.sa, t.pa, t.fa);
+    if (rot == D) {
+        t.cb = t.ca, t.sb = t.sa, t.pb = 4 * l, t.fb = false;
+    } else {
+        one(D / 2 + 4 * l, t.cb, t.sb, t.pb, t.fb);
+    }
+}
+
+// x1 cos - x2 sin or x2 cos + x1 sin, every product and sum rounded by itself.
+__device__ __forceinline__ Four turned(const Four& x, const Four& partner, const float4& c, const float4& s, bool first) {
     const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    Four y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float a = __fmul_rn(x.v[i], cc[i]), b = __fmul_rn(other.v[i], ss[i]);
-        x.v[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
+        const float p = __fmul_rn(x.v[i], cc[i]), q = __fmul_rn(partner.v[i], ss[i]);
+        y.v[i] = first ? __fsub_rn(p, q) : __fadd_rn(p, q);
+    }
+    return y;
+}
+
+template <int D, bool Whole>
+__device__ __forceinline__ Pair rotated(uint2 ra, uint2 rb, const __nv_bfloat16* vec, const Turn& t) {
+    Pair x{unpack4(ra), unpack4(rb)};
+    if constexpr (Whole) {
+        return {turned(x.a, x.b, t.ca, t.sa, true), turned(x.b, x.a, t.ca, t.sa, false)};
+    } else {
+        if (t.pa >= 0) x.a = turned(x.a, unpack4(load4(vec + t.pa)), t.ca, t.sa, t.fa);
+        if (t.pb >= 0) x.b = turned(x.b, unpack4(load4(vec + t.pb)), t.cb, t.sb, t.fb);
+        return x;
     }
 }
 
-// The four codes of this lane (nibble i: channel 4 l + i) and its group's word.
-template <int G>
-__device__ __forceinline__ uint32_t quantize4(const Four& x, uint32_t& word) {
-    float lo = fminf(fminf(x.v[0], x.v[1]), fminf(x.v[2], x.v[3])), hi = fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
-    int finite = 1;
+__device__ __forceinline__ float low4(const Four& x) { return fminf(fminf(x.v[0], x.v[1]), fminf(x.v[2], x.v[3])); }
+__device__ __forceinline__ float high4(const Four& x) { return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3])); }
+// Largest magnitude, NaN if there is one (fmaxf drops it).
+__device__ __forceinline__ uint32_t size4(const Four& x) {
+    return max(max(__float_as_uint(x.v[0]) & 0x7fffffffu, __float_as_uint(x.v[1]) & 0x7fffffffu),
+               max(__float_as_uint(x.v[2]) & 0x7fffffffu, __float_as_uint(x.v[3]) & 0x7fffffffu));
+}
+
+struct Scale {
+    float m, s, inv;
+    uint32_t word;
+};
+// A group's scale from its extremes over `Lanes` neighbouring lanes.
+template <int Lanes>
+__device__ __forceinline__ Scale scale_of(float lo, float hi, uint32_t size) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) finite &= fabsf(x.v[i]) <= FLT_MAX;
-#pragma unroll
-    for (int o = 1; o < G / 4; o *= 2) {
+    for (int o = 1; o < Lanes; o *= 2) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        finite &= __shfl_xor_sync(0xffffffffu, finite, o);
     }
+    Scale r;
     const __nv_bfloat16 mb = __float2bfloat16_rn(lo);
-    const float m = __bfloat162float(mb);
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, m), 1.0f / 15.0f));
-    float s = __bfloat162float(sb);
-    if (!finite || !(s <= FLT_MAX) || !(fabsf(m) <= FLT_MAX)) {
-        word = 0x7fc0u;
-        return 0;
-    }
-    if (s < FLT_MIN) s = 0.0f;  // a group of one value, or one whose minimum was rounded up past its maximum
-    word = __float_as_uint(s) | __bfloat16_as_ushort(mb);
-    uint32_t codes = 0;
-    if (s > 0.0f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) codes |= static_cast<uint32_t>(min(max(__float2int_rn(__fdiv_rn(__fsub_rn(x.v[i], m), s)), 0), 15)) << (4 * i);
-    }
-    return codes;
+    r.m = __bfloat162float(mb);
+    r.s = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, r.m), 1.0f / 15.0f)));
+    if (r.s < FLT_MIN) r.s = 0.0f;  // a group of one value, or one whose minimum was rounded up past its maximum
+    r.word = __float_as_uint(r.s) | __bfloat16_as_ushort(mb);
+    // an infinity or a NaN in the group (an infinity shows in the extremes, a NaN only in its own lane), a range past fp32
+    const bool odd = size >= 0x7f800000u || !(r.s <= FLT_MAX) || !(fabsf(r.m) <= FLT_MAX);
+    const uint32_t lanes = Lanes == 32 ? 0xffffffffu : ((1u << Lanes) - 1) << ((threadIdx.x & 31) / Lanes * Lanes);
+    if (__ballot_sync(0xffffffffu, odd) & lanes) r.s = 0.0f, r.m = 0.0f, r.word = 0x7fc0u;
+    r.inv = r.s > 0.0f ? __frcp_rn(r.s) : 0.0f;
+    return r;
 }
 
-// Block: eight tokens, one per warp, and the heads of slice blockIdx.y. Neighbouring tokens of a sequence share V blocks,
-// so their pieces leave the SM close together.
-template <int D, int G>
+// rint((x - m) / s) clamped to a code. The product with 1 / s is off by less than 2^-21 of the quotient, so its rounding is the
+// quotient's unless what is left over is next to half a step; only there (bf16 values do lie there) the division is made.
+__device__ __forceinline__ uint32_t codes4(const Four& x, const Scale& g) {
+    uint32_t c = 0;
+    const float half = 0.5f * g.s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float d = __fsub_rn(x.v[i], g.m);
+        float k = rintf(d * g.inv);
+        if (fabsf(fabsf(fmaf(-k, g.s, d)) - half) <= g.s * 0x1p-14f) k = rintf(__fdiv_rn(d, g.s));
+        if (g.s == 0.0f) k = 0.0f;
+        c |= static_cast<uint32_t>(min(max(static_cast<int>(k), 0), 15)) << (4 * i);
+    }
+    return c;
+}
+
+// Block: eight tokens, one per warp, and the head vectors of slice blockIdx.y, kPer of them at a time. Neighbouring tokens
+// of a sequence share V blocks, so their pieces leave the SM close together.
+template <int D, int G, bool Whole>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
-    constexpr int kLanes = D / 4, kPer = 32 / kLanes;  // lanes of a head vector, head vectors of a warp
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes;
+    constexpr int L = D / 8, kPer = 32 / L, kAhead = 4;  // lanes of a head vector, head vectors of a warp, loads in flight
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
     pdl_release();
     pdl_wait();
     const int t = blockIdx.x * 8 + warp;
@@ -129,9 +185,21 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
         pos = -1;
     }
     const bool placed = known && pos >= 0;
+    // the walk over this slice's head vectors: q's, then k's and v's; a warp's step never holds q beside k or v
+    const int q_steps = (p.q_heads + kPer - 1) / kPer, kv_steps = (2 * p.pool.heads + kPer - 1) / kPer;
+    const int from = static_cast<int>(static_cast<long long>(q_steps + kv_steps) * blockIdx.y / gridDim.y);
+    const int to = static_cast<int>(static_cast<long long>(q_steps + kv_steps) * (blockIdx.y + 1) / gridDim.y);
+    if (!placed) {
+        for (int i = from; i < min(to, q_steps); ++i)
+            if (i * kPer + sub < p.q_heads) {
+                __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + i * kPer + sub) * D + 4 * l;
+                store4(q, Four{}), store4(q + D / 2, Four{});
+            }
+        return;
+    }
     unsigned char* tile = nullptr;  // of KV head 0
-    const int tiles = p.pool.page_size / kv4::kTile;
-    if (placed) {
+    const int tiles = p.pool.page_size / kv4::kTile, in_tile = pos % kv4::kTile;
+    if (to > q_steps) {
         const int page = p.batch.table[static_cast<size_t>(b) * p.batch.width + pos / p.pool.page_size];
         if (page < 0 || page >= p.pool.pages) {
             if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
@@ -139,48 +207,72 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
             tile = p.pool.data + (static_cast<size_t>(page) * p.pool.heads * tiles + pos % p.pool.page_size / kv4::kTile) * p.pool.tile_bytes;
         }
     }
-    const int in_tile = placed ? pos % kv4::kTile : 0;
-    const float* cs = p.cos_sin + static_cast<size_t>(placed ? pos : 0) * p.rot;
-    const int total = p.q_heads + 2 * p.pool.heads;
+    Turn turn;
+    turn_of<D>(turn, l, p.cos_sin + static_cast<size_t>(pos) * p.rot, p.rot);
     const __nv_bfloat16* row = p.qkv + static_cast<size_t>(t) * p.stride;
 
-    for (int h0 = blockIdx.y * kPer; h0 < total; h0 += gridDim.y * kPer) {
-        const int h = h0 + lane / kLanes;
-        const bool here = h < total;
-        Four x = {};
-        if (placed && here) x = load4(row + static_cast<size_t>(h) * D + 4 * l);
-        // the shuffles below are the whole warp's: a warp of two head vectors may hold one of each kind
-        if (p.rot > 0 && placed) {
-            Four y = x;
-            rotate<D>(y, l, cs, p.rot);
-            if (h < p.q_heads + p.pool.heads) x = y;
-        }
-        uint32_t word = 0, codes = 0;
-        if (h0 + kPer > p.q_heads) codes = quantize4<G>(x, word);
-        const int kv = (h - p.q_heads) % p.pool.heads;
-        const bool is_k = h < p.q_heads + p.pool.heads;
-        // K: two lanes make a 32-bit word; V: the lanes of one run put their half words together
-        const uint32_t upper = __shfl_down_sync(0xffffffffu, codes, 1);
-        uint32_t piece[D / 64];
+    for (int i0 = from; i0 < min(to, q_steps); i0 += kAhead) {
+        uint2 ra[kAhead] = {}, rb[kAhead] = {};
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i)
-            piece[i] = __shfl_sync(0xffffffffu, codes, (l & 7) + 16 * i, kLanes) | __shfl_sync(0xffffffffu, codes, (l & 7) + 16 * i + 8, kLanes) << 16;
-        if (!here) continue;
-        if (h < p.q_heads) {
-            store4(p.q_out + (static_cast<size_t>(t) * p.q_heads + h) * D + 4 * l, x);
-            continue;
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = (i0 + j) * kPer + sub;
+            if (i0 + j < min(to, q_steps) && h < p.q_heads) ra[j] = load4(row + h * D + 4 * l), rb[j] = load4(row + h * D + D / 2 + 4 * l);
         }
-        if (tile == nullptr) continue;
-        unsigned char* at = tile + static_cast<size_t>(kv) * tiles * p.pool.tile_bytes;
-        if (is_k) {
-            if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(at + kv4::k_word_at(D, in_tile, 4 * l)) = codes | upper << 16;
-        } else if (l < 8) {
-            unsigned char* to = at + kv4::v_codes_at(D) + kv4::v_piece_at(D, in_tile, l);
-            if constexpr (D == 128) *reinterpret_cast<uint2*>(to) = make_uint2(piece[0], piece[D / 64 - 1]);
-            else *reinterpret_cast<uint32_t*>(to) = piece[0];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = (i0 + j) * kPer + sub;
+            if (i0 + j >= min(to, q_steps) || h >= p.q_heads) continue;
+            const Pair y = rotated<D, Whole>(ra[j], rb[j], row + h * D, turn);
+            __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + h) * D + 4 * l;
+            store4(q, y.a), store4(q + D / 2, y.b);
         }
-        if (l % (G / 4) == 0)
-            *reinterpret_cast<uint32_t*>(at + (is_k ? kv4::k_words_at(D) : kv4::v_words_at(D, G)) + (in_tile * (D / G) + 4 * l / G) * 4) = word;
+    }
+    if (tile == nullptr) return;
+    const __nv_bfloat16* kv_row = row + static_cast<size_t>(p.q_heads) * D;
+    for (int i0 = max(from, q_steps) - q_steps; i0 < to - q_steps; i0 += 2) {
+        uint2 ra[2] = {}, rb[2] = {};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int h = (i0 + j) * kPer + sub;
+            if (i0 + j < to - q_steps && h < 2 * p.pool.heads) ra[j] = load4(kv_row + h * D + 4 * l), rb[j] = load4(kv_row + h * D + D / 2 + 4 * l);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (i0 + j >= to - q_steps) break;  // the whole warp
+            const int h = (i0 + j) * kPer + sub;
+            const bool is_k = h < p.pool.heads;
+            Pair x{unpack4(ra[j]), unpack4(rb[j])};
+            if (is_k) x = rotated<D, Whole>(ra[j], rb[j], kv_row + h * D, turn);
+            uint32_t ca, cb, wa, wb;
+            if constexpr (G == D) {
+                const Scale g = scale_of<L>(fminf(low4(x.a), low4(x.b)), fmaxf(high4(x.a), high4(x.b)), max(size4(x.a), size4(x.b)));
+                ca = codes4(x.a, g), cb = codes4(x.b, g), wa = wb = g.word;
+            } else {
+                const Scale ga = scale_of<G / 4>(low4(x.a), high4(x.a), size4(x.a)), gb = scale_of<G / 4>(low4(x.b), high4(x.b), size4(x.b));
+                ca = codes4(x.a, ga), cb = codes4(x.b, gb), wa = ga.word, wb = gb.word;
+            }
+            // K: two lanes make a 32-bit word of a and one of b; V: the lanes of one run put their half words together
+            const uint32_t both = ca | cb << 16;
+            const uint32_t next = __shfl_xor_sync(0xffffffffu, both, 1), across = __shfl_xor_sync(0xffffffffu, both, 8);
+            if (h >= 2 * p.pool.heads) continue;
+            unsigned char* at = tile + static_cast<size_t>(is_k ? h : h - p.pool.heads) * tiles * p.pool.tile_bytes;
+            if (is_k) {
+                if ((l & 1) == 0) {
+                    *reinterpret_cast<uint32_t*>(at + kv4::k_word_at(D, in_tile, 4 * l)) = __byte_perm(both, next, 0x5410);
+                    *reinterpret_cast<uint32_t*>(at + kv4::k_word_at(D, in_tile, D / 2 + 4 * l)) = __byte_perm(both, next, 0x7632);
+                }
+            } else if (l < 8) {
+                unsigned char* piece = at + kv4::v_codes_at(D) + kv4::v_piece_at(D, in_tile, l);
+                if constexpr (D == 128) *reinterpret_cast<uint2*>(piece) = make_uint2(__byte_perm(both, across, 0x5410), __byte_perm(both, across, 0x7632));
+                else *reinterpret_cast<uint32_t*>(piece) = both;
+            }
+            uint32_t* words = reinterpret_cast<uint32_t*>(at + (is_k ? kv4::k_words_at(D) : kv4::v_words_at(D, G))) + in_tile * (D / G);
+            if constexpr (G == D) {
+                if (l == 0) words[0] = wa;
+            } else {
+                if (l % (G / 4) == 0) words[4 * l / G] = wa, words[(D / 2 + 4 * l) / G] = wb;
+            }
+        }
     }
 }
 
@@ -231,14 +323,14 @@ int for_shape(int d, int group, A&&... a) {
 template <int D, int G>
 struct Append {
     static int run(const AppendParams& p, int sms, cudaStream_t stream) {
-        const int blocks = cdiv(p.batch.rows, 8), vectors = cdiv(p.q_heads + 2 * p.pool.heads, 128 / D);
-        // few tokens: a slice of heads per block until the SMs hold eight blocks each
-        const int slices = max(1, min(vectors, 8 * sms / blocks));
-        SPK_CUDA(launch_chained(kv4_append_kernel<D, G>, dim3(blocks, slices), dim3(256), 0, stream, p));
+        constexpr int kPer = 256 / D;
+        const int blocks = cdiv(p.batch.rows, 8), steps = cdiv(p.q_heads, kPer) + cdiv(2 * p.pool.heads, kPer);
+        // few tokens: the heads are sliced over blocks until the SMs hold eight blocks each
+        const int slices = std::max(1, std::min(steps, 8 * sms / blocks));
+        auto kernel = p.rot == D ? kv4_append_kernel<D, G, true> : kv4_append_kernel<D, G, false>;
+        SPK_CUDA(launch_chained(kernel, dim3(blocks, slices), dim3(256), 0, stream, p));
         return SPK_OK;
     }
-    static int max(int a, int b) { return a > b ? a : b; }
-    static int min(int a, int b) { return a < b ? a : b; }
 };
 template <int D, int G>
 struct Read {

@@ -698,7 +698,7 @@ def kv4_append(qkv, pool, page_table, lens, cos_sin, q_offsets, head_dim: int, g
             _fail(f"cos_sin must be [positions, a multiple of 8 up to {head_dim}] and 16-byte aligned, got {list(cos_sin.shape)}")
     zero_rest = 0
     if q_out is None:
-        q_out = torch.empty((rows, q_heads, head_dim), dtype=_BF16, device=pool.device)
+        q_out = qkv.new_empty((rows, q_heads, head_dim))
         zero_rest = int(q_offsets is not None)
     else:
         _check_out(q_out, (rows, q_heads, head_dim), index, "q_out")
@@ -717,7 +717,8 @@ def kv4_read(pool, slots, head_dim: int, group: int):
     if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.dim() != 1 or slots.get_device() != index or not slots.is_contiguous():
         _fail("slots must be a contiguous int64 tensor [n] on the pool's device")
     n = slots.shape[0]
-    k, v = torch.empty((2, n, kv_heads, head_dim), dtype=_BF16, device=pool.device).unbind(0)
+    k = torch.empty((n, kv_heads, head_dim), dtype=_BF16, device=pool.device)
+    v = torch.empty_like(k)
     args = (pool.data_ptr(), pages, tiles * 16, kv_heads, head_dim, group, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _raw_stream(index))
     rc = _on_device(index, lambda: _spk_kv4_read(*args))
     if rc:
@@ -749,12 +750,12 @@ def kv4_attention(q, pool, page_table, lens, q_offsets, head_dim: int, group: in
         _fail(f"window must be 0 (none) or positive, got {window}")
     zero_rest = 0
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=pool.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         zero_rest = int(q_offsets is not None)
     else:
         _check_out(out, shape, index, "out")
     nbytes = _kv4_workspace_bytes(rows, seqs, q_heads, kv_heads, head_dim)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
+    ws = pool.new_empty(nbytes)
     args = (q.data_ptr(), stride, pool.data_ptr(), pages, tiles * 16, q_heads, kv_heads, head_dim, group, page_table.data_ptr(), width, lens.data_ptr(),
             _ptr(q_offsets), seqs, rows, scale, window, out.data_ptr(), zero_rest, ws.data_ptr(), nbytes, _raw_stream(index))
     rc = _on_device(index, lambda: _spk_kv4_attention(*args))
@@ -792,9 +793,8 @@ def add_rmsnorm(x, y, gain, eps: float, post_gain, gate, residual_scale: float):
             _fail(f"gate must be [{hidden}] or [{rows}, {hidden}], got {list(gate.shape)}")
         if g.shape[0] == 1:
             gate_stride = 0
-    dev = x.device
-    r = x if y is None else torch.empty((rows, hidden), dtype=_BF16, device=dev)
-    h = None if gain is None else torch.empty((rows, hidden), dtype=_BF16, device=dev)
+    r = x if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = None if gain is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     args = (x.data_ptr(), x_stride, _ptr(y), y_stride, _ptr(gain), _ptr(post_gain), _ptr(gate), gate_stride, residual_scale, eps,
             None if y is None else r.data_ptr(), _ptr(h), rows, hidden, _raw_stream(index))
     rc = _on_device(index, lambda: _spk_add_rmsnorm(*args))
