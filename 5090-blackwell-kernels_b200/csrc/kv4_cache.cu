@@ -103,25 +103,31 @@ __device__ __forceinline__ Pair rotated(uint2 ra, uint2 rb, const __nv_bfloat16*
     }
 }
 
-__device__ __forceinline__ float low4(const Four& x) { return fminf(fminf(x.v[0], x.v[1]), fminf(x.v[2], x.v[3])); }
-__device__ __forceinline__ float high4(const Four& x) { return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3])); }
-// Largest magnitude, NaN if there is one (fmaxf drops it).
-__device__ __forceinline__ uint32_t size4(const Four& x) {
-    return max(max(__float_as_uint(x.v[0]) & 0x7fffffffu, __float_as_uint(x.v[1]) & 0x7fffffffu),
-               max(__float_as_uint(x.v[2]) & 0x7fffffffu, __float_as_uint(x.v[3]) & 0x7fffffffu));
+// Minimum and maximum that hand a NaN on.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float low4(const Four& x) { return min_nan(min_nan(x.v[0], x.v[1]), min_nan(x.v[2], x.v[3])); }
+__device__ __forceinline__ float high4(const Four& x) { return max_nan(max_nan(x.v[0], x.v[1]), max_nan(x.v[2], x.v[3])); }
 
 struct Scale {
-    float m, s, inv;
+    float m, s, inv;  // minimum, scale, 1 / scale
     uint32_t word;
 };
 // A group's scale from its extremes over `Lanes` neighbouring lanes.
 template <int Lanes>
-__device__ __forceinline__ Scale scale_of(float lo, float hi, uint32_t size) {
+__device__ __forceinline__ Scale scale_of(float lo, float hi) {
 #pragma unroll
     for (int o = 1; o < Lanes; o *= 2) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     Scale r;
     const __nv_bfloat16 mb = __float2bfloat16_rn(lo);
@@ -129,28 +135,33 @@ __device__ __forceinline__ Scale scale_of(float lo, float hi, uint32_t size) {
     r.s = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, r.m), 1.0f / 15.0f)));
     if (r.s < FLT_MIN) r.s = 0.0f;  // a group of one value, or one whose minimum was rounded up past its maximum
     r.word = __float_as_uint(r.s) | __bfloat16_as_ushort(mb);
-    // an infinity or a NaN in the group (an infinity shows in the extremes, a NaN only in its own lane), a range past fp32
-    const bool odd = size >= 0x7f800000u || !(r.s <= FLT_MAX) || !(fabsf(r.m) <= FLT_MAX);
-    const uint32_t lanes = Lanes == 32 ? 0xffffffffu : ((1u << Lanes) - 1) << ((threadIdx.x & 31) / Lanes * Lanes);
-    if (__ballot_sync(0xffffffffu, odd) & lanes) r.s = 0.0f, r.m = 0.0f, r.word = 0x7fc0u;
-    r.inv = r.s > 0.0f ? __frcp_rn(r.s) : 0.0f;
+    // an infinity or a NaN in the group, or a range past fp32
+    if (!(r.s <= FLT_MAX) || !(fabsf(r.m) <= FLT_MAX)) r.s = 0.0f, r.m = 0.0f, r.word = 0x7fc0u;
+    r.inv = r.s > 0.0f ? __fdividef(1.0f, r.s) : 0.0f;
     return r;
 }
 
-// rint((x - m) / s) clamped to a code. The product with 1 / s is off by less than 2^-21 of the quotient, so its rounding is the
-// quotient's unless what is left over is next to half a step; only there (bf16 values do lie there) the division is made.
+// rint((x - m) / s) clamped to a code, four of them in the low 16 bits. The quotient has to be the correctly rounded one: bf16
+// values often lie exactly on the border between two codes. q + (d - q s) / s from a first q = d (1 / s) is that: d - q s is
+// exact, what the last product leaves is 2^-45 of the quotient, and a quotient of 24 bits by s's 8 is never closer than
+// 2^-33 to where the rounding turns. (Below 2^-100 the remainder falls out of fp32's range; there the division is
+// made.) The rounding to an integer is an addition of 1.5 x 2^23, which leaves it in the low bits.
 __device__ __forceinline__ uint32_t codes4(const Four& x, const Scale& g) {
-    uint32_t c = 0;
-    const float half = 0.5f * g.s;
+    constexpr float kRound = 12582912.0f;
+    int k[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float d = __fsub_rn(x.v[i], g.m);
-        float k = rintf(d * g.inv);
-        if (fabsf(fabsf(fmaf(-k, g.s, d)) - half) <= g.s * 0x1p-14f) k = rintf(__fdiv_rn(d, g.s));
-        if (g.s == 0.0f) k = 0.0f;
-        c |= static_cast<uint32_t>(min(max(static_cast<int>(k), 0), 15)) << (4 * i);
+        const float d = __fsub_rn(x.v[i], g.m), q = d * g.inv;
+        k[i] = __float_as_int(fmaf(fmaf(-q, g.s, d), g.inv, q) + kRound);
     }
-    return c;
+    if (g.s < 0x1p-100f && g.s > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = __float_as_int(__fdiv_rn(__fsub_rn(x.v[i], g.m), g.s) + kRound);
+    }
+    constexpr int kZero = 0x4b400000;  // the bits of kRound: code 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = min(max(k[i], kZero), kZero + 15);
+    return static_cast<uint32_t>(k[0]) + 16u * k[1] + 256u * k[2] + 4096u * k[3];
 }
 
 // Block: eight tokens, one per warp, and the head vectors of slice blockIdx.y, kPer of them at a time. Neighbouring tokens
@@ -185,12 +196,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
         pos = -1;
     }
     const bool placed = known && pos >= 0;
-    // the walk over this slice's head vectors: q's, then k's and v's; a warp's step never holds q beside k or v
+    // this slice's head vectors: k's and v's, the longer work, then q's; a warp's step never holds q beside k or v
     const int q_steps = (p.q_heads + kPer - 1) / kPer, kv_steps = (2 * p.pool.heads + kPer - 1) / kPer;
     const int from = static_cast<int>(static_cast<long long>(q_steps + kv_steps) * blockIdx.y / gridDim.y);
     const int to = static_cast<int>(static_cast<long long>(q_steps + kv_steps) * (blockIdx.y + 1) / gridDim.y);
+    const int q_from = max(from - kv_steps, 0), q_to = to - kv_steps, kv_to = min(to, kv_steps);
     if (!placed) {
-        for (int i = from; i < min(to, q_steps); ++i)
+        for (int i = q_from; i < q_to; ++i)
             if (i * kPer + sub < p.q_heads) {
                 __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + i * kPer + sub) * D + 4 * l;
                 store4(q, Four{}), store4(q + D / 2, Four{});
@@ -199,7 +211,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     }
     unsigned char* tile = nullptr;  // of KV head 0
     const int tiles = p.pool.page_size / kv4::kTile, in_tile = pos % kv4::kTile;
-    if (to > q_steps) {
+    if (from < kv_to) {
         const int page = p.batch.table[static_cast<size_t>(b) * p.batch.width + pos / p.pool.page_size];
         if (page < 0 || page >= p.pool.pages) {
             if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
@@ -211,48 +223,31 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     turn_of<D>(turn, l, p.cos_sin + static_cast<size_t>(pos) * p.rot, p.rot);
     const __nv_bfloat16* row = p.qkv + static_cast<size_t>(t) * p.stride;
 
-    for (int i0 = from; i0 < min(to, q_steps); i0 += kAhead) {
-        uint2 ra[kAhead] = {}, rb[kAhead] = {};
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int h = (i0 + j) * kPer + sub;
-            if (i0 + j < min(to, q_steps) && h < p.q_heads) ra[j] = load4(row + h * D + 4 * l), rb[j] = load4(row + h * D + D / 2 + 4 * l);
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int h = (i0 + j) * kPer + sub;
-            if (i0 + j >= min(to, q_steps) || h >= p.q_heads) continue;
-            const Pair y = rotated<D, Whole>(ra[j], rb[j], row + h * D, turn);
-            __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + h) * D + 4 * l;
-            store4(q, y.a), store4(q + D / 2, y.b);
-        }
-    }
-    if (tile == nullptr) return;
     const __nv_bfloat16* kv_row = row + static_cast<size_t>(p.q_heads) * D;
-    for (int i0 = max(from, q_steps) - q_steps; i0 < to - q_steps; i0 += 2) {
+    for (int i0 = from; i0 < kv_to && tile != nullptr; i0 += 2) {
         uint2 ra[2] = {}, rb[2] = {};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int h = (i0 + j) * kPer + sub;
-            if (i0 + j < to - q_steps && h < 2 * p.pool.heads) ra[j] = load4(kv_row + h * D + 4 * l), rb[j] = load4(kv_row + h * D + D / 2 + 4 * l);
+            if (i0 + j < kv_to && h < 2 * p.pool.heads) ra[j] = load4(kv_row + h * D + 4 * l), rb[j] = load4(kv_row + h * D + D / 2 + 4 * l);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            if (i0 + j >= to - q_steps) break;  // the whole warp
+            if (i0 + j >= kv_to) break;  // the whole warp
             const int h = (i0 + j) * kPer + sub;
             const bool is_k = h < p.pool.heads;
             Pair x{unpack4(ra[j]), unpack4(rb[j])};
             if (is_k) x = rotated<D, Whole>(ra[j], rb[j], kv_row + h * D, turn);
             uint32_t ca, cb, wa, wb;
             if constexpr (G == D) {
-                const Scale g = scale_of<L>(fminf(low4(x.a), low4(x.b)), fmaxf(high4(x.a), high4(x.b)), max(size4(x.a), size4(x.b)));
+                const Scale g = scale_of<L>(min_nan(low4(x.a), low4(x.b)), max_nan(high4(x.a), high4(x.b)));
                 ca = codes4(x.a, g), cb = codes4(x.b, g), wa = wb = g.word;
             } else {
-                const Scale ga = scale_of<G / 4>(low4(x.a), high4(x.a), size4(x.a)), gb = scale_of<G / 4>(low4(x.b), high4(x.b), size4(x.b));
+                const Scale ga = scale_of<G / 4>(low4(x.a), high4(x.a)), gb = scale_of<G / 4>(low4(x.b), high4(x.b));
                 ca = codes4(x.a, ga), cb = codes4(x.b, gb), wa = ga.word, wb = gb.word;
             }
             // K: two lanes make a 32-bit word of a and one of b; V: the lanes of one run put their half words together
-            const uint32_t both = ca | cb << 16;
+            const uint32_t both = __byte_perm(ca, cb, 0x5410);
             const uint32_t next = __shfl_xor_sync(0xffffffffu, both, 1), across = __shfl_xor_sync(0xffffffffu, both, 8);
             if (h >= 2 * p.pool.heads) continue;
             unsigned char* at = tile + static_cast<size_t>(is_k ? h : h - p.pool.heads) * tiles * p.pool.tile_bytes;
@@ -274,6 +269,22 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
             }
         }
     }
+    for (int i0 = q_from; i0 < q_to; i0 += kAhead) {
+        uint2 ra[kAhead] = {}, rb[kAhead] = {};
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = (i0 + j) * kPer + sub;
+            if (i0 + j < q_to && h < p.q_heads) ra[j] = load4(row + h * D + 4 * l), rb[j] = load4(row + h * D + D / 2 + 4 * l);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = (i0 + j) * kPer + sub;
+            if (i0 + j >= q_to || h >= p.q_heads) continue;
+            const Pair y = rotated<D, Whole>(ra[j], rb[j], row + h * D, turn);
+            __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + h) * D + 4 * l;
+            store4(q, y.a), store4(q + D / 2, y.b);
+        }
+    }
 }
 
 struct ReadParams {
@@ -284,34 +295,44 @@ struct ReadParams {
     int* status;
 };
 
-// A warp reads one token of one head, K and V: lane l the 4 channels 4 l .. (D = 128) or the halves of the warp one tensor each.
+// A warp reads a token: D / 8 lanes a head vector, eight channels each, the vectors of slice blockIdx.y.
 template <int D, int G>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadParams p) {
+    constexpr int L = D / 8, kPer = 32 / L;
     pdl_release();
     pdl_wait();
-    constexpr int kQuads = D / 4;
-    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;  // (slot, head, K or V, quad)
-    const int quad = static_cast<int>(i % kQuads);
-    const bool is_v = (i / kQuads) & 1;
-    const long long vec = i / (2 * kQuads);
-    const int head = static_cast<int>(vec % p.pool.heads);
-    const long long n = vec / p.pool.heads;
+    const int lane = threadIdx.x & 31, ch = 8 * (lane % L), sub = lane / L, n = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (n >= p.n) return;
     const long long slot = p.slots[n];
-    Four x = {};
-    if (slot >= 0 && slot < static_cast<long long>(p.pool.pages) * p.pool.page_size) {
-        const int tiles = p.pool.page_size / kv4::kTile, in_page = static_cast<int>(slot % p.pool.page_size), t = in_page % kv4::kTile;
-        const unsigned char* tile = p.pool.data + ((static_cast<size_t>(slot / p.pool.page_size) * p.pool.heads + head) * tiles + in_page / kv4::kTile) * p.pool.tile_bytes;
-        const int ch = 4 * quad;
-        const unsigned char* at = is_v ? tile + kv4::v_codes_at(D) + kv4::v_piece_at(D, t, ch % 32 / 4) + ch / 32 * 2 : tile + kv4::k_word_at(D, t, ch & ~7) + ch % 8 / 2;
-        const uint32_t codes = *reinterpret_cast<const uint16_t*>(at);
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + (is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D)) + (t * (D / G) + ch / G) * 4);
+    const bool there = slot >= 0 && slot < static_cast<long long>(p.pool.pages) * p.pool.page_size;
+    if (slot >= 0 && !there) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+    const long long page = there ? slot / p.pool.page_size : 0;
+    const int tiles = p.pool.page_size / kv4::kTile, in_page = there ? static_cast<int>(slot - page * p.pool.page_size) : 0, t = in_page % kv4::kTile;
+    const unsigned char* tile = p.pool.data + (static_cast<size_t>(page) * p.pool.heads * tiles + in_page / kv4::kTile) * p.pool.tile_bytes;
+    const int k_at = kv4::k_word_at(D, t, ch), v_at = kv4::v_codes_at(D) + kv4::v_piece_at(D, t, ch % 32 / 4) + ch / 32 * 2;
+    const int word = (t * (D / G) + ch / G) * 4;
+#pragma unroll 4
+    for (int i = blockIdx.y * kPer + sub; i < 2 * p.pool.heads; i += gridDim.y * kPer) {
+        const bool is_v = i >= p.pool.heads;
+        const int head = is_v ? i - p.pool.heads : i;
+        uint32_t out[4] = {};
+        if (there) {
+            const unsigned char* at = tile + static_cast<size_t>(head) * tiles * p.pool.tile_bytes;
+            uint32_t codes;
+            if (is_v) codes = *reinterpret_cast<const uint16_t*>(at + v_at) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + v_at + D / 2)) << 16;
+            else codes = *reinterpret_cast<const uint32_t*>(at + k_at);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + (is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D)) + word);
+            float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] = fmaf(static_cast<float>(codes >> (4 * j) & 15u), kv4::word_scale(word), kv4::word_min(word));
-    } else if (slot >= 0) {
-        atomicCAS(p.status, 0, SPK_BAD_INDEX);
+            for (int j = 0; j < 8; ++j) x[j] = fmaf(__uint_as_float((codes >> (4 * j) & 15u) | 0x4b000000u) - 8388608.0f, kv4::word_scale(w), kv4::word_min(w));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                out[j] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
+        *reinterpret_cast<uint4*>((is_v ? p.v : p.k) + (static_cast<size_t>(n) * p.pool.heads + head) * D + ch) = make_uint4(out[0], out[1], out[2], out[3]);
     }
-    store4((is_v ? p.v : p.k) + (n * p.pool.heads + head) * D + 4 * quad, x);
 }
 
 template <template <int, int> class F, typename... A>
@@ -325,8 +346,8 @@ struct Append {
     static int run(const AppendParams& p, int sms, cudaStream_t stream) {
         constexpr int kPer = 256 / D;
         const int blocks = cdiv(p.batch.rows, 8), steps = cdiv(p.q_heads, kPer) + cdiv(2 * p.pool.heads, kPer);
-        // few tokens: the heads are sliced over blocks until the SMs hold eight blocks each
-        const int slices = std::max(1, std::min(steps, 8 * sms / blocks));
+        // the heads are sliced over blocks until there are several rounds of them (four live on an SM), or one step each
+        const int slices = std::max(1, std::min(steps, 16 * sms / blocks));
         auto kernel = p.rot == D ? kv4_append_kernel<D, G, true> : kv4_append_kernel<D, G, false>;
         SPK_CUDA(launch_chained(kernel, dim3(blocks, slices), dim3(256), 0, stream, p));
         return SPK_OK;
@@ -334,9 +355,10 @@ struct Append {
 };
 template <int D, int G>
 struct Read {
-    static int run(const ReadParams& p, cudaStream_t stream) {
-        const int64_t threads = int64_t{p.n} * p.pool.heads * 2 * (D / 4);
-        SPK_CUDA(launch_chained(kv4_read_kernel<D, G>, dim3(static_cast<unsigned>(cdiv64(threads, 256))), dim3(256), 0, stream, p));
+    static int run(const ReadParams& p, int sms, cudaStream_t stream) {
+        const int blocks = cdiv(p.n, 8), steps = cdiv(2 * p.pool.heads, 256 / D);
+        const int slices = std::max(1, std::min(steps, 16 * sms / blocks));
+        SPK_CUDA(launch_chained(kv4_read_kernel<D, G>, dim3(blocks, slices), dim3(256), 0, stream, p));
         return SPK_OK;
     }
 };
@@ -384,5 +406,5 @@ extern "C" int spk_kv4_read(const void* pool, int pages, int page_size, int kv_h
     p.pool = {static_cast<unsigned char*>(const_cast<void*>(pool)), pages, page_size, kv_heads, kv4::tile_bytes(head_dim, group)};
     p.slots = reinterpret_cast<const long long*>(slots), p.n = n;
     p.k = static_cast<__nv_bfloat16*>(k), p.v = static_cast<__nv_bfloat16*>(v), p.status = dev->status;
-    return for_shape<Read>(head_dim, group, p, static_cast<cudaStream_t>(stream));
+    return for_shape<Read>(head_dim, group, p, dev->sm_count, static_cast<cudaStream_t>(stream));
 }
