@@ -1,0 +1,32 @@
+// What the two attention kernels over the 4-bit cache share: the arguments of a call, and which of its sequences goes to which.
+#pragma once
+
+#include "kv4_layout.cuh"
+
+namespace spk::kv4 {
+
+struct AttendParams {
+    const __nv_bfloat16* q;
+    long long stride;
+    Pool pool;
+    Batch batch;
+    int q_heads, window, zero_rest;
+    int prompts;  // whether sequences with many rows are another launch's (kv4_prompt.cu)
+    float scale;
+    __nv_bfloat16* out;
+    int4* pieces;     // of kv4_attention.cu, in the workspace
+    float* partials;
+    int* status;
+};
+
+// A sequence is a prompt from kPromptRows rows a KV head up (rows: new tokens x query heads of a KV head), and prompts are
+// taken in blocks of kBlockRows rows a CTA. With fewer than kPromptBlocks blocks in the call they would leave most SMs idle,
+// while the other kernel cuts the keys as well.
+constexpr int kPromptRows = 128, kBlockRows = 256, kPromptBlocks = 32;
+
+__host__ __device__ inline long long prompt_blocks(long long rows) { return rows >= kPromptRows ? (rows + kBlockRows - 1) / kBlockRows : 0; }
+
+// kv4_prompt.cu: the call's prompts; nothing if they are too few.
+int attend_prompts(const AttendParams& p, int head_dim, int group, DeviceState* dev, cudaStream_t stream);
+
+}  // namespace spk::kv4

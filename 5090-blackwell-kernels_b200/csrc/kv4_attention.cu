@@ -22,14 +22,15 @@
 // through a ring of its own filled by bulk copies. What a warp holds of a piece that is cut across warps is added up in
 // the CTA at its end, what crosses CTAs goes through the workspace to a second, chained launch; always in the order of the
 // units: the same bits every run.
-#include "kv4_layout.cuh"
+#include <algorithm>
+
+#include "kv4_attend.cuh"
 #include "ptx_sm100.cuh"
 
 namespace spk {
 namespace {
 
-using kv4::Batch;
-using kv4::Pool;
+using kv4::AttendParams;
 
 constexpr int kSteps = 2;     // 16-token tiles of a ring stage
 constexpr int kMinUnits = 8;  // a CTA gets at least this many units
@@ -39,19 +40,6 @@ constexpr int kLead = 6;
 constexpr int kMaxWarps = 11;  // consuming warps of a CTA, of any form
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
-
-struct AttendParams {
-    const __nv_bfloat16* q;
-    long long stride;
-    Pool pool;
-    Batch batch;
-    int q_heads, window, zero_rest;
-    float scale;
-    __nv_bfloat16* out;
-    int4* pieces;     // [grid] (CTAs that share the piece begun in this CTA, or 0; sequence; row block; KV head)
-    float* partials;  // [grid][2 + warps][rows][D + 2]: a piece continued from the CTA before, a piece begun here, the warps' own
-    int* status;
-};
 
 // H = 2 is the form for at most four rows a KV head (NQ = 1): a row has two of the eight columns, each for half of the
 // groups, so that the scales of one group are all a column ever meets.
@@ -76,16 +64,18 @@ struct SplitCfg {
 struct Seq {
     int b, first, count, len;  // its rows of q, its tokens
     int lo, hi;                // tiles of 16 tokens that any of its rows sees
+    bool other;                // a prompt, and the prompts are another launch's
     long long begin, units;    // units before it, its own: row blocks x KV heads x (lead + tiles)
 };
 
-__device__ __forceinline__ void load_seq(const AttendParams& p, int rows, Seq& s) {
+__device__ __forceinline__ void load_seq(const AttendParams& p, int rows, bool prompts, Seq& s) {
     kv4::rows_of(p.batch, s.b, s.first, s.count);
     s.len = kv4::length_of(p.batch, p.pool.page_size, s.b, p.status);
     s.hi = s.count > 0 ? (s.len + kv4::kTile - 1) / kv4::kTile : 0;
     s.lo = p.window > 0 && s.count > 0 ? max(0, s.len - s.count - p.window + 1) / kv4::kTile : 0;
     const int group = p.q_heads / p.pool.heads;
-    s.units = static_cast<long long>((s.count * group + rows - 1) / rows) * p.pool.heads * (s.hi > s.lo ? s.hi - s.lo + kLead : 0);
+    s.other = prompts && kv4::prompt_blocks(static_cast<long long>(s.count) * group) > 0;
+    s.units = s.other ? 0 : static_cast<long long>((s.count * group + rows - 1) / rows) * p.pool.heads * (s.hi > s.lo ? s.hi - s.lo + kLead : 0);
 }
 
 // What a range holds of one (sequence, block of rows, KV head).
@@ -97,11 +87,11 @@ struct Piece {
 };
 
 // The piece at unit u; s is the sequence that holds an earlier unit, and becomes the one that holds u.
-__device__ __forceinline__ Piece piece_at(const AttendParams& p, int rows, long long u, long long end, Seq& s) {
+__device__ __forceinline__ Piece piece_at(const AttendParams& p, int rows, bool prompts, long long u, long long end, Seq& s) {
     while (s.begin + s.units <= u) {
         s.begin += s.units;
         ++s.b;
-        load_seq(p, rows, s);
+        load_seq(p, rows, prompts, s);
     }
     const int n = s.hi - s.lo + kLead;
     const long long local = u - s.begin;
@@ -437,6 +427,21 @@ kv4_attend_split_kernel(const AttendParams p) {
     const int chunk = (p.batch.seqs + kThreads - 1) / kThreads;
     long long* chunk_start = reinterpret_cast<long long*>(smem);  // in the ring's memory, before it is used
     long long total;
+    bool prompts = false;
+    if (p.prompts) {  // as the other launch counts them
+        __shared__ int blocks;
+        if (threadIdx.x == 0) blocks = 0;
+        __syncthreads();
+        long long n = 0;
+        for (int b = threadIdx.x; b < p.batch.seqs; b += kThreads) {
+            int first, count;
+            kv4::rows_of(p.batch, b, first, count);
+            n += kv4::prompt_blocks(static_cast<long long>(count) * group) * p.pool.heads;
+        }
+        if (n > 0) atomicAdd(&blocks, static_cast<int>(min(n, 1ll << 20)));
+        __syncthreads();
+        prompts = blocks >= kv4::kPromptBlocks;
+    }
     {
         __shared__ long long warp_sum[W + 1];
         __shared__ int empties, empty_seqs[kv4::kMaxSeqs / kMinGrid];  // of the ones that fall to this CTA
@@ -447,9 +452,9 @@ kv4_attend_split_kernel(const AttendParams p) {
             Seq s;
             s.b = threadIdx.x * chunk + i;
             if (s.b >= p.batch.seqs) break;
-            load_seq(p, R, s);
+            load_seq(p, R, prompts, s);
             units += s.units;
-            if (s.units == 0 && s.count > 0 && s.b % gridDim.x == blockIdx.x) empty_seqs[atomicAdd(&empties, 1)] = s.b;
+            if (s.units == 0 && !s.other && s.count > 0 && s.b % gridDim.x == blockIdx.x) empty_seqs[atomicAdd(&empties, 1)] = s.b;
         }
         long long run = units;
 #pragma unroll
@@ -496,7 +501,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         }
         seq.b = min(at * chunk, p.batch.seqs - 1);
         seq.begin = chunk_start[at];
-        load_seq(p, R, seq);
+        load_seq(p, R, prompts, seq);
     }
     ptx::fence_proxy_async();
     __syncthreads();  // chunk_start has been read: its place is the copies' now
@@ -513,7 +518,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         auto settle = [&]() {  // to this lane's next step; false at the end of the range
             while (left <= 0) {
                 if (u >= end) return false;
-                const Piece s = piece_at(p, R, u, end, seq);
+                const Piece s = piece_at(p, R, prompts, u, end, seq);
                 u += s.units;
                 left = s.tiles;
                 at = s.tile0 / tiles_per_page, in_page = s.tile0 - at * tiles_per_page;
@@ -570,7 +575,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         bool alive = true;
         State<D, G, NQ, H> st;
         for (long long u = start; u < end;) {
-            const Piece s = piece_at(p, R, u, end, seq);
+            const Piece s = piece_at(p, R, prompts, u, end, seq);
             u += s.units;
             if (s.tiles == 0) continue;
             write_task<D, G, NQ, H>(p, seq, s, task, lane);
@@ -803,6 +808,13 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     p.pieces = static_cast<int4*>(workspace);
     p.partials = reinterpret_cast<float*>(p.pieces + kMaxGrid);
     auto stream = static_cast<cudaStream_t>(stream_);
+    // the most blocks of prompts there can be decides whether they are looked for at all
+    const int64_t all_rows = int64_t{rows} * (q_heads / kv_heads);
+    p.prompts = q_offsets != nullptr && all_rows >= kv4::kPromptRows &&
+                (all_rows / kv4::kBlockRows + std::min<int64_t>(seqs, all_rows / kv4::kPromptRows)) * kv_heads >= kv4::kPromptBlocks;
+    if (p.prompts) {
+        if (int rc = kv4::attend_prompts(p, head_dim, group, dev, stream)) return rc;
+    }
     const int per_block = rows_per_block(rows, seqs, q_heads / kv_heads, head_dim / group);
     if (head_dim == 64) return group == 32 ? attend_rows<64, 32>(p, per_block, dev, stream) : attend_rows<64, 64>(p, per_block, dev, stream);
     return group == 32 ? attend_rows<128, 32>(p, per_block, dev, stream) : group == 64 ? attend_rows<128, 64>(p, per_block, dev, stream) : attend_rows<128, 128>(p, per_block, dev, stream);

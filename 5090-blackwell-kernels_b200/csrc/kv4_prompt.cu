@@ -1,0 +1,518 @@
+// Attention of many rows over the 4-bit paged KV cache (prompts; the mathematics and the argument checks: kv4_attention.cu).
+//
+// A CTA takes 256 rows (new tokens x query heads of one KV head of a sequence) in two tiles of 128, one row a TMEM lane, and
+// walks the keys 64 at a time:
+//     S [row][key] = Q' K'^T        P = 2^(S c + b)        O [row][channel] += P V'
+// with tcgen05.mma on fp16 operands, Q' and P (in S's place) from TMEM, K' and V' from shared memory. Four warps turn codes
+// and words into K' and V': 16 tokens a warp, every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
+// the 16 tokens' largest |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the
+// keys; for the values 2^e joins the softmax's exponent: with M the running maximum of score + e,
+//     P = 2^(score + e - M) <= 2^8,      sum += P 2^-e,      out = O / sum,
+// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread; a maximum that grows by less than 2^8 is
+// left alone, so O (in TMEM) is rarely touched between the MMAs. While one tile's row warps work on S the tensor cores
+// have the other tile.
+// K' rows are keys, 128 bytes = 64 channels wide (the order of the channels inside eights is the codes' own; Q' is
+// stored in the same order); V' rows are keys too, and the MMA reads them MN-major; the order of its columns is the codes',
+// put right when O is written.
+#include <algorithm>
+
+#include "kv4_attend.cuh"
+#include "umma_sm100.cuh"
+
+namespace spk {
+namespace {
+
+using kv4::AttendParams;
+
+constexpr int kKeys = 64, kRowWarps = 8, kCodeWarps = 4, kThreadsP = 32 * (kRowWarps + kCodeWarps + 1);
+constexpr int kInfos = 4;       // steps whose exponents are kept: the code warps are at most two ahead of a row warp
+constexpr float kLazy = 8.0f;   // powers of two that P may exceed 1 by
+constexpr int kFit = 14;        // |K'|, |V'| < 2^14
+
+// What the code warps say of 16 keys.
+struct TileInfo {
+    float k_unit, v_exp, v_unit;  // 2^(e - 14) of the keys; e of the values, 2^-e
+    uint32_t bad_k, bad_v[4];     // keys whose words are not finite, in K, and in V by group
+};
+
+template <int D, int G>
+struct PromptCfg {
+    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 3;
+    static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
+    static constexpr int kSmem = 1024 + 4 * kOperand + kCodeWarps * kRaw * kTile + 16;
+    // TMEM columns: S (P in its first half) and Q' of both tiles, then O
+    static constexpr int kS = 0, kQ = 128, kO = kQ + D, kCols = 512;
+    static_assert(kO + 2 * D <= kCols, "TMEM");
+};
+
+struct PromptBars {
+    uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], info[kInfos], raw[kCodeWarps][3];
+};
+
+// Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
+__device__ __forceinline__ uint4 values8(uint32_t w, uint32_t s, uint32_t m) {
+    const uint32_t w8 = w >> 8;
+    return make_uint4(ptx::f16x2_fma(ptx::f16x2_sub(ptx::lop3_and_or(w, 0x000f000fu, 0x64006400u), 0x64006400u), s, m),
+                      ptx::f16x2_fma(ptx::f16x2_sub(ptx::lop3_and_or(w, 0x00f000f0u, 0x54005400u), 0x54005400u), s, m),
+                      ptx::f16x2_fma(ptx::f16x2_sub(ptx::lop3_and_or(w8, 0x000f000fu, 0x64006400u), 0x64006400u), s, m),
+                      ptx::f16x2_fma(ptx::f16x2_sub(ptx::lop3_and_or(w8, 0x00f000f0u, 0x54005400u), 0x54005400u), s, m));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
+
+// Exponent above every |m| + 15 s of a warp's words (0 words for what is not there), at least -100.
+__device__ __forceinline__ int exponent_of(uint32_t largest) {
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    return max(static_cast<int>(largest >> 23) - 126, -100);
+}
+
+template <int D, int G>
+__global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const AttendParams p) {
+    using Cfg = PromptCfg<D, G>;
+    constexpr int NG = D / G, NC = D / 8;  // groups and chunks of eight channels of a head vector
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+    unsigned char *k_smem = smem, *v_smem = smem + 2 * Cfg::kOperand, *raw_smem = smem + 4 * Cfg::kOperand;
+    __shared__ PromptBars bars;
+    __shared__ TileInfo infos[kInfos][kCodeWarps];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_seq, s_block;
+    __shared__ int counts[kThreadsP];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = p.q_heads / p.pool.heads, tiles_per_page = p.pool.page_size / kv4::kTile;
+    pdl_wait();
+
+    // ---- this CTA's sequence and block of rows: the last blocks, which see the most keys, first ---------------------------
+    const int head = blockIdx.x % p.pool.heads, order = blockIdx.x / p.pool.heads;
+    const int chunk = (p.batch.seqs + kThreadsP - 1) / kThreadsP;
+    auto blocks_of = [&](int b) {
+        int first, count;
+        kv4::rows_of(p.batch, b, first, count);
+        return static_cast<int>(kv4::prompt_blocks(static_cast<long long>(count) * group));
+    };
+    int n = 0;
+    for (int i = 0; i < chunk; ++i)
+        if (static_cast<int>(threadIdx.x) * chunk + i < p.batch.seqs) n += blocks_of(threadIdx.x * chunk + i);
+    counts[threadIdx.x] = n;
+    if (threadIdx.x == 0) s_seq = -1;
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int t = 0; t < kThreadsP; ++t) {
+        if (t < static_cast<int>(threadIdx.x)) before += counts[t];
+        total += counts[t];
+    }
+    if (order >= total || static_cast<long long>(total) * p.pool.heads < kv4::kPromptBlocks) return;
+    const int want = total - 1 - order;
+    if (want >= before && want < before + n) {
+        int at = want - before, b = threadIdx.x * chunk;
+        while (at >= blocks_of(b)) at -= blocks_of(b++);
+        s_seq = b, s_block = at;
+    }
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(&bars.q_ready, kRowWarps);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&bars.k_full[i], kCodeWarps), ptx::mbar_init(&bars.v_full[i], kCodeWarps);
+            ptx::mbar_init(&bars.k_empty[i], 1), ptx::mbar_init(&bars.v_empty[i], 1);
+            ptx::mbar_init(&bars.s_full[i], 1), ptx::mbar_init(&bars.p_full[i], 4), ptx::mbar_init(&bars.o_full[i], 1);
+        }
+        for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], kCodeWarps);
+        for (int w = 0; w < kCodeWarps; ++w)
+            for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw[w][i], 1);
+        ptx::fence_mbar_init();
+    }
+    if (warp == kRowWarps + kCodeWarps) umma::tmem_alloc(&tmem_slot, Cfg::kCols);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    pdl_release();  // only now: a kernel that starts beside this one may want TMEM too
+
+    const int b = s_seq, block = s_block;
+    int first, count;
+    kv4::rows_of(p.batch, b, first, count);
+    const int len = kv4::length_of(p.batch, p.pool.page_size, b, p.status), rows = count * group;
+    // tokens that any row of the block sees: [any_lo, any_hi)
+    const int last_row = min(rows, (block + 1) * kv4::kBlockRows) - 1;
+    const int first_pos = len - count + block * kv4::kBlockRows / group, any_hi = max(0, len - count + last_row / group + 1);
+    const int any_lo = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;
+    const int key0 = any_lo / kKeys * kKeys, steps = any_hi > key0 ? (any_hi - key0 + kKeys - 1) / kKeys : 0;
+    const int tiles = last_row - block * kv4::kBlockRows >= 128 ? 2 : 1;  // tiles of 128 rows
+    constexpr uint32_t kAll = 0xffffffffu;
+
+    if (warp < kRowWarps) {
+        // ---- a row a thread ------------------------------------------------------------------------------------------------
+        const int tile = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const int row = block * kv4::kBlockRows + tile * 128 + (warp & 3) * 32 + lane;
+        const bool there = row < rows;
+        const int token = there ? row / group : 0;
+        const __nv_bfloat16* q = p.q + static_cast<long long>(first + token) * p.stride + static_cast<long long>(head * group + (there ? row - token * group : 0)) * D;
+        __nv_bfloat16* out = p.out + (static_cast<size_t>(first + token) * p.q_heads + head * group + (there ? row - token * group : 0)) * D;
+        const int pos = len - count + token;
+        const int hi = there ? max(0, pos + 1) : 0, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        uint32_t most = 0;
+#pragma unroll 4
+        for (int i = 0; i < NC; ++i) {
+            const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(q) + i) : uint4{};
+            most = __vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+        }
+        const int e = static_cast<int>(max(most >> 16, most & 0xffffu) >> 7);  // biased exponent of the row's largest |q|
+        const bool finite = e < 255;
+        float down = __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23);
+        if (p.scale < 0.0f) down = -down;
+        const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
+        const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
+        const bool work = tile < tiles && steps > 0;
+        if (work) {
+#pragma unroll
+            for (int part = 0; part < D / 64; ++part) {
+                uint32_t r[32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 w = there && finite ? __ldg(reinterpret_cast<const uint4*>(q) + part * 8 + i) : uint4{};
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                    float h[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[2 * k] = __uint_as_float(u[k] << 16) * down, h[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[4 * i + k] = ptx::f16x2_pack(h[k], h[k + 4]);
+                }
+                umma::tmem_st_32x32(tmem + lanes + Cfg::kQ + tile * (D / 2) + part * 32, r);
+            }
+            umma::tmem_st_wait();
+        }
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars.q_ready);
+
+        const int all_hi = __reduce_min_sync(kAll, there ? hi : INT32_MAX), all_lo = __reduce_max_sync(kAll, there ? lo : 0);
+        float top = -INFINITY, sum = 0.0f;
+        uint32_t poison = 0;  // groups of channels in which this row sees a value that is no number
+        bool alive = true;
+        const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 64, o_at = tmem + lanes + Cfg::kO + tile * D;
+        for (int j = 0; work && j < steps; ++j) {
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.info[j % kInfos], (j / kInfos) & 1, p.status));
+            const TileInfo* info = infos[j % kInfos];
+            float unit[4], v_exp[4], v_unit[4];
+            uint32_t bad = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                unit[t] = fmaxf(info[t].k_unit * mult, 1.2e-38f), v_exp[t] = info[t].v_exp, v_unit[t] = info[t].v_unit;
+                bad |= info[t].bad_k;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) bad |= info[t].bad_v[k];
+            }
+            const int base = key0 + j * kKeys;
+            if (bad) {
+                for (int t = 0; t < 4; ++t)
+                    for (int i = 0; i < kv4::kTile; ++i) {
+                        const int key = base + kv4::kTile * t + i;
+                        if (key < lo || key >= hi) continue;
+                        if (info[t].bad_k >> i & 1) poison = (1u << NG) - 1;
+                        for (int k = 0; k < NG; ++k) poison |= (info[t].bad_v[k] >> i & 1) << k;
+                    }
+            }
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[tile], j & 1, p.status));
+            umma::fence_after_sync();
+            uint32_t a0[32], a1[32];
+            umma::tmem_ld_32x32(s_at, a0);
+            umma::tmem_ld_32x32(s_at + 32, a1);
+            umma::tmem_ld_wait();
+            float x[64];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(a0[i]), x[i + 32] = __uint_as_float(a1[i]);
+            if (base < all_lo || base + kKeys > all_hi) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (base + i < lo || base + i >= hi) x[i] = -INFINITY;
+            }
+            float most_here = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float m = x[16 * t];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
+                most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
+            }
+            if (__any_sync(kAll, most_here > top + kLazy)) {
+                const float now = fmaxf(top, most_here), keep = top == -INFINITY ? 0.0f : exp2f(top - now);
+                if (j > 0) {
+#pragma unroll 1
+                    for (int at = 0; at < D; at += 32) {
+                        uint32_t r[32];
+                        umma::tmem_ld_32x32(o_at + at, r);
+                        umma::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * keep);
+                        umma::tmem_st_32x32(o_at + at, r);
+                    }
+                }
+                sum *= keep, top = now;
+            }
+            uint32_t pr[32];
+            const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float add = v_exp[t] - shift;
+                float part = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float u = ptx::exp2_fast(fmaf(x[16 * t + i], unit[t], add)), v = ptx::exp2_fast(fmaf(x[16 * t + i + 1], unit[t], add));
+                    part += u + v;
+                    pr[8 * t + i / 2] = ptx::f16x2_pack(u, v);
+                }
+                sum = fmaf(part, v_unit[t], sum);
+            }
+            umma::tmem_st_32x32(s_at, pr);
+            umma::tmem_st_wait();
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.p_full[tile]);
+        }
+        if (work && alive) __all_sync(kAll, ptx::mbar_wait(&bars.o_full[tile], 0, p.status));
+        umma::fence_after_sync();
+        if (!finite && hi > lo) poison = ~0u;
+        const float inv = sum == 0.0f ? 0.0f : power_of_two(-kFit) / sum;
+        if (tile < tiles) {
+#pragma unroll
+            for (int at = 0; at < D / 32; ++at) {
+                uint32_t r[32] = {};
+                if (work) {
+                    umma::tmem_ld_32x32(o_at + 32 * at, r);
+                    umma::tmem_ld_wait();
+                }
+                // column (D = 128): 16 g + 8 (u / 2) + 2 n + u % 2; (D = 64): 8 g + 2 n + u; channel 32 u + 4 g + n
+#pragma unroll
+                for (int u = 0; u < D / 32; ++u)
+#pragma unroll
+                    for (int half = 0; half < (D == 64 ? 2 : 1); ++half) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float f[2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int ch = 8 * half + 2 * k + y, g = ch / 4, nn = ch % 4;  // g within this run of 32 columns
+                                const int col = D == 128 ? 16 * g + 8 * (u / 2) + 2 * nn + u % 2 : 8 * g + 2 * nn + u;
+                                f[y] = poison >> (32 * u / G) & 1 ? __uint_as_float(0x7fc00000u) : __uint_as_float(r[col]) * inv;
+                            }
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]);
+                            o[k] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                        if (there) *reinterpret_cast<uint4*>(out + 32 * u + (D == 128 ? 8 : 16) * at + 8 * half) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+            }
+        }
+    } else if (warp < kRowWarps + kCodeWarps) {
+        // ---- 16 keys of every step a warp: codes and words to K' and V' -----------------------------------------------------
+        const int w = warp - kRowWarps;
+        unsigned char* raw = raw_smem + w * Cfg::kRaw * Cfg::kTile;
+        uint64_t* raw_full = bars.raw[w];
+        const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
+        uint32_t got = 0;  // tiles of the ring that hold something, by slot
+        // the tile of step j, if there is one: one copy
+        auto fetch = [&](int j) {
+            const int key = key0 + j * kKeys + w * kv4::kTile, slot = j % Cfg::kRaw;
+            got &= ~(1u << slot);
+            if (j >= steps || key >= any_hi) return;
+            const int at = key / kv4::kTile, page = __ldg(table + at / tiles_per_page);
+            if (page < 0 || page >= p.pool.pages) {
+                if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                return;
+            }
+            got |= 1u << slot;
+            if (lane == 0) {
+                ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kTile);
+                ptx::bulk_g2s(raw + slot * Cfg::kTile, p.pool.data + ((static_cast<size_t>(page) * p.pool.heads + head) * tiles_per_page + at % tiles_per_page) * Cfg::kTile,
+                              Cfg::kTile, &raw_full[slot]);
+            }
+        };
+        for (int j = 0; j < Cfg::kRaw; ++j) fetch(j);
+        uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
+        bool alive = true;
+        const int t = lane >> 1, h = lane & 1;                            // K: a lane has half of a key's row
+        const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;      // V: run g of four keys of a block of eight
+        for (int j = 0; j < steps; ++j) {
+            const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
+            const bool here = got >> slot & 1;
+            if (here) {
+                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
+                raw_phase ^= 1u << slot;
+            }
+            const unsigned char* tile = raw + slot * Cfg::kTile;
+            // a word, 0 for a key that no row sees or whose word is not finite
+            auto word_at = [&](int at, int key, int k, bool& bad) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + at + (key * NG + k) * 4);
+                const bool seen = here && base + key >= any_lo && base + key < any_hi;
+                bad = seen && ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u);
+                return seen && !bad ? x : 0u;
+            };
+            auto size_of = [](uint32_t x) { return __float_as_uint(fminf(fmaf(15.0f, fabsf(kv4::word_scale(x)), fabsf(kv4::word_min(x))), 3.4e38f)); };
+            // K words of this lane's key, V words of its four keys; exponents and what is not finite over the warp
+            uint32_t kw[NG], vw[4][NG], k_size = 0, v_size = 0, bad_k = 0, bad_v[NG];
+            bool bad;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                kw[k] = word_at(kv4::k_words_at(D), t, k, bad);
+                if (bad) bad_k |= 1u << t;
+                k_size = max(k_size, size_of(kw[k]));
+                bad_v[k] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vw[i][k] = word_at(kv4::v_words_at(D, G), 8 * blk + 4 * th + i, k, bad);
+                    if (bad) bad_v[k] |= 1u << (8 * blk + 4 * th + i);
+                    v_size = max(v_size, size_of(vw[i][k]));
+                }
+            }
+            const int k_exp = exponent_of(k_size), v_exp = exponent_of(v_size);
+            bad_k = __reduce_or_sync(kAll, bad_k);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
+            if (lane == 0) {
+                TileInfo& info = infos[j % kInfos][w];
+                info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
+                info.bad_k = bad_k;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) info.bad_v[k] = bad_v[k];
+            }
+            // ---- K'
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);  // its place was free: the row warps are past step j - 4
+            {
+                const float f = power_of_two(kFit - k_exp);
+                uint32_t s2[NG], m2[NG];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    const float s = kv4::word_scale(kw[k]) * f, m = kv4::word_min(kw[k]) * f;
+                    s2[k] = ptx::f16x2_pack(s, s), m2[k] = ptx::f16x2_pack(m, m);
+                }
+                unsigned char* to = k_smem + stage * Cfg::kOperand;
+                const int row = w * kv4::kTile + t;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
+                    const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
+                    uint32_t code[D / 32];
+                    if constexpr (D == 128) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(at);
+                        code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(at);
+                        code[0] = v.x, code[1] = v.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const int chunk = 4 * i + 2 * h + r;  // channels 8 chunk .. + 7
+                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = values8(code[i], s2[32 * i / G], m2[32 * i / G]);
+                    }
+                }
+            }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.k_full[stage]);
+            // ---- V'
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.v_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
+            {
+                const float f = power_of_two(kFit - v_exp);
+                unsigned char* to = v_smem + stage * Cfg::kOperand;
+                const unsigned char* at = tile + kv4::v_codes_at(D) + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
+                uint32_t code[4][D / 64];
+                if constexpr (D == 128) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 16);
+                    code[0][0] = a.x, code[0][D / 64 - 1] = a.y, code[1][0] = a.z, code[1][D / 64 - 1] = a.w;
+                    code[2][0] = c.x, code[2][D / 64 - 1] = c.y, code[3][0] = c.z, code[3][D / 64 - 1] = c.w;
+                } else {
+                    const uint4 a = *reinterpret_cast<const uint4*>(at);
+                    code[0][0] = a.x, code[1][0] = a.y, code[2][0] = a.z, code[3][0] = a.w;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = w * kv4::kTile + 8 * blk + 4 * th + i;
+                    float s[NG], m[NG];
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) s[k] = kv4::word_scale(vw[i][k]) * f, m[k] = kv4::word_min(vw[i][k]) * f;
+#pragma unroll
+                    for (int jw = 0; jw < D / 64; ++jw) {  // units 2 jw (low halves) and 2 jw + 1 (high)
+                        const int ka = 64 * jw / G, kb = (64 * jw + 32) / G, chunk = D / 64 * g + jw;
+                        *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+                            values8(code[i][jw], ptx::f16x2_pack(s[ka], s[kb]), ptx::f16x2_pack(m[ka], m[kb]));
+                    }
+                }
+            }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.v_full[stage]);
+            fetch(j + Cfg::kRaw);
+        }
+    } else if (steps > 0) {
+        // ---- the MMAs ----------------------------------------------------------------------------------------------------------
+        constexpr uint32_t s_desc = umma::instr_desc(128, kKeys, 0, 0), o_desc = umma::instr_desc_b_mn(128, D, 0, 0);
+        bool ok = __all_sync(kAll, ptx::mbar_wait(&bars.q_ready, 0, p.status));
+        auto scores = [&](int i, int stage) {
+            const uint64_t k0 = umma::smem_desc_k128(k_smem + stage * Cfg::kOperand);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                umma::mma_f16_tmem_a(tmem + Cfg::kS + i * 64, tmem + Cfg::kQ + i * (D / 2) + 8 * k, umma::desc_advance(k0, (k / 4) * (kKeys * 128) + (k % 4) * 32), s_desc, k > 0);
+            umma::mma_commit(&bars.s_full[i]);
+        };
+        if (ok) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[0], 0, p.status));
+        umma::fence_after_sync();
+        if (ok && umma::elect_one()) {
+            for (int i = 0; i < tiles; ++i) scores(i, 0);
+            umma::mma_commit(&bars.k_empty[0]);
+        }
+        __syncwarp();
+        for (int j = 0; ok && j < steps; ++j) {
+            const int stage = j & 1, next = (j + 1) & 1;
+            ok = __all_sync(kAll, ptx::mbar_wait(&bars.v_full[stage], (j >> 1) & 1, p.status));
+            for (int i = 0; ok && i < tiles; ++i) {
+                ok = __all_sync(kAll, ptx::mbar_wait(&bars.p_full[i], j & 1, p.status));
+                if (ok && i == 0 && j + 1 < steps) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[next], ((j + 1) >> 1) & 1, p.status));
+                if (!ok) break;
+                umma::fence_after_sync();
+                if (umma::elect_one()) {
+                    const uint64_t v0 = umma::smem_desc_mn128(v_smem + stage * Cfg::kOperand, kKeys * 128);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma::mma_f16_tmem_a(tmem + Cfg::kO + i * D, tmem + Cfg::kS + i * 64 + 8 * k, umma::desc_advance(v0, k * 2048), o_desc, j > 0 || k > 0);
+                    if (i == tiles - 1) umma::mma_commit(&bars.v_empty[stage]);
+                    if (j + 1 < steps) {
+                        scores(i, next);
+                        if (i == tiles - 1) umma::mma_commit(&bars.k_empty[next]);
+                    } else {
+                        umma::mma_commit(&bars.o_full[i]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == kRowWarps + kCodeWarps) umma::tmem_dealloc(tmem, Cfg::kCols);
+}
+
+template <int D, int G>
+int launch_prompts(const AttendParams& p, DeviceState* dev, cudaStream_t stream) {
+    using Cfg = PromptCfg<D, G>;
+    auto kernel = kv4_attend_prompt_kernel<D, G>;
+    static bool configured[kMaxDevices] = {};
+    if (!configured[dev->device]) {
+        SPK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+        configured[dev->device] = true;
+    }
+    const int64_t rows = int64_t{p.batch.rows} * (p.q_heads / p.pool.heads);
+    const int64_t blocks = rows / kv4::kBlockRows + std::min<int64_t>(p.batch.seqs, rows / kv4::kPromptRows);
+    SPK_REQUIRE(blocks * p.pool.heads < (int64_t{1} << 31), "kv4_attention: too many rows for one call");
+    SPK_CUDA(launch_chained(kernel, dim3(static_cast<unsigned>(blocks * p.pool.heads)), dim3(kThreadsP), Cfg::kSmem, stream, p));
+    return SPK_OK;
+}
+
+}  // namespace
+
+int kv4::attend_prompts(const AttendParams& p, int d, int group, DeviceState* dev, cudaStream_t stream) {
+    if (d == 64) return group == 32 ? launch_prompts<64, 32>(p, dev, stream) : launch_prompts<64, 64>(p, dev, stream);
+    return group == 32 ? launch_prompts<128, 32>(p, dev, stream) : group == 64 ? launch_prompts<128, 64>(p, dev, stream) : launch_prompts<128, 128>(p, dev, stream);
+}
+
+}  // namespace spk

@@ -56,6 +56,18 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         : "r"(taddr)
         : "memory");
 }
+// The reverse: 32 registers of a lane into 32 consecutive columns.
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---- descriptors ---------------------------------------------------------------------------------
@@ -67,6 +79,12 @@ __device__ __forceinline__ uint64_t smem_desc_k128(const void* tile) {
     const uint64_t addr = (ptx::smem_u32(tile) & 0x3FFFFu) >> 4;
     return addr | (uint64_t{1} << 16) | (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
 }
+// Descriptor of an MN-major SWIZZLE_128B tile of 16-bit elements: a k is a row of 128 bytes (64 elements of m or n), the next
+// 64 elements are `block` bytes on, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn128(const void* tile, uint32_t block) {
+    const uint64_t addr = (ptx::smem_u32(tile) & 0x3FFFFu) >> 4;
+    return addr | (uint64_t{block >> 4} << 16) | (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
 // The descriptor of the same tile advanced by `bytes` along K inside the swizzle atom.
 __device__ __forceinline__ uint64_t desc_advance(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 
@@ -76,6 +94,9 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n, int a_fmt, int b
     return (1u << 4) | (static_cast<uint32_t>(a_fmt) << 7) | (static_cast<uint32_t>(b_fmt) << 10) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+
+// The same with operand B MN-major.
+__host__ __device__ constexpr uint32_t instr_desc_b_mn(int m, int n, int a_fmt, int b_fmt) { return instr_desc(m, n, a_fmt, b_fmt) | (1u << 16); }
 
 // ---- MMA -----------------------------------------------------------------------------------------
 
@@ -93,6 +114,14 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(tmem_d),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(0u)
+        : "memory");
+}
+// The same with operand A in TMEM (a lane per row, two elements of k per column).
+__device__ __forceinline__ void mma_f16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
         : "memory");
 }
 // True in exactly one lane of a fully converged warp. The MMA warp runs its loop warp-wide and puts
