@@ -24,22 +24,32 @@ namespace {
 
 using kv4::AttendParams;
 
-constexpr int kKeys = 64, kRowWarps = 8, kCodeWarps = 4, kThreadsP = 32 * (kRowWarps + kCodeWarps + 1);
+// Four warpgroups: two of row warps, one of code warps, one whose first warp issues the MMAs. The registers are dealt out
+// again by warpgroup (168 + 168 + 104 + 72 = 4 x 128).
+constexpr int kKeys = 64, kRowWarps = 8, kCodeWarps = 4, kThreadsP = 512;
+constexpr int kRowRegs = 168, kCodeRegs = 104, kMmaRegs = 72;
 constexpr int kInfos = 4;       // steps whose exponents are kept: the code warps are at most two ahead of a row warp
 constexpr float kLazy = 8.0f;   // powers of two that P may exceed 1 by
 constexpr int kFit = 14;        // |K'|, |V'| < 2^14
 
 // What the code warps say of 16 keys.
-struct TileInfo {
-    float k_unit, v_exp, v_unit;  // 2^(e - 14) of the keys; e of the values, 2^-e
-    uint32_t bad_k, bad_v[4];     // keys whose words are not finite, in K, and in V by group
+struct alignas(16) TileInfo {
+    float k_unit, v_exp, v_unit;   // 2^(e - 14) of the keys; e of the values, 2^-e
+    uint32_t bad;                  // whether any word is not finite
+    uint32_t bad_k, bad_v[4];      // then the keys, in K, and in V by group
 };
+
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D, int G>
 struct PromptCfg {
     static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 3;
     static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
-    static constexpr int kSmem = 1024 + 4 * kOperand + kCodeWarps * kRaw * kTile + 16;
+    static constexpr int kWords = 32 * (D / G);     // words of a tile, K's and V's
+    static constexpr int kSmem = 1024 + 4 * kOperand + kCodeWarps * (kRaw * kTile + kWords * 8) + 16;
     // TMEM columns: S (P in its first half) and Q' of both tiles, then O
     static constexpr int kS = 0, kQ = 128, kO = kQ + D, kCols = 512;
     static_assert(kO + 2 * D <= kCols, "TMEM");
@@ -76,7 +86,6 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     __shared__ TileInfo infos[kInfos][kCodeWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_block;
-    __shared__ int counts[kThreadsP];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.q_heads / p.pool.heads, tiles_per_page = p.pool.page_size / kv4::kTile;
@@ -93,13 +102,20 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     int n = 0;
     for (int i = 0; i < chunk; ++i)
         if (static_cast<int>(threadIdx.x) * chunk + i < p.batch.seqs) n += blocks_of(threadIdx.x * chunk + i);
-    counts[threadIdx.x] = n;
-    if (threadIdx.x == 0) s_seq = -1;
+    // the blocks before this thread's chunk, and all of them: each warp sums the warps before it
+    __shared__ int warp_blocks[kThreadsP / 32];
+    int run = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += up;
+    }
+    if (lane == 31) warp_blocks[warp] = run;
     __syncthreads();
-    int before = 0, total = 0;
-    for (int t = 0; t < kThreadsP; ++t) {
-        if (t < static_cast<int>(threadIdx.x)) before += counts[t];
-        total += counts[t];
+    int before = run - n, total = 0;
+    for (int w = 0; w < kThreadsP / 32; ++w) {
+        if (w < warp) before += warp_blocks[w];
+        total += warp_blocks[w];
     }
     if (order >= total || static_cast<long long>(total) * p.pool.heads < kv4::kPromptBlocks) return;
     const int want = total - 1 - order;
@@ -140,6 +156,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     constexpr uint32_t kAll = 0xffffffffu;
 
     if (warp < kRowWarps) {
+        registers_up<kRowRegs>();
         // ---- a row a thread ------------------------------------------------------------------------------------------------
         const int tile = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -197,15 +214,14 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             uint32_t bad = 0;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                unit[t] = fmaxf(info[t].k_unit * mult, 1.2e-38f), v_exp[t] = info[t].v_exp, v_unit[t] = info[t].v_unit;
-                bad |= info[t].bad_k;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) bad |= info[t].bad_v[k];
+                const float4 of = *reinterpret_cast<const float4*>(&info[t]);
+                unit[t] = fmaxf(of.x * mult, 1.2e-38f), v_exp[t] = of.y, v_unit[t] = of.z;
+                bad |= __float_as_uint(of.w);
             }
             const int base = key0 + j * kKeys;
             if (bad) {
                 for (int t = 0; t < 4; ++t)
-                    for (int i = 0; i < kv4::kTile; ++i) {
+                    for (int i = 0; i < kv4::kTile && info[t].bad; ++i) {
                         const int key = base + kv4::kTile * t + i;
                         if (key < lo || key >= hi) continue;
                         if (info[t].bad_k >> i & 1) poison = (1u << NG) - 1;
@@ -304,91 +320,103 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             }
         }
     } else if (warp < kRowWarps + kCodeWarps) {
+        registers_down<kCodeRegs>();
         // ---- 16 keys of every step a warp: codes and words to K' and V' -----------------------------------------------------
         const int w = warp - kRowWarps;
         unsigned char* raw = raw_smem + w * Cfg::kRaw * Cfg::kTile;
+        uint2* scales = reinterpret_cast<uint2*>(raw_smem + kCodeWarps * Cfg::kRaw * Cfg::kTile) + w * Cfg::kWords;  // (s, s), (m, m) of every word
         uint64_t* raw_full = bars.raw[w];
         const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
-        uint32_t got = 0;  // tiles of the ring that hold something, by slot
-        // the tile of step j, if there is one: one copy
-        auto fetch = [&](int j) {
-            const int key = key0 + j * kKeys + w * kv4::kTile, slot = j % Cfg::kRaw;
+        const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
+        const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
+        // the tile that is fetched next: its first key, its place in the table, its page's number (read a step early)
+        int next_key = key0 + w * kv4::kTile, next_at = next_key / kv4::kTile / tiles_per_page, next_in = next_key / kv4::kTile % tiles_per_page, next_page = -1;
+        if (next_key < any_hi) next_page = __ldg(table + next_at);
+        uint32_t got = 0;  // slots of the ring that hold a tile
+        auto fetch = [&](int slot) {
             got &= ~(1u << slot);
-            if (j >= steps || key >= any_hi) return;
-            const int at = key / kv4::kTile, page = __ldg(table + at / tiles_per_page);
-            if (page < 0 || page >= p.pool.pages) {
-                if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
-                return;
+            if (next_key >= any_hi) return;
+            if (next_page >= 0 && next_page < p.pool.pages) {
+                got |= 1u << slot;
+                if (lane == 0) {
+                    ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kTile);
+                    ptx::bulk_g2s(raw + slot * Cfg::kTile, pool + next_page * page_bytes + next_in * Cfg::kTile, Cfg::kTile, &raw_full[slot]);
+                }
+            } else if (lane == 0) {
+                atomicCAS(p.status, 0, SPK_BAD_INDEX);
             }
-            got |= 1u << slot;
-            if (lane == 0) {
-                ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kTile);
-                ptx::bulk_g2s(raw + slot * Cfg::kTile, p.pool.data + ((static_cast<size_t>(page) * p.pool.heads + head) * tiles_per_page + at % tiles_per_page) * Cfg::kTile,
-                              Cfg::kTile, &raw_full[slot]);
-            }
+            next_key += kKeys, next_in += kKeys / kv4::kTile;
+            while (next_in >= tiles_per_page) next_in -= tiles_per_page, ++next_at;
+            if (next_key < any_hi) next_page = __ldg(table + next_at);
         };
-        for (int j = 0; j < Cfg::kRaw; ++j) fetch(j);
+        for (int i = 0; i < Cfg::kRaw; ++i) fetch(i);
         uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
         bool alive = true;
+        int slot = 0;
         const int t = lane >> 1, h = lane & 1;                            // K: a lane has half of a key's row
         const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;      // V: run g of four keys of a block of eight
         for (int j = 0; j < steps; ++j) {
-            const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
+            const int stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
             const bool here = got >> slot & 1;
             if (here) {
                 if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
                 raw_phase ^= 1u << slot;
             }
             const unsigned char* tile = raw + slot * Cfg::kTile;
-            // a word, 0 for a key that no row sees or whose word is not finite
-            auto word_at = [&](int at, int key, int k, bool& bad) {
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + at + (key * NG + k) * 4);
-                const bool seen = here && base + key >= any_lo && base + key < any_hi;
-                bad = seen && ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u);
-                return seen && !bad ? x : 0u;
-            };
-            auto size_of = [](uint32_t x) { return __float_as_uint(fminf(fmaf(15.0f, fabsf(kv4::word_scale(x)), fabsf(kv4::word_min(x))), 3.4e38f)); };
-            // K words of this lane's key, V words of its four keys; exponents and what is not finite over the warp
-            uint32_t kw[NG], vw[4][NG], k_size = 0, v_size = 0, bad_k = 0, bad_v[NG];
-            bool bad;
+            // ---- the words, one or a few a lane (K's, then V's): their sizes, and what is not finite; 0 for a key no row sees
+            float s[NG], m[NG];
+            uint32_t k_size = 0, v_size = 0, odd = 0;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                kw[k] = word_at(kv4::k_words_at(D), t, k, bad);
-                if (bad) bad_k |= 1u << t;
-                k_size = max(k_size, size_of(kw[k]));
-                bad_v[k] = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vw[i][k] = word_at(kv4::v_words_at(D, G), 8 * blk + 4 * th + i, k, bad);
-                    if (bad) bad_v[k] |= 1u << (8 * blk + 4 * th + i);
-                    v_size = max(v_size, size_of(vw[i][k]));
-                }
+            for (int i = 0; i < NG; ++i) {
+                const int at = lane + 32 * i, key = at % (16 * NG) / NG;
+                uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + at * 4);
+                if (!here || base + key < any_lo || base + key >= any_hi) x = 0;
+                if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
+                s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
+                const uint32_t size = __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f));
+                if (at < 16 * NG) k_size = max(k_size, size); else v_size = max(v_size, size);
             }
             const int k_exp = exponent_of(k_size), v_exp = exponent_of(v_size);
-            bad_k = __reduce_or_sync(kAll, bad_k);
+            const float k_fit = power_of_two(kFit - k_exp), v_fit = power_of_two(kFit - v_exp);
 #pragma unroll
-            for (int k = 0; k < NG; ++k) bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
-            if (lane == 0) {
-                TileInfo& info = infos[j % kInfos][w];
-                info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
-                info.bad_k = bad_k;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) info.bad_v[k] = bad_v[k];
+            for (int i = 0; i < NG; ++i) {
+                const float f = lane + 32 * i < 16 * NG ? k_fit : v_fit;
+                scales[lane + 32 * i] = make_uint2(ptx::f16x2_pack(s[i] * f, s[i] * f), ptx::f16x2_pack(m[i] * f, m[i] * f));
             }
-            // ---- K'
-            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);  // its place was free: the row warps are past step j - 4
-            {
-                const float f = power_of_two(kFit - k_exp);
-                uint32_t s2[NG], m2[NG];
+            const bool any_odd = __any_sync(kAll, odd != 0);
+            TileInfo& info = infos[j % kInfos][w];  // its place is free: the row warps are past step j - 4
+            if (lane == 0) {
+                info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
+                info.bad = any_odd;
+            }
+            if (any_odd) {
+                uint32_t bad_k = 0, bad_v[NG] = {};
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int at = lane + 32 * i, key = at % (16 * NG) / NG;
+                    if (!(odd >> i & 1)) continue;
+                    if (at < 16 * NG) bad_k |= 1u << key;
+#pragma unroll
+                    for (int k = 0; k < NG; ++k)
+                        if (at >= 16 * NG && at % NG == k) bad_v[k] |= 1u << key;
+                }
+                bad_k = __reduce_or_sync(kAll, bad_k);
+                if (lane == 0) info.bad_k = bad_k;
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
-                    const float s = kv4::word_scale(kw[k]) * f, m = kv4::word_min(kw[k]) * f;
-                    s2[k] = ptx::f16x2_pack(s, s), m2[k] = ptx::f16x2_pack(m, m);
+                    bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
+                    if (lane == 0) info.bad_v[k] = bad_v[k];
                 }
-                unsigned char* to = k_smem + stage * Cfg::kOperand;
-                const int row = w * kv4::kTile + t;
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);
+            // ---- K'
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
+            {
+                uint2 sm[NG];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
+                unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
                     const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
@@ -401,10 +429,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         code[0] = v.x, code[1] = v.y;
                     }
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        const int chunk = 4 * i + 2 * h + r;  // channels 8 chunk .. + 7
-                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = values8(code[i], s2[32 * i / G], m2[32 * i / G]);
-                    }
+                    for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
+                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
                 }
             }
             ptx::fence_proxy_async();
@@ -413,8 +439,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             // ---- V'
             if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.v_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
             {
-                const float f = power_of_two(kFit - v_exp);
-                unsigned char* to = v_smem + stage * Cfg::kOperand;
+                unsigned char* to = v_smem + stage * Cfg::kOperand + (w * kv4::kTile + 8 * blk + 4 * th) * 128;
                 const unsigned char* at = tile + kv4::v_codes_at(D) + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
                 uint32_t code[4][D / 64];
                 if constexpr (D == 128) {
@@ -427,24 +452,26 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = w * kv4::kTile + 8 * blk + 4 * th + i;
-                    float s[NG], m[NG];
+                    uint2 sm[NG];
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) s[k] = kv4::word_scale(vw[i][k]) * f, m[k] = kv4::word_min(vw[i][k]) * f;
+                    for (int k = 0; k < NG; ++k) sm[k] = scales[16 * NG + (8 * blk + 4 * th + i) * NG + k];
 #pragma unroll
                     for (int jw = 0; jw < D / 64; ++jw) {  // units 2 jw (low halves) and 2 jw + 1 (high)
                         const int ka = 64 * jw / G, kb = (64 * jw + 32) / G, chunk = D / 64 * g + jw;
-                        *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-                            values8(code[i][jw], ptx::f16x2_pack(s[ka], s[kb]), ptx::f16x2_pack(m[ka], m[kb]));
+                        const uint32_t s2 = ka == kb ? sm[ka].x : __byte_perm(sm[ka].x, sm[kb].x, 0x5410), m2 = ka == kb ? sm[ka].y : __byte_perm(sm[ka].y, sm[kb].y, 0x5410);
+                        *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + i * 128 + (((chunk & 7) ^ (4 * th + i)) << 4)) = values8(code[i][jw], s2, m2);
                     }
                 }
             }
             ptx::fence_proxy_async();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&bars.v_full[stage]);
-            fetch(j + Cfg::kRaw);
+            fetch(slot);
+            if (++slot == Cfg::kRaw) slot = 0;
         }
-    } else if (steps > 0) {
+    } else {
+        registers_down<kMmaRegs>();
+        if (warp == kRowWarps + kCodeWarps && steps > 0) {
         // ---- the MMAs ----------------------------------------------------------------------------------------------------------
         constexpr uint32_t s_desc = umma::instr_desc(128, kKeys, 0, 0), o_desc = umma::instr_desc_b_mn(128, D, 0, 0);
         bool ok = __all_sync(kAll, ptx::mbar_wait(&bars.q_ready, 0, p.status));
@@ -486,6 +513,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 __syncwarp();
             }
         }
+    }
     }
     umma::fence_before_sync();
     __syncthreads();
