@@ -3,7 +3,7 @@
 // A CTA takes 256 rows (new tokens x query heads of one KV head of a sequence) in two tiles of 128, one row a TMEM lane, and
 // walks the keys 64 at a time:
 //     S [row][key] = Q' K'^T        P = 2^(S c + b)        O [row][channel] += P V'
-// with tcgen05.mma on fp16 operands, Q' and P (in S's place) from TMEM, K' and V' from shared memory. Four warps turn codes
+// with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Four warps turn codes
 // and words into K' and V': 16 tokens a warp, every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
 // the 16 tokens' largest |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the
 // keys; for the values 2^e joins the softmax's exponent: with M the running maximum of score + e,
@@ -28,7 +28,7 @@ using kv4::AttendParams;
 // again by warpgroup (168 + 168 + 104 + 72 = 4 x 128).
 constexpr int kKeys = 64, kRowWarps = 8, kCodeWarps = 4, kThreadsP = 512;
 constexpr int kRowRegs = 168, kCodeRegs = 104, kMmaRegs = 72;
-constexpr int kInfos = 4;       // steps whose exponents are kept: the code warps are at most two ahead of a row warp
+constexpr int kInfos = 8;       // steps whose exponents are kept: the code warps are at most four ahead of a row warp
 constexpr float kLazy = 8.0f;   // powers of two that P may exceed 1 by
 constexpr int kFit = 14;        // |K'|, |V'| < 2^14
 
@@ -46,17 +46,19 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 
 template <int D, int G>
 struct PromptCfg {
-    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 3;
+    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 4;
+    static constexpr int kRows = 128 * D * 2;       // Q' of a tile of rows
     static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
     static constexpr int kWords = 32 * (D / G);     // words of a tile, K's and V's
-    static constexpr int kSmem = 1024 + 4 * kOperand + kCodeWarps * (kRaw * kTile + kWords * 8) + 16;
-    // TMEM columns: S (P in its first half) and Q' of both tiles, then O
-    static constexpr int kS = 0, kQ = 128, kO = kQ + D, kCols = 512;
+    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + kCodeWarps * kRaw * (kTile + kWords * 8) + 16;
+    // TMEM columns: S of both tiles, two buffers each (P in a buffer's first half), then O
+    static constexpr int kS = 0, kO = 256, kCols = 512;
     static_assert(kO + 2 * D <= kCols, "TMEM");
 };
 
 struct PromptBars {
-    uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], info[kInfos], raw[kCodeWarps][3];
+    // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by warp and slot
+    uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], info[kInfos], raw[kCodeWarps][4];
 };
 
 // Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     constexpr int NG = D / G, NC = D / 8;  // groups and chunks of eight channels of a head vector
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
-    unsigned char *k_smem = smem, *v_smem = smem + 2 * Cfg::kOperand, *raw_smem = smem + 4 * Cfg::kOperand;
+    unsigned char *q_smem = smem, *k_smem = q_smem + 2 * Cfg::kRows, *v_smem = k_smem + 2 * Cfg::kOperand, *raw_smem = v_smem + 2 * Cfg::kOperand;
     __shared__ PromptBars bars;
     __shared__ TileInfo infos[kInfos][kCodeWarps];
     __shared__ uint32_t tmem_slot;
@@ -129,7 +131,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&bars.k_full[i], kCodeWarps), ptx::mbar_init(&bars.v_full[i], kCodeWarps);
             ptx::mbar_init(&bars.k_empty[i], 1), ptx::mbar_init(&bars.v_empty[i], 1);
-            ptx::mbar_init(&bars.s_full[i], 1), ptx::mbar_init(&bars.p_full[i], 4), ptx::mbar_init(&bars.o_full[i], 1);
+            for (int k = 0; k < 2; ++k) ptx::mbar_init(&bars.s_full[i][k], 1), ptx::mbar_init(&bars.p_full[i][k], 4), ptx::mbar_init(&bars.pv_done[i][k], 1);
+            ptx::mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], kCodeWarps);
         for (int w = 0; w < kCodeWarps; ++w)
@@ -181,24 +184,20 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
         const bool work = tile < tiles && steps > 0;
         if (work) {
+            const int r = (warp & 3) * 32 + lane;
+            unsigned char* to = q_smem + tile * Cfg::kRows + r * 128;
+#pragma unroll 4
+            for (int i = 0; i < NC; ++i) {
+                const uint4 w = there && finite ? __ldg(reinterpret_cast<const uint4*>(q) + i) : uint4{};
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                float h[8];
 #pragma unroll
-            for (int part = 0; part < D / 64; ++part) {
-                uint32_t r[32];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint4 w = there && finite ? __ldg(reinterpret_cast<const uint4*>(q) + part * 8 + i) : uint4{};
-                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-                    float h[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) h[2 * k] = __uint_as_float(u[k] << 16) * down, h[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) r[4 * i + k] = ptx::f16x2_pack(h[k], h[k + 4]);
-                }
-                umma::tmem_st_32x32(tmem + lanes + Cfg::kQ + tile * (D / 2) + part * 32, r);
+                for (int k = 0; k < 4; ++k) h[2 * k] = __uint_as_float(u[k] << 16) * down, h[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+                *reinterpret_cast<uint4*>(to + (i >> 3) * (128 * 128) + (((i & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(ptx::f16x2_pack(h[0], h[4]), ptx::f16x2_pack(h[1], h[5]), ptx::f16x2_pack(h[2], h[6]), ptx::f16x2_pack(h[3], h[7]));
             }
-            umma::tmem_st_wait();
         }
-        umma::fence_before_sync();
+        ptx::fence_proxy_async();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars.q_ready);
 
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         float top = -INFINITY, sum = 0.0f;
         uint32_t poison = 0;  // groups of channels in which this row sees a value that is no number
         bool alive = true;
-        const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 64, o_at = tmem + lanes + Cfg::kO + tile * D;
+        const uint32_t o_at = tmem + lanes + Cfg::kO + tile * D;
         for (int j = 0; work && j < steps; ++j) {
             if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.info[j % kInfos], (j / kInfos) & 1, p.status));
             const TileInfo* info = infos[j % kInfos];
@@ -228,7 +227,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         for (int k = 0; k < NG; ++k) poison |= (info[t].bad_v[k] >> i & 1) << k;
                     }
             }
-            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[tile], j & 1, p.status));
+            const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 128 + (j & 1) * 64;
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[tile][j & 1], (j >> 1) & 1, p.status));
             umma::fence_after_sync();
             uint32_t a0[32], a1[32];
             umma::tmem_ld_32x32(s_at, a0);
@@ -253,6 +253,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             if (__any_sync(kAll, most_here > top + kLazy)) {
                 const float now = fmaxf(top, most_here), keep = top == -INFINITY ? 0.0f : exp2f(top - now);
                 if (j > 0) {
+                    // O is the MMAs' until those of step j - 1 are done. Step j's wait for P, so this barrier cannot be a round
+                    // further; nor a round behind: S of step j - 1, which this row has had, came after the MMAs of step j - 3
+                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.pv_done[tile][(j - 1) & 1], ((j - 1) >> 1) & 1, p.status));
+                    umma::fence_after_sync();
 #pragma unroll 1
                     for (int at = 0; at < D; at += 32) {
                         uint32_t r[32];
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             umma::tmem_st_wait();
             umma::fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&bars.p_full[tile]);
+            if (lane == 0) ptx::mbar_arrive(&bars.p_full[tile][j & 1]);
         }
         if (work && alive) __all_sync(kAll, ptx::mbar_wait(&bars.o_full[tile], 0, p.status));
         umma::fence_after_sync();
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         // ---- 16 keys of every step a warp: codes and words to K' and V' -----------------------------------------------------
         const int w = warp - kRowWarps;
         unsigned char* raw = raw_smem + w * Cfg::kRaw * Cfg::kTile;
-        uint2* scales = reinterpret_cast<uint2*>(raw_smem + kCodeWarps * Cfg::kRaw * Cfg::kTile) + w * Cfg::kWords;  // (s, s), (m, m) of every word
+        uint2* scale_ring = reinterpret_cast<uint2*>(raw_smem + kCodeWarps * Cfg::kRaw * Cfg::kTile) + w * Cfg::kRaw * Cfg::kWords;  // (s, s), (m, m) of every word
         uint64_t* raw_full = bars.raw[w];
         const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
         const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
@@ -352,93 +356,99 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         for (int i = 0; i < Cfg::kRaw; ++i) fetch(i);
         uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
         bool alive = true;
-        int slot = 0;
         const int t = lane >> 1, h = lane & 1;                            // K: a lane has half of a key's row
         const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;      // V: run g of four keys of a block of eight
-        for (int j = 0; j < steps; ++j) {
-            const int stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
-            const bool here = got >> slot & 1;
-            if (here) {
-                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
-                raw_phase ^= 1u << slot;
-            }
-            const unsigned char* tile = raw + slot * Cfg::kTile;
-            // ---- the words, one or a few a lane (K's, then V's): their sizes, and what is not finite; 0 for a key no row sees
-            float s[NG], m[NG];
-            uint32_t k_size = 0, v_size = 0, odd = 0;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int at = lane + 32 * i, key = at % (16 * NG) / NG;
-                uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + at * 4);
-                if (!here || base + key < any_lo || base + key >= any_hi) x = 0;
-                if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
-                s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
-                const uint32_t size = __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f));
-                if (at < 16 * NG) k_size = max(k_size, size); else v_size = max(v_size, size);
-            }
-            const int k_exp = exponent_of(k_size), v_exp = exponent_of(v_size);
-            const float k_fit = power_of_two(kFit - k_exp), v_fit = power_of_two(kFit - v_exp);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const float f = lane + 32 * i < 16 * NG ? k_fit : v_fit;
-                scales[lane + 32 * i] = make_uint2(ptx::f16x2_pack(s[i] * f, s[i] * f), ptx::f16x2_pack(m[i] * f, m[i] * f));
-            }
-            const bool any_odd = __any_sync(kAll, odd != 0);
-            TileInfo& info = infos[j % kInfos][w];  // its place is free: the row warps are past step j - 4
-            if (lane == 0) {
-                info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
-                info.bad = any_odd;
-            }
-            if (any_odd) {
-                uint32_t bad_k = 0, bad_v[NG] = {};
+        // K' of step j, then V' of the step before: the MMAs are to have the next scores ready when a row warp is done
+        for (int j = 0; j <= steps; ++j) {
+            if (j < steps) {
+                const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
+                uint2* scales = scale_ring + slot * Cfg::kWords;
+                const bool here = got >> slot & 1;
+                if (here) {
+                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
+                    raw_phase ^= 1u << slot;
+                }
+                const unsigned char* tile = raw + slot * Cfg::kTile;
+                // ---- the words, one or a few a lane (K's, then V's): their sizes, and what is not finite; 0 for a key no row sees
+                float s[NG], m[NG];
+                uint32_t k_size = 0, v_size = 0, odd = 0;
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const int at = lane + 32 * i, key = at % (16 * NG) / NG;
-                    if (!(odd >> i & 1)) continue;
-                    if (at < 16 * NG) bad_k |= 1u << key;
-#pragma unroll
-                    for (int k = 0; k < NG; ++k)
-                        if (at >= 16 * NG && at % NG == k) bad_v[k] |= 1u << key;
+                    uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + at * 4);
+                    if (!here || base + key < any_lo || base + key >= any_hi) x = 0;
+                    if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
+                    s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
+                    const uint32_t size = __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f));
+                    if (at < 16 * NG) k_size = max(k_size, size); else v_size = max(v_size, size);
                 }
-                bad_k = __reduce_or_sync(kAll, bad_k);
-                if (lane == 0) info.bad_k = bad_k;
+                const int k_exp = exponent_of(k_size), v_exp = exponent_of(v_size);
+                const float k_fit = power_of_two(kFit - k_exp), v_fit = power_of_two(kFit - v_exp);
 #pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
-                    if (lane == 0) info.bad_v[k] = bad_v[k];
+                for (int i = 0; i < NG; ++i) {
+                    const float f = lane + 32 * i < 16 * NG ? k_fit : v_fit;
+                    scales[lane + 32 * i] = make_uint2(ptx::f16x2_pack(s[i] * f, s[i] * f), ptx::f16x2_pack(m[i] * f, m[i] * f));
                 }
-            }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);
-            // ---- K'
-            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
-            {
-                uint2 sm[NG];
+                const bool any_odd = __any_sync(kAll, odd != 0);
+                TileInfo& info = infos[j % kInfos][w];  // its place is free: V' of step j - 2 had its place, so the row warps are past step j - 4
+                if (lane == 0) {
+                    info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
+                    info.bad = any_odd;
+                }
+                if (any_odd) {
+                    uint32_t bad_k = 0, bad_v[NG] = {};
 #pragma unroll
-                for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
-                unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
+                    for (int i = 0; i < NG; ++i) {
+                        const int at = lane + 32 * i, key = at % (16 * NG) / NG;
+                        if (!(odd >> i & 1)) continue;
+                        if (at < 16 * NG) bad_k |= 1u << key;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
-                    const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
-                    uint32_t code[D / 32];
-                    if constexpr (D == 128) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(at);
-                        code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(at);
-                        code[0] = v.x, code[1] = v.y;
+                        for (int k = 0; k < NG; ++k)
+                            if (at >= 16 * NG && at % NG == k) bad_v[k] |= 1u << key;
                     }
+                    bad_k = __reduce_or_sync(kAll, bad_k);
+                    if (lane == 0) info.bad_k = bad_k;
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
-                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
+                    for (int k = 0; k < NG; ++k) {
+                        bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
+                        if (lane == 0) info.bad_v[k] = bad_v[k];
+                    }
                 }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);
+                // ---- K'
+                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
+                {
+                    uint2 sm[NG];
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
+                    unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
+                        const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
+                        uint32_t code[D / 32];
+                        if constexpr (D == 128) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(at);
+                            code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(at);
+                            code[0] = v.x, code[1] = v.y;
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
+                            *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
+                    }
+                }
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bars.k_full[stage]);
             }
-            ptx::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&bars.k_full[stage]);
             // ---- V'
-            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.v_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
-            {
+            if (j > 0) {
+                const int of = j - 1, slot = of % Cfg::kRaw, stage = of & 1;
+                const unsigned char* tile = raw + slot * Cfg::kTile;
+                const uint2* scales = scale_ring + slot * Cfg::kWords;
+                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.v_empty[stage], ((of >> 1) & 1) ^ 1, p.status));
                 unsigned char* to = v_smem + stage * Cfg::kOperand + (w * kv4::kTile + 8 * blk + 4 * th) * 128;
                 const unsigned char* at = tile + kv4::v_codes_at(D) + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
                 uint32_t code[4][D / 64];
@@ -462,58 +472,58 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + i * 128 + (((chunk & 7) ^ (4 * th + i)) << 4)) = values8(code[i][jw], s2, m2);
                     }
                 }
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&bars.v_full[stage]);
+                fetch(slot);
             }
-            ptx::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&bars.v_full[stage]);
-            fetch(slot);
-            if (++slot == Cfg::kRaw) slot = 0;
         }
     } else {
         registers_down<kMmaRegs>();
         if (warp == kRowWarps + kCodeWarps && steps > 0) {
-        // ---- the MMAs ----------------------------------------------------------------------------------------------------------
-        constexpr uint32_t s_desc = umma::instr_desc(128, kKeys, 0, 0), o_desc = umma::instr_desc_b_mn(128, D, 0, 0);
-        bool ok = __all_sync(kAll, ptx::mbar_wait(&bars.q_ready, 0, p.status));
-        auto scores = [&](int i, int stage) {
-            const uint64_t k0 = umma::smem_desc_k128(k_smem + stage * Cfg::kOperand);
+            // ---- the MMAs: the scores run two steps ahead of the values -----------------------------------------------------
+            constexpr uint32_t s_desc = umma::instr_desc(128, kKeys, 0, 0), o_desc = umma::instr_desc_b_mn(128, D, 0, 0);
+            auto scores = [&](int i, int j) {  // by the elected lane
+                const uint64_t q0 = umma::smem_desc_k128(q_smem + i * Cfg::kRows), k0 = umma::smem_desc_k128(k_smem + (j & 1) * Cfg::kOperand);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                umma::mma_f16_tmem_a(tmem + Cfg::kS + i * 64, tmem + Cfg::kQ + i * (D / 2) + 8 * k, umma::desc_advance(k0, (k / 4) * (kKeys * 128) + (k % 4) * 32), s_desc, k > 0);
-            umma::mma_commit(&bars.s_full[i]);
-        };
-        if (ok) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[0], 0, p.status));
-        umma::fence_after_sync();
-        if (ok && umma::elect_one()) {
-            for (int i = 0; i < tiles; ++i) scores(i, 0);
-            umma::mma_commit(&bars.k_empty[0]);
-        }
-        __syncwarp();
-        for (int j = 0; ok && j < steps; ++j) {
-            const int stage = j & 1, next = (j + 1) & 1;
-            ok = __all_sync(kAll, ptx::mbar_wait(&bars.v_full[stage], (j >> 1) & 1, p.status));
-            for (int i = 0; ok && i < tiles; ++i) {
-                ok = __all_sync(kAll, ptx::mbar_wait(&bars.p_full[i], j & 1, p.status));
-                if (ok && i == 0 && j + 1 < steps) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[next], ((j + 1) >> 1) & 1, p.status));
-                if (!ok) break;
+                for (int k = 0; k < D / 16; ++k)
+                    umma::mma_f16(tmem + Cfg::kS + i * 128 + (j & 1) * 64, umma::desc_advance(q0, (k / 4) * (128 * 128) + (k % 4) * 32),
+                                  umma::desc_advance(k0, (k / 4) * (kKeys * 128) + (k % 4) * 32), s_desc, k > 0);
+                umma::mma_commit(&bars.s_full[i][j & 1]);
+                if (i == tiles - 1) umma::mma_commit(&bars.k_empty[j & 1]);
+            };
+            bool ok = __all_sync(kAll, ptx::mbar_wait(&bars.q_ready, 0, p.status));
+            for (int j = 0; ok && j < min(steps, 2); ++j) {
+                ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[j], 0, p.status));
                 umma::fence_after_sync();
-                if (umma::elect_one()) {
-                    const uint64_t v0 = umma::smem_desc_mn128(v_smem + stage * Cfg::kOperand, kKeys * 128);
-#pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma::mma_f16_tmem_a(tmem + Cfg::kO + i * D, tmem + Cfg::kS + i * 64 + 8 * k, umma::desc_advance(v0, k * 2048), o_desc, j > 0 || k > 0);
-                    if (i == tiles - 1) umma::mma_commit(&bars.v_empty[stage]);
-                    if (j + 1 < steps) {
-                        scores(i, next);
-                        if (i == tiles - 1) umma::mma_commit(&bars.k_empty[next]);
-                    } else {
-                        umma::mma_commit(&bars.o_full[i]);
-                    }
-                }
+                if (ok && umma::elect_one())
+                    for (int i = 0; i < tiles; ++i) scores(i, j);
                 __syncwarp();
             }
+            for (int j = 0; ok && j < steps; ++j) {
+                const int stage = j & 1, round = (j >> 1) & 1;
+                ok = __all_sync(kAll, ptx::mbar_wait(&bars.v_full[stage], round, p.status));
+                for (int i = 0; ok && i < tiles; ++i) {
+                    ok = __all_sync(kAll, ptx::mbar_wait(&bars.p_full[i][stage], round, p.status));
+                    umma::fence_after_sync();
+                    if (ok && umma::elect_one()) {
+                        const uint64_t v0 = umma::smem_desc_mn128(v_smem + stage * Cfg::kOperand, kKeys * 128);
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            umma::mma_f16_tmem_a(tmem + Cfg::kO + i * D, tmem + Cfg::kS + i * 128 + stage * 64 + 8 * k, umma::desc_advance(v0, k * 2048), o_desc, j > 0 || k > 0);
+                        umma::mma_commit(j + 1 < steps ? &bars.pv_done[i][stage] : &bars.o_full[i]);
+                        if (i == tiles - 1) umma::mma_commit(&bars.v_empty[stage]);
+                    }
+                    __syncwarp();
+                    if (j + 2 < steps) {  // into the buffer whose P has just been taken: MMAs of a CTA run in their order
+                        if (ok && i == 0) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[stage], round ^ 1, p.status));
+                        umma::fence_after_sync();
+                        if (ok && umma::elect_one()) scores(i, j + 2);
+                        __syncwarp();
+                    }
+                }
+            }
         }
-    }
     }
     umma::fence_before_sync();
     __syncthreads();
