@@ -3,7 +3,7 @@
 // A CTA takes 256 rows (new tokens x query heads of one KV head of a sequence) in two tiles of 128, one row a TMEM lane, and
 // walks the keys 64 at a time:
 //     S [row][key] = Q' K'^T        P = 2^(S c + b)        O [row][channel] += P V'
-// with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Four warps turn codes
+// with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Eight warps turn codes
 // and words into K' and V': 16 tokens a warp, every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
 // the 16 tokens' largest |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the
 // keys; for the values 2^e joins the softmax's exponent: with M the running maximum of score + e,
@@ -24,19 +24,21 @@ namespace {
 
 using kv4::AttendParams;
 
-// Four warpgroups: two of row warps, one of code warps, one whose first warp issues the MMAs. The registers are dealt out
-// again by warpgroup (168 + 168 + 104 + 72 = 4 x 128).
-constexpr int kKeys = 64, kRowWarps = 8, kCodeWarps = 4, kThreadsP = 512;
-constexpr int kRowRegs = 168, kCodeRegs = 104, kMmaRegs = 72;
+// Five warpgroups: two of row warps, one that makes K', one that makes V', one whose first two warps issue the MMAs. The
+// registers are dealt out again by warpgroup: 2 x 144 + 2 x 72 + 48 = 5 x 96.
+constexpr int kKeys = 64, kRowWarps = 8, kKWarp = 8, kVWarp = 12, kMmaWarp = 16, kThreadsP = 640;
+constexpr int kRowRegs = 144, kCodeRegs = 72, kMmaRegs = 48;
 constexpr int kInfos = 8;       // steps whose exponents are kept: the code warps are at most four ahead of a row warp
 constexpr float kLazy = 8.0f;   // powers of two that P may exceed 1 by
 constexpr int kFit = 14;        // |K'|, |V'| < 2^14
 
-// What the code warps say of 16 keys.
+// What the code warps say of 16 keys: of the keys 2^(e - 14), and which are not finite; of the values e and 2^-e (negative if any
+// is not finite), and then which, by group.
 struct alignas(16) TileInfo {
-    float k_unit, v_exp, v_unit;   // 2^(e - 14) of the keys; e of the values, 2^-e
-    uint32_t bad;                  // whether any word is not finite
-    uint32_t bad_k, bad_v[4];      // then the keys, in K, and in V by group
+    float k_unit;
+    uint32_t bad_k;
+    float v_exp, v_unit;
+    uint32_t bad_v[4];
 };
 
 template <int N>
@@ -49,8 +51,9 @@ struct PromptCfg {
     static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 4;
     static constexpr int kRows = 128 * D * 2;       // Q' of a tile of rows
     static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
-    static constexpr int kWords = 32 * (D / G);     // words of a tile, K's and V's
-    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + kCodeWarps * kRaw * (kTile + kWords * 8) + 16;
+    static constexpr int kWords = 16 * (D / G);             // words of 16 keys, K's or V's
+    static constexpr int kHalf = kv4::kTile * D / 2 + kWords * 4;  // their codes and words
+    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + 8 * (kRaw * kHalf + kWords * 8) + 16;
     // TMEM columns: S of both tiles, two buffers each (P in a buffer's first half), then O
     static constexpr int kS = 0, kO = 256, kCols = 512;
     static_assert(kO + 2 * D <= kCols, "TMEM");
@@ -58,7 +61,7 @@ struct PromptCfg {
 
 struct PromptBars {
     // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by warp and slot
-    uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], info[kInfos], raw[kCodeWarps][4];
+    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw[8][4];
 };
 
 // Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
     unsigned char *q_smem = smem, *k_smem = q_smem + 2 * Cfg::kRows, *v_smem = k_smem + 2 * Cfg::kOperand, *raw_smem = v_smem + 2 * Cfg::kOperand;
     __shared__ PromptBars bars;
-    __shared__ TileInfo infos[kInfos][kCodeWarps];
+    __shared__ TileInfo infos[kInfos][4];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_block;
 
@@ -129,17 +132,16 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     if (threadIdx.x == 0) {
         ptx::mbar_init(&bars.q_ready, kRowWarps);
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&bars.k_full[i], kCodeWarps), ptx::mbar_init(&bars.v_full[i], kCodeWarps);
-            ptx::mbar_init(&bars.k_empty[i], 1), ptx::mbar_init(&bars.v_empty[i], 1);
-            for (int k = 0; k < 2; ++k) ptx::mbar_init(&bars.s_full[i][k], 1), ptx::mbar_init(&bars.p_full[i][k], 4), ptx::mbar_init(&bars.pv_done[i][k], 1);
-            ptx::mbar_init(&bars.o_full[i], 1);
+            ptx::mbar_init(&bars.k_full[i], 4), ptx::mbar_init(&bars.v_full[i], 4);
+            for (int k = 0; k < 2; ++k) ptx::mbar_init(&bars.s_full[i][k], 1), ptx::mbar_init(&bars.p_full[i][k], 4);
+            ptx::mbar_init(&bars.before_last[i], 1), ptx::mbar_init(&bars.o_full[i], 1);
         }
-        for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], kCodeWarps);
-        for (int w = 0; w < kCodeWarps; ++w)
+        for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], 8);
+        for (int w = 0; w < 8; ++w)
             for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw[w][i], 1);
         ptx::fence_mbar_init();
     }
-    if (warp == kRowWarps + kCodeWarps) umma::tmem_alloc(&tmem_slot, Cfg::kCols);
+    if (warp == kMmaWarp) umma::tmem_alloc(&tmem_slot, Cfg::kCols);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
@@ -214,17 +216,17 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const float4 of = *reinterpret_cast<const float4*>(&info[t]);
-                unit[t] = fmaxf(of.x * mult, 1.2e-38f), v_exp[t] = of.y, v_unit[t] = of.z;
-                bad |= __float_as_uint(of.w);
+                unit[t] = fmaxf(of.x * mult, 1.2e-38f), v_exp[t] = of.z, v_unit[t] = fabsf(of.w);
+                bad |= __float_as_uint(of.y) | __float_as_uint(of.w) >> 31;
             }
             const int base = key0 + j * kKeys;
             if (bad) {
                 for (int t = 0; t < 4; ++t)
-                    for (int i = 0; i < kv4::kTile && info[t].bad; ++i) {
+                    for (int i = 0; i < kv4::kTile; ++i) {
                         const int key = base + kv4::kTile * t + i;
                         if (key < lo || key >= hi) continue;
                         if (info[t].bad_k >> i & 1) poison = (1u << NG) - 1;
-                        for (int k = 0; k < NG; ++k) poison |= (info[t].bad_v[k] >> i & 1) << k;
+                        for (int k = 0; k < NG && info[t].v_unit < 0.0f; ++k) poison |= (info[t].bad_v[k] >> i & 1) << k;
                     }
             }
             const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 128 + (j & 1) * 64;
@@ -253,9 +255,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             if (__any_sync(kAll, most_here > top + kLazy)) {
                 const float now = fmaxf(top, most_here), keep = top == -INFINITY ? 0.0f : exp2f(top - now);
                 if (j > 0) {
-                    // O is the MMAs' until those of step j - 1 are done. Step j's wait for P, so this barrier cannot be a round
-                    // further; nor a round behind: S of step j - 1, which this row has had, came after the MMAs of step j - 3
-                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.pv_done[tile][(j - 1) & 1], ((j - 1) >> 1) & 1, p.status));
+                    // O is the MMAs' until those of step j - 1 are done: S of step j + 1 comes after them
+                    uint64_t* done = j + 1 < steps ? &bars.s_full[tile][(j + 1) & 1] : &bars.before_last[tile];
+                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(done, j + 1 < steps ? ((j + 1) >> 1) & 1 : 0, p.status));
                     umma::fence_after_sync();
 #pragma unroll 1
                     for (int at = 0; at < D; at += 32) {
@@ -323,13 +325,16 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                     }
             }
         }
-    } else if (warp < kRowWarps + kCodeWarps) {
+    } else if (warp < kMmaWarp) {
         registers_down<kCodeRegs>();
-        // ---- 16 keys of every step a warp: codes and words to K' and V' -----------------------------------------------------
-        const int w = warp - kRowWarps;
-        unsigned char* raw = raw_smem + w * Cfg::kRaw * Cfg::kTile;
-        uint2* scale_ring = reinterpret_cast<uint2*>(raw_smem + kCodeWarps * Cfg::kRaw * Cfg::kTile) + w * Cfg::kRaw * Cfg::kWords;  // (s, s), (m, m) of every word
-        uint64_t* raw_full = bars.raw[w];
+        // ---- 16 keys of every step a warp: K's or V's codes and words to K' or V' ------------------------------------------
+        const bool is_v = warp >= kVWarp;
+        const int w = warp & 3, ring_of = warp - kKWarp;
+        unsigned char* raw = raw_smem + ring_of * Cfg::kRaw * Cfg::kHalf;
+        uint2* scales = reinterpret_cast<uint2*>(raw_smem + 8 * Cfg::kRaw * Cfg::kHalf) + ring_of * Cfg::kWords;  // (s, s), (m, m) of every word
+        uint64_t* raw_full = bars.raw[ring_of];
+        constexpr int kCodes = kv4::kTile * D / 2;
+        const int codes_at = is_v ? kv4::v_codes_at(D) : 0, words_at = is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D);
         const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
         const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
         const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
@@ -343,8 +348,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             if (next_page >= 0 && next_page < p.pool.pages) {
                 got |= 1u << slot;
                 if (lane == 0) {
-                    ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kTile);
-                    ptx::bulk_g2s(raw + slot * Cfg::kTile, pool + next_page * page_bytes + next_in * Cfg::kTile, Cfg::kTile, &raw_full[slot]);
+                    const unsigned char* from = pool + next_page * page_bytes + next_in * Cfg::kTile;
+                    ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kHalf);
+                    ptx::bulk_g2s(raw + slot * Cfg::kHalf, from + codes_at, kCodes, &raw_full[slot]);
+                    ptx::bulk_g2s(raw + slot * Cfg::kHalf + kCodes, from + words_at, Cfg::kWords * 4, &raw_full[slot]);
                 }
             } else if (lane == 0) {
                 atomicCAS(p.status, 0, SPK_BAD_INDEX);
@@ -356,101 +363,89 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         for (int i = 0; i < Cfg::kRaw; ++i) fetch(i);
         uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
         bool alive = true;
-        const int t = lane >> 1, h = lane & 1;                            // K: a lane has half of a key's row
-        const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;      // V: run g of four keys of a block of eight
-        // K' of step j, then V' of the step before: the MMAs are to have the next scores ready when a row warp is done
-        for (int j = 0; j <= steps; ++j) {
-            if (j < steps) {
-                const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
-                uint2* scales = scale_ring + slot * Cfg::kWords;
-                const bool here = got >> slot & 1;
-                if (here) {
-                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
-                    raw_phase ^= 1u << slot;
-                }
-                const unsigned char* tile = raw + slot * Cfg::kTile;
-                // ---- the words, one or a few a lane (K's, then V's): their sizes, and what is not finite; 0 for a key no row sees
-                float s[NG], m[NG];
-                uint32_t k_size = 0, v_size = 0, odd = 0;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const int at = lane + 32 * i, key = at % (16 * NG) / NG;
-                    uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kv4::k_words_at(D) + at * 4);
-                    if (!here || base + key < any_lo || base + key >= any_hi) x = 0;
-                    if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
-                    s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
-                    const uint32_t size = __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f));
-                    if (at < 16 * NG) k_size = max(k_size, size); else v_size = max(v_size, size);
-                }
-                const int k_exp = exponent_of(k_size), v_exp = exponent_of(v_size);
-                const float k_fit = power_of_two(kFit - k_exp), v_fit = power_of_two(kFit - v_exp);
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const float f = lane + 32 * i < 16 * NG ? k_fit : v_fit;
-                    scales[lane + 32 * i] = make_uint2(ptx::f16x2_pack(s[i] * f, s[i] * f), ptx::f16x2_pack(m[i] * f, m[i] * f));
-                }
-                const bool any_odd = __any_sync(kAll, odd != 0);
-                TileInfo& info = infos[j % kInfos][w];  // its place is free: V' of step j - 2 had its place, so the row warps are past step j - 4
-                if (lane == 0) {
-                    info.k_unit = power_of_two(k_exp - kFit), info.v_exp = static_cast<float>(v_exp), info.v_unit = power_of_two(-v_exp);
-                    info.bad = any_odd;
-                }
-                if (any_odd) {
-                    uint32_t bad_k = 0, bad_v[NG] = {};
-#pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        const int at = lane + 32 * i, key = at % (16 * NG) / NG;
-                        if (!(odd >> i & 1)) continue;
-                        if (at < 16 * NG) bad_k |= 1u << key;
-#pragma unroll
-                        for (int k = 0; k < NG; ++k)
-                            if (at >= 16 * NG && at % NG == k) bad_v[k] |= 1u << key;
-                    }
-                    bad_k = __reduce_or_sync(kAll, bad_k);
-                    if (lane == 0) info.bad_k = bad_k;
-#pragma unroll
-                    for (int k = 0; k < NG; ++k) {
-                        bad_v[k] = __reduce_or_sync(kAll, bad_v[k]);
-                        if (lane == 0) info.bad_v[k] = bad_v[k];
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);
-                // ---- K'
-                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.k_empty[stage], ((j >> 1) & 1) ^ 1, p.status));
-                {
-                    uint2 sm[NG];
-#pragma unroll
-                    for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
-                    unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
-                        const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
-                        uint32_t code[D / 32];
-                        if constexpr (D == 128) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(at);
-                            code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(at);
-                            code[0] = v.x, code[1] = v.y;
-                        }
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
-                            *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
-                    }
-                }
-                ptx::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&bars.k_full[stage]);
+        for (int j = 0; j < steps; ++j) {
+            const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
+            const bool here = got >> slot & 1;
+            if (here) {
+                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
+                raw_phase ^= 1u << slot;
             }
-            // ---- V'
-            if (j > 0) {
-                const int of = j - 1, slot = of % Cfg::kRaw, stage = of & 1;
-                const unsigned char* tile = raw + slot * Cfg::kTile;
-                const uint2* scales = scale_ring + slot * Cfg::kWords;
-                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.v_empty[stage], ((of >> 1) & 1) ^ 1, p.status));
+            const unsigned char* tile = raw + slot * Cfg::kHalf;
+            // ---- the words, one or a few a lane: their size, and what is not finite; 0 for a key that no row sees
+            constexpr int kPerLane = (Cfg::kWords + 31) / 32;
+            float s[kPerLane], m[kPerLane];
+            uint32_t size = 0, odd = 0;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const int at = (lane + 32 * i) % Cfg::kWords, key = base + at / NG;  // one group: the upper lanes repeat the lower
+                uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kCodes + at * 4);
+                if (!here || key < any_lo || key >= any_hi) x = 0;
+                if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
+                s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
+                size = max(size, __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f)));
+            }
+            const int e = exponent_of(size);
+            const float fit = power_of_two(kFit - e);
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) scales[(lane + 32 * i) % Cfg::kWords] = make_uint2(ptx::f16x2_pack(s[i] * fit, s[i] * fit), ptx::f16x2_pack(m[i] * fit, m[i] * fit));
+            // the row warps are past step j - 8, whose place this was: S of the step before the last but one came after their P
+            TileInfo& info = infos[j % kInfos][w];
+            uint32_t bad[NG] = {};
+            if (__any_sync(kAll, odd != 0)) {
+#pragma unroll
+                for (int i = 0; i < kPerLane; ++i) {
+                    const int at = (lane + 32 * i) % Cfg::kWords;
+#pragma unroll
+                    for (int k = 0; k < NG; ++k)
+                        if ((odd >> i & 1) && at % NG == k) bad[k] |= 1u << (at / NG);
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k) bad[k] = __reduce_or_sync(kAll, bad[k]);
+            }
+            if (lane == 0) {
+                uint32_t all = 0;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) all |= bad[k];
+                if (is_v) {
+                    info.v_exp = static_cast<float>(e), info.v_unit = all ? -power_of_two(-e) : power_of_two(-e);
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) info.bad_v[k] = bad[k];
+                } else {
+                    info.k_unit = power_of_two(e - kFit), info.bad_k = all;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&bars.info[j % kInfos]);
+            // ---- K's place is free once S of step j - 2 is there; V's once S of the step itself is, whose MMAs follow those on the
+            // values of step j - 2
+            const int after = is_v ? j : j - 2;
+            for (int i = 0; i < tiles && after >= 0; ++i)
+                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[i][after & 1], (after >> 1) & 1, p.status));
+            if (!is_v) {
+                const int t = lane >> 1, h = lane & 1;  // a lane has half of a key's row
+                uint2 sm[NG];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
+                unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
+                    const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
+                    uint32_t code[D / 32];
+                    if constexpr (D == 128) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(at);
+                        code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(at);
+                        code[0] = v.x, code[1] = v.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
+                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
+                }
+            } else {
+                const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;  // run g of four keys of a block of eight
                 unsigned char* to = v_smem + stage * Cfg::kOperand + (w * kv4::kTile + 8 * blk + 4 * th) * 128;
-                const unsigned char* at = tile + kv4::v_codes_at(D) + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
+                const unsigned char* at = tile + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
                 uint32_t code[4][D / 64];
                 if constexpr (D == 128) {
                     const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 16);
@@ -464,7 +459,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 for (int i = 0; i < 4; ++i) {
                     uint2 sm[NG];
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) sm[k] = scales[16 * NG + (8 * blk + 4 * th + i) * NG + k];
+                    for (int k = 0; k < NG; ++k) sm[k] = scales[(8 * blk + 4 * th + i) * NG + k];
 #pragma unroll
                     for (int jw = 0; jw < D / 64; ++jw) {  // units 2 jw (low halves) and 2 jw + 1 (high)
                         const int ka = 64 * jw / G, kb = (64 * jw + 32) / G, chunk = D / 64 * g + jw;
@@ -472,62 +467,56 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + i * 128 + (((chunk & 7) ^ (4 * th + i)) << 4)) = values8(code[i][jw], s2, m2);
                     }
                 }
-                ptx::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&bars.v_full[stage]);
-                fetch(slot);
             }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]);
+            fetch(slot);
         }
     } else {
         registers_down<kMmaRegs>();
-        if (warp == kRowWarps + kCodeWarps && steps > 0) {
-            // ---- the MMAs: the scores run two steps ahead of the values -----------------------------------------------------
+        const int i = warp - kMmaWarp;
+        if (i < tiles && steps > 0) {
+            // ---- the MMAs of a tile of rows, a warp for each (a warp's waits and commits alone take longer than a step's MMAs). The
+            // scores run two steps ahead of the values, into the buffer whose P the values have just taken: the MMAs of a
+            // thread run in their order, so one commit a step tells of both
             constexpr uint32_t s_desc = umma::instr_desc(128, kKeys, 0, 0), o_desc = umma::instr_desc_b_mn(128, D, 0, 0);
-            auto scores = [&](int i, int j) {  // by the elected lane
-                const uint64_t q0 = umma::smem_desc_k128(q_smem + i * Cfg::kRows), k0 = umma::smem_desc_k128(k_smem + (j & 1) * Cfg::kOperand);
+            const uint64_t q0 = umma::smem_desc_k128(q_smem + i * Cfg::kRows), k0 = umma::smem_desc_k128(k_smem), v0 = umma::smem_desc_mn128(v_smem, kKeys * 128);
+            const uint32_t s0 = tmem + Cfg::kS + i * 128, o0 = tmem + Cfg::kO + i * D;
+            auto scores = [&](int buffer) {  // by the elected lane
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    umma::mma_f16(tmem + Cfg::kS + i * 128 + (j & 1) * 64, umma::desc_advance(q0, (k / 4) * (128 * 128) + (k % 4) * 32),
-                                  umma::desc_advance(k0, (k / 4) * (kKeys * 128) + (k % 4) * 32), s_desc, k > 0);
-                umma::mma_commit(&bars.s_full[i][j & 1]);
-                if (i == tiles - 1) umma::mma_commit(&bars.k_empty[j & 1]);
+                    umma::mma_f16(s0 + buffer * 64, umma::desc_advance(q0, (k / 4) * (128 * 128) + (k % 4) * 32),
+                                  umma::desc_advance(k0, buffer * Cfg::kOperand + (k / 4) * (kKeys * 128) + (k % 4) * 32), s_desc, k > 0);
+                umma::mma_commit(&bars.s_full[i][buffer]);
             };
             bool ok = __all_sync(kAll, ptx::mbar_wait(&bars.q_ready, 0, p.status));
             for (int j = 0; ok && j < min(steps, 2); ++j) {
                 ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[j], 0, p.status));
                 umma::fence_after_sync();
-                if (ok && umma::elect_one())
-                    for (int i = 0; i < tiles; ++i) scores(i, j);
+                if (ok && umma::elect_one()) scores(j);
                 __syncwarp();
             }
             for (int j = 0; ok && j < steps; ++j) {
                 const int stage = j & 1, round = (j >> 1) & 1;
                 ok = __all_sync(kAll, ptx::mbar_wait(&bars.v_full[stage], round, p.status));
-                for (int i = 0; ok && i < tiles; ++i) {
-                    ok = __all_sync(kAll, ptx::mbar_wait(&bars.p_full[i][stage], round, p.status));
-                    umma::fence_after_sync();
-                    if (ok && umma::elect_one()) {
-                        const uint64_t v0 = umma::smem_desc_mn128(v_smem + stage * Cfg::kOperand, kKeys * 128);
+                if (ok && j + 2 < steps) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[stage], round ^ 1, p.status));
+                if (ok) ok = __all_sync(kAll, ptx::mbar_wait(&bars.p_full[i][stage], round, p.status));
+                umma::fence_after_sync();
+                if (ok && umma::elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            umma::mma_f16_tmem_a(tmem + Cfg::kO + i * D, tmem + Cfg::kS + i * 128 + stage * 64 + 8 * k, umma::desc_advance(v0, k * 2048), o_desc, j > 0 || k > 0);
-                        umma::mma_commit(j + 1 < steps ? &bars.pv_done[i][stage] : &bars.o_full[i]);
-                        if (i == tiles - 1) umma::mma_commit(&bars.v_empty[stage]);
-                    }
-                    __syncwarp();
-                    if (j + 2 < steps) {  // into the buffer whose P has just been taken: MMAs of a CTA run in their order
-                        if (ok && i == 0) ok = __all_sync(kAll, ptx::mbar_wait(&bars.k_full[stage], round ^ 1, p.status));
-                        umma::fence_after_sync();
-                        if (ok && umma::elect_one()) scores(i, j + 2);
-                        __syncwarp();
-                    }
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma::mma_f16_tmem_a(o0, s0 + stage * 64 + 8 * k, umma::desc_advance(v0, stage * Cfg::kOperand + k * 2048), o_desc, j > 0 || k > 0);
+                    if (j + 2 < steps) scores(stage);
+                    else umma::mma_commit(j + 1 < steps ? &bars.before_last[i] : &bars.o_full[i]);
                 }
+                __syncwarp();
             }
         }
     }
     umma::fence_before_sync();
     __syncthreads();
-    if (warp == kRowWarps + kCodeWarps) umma::tmem_dealloc(tmem, Cfg::kCols);
+    if (warp == kMmaWarp) umma::tmem_dealloc(tmem, Cfg::kCols);
 }
 
 template <int D, int G>
