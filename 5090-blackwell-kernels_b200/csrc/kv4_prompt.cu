@@ -4,12 +4,12 @@
 // walks the keys 64 at a time:
 //     S [row][key] = Q' K'^T        P = 2^(S c + b)        O [row][channel] += P V'
 // with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Eight warps turn codes
-// and words into K' and V': 16 tokens a warp, every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
+// and words into K' and V', every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
 // the 16 tokens' largest |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the
 // keys; for the values 2^e joins the softmax's exponent: with M the running maximum of score + e,
-//     P = 2^(score + e - M) <= 2^8,      sum += P 2^-e,      out = O / sum,
-// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread; a maximum that grows by less than 2^8 is
-// left alone, so O (in TMEM) is rarely touched between the MMAs. While one tile's row warps work on S the tensor cores
+//     P = 2^(score + e - M),      sum += P 2^-e,      out = O / sum,
+// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread; M is the maximum of a row's first keys and moves
+// only when weights would come near fp16's end, so O (in TMEM) is rarely touched between the MMAs and the maximum rarely looked for. While one tile's row warps work on S the tensor cores
 // have the other tile.
 // K' rows are keys, 128 bytes = 64 channels wide (the order of the channels inside eights is the codes' own; Q' is
 // stored in the same order); V' rows are keys too, and the MMA reads them MN-major; the order of its columns is the codes',
@@ -29,7 +29,7 @@ using kv4::AttendParams;
 constexpr int kKeys = 64, kRowWarps = 8, kKWarp = 8, kVWarp = 12, kMmaWarp = 16, kThreadsP = 640;
 constexpr int kRowRegs = 144, kCodeRegs = 72, kMmaRegs = 48;
 constexpr int kInfos = 8;       // steps whose exponents are kept: the code warps are at most four ahead of a row warp
-constexpr float kLazy = 8.0f;   // powers of two that P may exceed 1 by
+constexpr float kMost = 32768.0f;  // what 16 weights may add up to before the maximum moves: then none overflows fp16
 constexpr int kFit = 14;        // |K'|, |V'| < 2^14
 
 // What the code warps say of 16 keys: of the keys 2^(e - 14), and which are not finite; of the values e and 2^-e (negative if any
@@ -48,12 +48,12 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 
 template <int D, int G>
 struct PromptCfg {
-    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 4;
+    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 3;
     static constexpr int kRows = 128 * D * 2;       // Q' of a tile of rows
     static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
     static constexpr int kWords = 16 * (D / G);             // words of 16 keys, K's or V's
     static constexpr int kHalf = kv4::kTile * D / 2 + kWords * 4;  // their codes and words
-    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + 8 * (kRaw * kHalf + kWords * 8) + 16;
+    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + 16 * (kRaw * kHalf + kWords * 8) + 16;
     // TMEM columns: S of both tiles, two buffers each (P in a buffer's first half), then O
     static constexpr int kS = 0, kO = 256, kCols = 512;
     static_assert(kO + 2 * D <= kCols, "TMEM");
@@ -61,7 +61,7 @@ struct PromptCfg {
 
 struct PromptBars {
     // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by warp and slot
-    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw[8][4];
+    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw[8][3];
 };
 
 // Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     if (threadIdx.x == 0) {
         ptx::mbar_init(&bars.q_ready, kRowWarps);
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&bars.k_full[i], 4), ptx::mbar_init(&bars.v_full[i], 4);
+            ptx::mbar_init(&bars.k_full[i], 2), ptx::mbar_init(&bars.v_full[i], 2);
             for (int k = 0; k < 2; ++k) ptx::mbar_init(&bars.s_full[i][k], 1), ptx::mbar_init(&bars.p_full[i][k], 4);
             ptx::mbar_init(&bars.before_last[i], 1), ptx::mbar_init(&bars.o_full[i], 1);
         }
-        for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], 8);
+        for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], 4);
         for (int w = 0; w < 8; ++w)
             for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw[w][i], 1);
         ptx::fence_mbar_init();
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         if (lane == 0) ptx::mbar_arrive(&bars.q_ready);
 
         const int all_hi = __reduce_min_sync(kAll, there ? hi : INT32_MAX), all_lo = __reduce_max_sync(kAll, there ? lo : 0);
-        float top = -INFINITY, sum = 0.0f;
+        float top = hi > lo ? -INFINITY : 0.0f, sum = 0.0f;
         uint32_t poison = 0;  // groups of channels in which this row sees a value that is no number
         bool alive = true;
         const uint32_t o_at = tmem + lanes + Cfg::kO + tile * D;
@@ -244,15 +244,36 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 for (int i = 0; i < 64; ++i)
                     if (base + i < lo || base + i >= hi) x[i] = -INFINITY;
             }
-            float most_here = -INFINITY;
+            uint32_t pr[32];
+            float part[4];
+            // the weights under the present maximum, and their sums by 16 keys
+            auto weights = [&]() {
+                const float shift = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float m = x[16 * t];
+                for (int t = 0; t < 4; ++t) {
+                    const float2 by = make_float2(unit[t], unit[t]), add = make_float2(v_exp[t] - shift, v_exp[t] - shift);
+                    float2 all = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
-                most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
-            }
-            if (__any_sync(kAll, most_here > top + kLazy)) {
+                    for (int i = 0; i < 16; i += 2) {
+                        float2 e = ptx::fma2(make_float2(x[16 * t + i], x[16 * t + i + 1]), by, add);
+                        e.x = ptx::exp2_fast(e.x), e.y = ptx::exp2_fast(e.y);
+                        all = ptx::add2(all, e);
+                        pr[8 * t + i / 2] = ptx::f16x2_pack(e.x, e.y);
+                    }
+                    part[t] = all.x + all.y;
+                }
+            };
+            weights();
+            const bool over = !(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) <= kMost);
+            if (__any_sync(kAll, over || top == -INFINITY)) {  // a row's first keys, or much larger scores than it has had
+                float most_here = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    float m = x[16 * t];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
+                    most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
+                }
                 const float now = fmaxf(top, most_here), keep = top == -INFINITY ? 0.0f : exp2f(top - now);
                 if (j > 0) {
                     // O is the MMAs' until those of step j - 1 are done: S of step j + 1 comes after them
@@ -270,21 +291,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                     }
                 }
                 sum *= keep, top = now;
+                weights();
             }
-            uint32_t pr[32];
-            const float shift = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float add = v_exp[t] - shift;
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float u = ptx::exp2_fast(fmaf(x[16 * t + i], unit[t], add)), v = ptx::exp2_fast(fmaf(x[16 * t + i + 1], unit[t], add));
-                    part += u + v;
-                    pr[8 * t + i / 2] = ptx::f16x2_pack(u, v);
-                }
-                sum = fmaf(part, v_unit[t], sum);
-            }
+            for (int t = 0; t < 4; ++t) sum = fmaf(part[t], v_unit[t], sum);
             umma::tmem_st_32x32(s_at, pr);
             umma::tmem_st_wait();
             umma::fence_before_sync();
@@ -327,91 +337,111 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         }
     } else if (warp < kMmaWarp) {
         registers_down<kCodeRegs>();
-        // ---- 16 keys of every step a warp: K's or V's codes and words to K' or V' ------------------------------------------
+        // ---- 32 keys of every other step a warp: K's or V's codes and words to K' or V'. Two tiles at once and a step's time
+        // for each: a warp alone spends most of its time on latencies -----------------------------------------------------------
         const bool is_v = warp >= kVWarp;
-        const int w = warp & 3, ring_of = warp - kKWarp;
-        unsigned char* raw = raw_smem + ring_of * Cfg::kRaw * Cfg::kHalf;
-        uint2* scales = reinterpret_cast<uint2*>(raw_smem + 8 * Cfg::kRaw * Cfg::kHalf) + ring_of * Cfg::kWords;  // (s, s), (m, m) of every word
+        const int w = warp & 1, ring_of = warp - kKWarp;  // keys 32 w .. + 31 of the steps of parity warp / 2 % 2
+        unsigned char* raw = raw_smem + ring_of * Cfg::kRaw * 2 * Cfg::kHalf;
+        uint2* scales = reinterpret_cast<uint2*>(raw_smem + 8 * Cfg::kRaw * 2 * Cfg::kHalf) + ring_of * 2 * Cfg::kWords;  // (s, s), (m, m) of every word
         uint64_t* raw_full = bars.raw[ring_of];
         constexpr int kCodes = kv4::kTile * D / 2;
         const int codes_at = is_v ? kv4::v_codes_at(D) : 0, words_at = is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D);
         const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
         const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
         const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
-        // the tile that is fetched next: its first key, its place in the table, its page's number (read a step early)
-        int next_key = key0 + w * kv4::kTile, next_at = next_key / kv4::kTile / tiles_per_page, next_in = next_key / kv4::kTile % tiles_per_page, next_page = -1;
-        if (next_key < any_hi) next_page = __ldg(table + next_at);
-        uint32_t got = 0;  // slots of the ring that hold a tile
+        // the two tiles that are fetched next: their first keys, places in the table, pages' numbers (read a visit early)
+        int next_key[2], next_at[2], next_in[2], next_page[2] = {-1, -1};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            next_key[u] = key0 + (warp >> 1 & 1) * kKeys + (2 * w + u) * kv4::kTile;
+            next_at[u] = next_key[u] / kv4::kTile / tiles_per_page, next_in[u] = next_key[u] / kv4::kTile % tiles_per_page;
+            if (next_key[u] < any_hi) next_page[u] = __ldg(table + next_at[u]);
+        }
+        uint32_t got = 0;  // tiles of the ring that are there: bits 2 slot and 2 slot + 1
         auto fetch = [&](int slot) {
-            got &= ~(1u << slot);
-            if (next_key >= any_hi) return;
-            if (next_page >= 0 && next_page < p.pool.pages) {
-                got |= 1u << slot;
-                if (lane == 0) {
-                    const unsigned char* from = pool + next_page * page_bytes + next_in * Cfg::kTile;
-                    ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kHalf);
-                    ptx::bulk_g2s(raw + slot * Cfg::kHalf, from + codes_at, kCodes, &raw_full[slot]);
-                    ptx::bulk_g2s(raw + slot * Cfg::kHalf + kCodes, from + words_at, Cfg::kWords * 4, &raw_full[slot]);
-                }
-            } else if (lane == 0) {
-                atomicCAS(p.status, 0, SPK_BAD_INDEX);
+            got &= ~(3u << 2 * slot);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (next_key[u] >= any_hi) continue;
+                if (next_page[u] >= 0 && next_page[u] < p.pool.pages) got |= 1u << (2 * slot + u);
+                else if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
             }
-            next_key += kKeys, next_in += kKeys / kv4::kTile;
-            while (next_in >= tiles_per_page) next_in -= tiles_per_page, ++next_at;
-            if (next_key < any_hi) next_page = __ldg(table + next_at);
+            const uint32_t mine = got >> 2 * slot & 3u;
+            if (mine != 0 && lane == 0) {
+                ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kHalf * ((mine & 1) + (mine >> 1)));
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (mine >> u & 1) {
+                        const unsigned char* from = pool + next_page[u] * page_bytes + next_in[u] * Cfg::kTile;
+                        unsigned char* to = raw + (2 * slot + u) * Cfg::kHalf;
+                        ptx::bulk_g2s(to, from + codes_at, kCodes, &raw_full[slot]);
+                        ptx::bulk_g2s(to + kCodes, from + words_at, Cfg::kWords * 4, &raw_full[slot]);
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (next_key[u] >= any_hi) continue;
+                next_key[u] += 2 * kKeys, next_in[u] += 2 * kKeys / kv4::kTile;
+                while (next_in[u] >= tiles_per_page) next_in[u] -= tiles_per_page, ++next_at[u];
+                if (next_key[u] < any_hi) next_page[u] = __ldg(table + next_at[u]);
+            }
         };
         for (int i = 0; i < Cfg::kRaw; ++i) fetch(i);
         uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
         bool alive = true;
-        for (int j = 0; j < steps; ++j) {
-            const int slot = j % Cfg::kRaw, stage = j & 1, base = key0 + j * kKeys + w * kv4::kTile;
-            const bool here = got >> slot & 1;
+        int slot = 0;
+        for (int j = warp >> 1 & 1; j < steps; j += 2) {
+            const int stage = j & 1, base0 = key0 + j * kKeys + 2 * w * kv4::kTile;
+            const uint32_t here = got >> 2 * slot & 3u;
             if (here) {
                 if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
                 raw_phase ^= 1u << slot;
             }
-            const unsigned char* tile = raw + slot * Cfg::kHalf;
+            const unsigned char* tiles_at = raw + 2 * slot * Cfg::kHalf;
             // ---- the words, one or a few a lane: their size, and what is not finite; 0 for a key that no row sees
             constexpr int kPerLane = (Cfg::kWords + 31) / 32;
-            float s[kPerLane], m[kPerLane];
-            uint32_t size = 0, odd = 0;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-                const int at = (lane + 32 * i) % Cfg::kWords, key = base + at / NG;  // one group: the upper lanes repeat the lower
-                uint32_t x = *reinterpret_cast<const uint32_t*>(tile + kCodes + at * 4);
-                if (!here || key < any_lo || key >= any_hi) x = 0;
-                if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
-                s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
-                size = max(size, __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f)));
-            }
-            const int e = exponent_of(size);
-            const float fit = power_of_two(kFit - e);
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) scales[(lane + 32 * i) % Cfg::kWords] = make_uint2(ptx::f16x2_pack(s[i] * fit, s[i] * fit), ptx::f16x2_pack(m[i] * fit, m[i] * fit));
-            // the row warps are past step j - 8, whose place this was: S of the step before the last but one came after their P
-            TileInfo& info = infos[j % kInfos][w];
-            uint32_t bad[NG] = {};
-            if (__any_sync(kAll, odd != 0)) {
+            for (int u = 0; u < 2; ++u) {
+                float s[kPerLane], m[kPerLane];
+                uint32_t size = 0, odd = 0;
 #pragma unroll
                 for (int i = 0; i < kPerLane; ++i) {
-                    const int at = (lane + 32 * i) % Cfg::kWords;
-#pragma unroll
-                    for (int k = 0; k < NG; ++k)
-                        if ((odd >> i & 1) && at % NG == k) bad[k] |= 1u << (at / NG);
+                    const int at = (lane + 32 * i) % Cfg::kWords, key = base0 + u * kv4::kTile + at / NG;  // one group: the upper lanes repeat the lower
+                    uint32_t x = *reinterpret_cast<const uint32_t*>(tiles_at + u * Cfg::kHalf + kCodes + at * 4);
+                    if (!(here >> u & 1) || key < any_lo || key >= any_hi) x = 0;
+                    if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
+                    s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
+                    size = max(size, __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f)));
                 }
+                const int e = exponent_of(size);
+                const float fit = power_of_two(kFit - e);
 #pragma unroll
-                for (int k = 0; k < NG; ++k) bad[k] = __reduce_or_sync(kAll, bad[k]);
-            }
-            if (lane == 0) {
-                uint32_t all = 0;
+                for (int i = 0; i < kPerLane; ++i)
+                    scales[u * Cfg::kWords + (lane + 32 * i) % Cfg::kWords] = make_uint2(ptx::f16x2_pack(s[i] * fit, s[i] * fit), ptx::f16x2_pack(m[i] * fit, m[i] * fit));
+                TileInfo& info = infos[j % kInfos][2 * w + u];  // its place is free: the row warps are far past step j - 8
+                uint32_t bad[NG] = {};
+                if (__any_sync(kAll, odd != 0)) {
 #pragma unroll
-                for (int k = 0; k < NG; ++k) all |= bad[k];
-                if (is_v) {
-                    info.v_exp = static_cast<float>(e), info.v_unit = all ? -power_of_two(-e) : power_of_two(-e);
+                    for (int i = 0; i < kPerLane; ++i) {
+                        const int at = (lane + 32 * i) % Cfg::kWords;
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) info.bad_v[k] = bad[k];
-                } else {
-                    info.k_unit = power_of_two(e - kFit), info.bad_k = all;
+                        for (int k = 0; k < NG; ++k)
+                            if ((odd >> i & 1) && at % NG == k) bad[k] |= 1u << (at / NG);
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) bad[k] = __reduce_or_sync(kAll, bad[k]);
+                }
+                if (lane == 0) {
+                    uint32_t all = 0;
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) all |= bad[k];
+                    if (is_v) {
+                        info.v_exp = static_cast<float>(e), info.v_unit = all ? -power_of_two(-e) : power_of_two(-e);
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) info.bad_v[k] = bad[k];
+                    } else {
+                        info.k_unit = power_of_two(e - kFit), info.bad_k = all;
+                    }
                 }
             }
             __syncwarp();
@@ -423,48 +453,55 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[i][after & 1], (after >> 1) & 1, p.status));
             if (!is_v) {
                 const int t = lane >> 1, h = lane & 1;  // a lane has half of a key's row
-                uint2 sm[NG];
 #pragma unroll
-                for (int k = 0; k < NG; ++k) sm[k] = scales[t * NG + k];
-                unsigned char* to = k_smem + stage * Cfg::kOperand + (w * kv4::kTile + t) * 128;
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned char* tile = tiles_at + u * Cfg::kHalf;
+                    uint2 sm[NG];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
-                    const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
-                    uint32_t code[D / 32];
-                    if constexpr (D == 128) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(at);
-                        code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(at);
-                        code[0] = v.x, code[1] = v.y;
+                    for (int k = 0; k < NG; ++k) sm[k] = scales[u * Cfg::kWords + t * NG + k];
+                    unsigned char* to = k_smem + stage * Cfg::kOperand + ((2 * w + u) * kv4::kTile + t) * 128;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {  // runs 2 h and 2 h + 1
+                        const unsigned char* at = tile + t * (D / 2) + (2 * h + r) * (D / 8);
+                        uint32_t code[D / 32];
+                        if constexpr (D == 128) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(at);
+                            code[0] = v.x, code[1] = v.y, code[D / 32 - 2] = v.z, code[D / 32 - 1] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(at);
+                            code[0] = v.x, code[1] = v.y;
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
+                            *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
                     }
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i)  // channels 8 chunk .. + 7, chunk = 4 i + 2 h + r
-                        *reinterpret_cast<uint4*>(to + (i / 2) * (kKeys * 128) + ((((4 * i + 2 * h + r) & 7) ^ (t & 7)) << 4)) = values8(code[i], sm[32 * i / G].x, sm[32 * i / G].y);
                 }
             } else {
                 const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;  // run g of four keys of a block of eight
-                unsigned char* to = v_smem + stage * Cfg::kOperand + (w * kv4::kTile + 8 * blk + 4 * th) * 128;
-                const unsigned char* at = tile + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
-                uint32_t code[4][D / 64];
-                if constexpr (D == 128) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 16);
-                    code[0][0] = a.x, code[0][D / 64 - 1] = a.y, code[1][0] = a.z, code[1][D / 64 - 1] = a.w;
-                    code[2][0] = c.x, code[2][D / 64 - 1] = c.y, code[3][0] = c.z, code[3][D / 64 - 1] = c.w;
-                } else {
-                    const uint4 a = *reinterpret_cast<const uint4*>(at);
-                    code[0][0] = a.x, code[1][0] = a.y, code[2][0] = a.z, code[3][0] = a.w;
-                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint2 sm[NG];
+                for (int u = 0; u < 2; ++u) {
+                    unsigned char* to = v_smem + stage * Cfg::kOperand + ((2 * w + u) * kv4::kTile + 8 * blk + 4 * th) * 128;
+                    const unsigned char* at = tiles_at + u * Cfg::kHalf + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
+                    uint32_t code[4][D / 64];
+                    if constexpr (D == 128) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 16);
+                        code[0][0] = a.x, code[0][D / 64 - 1] = a.y, code[1][0] = a.z, code[1][D / 64 - 1] = a.w;
+                        code[2][0] = c.x, code[2][D / 64 - 1] = c.y, code[3][0] = c.z, code[3][D / 64 - 1] = c.w;
+                    } else {
+                        const uint4 a = *reinterpret_cast<const uint4*>(at);
+                        code[0][0] = a.x, code[1][0] = a.y, code[2][0] = a.z, code[3][0] = a.w;
+                    }
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) sm[k] = scales[(8 * blk + 4 * th + i) * NG + k];
+                    for (int i = 0; i < 4; ++i) {
+                        uint2 sm[NG];
 #pragma unroll
-                    for (int jw = 0; jw < D / 64; ++jw) {  // units 2 jw (low halves) and 2 jw + 1 (high)
-                        const int ka = 64 * jw / G, kb = (64 * jw + 32) / G, chunk = D / 64 * g + jw;
-                        const uint32_t s2 = ka == kb ? sm[ka].x : __byte_perm(sm[ka].x, sm[kb].x, 0x5410), m2 = ka == kb ? sm[ka].y : __byte_perm(sm[ka].y, sm[kb].y, 0x5410);
-                        *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + i * 128 + (((chunk & 7) ^ (4 * th + i)) << 4)) = values8(code[i][jw], s2, m2);
+                        for (int k = 0; k < NG; ++k) sm[k] = scales[u * Cfg::kWords + (8 * blk + 4 * th + i) * NG + k];
+#pragma unroll
+                        for (int jw = 0; jw < D / 64; ++jw) {  // units 2 jw (low halves) and 2 jw + 1 (high)
+                            const int ka = 64 * jw / G, kb = (64 * jw + 32) / G, chunk = D / 64 * g + jw;
+                            const uint32_t s2 = ka == kb ? sm[ka].x : __byte_perm(sm[ka].x, sm[kb].x, 0x5410), m2 = ka == kb ? sm[ka].y : __byte_perm(sm[ka].y, sm[kb].y, 0x5410);
+                            *reinterpret_cast<uint4*>(to + (chunk >> 3) * (kKeys * 128) + i * 128 + (((chunk & 7) ^ (4 * th + i)) << 4)) = values8(code[i][jw], s2, m2);
+                        }
                     }
                 }
             }
@@ -472,6 +509,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]);
             fetch(slot);
+            if (++slot == Cfg::kRaw) slot = 0;
         }
     } else {
         registers_down<kMmaRegs>();
