@@ -48,20 +48,20 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 
 template <int D, int G>
 struct PromptCfg {
-    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 3;
+    static constexpr int kTile = kv4::tile_bytes(D, G), kRaw = 4;
     static constexpr int kRows = 128 * D * 2;       // Q' of a tile of rows
     static constexpr int kOperand = kKeys * D * 2;  // K' or V' of a step
     static constexpr int kWords = 16 * (D / G);             // words of 16 keys, K's or V's
-    static constexpr int kHalf = kv4::kTile * D / 2 + kWords * 4;  // their codes and words
-    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + 16 * (kRaw * kHalf + kWords * 8) + 16;
+    static constexpr int kStep = kKeys / kv4::kTile * kTile;  // the cache's bytes of a step
+    static constexpr int kSmem = 1024 + 2 * kRows + 4 * kOperand + kRaw * kStep + 16 * kWords * 8 + 16;
     // TMEM columns: S of both tiles, two buffers each (P in a buffer's first half), then O
     static constexpr int kS = 0, kO = 256, kCols = 512;
     static_assert(kO + 2 * D <= kCols, "TMEM");
 };
 
 struct PromptBars {
-    // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by warp and slot
-    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw[8][3];
+    // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by slot
+    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw_full[4], raw_empty[4];
 };
 
 // Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     unsigned char *q_smem = smem, *k_smem = q_smem + 2 * Cfg::kRows, *v_smem = k_smem + 2 * Cfg::kOperand, *raw_smem = v_smem + 2 * Cfg::kOperand;
     __shared__ PromptBars bars;
     __shared__ TileInfo infos[kInfos][4];
+    __shared__ uint32_t raw_there[Cfg::kRaw];  // which tiles of a slot were copied
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_block;
 
@@ -137,8 +138,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             ptx::mbar_init(&bars.before_last[i], 1), ptx::mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], 4);
-        for (int w = 0; w < 8; ++w)
-            for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw[w][i], 1);
+        for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw_full[i], 1), ptx::mbar_init(&bars.raw_empty[i], 4);
         ptx::fence_mbar_init();
     }
     if (warp == kMmaWarp) umma::tmem_alloc(&tmem_slot, Cfg::kCols);
@@ -209,6 +209,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         bool alive = true;
         const uint32_t o_at = tmem + lanes + Cfg::kO + tile * D;
         for (int j = 0; work && j < steps; ++j) {
+            const int base = key0 + j * kKeys;
+            const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 128 + (j & 1) * 64;
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[tile][j & 1], (j >> 1) & 1, p.status));
+            umma::fence_after_sync();
             if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.info[j % kInfos], (j / kInfos) & 1, p.status));
             const TileInfo* info = infos[j % kInfos];
             float unit[4], v_exp[4], v_unit[4];
@@ -219,7 +223,6 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 unit[t] = fmaxf(of.x * mult, 1.2e-38f), v_exp[t] = of.z, v_unit[t] = fabsf(of.w);
                 bad |= __float_as_uint(of.y) | __float_as_uint(of.w) >> 31;
             }
-            const int base = key0 + j * kKeys;
             if (bad) {
                 for (int t = 0; t < 4; ++t)
                     for (int i = 0; i < kv4::kTile; ++i) {
@@ -229,25 +232,39 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         for (int k = 0; k < NG && info[t].v_unit < 0.0f; ++k) poison |= (info[t].bad_v[k] >> i & 1) << k;
                     }
             }
-            const uint32_t s_at = tmem + lanes + Cfg::kS + tile * 128 + (j & 1) * 64;
-            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[tile][j & 1], (j >> 1) & 1, p.status));
-            umma::fence_after_sync();
-            uint32_t a0[32], a1[32];
-            umma::tmem_ld_32x32(s_at, a0);
-            umma::tmem_ld_32x32(s_at + 32, a1);
-            umma::tmem_ld_wait();
-            float x[64];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(a0[i]), x[i + 32] = __uint_as_float(a1[i]);
-            if (base < all_lo || base + kKeys > all_hi) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (base + i < lo || base + i >= hi) x[i] = -INFINITY;
-            }
+            // The weights under the present maximum. A row's first keys need it found, and so do scores so much larger than before that 16
+            // weights add up to more than kMost: then S is read again (P does not yet stand in its place)
             uint32_t pr[32];
-            float part[4];
-            // the weights under the present maximum, and their sums by 16 keys
-            auto weights = [&]() {
+            float part[4], keep = 1.0f, now = 0.0f;
+            bool look = __any_sync(kAll, top == -INFINITY);
+#pragma unroll 1
+            for (int tries = 0; tries < 2; ++tries) {
+                float x[64];
+                {
+                    uint32_t a0[32], a1[32];
+                    umma::tmem_ld_32x32(s_at, a0);
+                    umma::tmem_ld_32x32(s_at + 32, a1);
+                    umma::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(a0[i]), x[i + 32] = __uint_as_float(a1[i]);
+                }
+                if (base < all_lo || base + kKeys > all_hi) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (base + i < lo || base + i >= hi) x[i] = -INFINITY;
+                }
+                if (look) {
+                    float most_here = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        float m = x[16 * t];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
+                        most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
+                    }
+                    keep = top == -INFINITY ? 0.0f : exp2f(top - fmaxf(top, most_here));
+                    top = fmaxf(top, most_here);
+                }
                 const float shift = top == -INFINITY ? 0.0f : top;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -262,19 +279,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                     }
                     part[t] = all.x + all.y;
                 }
-            };
-            weights();
-            const bool over = !(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) <= kMost);
-            if (__any_sync(kAll, over || top == -INFINITY)) {  // a row's first keys, or much larger scores than it has had
-                float most_here = -INFINITY;
+                if (look || !__any_sync(kAll, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) > kMost)) break;
+                look = true;
+            }
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    float m = x[16 * t];
-#pragma unroll
-                    for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
-                    most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
-                }
-                const float now = fmaxf(top, most_here), keep = top == -INFINITY ? 0.0f : exp2f(top - now);
+            for (int t = 0; t < 4; ++t) now = fmaf(part[t], v_unit[t], now);
+            umma::tmem_st_32x32(s_at, pr);
+            if (look) {
                 if (j > 0) {
                     // O is the MMAs' until those of step j - 1 are done: S of step j + 1 comes after them
                     uint64_t* done = j + 1 < steps ? &bars.s_full[tile][(j + 1) & 1] : &bars.before_last[tile];
@@ -290,12 +301,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         umma::tmem_st_32x32(o_at + at, r);
                     }
                 }
-                sum *= keep, top = now;
-                weights();
+                sum *= keep;
             }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) sum = fmaf(part[t], v_unit[t], sum);
-            umma::tmem_st_32x32(s_at, pr);
+            sum += now;
             umma::tmem_st_wait();
             umma::fence_before_sync();
             __syncwarp();
@@ -340,64 +348,15 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         // ---- 32 keys of every other step a warp: K's or V's codes and words to K' or V'. Two tiles at once and a step's time
         // for each: a warp alone spends most of its time on latencies -----------------------------------------------------------
         const bool is_v = warp >= kVWarp;
-        const int w = warp & 1, ring_of = warp - kKWarp;  // keys 32 w .. + 31 of the steps of parity warp / 2 % 2
-        unsigned char* raw = raw_smem + ring_of * Cfg::kRaw * 2 * Cfg::kHalf;
-        uint2* scales = reinterpret_cast<uint2*>(raw_smem + 8 * Cfg::kRaw * 2 * Cfg::kHalf) + ring_of * 2 * Cfg::kWords;  // (s, s), (m, m) of every word
-        uint64_t* raw_full = bars.raw[ring_of];
-        constexpr int kCodes = kv4::kTile * D / 2;
+        const int w = warp & 1;  // keys 32 w .. + 31 of the steps of parity warp / 2 % 2
+        uint2* scales = reinterpret_cast<uint2*>(raw_smem + Cfg::kRaw * Cfg::kStep) + (warp - kKWarp) * 2 * Cfg::kWords;  // (s, s), (m, m) of every word
         const int codes_at = is_v ? kv4::v_codes_at(D) : 0, words_at = is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D);
-        const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
-        const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
-        const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
-        // the two tiles that are fetched next: their first keys, places in the table, pages' numbers (read a visit early)
-        int next_key[2], next_at[2], next_in[2], next_page[2] = {-1, -1};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            next_key[u] = key0 + (warp >> 1 & 1) * kKeys + (2 * w + u) * kv4::kTile;
-            next_at[u] = next_key[u] / kv4::kTile / tiles_per_page, next_in[u] = next_key[u] / kv4::kTile % tiles_per_page;
-            if (next_key[u] < any_hi) next_page[u] = __ldg(table + next_at[u]);
-        }
-        uint32_t got = 0;  // tiles of the ring that are there: bits 2 slot and 2 slot + 1
-        auto fetch = [&](int slot) {
-            got &= ~(3u << 2 * slot);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (next_key[u] >= any_hi) continue;
-                if (next_page[u] >= 0 && next_page[u] < p.pool.pages) got |= 1u << (2 * slot + u);
-                else if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
-            }
-            const uint32_t mine = got >> 2 * slot & 3u;
-            if (mine != 0 && lane == 0) {
-                ptx::mbar_arrive_expect_tx(&raw_full[slot], Cfg::kHalf * ((mine & 1) + (mine >> 1)));
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (mine >> u & 1) {
-                        const unsigned char* from = pool + next_page[u] * page_bytes + next_in[u] * Cfg::kTile;
-                        unsigned char* to = raw + (2 * slot + u) * Cfg::kHalf;
-                        ptx::bulk_g2s(to, from + codes_at, kCodes, &raw_full[slot]);
-                        ptx::bulk_g2s(to + kCodes, from + words_at, Cfg::kWords * 4, &raw_full[slot]);
-                    }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (next_key[u] >= any_hi) continue;
-                next_key[u] += 2 * kKeys, next_in[u] += 2 * kKeys / kv4::kTile;
-                while (next_in[u] >= tiles_per_page) next_in[u] -= tiles_per_page, ++next_at[u];
-                if (next_key[u] < any_hi) next_page[u] = __ldg(table + next_at[u]);
-            }
-        };
-        for (int i = 0; i < Cfg::kRaw; ++i) fetch(i);
-        uint32_t raw_phase = 0;  // by slot: a slot's barrier turns only when it was filled
         bool alive = true;
-        int slot = 0;
         for (int j = warp >> 1 & 1; j < steps; j += 2) {
-            const int stage = j & 1, base0 = key0 + j * kKeys + 2 * w * kv4::kTile;
-            const uint32_t here = got >> 2 * slot & 3u;
-            if (here) {
-                if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&raw_full[slot], raw_phase >> slot & 1, p.status));
-                raw_phase ^= 1u << slot;
-            }
-            const unsigned char* tiles_at = raw + 2 * slot * Cfg::kHalf;
+            const int stage = j & 1, slot = j % Cfg::kRaw, base0 = key0 + j * kKeys + 2 * w * kv4::kTile;
+            if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.raw_full[slot], (j / Cfg::kRaw) & 1, p.status));
+            const uint32_t here = raw_there[slot] >> 2 * w;
+            const unsigned char* tiles_at = raw_smem + slot * Cfg::kStep + 2 * w * Cfg::kTile;
             // ---- the words, one or a few a lane: their size, and what is not finite; 0 for a key that no row sees
             constexpr int kPerLane = (Cfg::kWords + 31) / 32;
 #pragma unroll
@@ -407,7 +366,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
 #pragma unroll
                 for (int i = 0; i < kPerLane; ++i) {
                     const int at = (lane + 32 * i) % Cfg::kWords, key = base0 + u * kv4::kTile + at / NG;  // one group: the upper lanes repeat the lower
-                    uint32_t x = *reinterpret_cast<const uint32_t*>(tiles_at + u * Cfg::kHalf + kCodes + at * 4);
+                    uint32_t x = *reinterpret_cast<const uint32_t*>(tiles_at + u * Cfg::kTile + words_at + at * 4);
                     if (!(here >> u & 1) || key < any_lo || key >= any_hi) x = 0;
                     if ((x & 0x7f800000u) == 0x7f800000u || (x & 0x7f80u) == 0x7f80u) x = 0, odd |= 1u << i;
                     s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
@@ -455,7 +414,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 const int t = lane >> 1, h = lane & 1;  // a lane has half of a key's row
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const unsigned char* tile = tiles_at + u * Cfg::kHalf;
+                    const unsigned char* tile = tiles_at + u * Cfg::kTile;
                     uint2 sm[NG];
 #pragma unroll
                     for (int k = 0; k < NG; ++k) sm[k] = scales[u * Cfg::kWords + t * NG + k];
@@ -481,7 +440,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     unsigned char* to = v_smem + stage * Cfg::kOperand + ((2 * w + u) * kv4::kTile + 8 * blk + 4 * th) * 128;
-                    const unsigned char* at = tiles_at + u * Cfg::kHalf + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
+                    const unsigned char* at = tiles_at + u * Cfg::kTile + codes_at + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
                     uint32_t code[4][D / 64];
                     if constexpr (D == 128) {
                         const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 16);
@@ -507,14 +466,44 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             }
             ptx::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]);
-            fetch(slot);
-            if (++slot == Cfg::kRaw) slot = 0;
+            if (lane == 0) ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]), ptx::mbar_arrive(&bars.raw_empty[slot]);
         }
     } else {
         registers_down<kMmaRegs>();
         const int i = warp - kMmaWarp;
-        if (i < tiles && steps > 0) {
+        if (i == 2) {
+            // ---- the copies, a step at a time; page numbers (a lane a tile) a step early ------------------------------------
+            const int32_t* table = p.batch.table + static_cast<size_t>(b) * p.batch.width;
+            const unsigned char* pool = p.pool.data + static_cast<size_t>(head) * tiles_per_page * Cfg::kTile;
+            const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
+            int key = key0 + (lane & 3) * kv4::kTile, at = key / kv4::kTile / tiles_per_page, in_page = key / kv4::kTile % tiles_per_page, page = -1;
+            if (key < any_hi) page = __ldg(table + at);
+            bool ok = true;
+            for (int j = 0; ok && j < steps; ++j) {
+                const int slot = j % Cfg::kRaw;
+                if (j >= Cfg::kRaw) ok = __all_sync(kAll, ptx::mbar_wait(&bars.raw_empty[slot], (j / Cfg::kRaw - 1) & 1, p.status));
+                const bool good = key < any_hi && page >= 0 && page < p.pool.pages;
+                if (key < any_hi && !good && lane < 4) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                const uint32_t there = __ballot_sync(kAll, good) & 15u;
+                const int first_page = __shfl_sync(kAll, page, 0);
+                const bool one = __ballot_sync(kAll, good && page == first_page) == kAll && __shfl_sync(kAll, in_page, 0) + 3 < tiles_per_page;
+                if (lane == 0) {
+                    raw_there[slot] = there;
+                    ptx::mbar_arrive_expect_tx(&bars.raw_full[slot], __popc(there) * Cfg::kTile);
+                }
+                __syncwarp();
+                unsigned char* to = raw_smem + slot * Cfg::kStep;
+                const unsigned char* from = pool + page * page_bytes + in_page * Cfg::kTile;
+                if (one) {  // all of the step in one page
+                    if (lane == 0) ptx::bulk_g2s(to, from, Cfg::kStep, &bars.raw_full[slot]);
+                } else if (lane < 4 && good) {
+                    ptx::bulk_g2s(to + lane * Cfg::kTile, from, Cfg::kTile, &bars.raw_full[slot]);
+                }
+                key += kKeys, in_page += kKeys / kv4::kTile;
+                while (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
+                if (key < any_hi) page = __ldg(table + at);
+            }
+        } else if (i < tiles && steps > 0) {
             // ---- the MMAs of a tile of rows, a warp for each (a warp's waits and commits alone take longer than a step's MMAs). The
             // scores run two steps ahead of the values, into the buffer whose P the values have just taken: the MMAs of a
             // thread run in their order, so one commit a step tells of both
