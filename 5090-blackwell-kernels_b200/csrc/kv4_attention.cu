@@ -35,8 +35,9 @@ using kv4::AttendParams;
 constexpr int kSteps = 2;     // 16-token tiles of a ring stage
 constexpr int kMinUnits = 8;  // a CTA gets at least this many units
 // Units that stand in front of a piece's tiles for what its beginning costs (q, the lengths, the end's sums). Without them
-// a batch with short sequences waits for the warps that got many (64 x 4k, ragged: 60.1 us with 0, 56.6 / 47.7 / 45.4 with 1 / 3 / 6).
-constexpr int kLead = 6;
+// a batch with short sequences waits for the warps that got many (64 x 4k, ragged: 60.1 us with 0, 56.6 / 47.7 / 43.5 / 42.0 / 43.3
+// with 1 / 3 / 6 / 10 / 16).
+constexpr int kLead = 10;
 constexpr int kMaxWarps = 11;  // consuming warps of a CTA, of any form
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
@@ -720,16 +721,29 @@ __global__ void __launch_bounds__(256) kv4_attend_add_kernel(const AttendParams 
     for (int i = threadIdx.x; i < R * (D / 4); i += 256) {
         const int row = i / (D / 4), ch = i % (D / 4) * 4, r = piece.z * R + row;
         if (r >= count * group) break;
-        float m = -INFINITY;
-        for (int k = 0; k < piece.x; ++k) m = fmaxf(m, part(k)[R * D + 2 * row]);
-        float l = 0.0f;
+        // four parts' loads at a time, the sums on their running maximum
+        float m = -INFINITY, l = 0.0f;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < piece.x; ++k) {
-            const float* from = part(k);
-            const float t = from[R * D + 2 * row], w = t == -INFINITY ? 0.0f : ptx::exp2_fast(t - m);
-            const float4 v = *reinterpret_cast<const float4*>(from + row * D + ch);
-            a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
-            l = fmaf(from[R * D + 2 * row + 1], w, l);
+        for (int k0 = 0; k0 < piece.x; k0 += 4) {
+            float2 ms[4];
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                ms[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k0 + k < piece.x) {
+                    const float* from = part(k0 + k);
+                    ms[k] = *reinterpret_cast<const float2*>(from + R * D + 2 * row), v[k] = *reinterpret_cast<const float4*>(from + row * D + ch);
+                }
+            }
+            const float now = fmaxf(fmaxf(fmaxf(ms[0].x, ms[1].x), fmaxf(ms[2].x, ms[3].x)), m);
+            const float keep = m == -INFINITY ? 0.0f : ptx::exp2_fast(m - now);
+            a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep, l *= keep, m = now;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = ms[k].x == -INFINITY ? 0.0f : ptx::exp2_fast(ms[k].x - now);
+                a.x = fmaf(v[k].x, w, a.x), a.y = fmaf(v[k].y, w, a.y), a.z = fmaf(v[k].z, w, a.z), a.w = fmaf(v[k].w, w, a.w);
+                l = fmaf(ms[k].y, w, l);
+            }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
