@@ -803,12 +803,12 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     if (int rc = kv4::check("kv4_attention", pool, pages, page_size, kv_heads, head_dim, group)) return rc;
     AttendParams p{};
     p.batch = {page_table, lens, q_offsets, seqs, rows, table_width};
-    if (int rc = kv4::check_batch("kv4_attention", p.batch)) return rc;
+    if (int rc = kv4::check_batch("kv4_attention", p.batch, page_size)) return rc;
     SPK_REQUIRE(q_heads >= 1 && q_heads <= 16384 && q_heads % kv_heads == 0, "kv4_attention: q_heads must be a multiple of kv_heads, at most 16384, got %d and %d", q_heads, kv_heads);
     SPK_REQUIRE(window >= 0, "kv4_attention: window must be 0 (none) or positive, got %d", window);
     SPK_REQUIRE(scale == scale && scale >= -3e38f && scale <= 3e38f, "kv4_attention: scale must be finite");
     if (rows == 0) return SPK_OK;
-    SPK_REQUIRE(q && out && aligned16(q) && aligned16(out), "kv4_attention: q and out must be 16-byte aligned device pointers");
+    SPK_REQUIRE(q && out && q != out && aligned16(q) && aligned16(out), "kv4_attention: q and out must be two 16-byte aligned device pointers");
     SPK_REQUIRE(q_stride >= static_cast<long long>(q_heads) * head_dim && q_stride % 8 == 0, "kv4_attention: rows of q must be at least q_heads head_dim apart and a multiple of 8, got %lld", q_stride);
     SPK_REQUIRE(static_cast<long long>(rows) * (q_heads / kv_heads) <= INT32_MAX / 2, "kv4_attention: rows x query heads per KV head must stay below 2^30");
     SPK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= spk_kv4_attention_workspace(rows, seqs, q_heads, kv_heads, head_dim),
@@ -817,7 +817,7 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     if (int rc = device_state(&dev)) return rc;
     p.q = static_cast<const __nv_bfloat16*>(q), p.stride = q_stride;
     p.pool = {static_cast<unsigned char*>(const_cast<void*>(pool)), pages, page_size, kv_heads, kv4::tile_bytes(head_dim, group)};
-    p.q_heads = q_heads, p.window = window, p.zero_rest = zero_rest, p.scale = scale;
+    p.q_heads = q_heads, p.window = window < 1 << 30 ? window : 0, p.zero_rest = zero_rest, p.scale = scale;
     p.out = static_cast<__nv_bfloat16*>(out), p.status = dev->status;
     p.pieces = static_cast<int4*>(workspace);
     p.partials = reinterpret_cast<float*>(p.pieces + kMaxGrid);

@@ -375,11 +375,12 @@ extern "C" int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool,
     if (int rc = kv4::check("kv4_append", pool, pages, page_size, kv_heads, head_dim, group)) return rc;
     AppendParams p{};
     p.batch = {page_table, lens, q_offsets, seqs, rows, table_width};
-    if (int rc = kv4::check_batch("kv4_append", p.batch)) return rc;
+    if (int rc = kv4::check_batch("kv4_append", p.batch, page_size)) return rc;
     SPK_REQUIRE(q_heads >= 0 && q_heads <= 16384, "kv4_append: q_heads must be in [0, 16384], got %d", q_heads);
     SPK_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 8 == 0, "kv4_append: the rotated channels must be a multiple of 8, at most head_dim, got %d", rot_dim);
     if (rows == 0) return SPK_OK;
     SPK_REQUIRE(qkv && (q_out || q_heads == 0) && (cos_sin || rot_dim == 0), "kv4_append: null pointer");
+    SPK_REQUIRE(q_heads == 0 || qkv != q_out, "kv4_append: q_out must not be qkv's memory");
     SPK_REQUIRE(rot_dim == 0 || positions >= 1, "kv4_append: the table of the rotation is empty");
     SPK_REQUIRE(aligned16(qkv) && aligned16(q_out) && aligned16(cos_sin), "kv4_append: qkv, q_out and cos_sin must be 16-byte aligned");
     SPK_REQUIRE(qkv_stride >= static_cast<long long>(q_heads + 2 * kv_heads) * head_dim && qkv_stride % 8 == 0,

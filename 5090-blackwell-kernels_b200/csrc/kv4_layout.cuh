@@ -82,8 +82,9 @@ inline int check(const char* what, const void* pool, int pages, int page_size, i
     if (pages < 1 || kv_heads < 1 || kv_heads > 1024) return fail(SPK_INVALID, "%s: needs at least one page and 1 to 1024 KV heads, got pages=%d kv_heads=%d", what, pages, kv_heads);
     return SPK_OK;
 }
-inline int check_batch(const char* what, const Batch& s) {
+inline int check_batch(const char* what, const Batch& s, int page_size) {
     if (s.seqs < 0 || s.rows < 0 || s.width < 0 || s.seqs > kMaxSeqs) return fail(SPK_INVALID, "%s: needs 0 to %d sequences and no negative sizes, got sequences=%d rows=%d table width=%d", what, kMaxSeqs, s.seqs, s.rows, s.width);
+    if (static_cast<long long>(s.width) * page_size > 1 << 30) return fail(SPK_INVALID, "%s: a row of the page table may hold 2^30 tokens, got %d pages of %d", what, s.width, page_size);
     if (s.rows > 0 && s.seqs > 0 && (s.lens == nullptr || (s.table == nullptr && s.width > 0))) return fail(SPK_INVALID, "%s: null page table or lengths", what);
     if (s.offsets == nullptr && s.rows != s.seqs) return fail(SPK_INVALID, "%s: without q_offsets every sequence has one row, got %d rows and %d sequences", what, s.rows, s.seqs);
     return SPK_OK;

@@ -701,7 +701,8 @@ def kv4_append(qkv, pool, page_table, lens, cos_sin, q_offsets, head_dim: int, g
         q_out = qkv.new_empty((rows, q_heads, head_dim))
         zero_rest = int(q_offsets is not None)
     else:
-        _check_out(q_out, (rows, q_heads, head_dim), index, "q_out")
+        if _check_out(q_out, (rows, q_heads, head_dim), index, "q_out") == qkv.data_ptr() and rows and q_heads:
+            _fail("q_out must not be qkv's memory")
     args = (qkv.data_ptr(), stride, pool.data_ptr(), pages, tiles * 16, q_heads, kv_heads, head_dim, group, page_table.data_ptr(), width, lens.data_ptr(),
             _ptr(q_offsets), seqs, rows, _ptr(cos_sin), positions, rot, q_out.data_ptr(), zero_rest, _raw_stream(index))
     rc = _on_device(index, lambda: _spk_kv4_append(*args))
@@ -745,7 +746,7 @@ def kv4_attention(q, pool, page_table, lens, q_offsets, head_dim: int, group: in
     if stride < q_heads * head_dim or stride & 7 or q.data_ptr() & 15:
         _fail("q needs 16-byte aligned rows that do not overlap")
     seqs, width = _check_batch("kv4_attention", rows, index, page_table, lens, q_offsets)
-    window = int(window)
+    window, scale = min(int(window), 1 << 30), float(scale)
     if window < 0:
         _fail(f"window must be 0 (none) or positive, got {window}")
     zero_rest = 0
@@ -753,7 +754,8 @@ def kv4_attention(q, pool, page_table, lens, q_offsets, head_dim: int, group: in
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         zero_rest = int(q_offsets is not None)
     else:
-        _check_out(out, shape, index, "out")
+        if _check_out(out, shape, index, "out") == q.data_ptr() and rows:
+            _fail("out must not be q's memory")
     nbytes = _kv4_workspace_bytes(rows, seqs, q_heads, kv_heads, head_dim)
     ws = pool.new_empty(nbytes)
     args = (q.data_ptr(), stride, pool.data_ptr(), pages, tiles * 16, q_heads, kv_heads, head_dim, group, page_table.data_ptr(), width, lens.data_ptr(),
@@ -772,6 +774,9 @@ def add_rmsnorm(x, y, gain, eps: float, post_gain, gate, residual_scale: float):
     index = x.get_device()
     if hidden < 8 or hidden & 7 or hidden > 65536:
         _fail(f"add_rmsnorm needs hidden a multiple of 8 up to 65536, got {hidden}")
+    if rows >= 1 << 31:
+        _fail(f"add_rmsnorm takes fewer than 2^31 rows, got {rows}")
+    eps, residual_scale = float(eps), float(residual_scale)
     x_stride = _row_strided(x, "x", hidden, index)
     y_stride = gate_stride = 0
     if y is not None:

@@ -177,7 +177,7 @@ SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int3
  * sequence (rows == seqs). Row i of n of a sequence thus has position lens - n + i; a row of negative position is
  * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest. A page outside the pool, a
  * length outside the table and a position outside the rotation's table are skipped and reported as SPK_BAD_INDEX by
- * spk_device_status. seqs <= 4096. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
+ * spk_device_status. seqs <= 4096, table_width * page_size <= 2^30. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
 SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported pair */
 /* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
  * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16
@@ -193,7 +193,7 @@ SPK_API int spk_kv4_read(const void* pool, int pages, int page_size, int kv_head
                          void* k, void* v, void* stream);
 /* out bf16 [rows][q_heads][head_dim] = softmax(scale q k^T) v over the tokens at positions <= the row's own (window > 0:
  * only the last `window` of them), fp32 sums; zeros where there are none. q bf16, rows q_stride elements apart; q_heads a
- * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads). workspace: spk_kv4_attention_workspace(...) bytes of
+ * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads); out must not be q's memory. workspace: spk_kv4_attention_workspace(...) bytes of
  * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter. */
 SPK_API long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim);
 SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,

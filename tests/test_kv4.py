@@ -255,6 +255,45 @@ def test_nan_and_infinity_reach_only_their_readers(sk):
     assert torch.isnan(only[9:14, :2, :64]).all() and not torch.isnan(only[14:20]).any() and not torch.isnan(only[:9]).any()
 
 
+@pytest.mark.parametrize("hq", [4, 12, 24])
+def test_queries_that_are_no_numbers(sk, hq):
+    """A NaN or an infinity in a query spoils its own row and head, and not a row that sees nothing."""
+    g = torch.Generator().manual_seed(21)
+    cache, table = _filled(sk, g, [40, 0, 9], 16, 2, 128, 64)
+    lens = torch.tensor([40, 0, 9], dtype=torch.int32).cuda()
+    q = _bf16(g, 3, hq, 128)
+    good = sk.kv4_attention(q.cuda(), cache, table.cuda(), lens)
+    q[0, 1, 5], q[2, hq - 1, 77], q[1, 0, 0] = float("nan"), float("inf"), float("nan")
+    got = sk.kv4_attention(q.cuda(), cache, table.cuda(), lens)
+    spoiled = torch.zeros(3, hq, dtype=torch.bool)
+    spoiled[0, 1] = spoiled[2, hq - 1] = True
+    assert torch.isnan(got[spoiled]).all() and torch.equal(got[~spoiled], good[~spoiled]) and (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("seqs", [257, 700, 4096])
+def test_many_sequences(sk, seqs):
+    """More sequences than a block has threads, most of them short or empty, one row each and several."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 20, (seqs,), generator=g)
+    lens[seqs // 2] = 300
+    page, hkv, hq, d = 32, 1, 2, 64
+    width = 10
+    table = torch.randint(0, 40, (seqs, width), generator=g).to(torch.int32)  # pages shared for reading
+    cache = sk.KV4Cache(40, hkv, d, page, 32)
+    fill = torch.arange(40, dtype=torch.int32).reshape(1, 40)
+    off = torch.tensor([0, 40 * page], dtype=torch.int32).cuda()
+    sk.kv4_append(_bf16(g, 40 * page, 2 * d).cuda(), cache, fill.cuda(), torch.tensor([40 * page], dtype=torch.int32).cuda(), None, off)
+    k, v = ref.unpack(cache.pool, d, 32)
+    news = torch.minimum(lens, torch.randint(0, 4, (seqs,), generator=g))
+    for offs in (None, [0] + news.cumsum(0).tolist()):
+        rows = seqs if offs is None else offs[-1]
+        q = _bf16(g, rows, hq, d)
+        got = sk.kv4_attention(q.cuda(), cache, table.cuda(), lens.to(torch.int32).cuda(), None if offs is None else torch.tensor(offs, dtype=torch.int32).cuda())
+        want, slack = ref.attention(q, k, v, table.tolist(), lens.tolist(), offs, d ** -0.5, 0)
+        _check(got, want, slack, f"{seqs} {offs is None}")
+    assert sk._C.device_status() == 0
+
+
 def test_bad_indices_are_reported_and_left_out(sk):
     """A page outside the pool, a length past the table, a position past the rotation's table, a slot past the pool."""
     g = torch.Generator().manual_seed(16)
@@ -414,6 +453,9 @@ def test_refusals(sk):
         lambda: sk.kv4_append(qkv, cache, table, lens, torch.zeros(4, 20).cuda()),
         lambda: sk.kv4_append(qkv, cache, table, lens, torch.zeros(4, 136).cuda()),
         lambda: sk.kv4_append(qkv, cache, table, lens, torch.zeros(4, 128).cuda().double()),
+        lambda: sk.kv4_attention(q, cache, table, lens, out=q),
+        lambda: sk.kv4_attention(q.repeat(2500, 1, 1)[:4097], cache, table[:1].repeat(4097, 1), lens[:1].repeat(4097)),
+        lambda: sk.kv4_attention(q, cache, torch.zeros(2, (1 << 26) + 1, dtype=torch.int32).cuda(), lens),
         lambda: sk.kv4_read(cache, lens),
         lambda: sk.kv4_read(cache, torch.zeros(2, dtype=torch.int64)),
     ]

@@ -1,0 +1,88 @@
+"""Without a GPU: what the C entry points of the 4-bit cache and the residual norm refuse before they touch CUDA, with the
+status and a message that names the argument; and the bytes of a tile."""
+
+import ctypes
+import os
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+i, p, ll, f = ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = ctypes.CDLL(os.path.join(ROOT, "5090-blackwell-kernels_b200", "lib", "libspark_b200.so"))
+    lib.spk_last_error.restype = ctypes.c_char_p
+    lib.spk_kv4_attention_workspace.restype = ll
+    lib.spk_kv4_append.argtypes = [p, ll, p, i, i, i, i, i, i, p, i, p, p, i, i, p, i, i, p, i, p]
+    lib.spk_kv4_read.argtypes = [p, i, i, i, i, i, p, i, p, p, p]
+    lib.spk_kv4_attention.argtypes = [p, ll, p, i, i, i, i, i, i, p, i, p, p, i, i, f, i, p, i, p, ll, p]
+    lib.spk_add_rmsnorm.argtypes = [p, ll, p, ll, p, p, p, ll, f, f, p, p, i, i, p]
+    return lib
+
+
+@pytest.fixture(scope="module")
+def at():
+    buf = ctypes.create_string_buffer(256)
+    base = ctypes.addressof(buf)
+    yield lambda k: base + (-base) % 16 + 16 * k
+    del buf
+
+
+def _refused(lib, rc, word):
+    assert rc == 1 and word in lib.spk_last_error().decode(), (rc, lib.spk_last_error())
+
+
+def test_tile_bytes(lib):
+    assert [lib.spk_kv4_tile_bytes(d, g) for d, g in ((64, 32), (64, 64), (128, 32), (128, 64), (128, 128))] == [1280, 1152, 2560, 2304, 2176]
+    assert [lib.spk_kv4_tile_bytes(d, g) for d, g in ((64, 128), (96, 32), (128, 16), (0, 0), (256, 64))] == [0] * 5
+
+
+def test_attention(lib, at):
+    def call(**kw):
+        a = dict(q=at(0), stride=512, pool=at(1), pages=4, page=16, hq=4, hkv=2, d=128, g=64, table=at(2), width=2, lens=at(3), off=None, seqs=2, rows=2,
+                 scale=0.1, window=0, out=at(4), rest=0, ws=at(5), wsb=1 << 40, stream=None)
+        a.update(kw)
+        return lib.spk_kv4_attention(*a.values())
+
+    for kw, word in ((dict(pool=None), "pool"), (dict(pool=at(1) + 8), "pool"), (dict(d=96), "head_dim"), (dict(g=48), "group"), (dict(d=64, g=128), "group"),
+                     (dict(page=24), "page_size"), (dict(page=0), "page_size"), (dict(page=2048), "page_size"), (dict(pages=0), "page"), (dict(hkv=0), "KV heads"),
+                     (dict(seqs=4097, rows=4097), "4096"), (dict(seqs=-1), "sequences"), (dict(rows=3), "q_offsets"), (dict(width=1 << 27), "2^30"),
+                     (dict(lens=None), "lengths"), (dict(table=None), "page table"), (dict(hq=3), "q_heads"), (dict(window=-1), "window"),
+                     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=None), "q and out"), (dict(out=at(0)), "q and out"),
+                     (dict(out=at(4) + 2), "q and out"), (dict(stride=511), "rows of q"), (dict(stride=504), "rows of q"), (dict(ws=None), "workspace"),
+                     (dict(wsb=16), "workspace")):
+        _refused(lib, call(**kw), word)
+    assert call(seqs=0, rows=0) == 0  # nothing to do: nothing touched
+
+
+def test_append_and_read(lib, at):
+    def call(**kw):
+        a = dict(qkv=at(0), stride=1024, pool=at(1), pages=4, page=16, hq=4, hkv=2, d=128, g=64, table=at(2), width=2, lens=at(3), off=None, seqs=2, rows=2,
+                 cs=at(6), positions=8, rot=128, q=at(4), rest=0, stream=None)
+        a.update(kw)
+        return lib.spk_kv4_append(*a.values())
+
+    for kw, word in ((dict(pool=None), "pool"), (dict(d=80), "head_dim"), (dict(rot=136), "rotated"), (dict(rot=20), "rotated"), (dict(positions=0), "rotation"),
+                     (dict(cs=None), "null"), (dict(cs=at(6) + 4), "aligned"), (dict(qkv=None), "null"), (dict(q=None), "null"), (dict(q=at(0)), "memory"),
+                     (dict(stride=1016), "apart"), (dict(stride=1028), "apart"), (dict(hq=-1), "q_heads"), (dict(rows=3), "q_offsets")):
+        _refused(lib, call(**kw), word)
+    assert call(seqs=0, rows=0) == 0
+    _refused(lib, lib.spk_kv4_read(at(1), 4, 16, 2, 128, 64, None, 3, at(2), at(3), None), "null")
+    _refused(lib, lib.spk_kv4_read(at(1), 4, 16, 2, 128, 64, at(0), -1, at(2), at(3), None), "slots")
+    assert lib.spk_kv4_read(at(1), 4, 16, 2, 128, 64, None, 0, None, None, None) == 0
+
+
+def test_norm(lib, at):
+    def call(**kw):
+        a = dict(x=at(0), xs=64, y=at(1), ys=64, gain=at(2), post=None, gate=None, gs=0, scale=1.0, eps=1e-5, r=at(3), h=at(4), rows=2, hidden=64, stream=None)
+        a.update(kw)
+        return lib.spk_add_rmsnorm(*a.values())
+
+    for kw, word in ((dict(hidden=60), "hidden"), (dict(hidden=0), "hidden"), (dict(hidden=65544), "hidden"), (dict(rows=-1), "hidden"), (dict(eps=-1.0), "eps"),
+                     (dict(eps=float("nan")), "eps"), (dict(x=None), "need y"), (dict(y=None, scale=0.5), "need y"), (dict(y=None, post=at(2)), "need y"),
+                     (dict(r=None), "goes with"), (dict(h=None), "goes with"), (dict(gain=None), "goes with"), (dict(y=None, gain=None, h=None), "goes with"),
+                     (dict(x=at(0) + 2), "aligned"), (dict(xs=68), "strides"), (dict(gs=-8), "strides")):
+        _refused(lib, call(**kw), word)
+    assert call(rows=0) == 0
