@@ -705,51 +705,69 @@ kv4_attend_split_kernel(const AttendParams p) {
     if (threadIdx.x == 0) p.pieces[blockIdx.x] = entry;
 }
 
-// Adds the parts of the pieces that were cut across CTAs: block i those of the piece that began in CTA i of the launch before.
+// Adds the parts of the pieces that were cut across CTAs: block (i, j) rows 4 j .. + 3 of the piece that began in CTA i of the launch
+// before. A long sequence alone has a part in every fifth CTA: groups of threads take every so-manieth part, four loads at a time.
+constexpr int kAddThreads = 512;
+
 template <int D, int R, int W>
-__global__ void __launch_bounds__(256) kv4_attend_add_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kAddThreads) kv4_attend_add_kernel(const AttendParams p) {
     pdl_release();
     pdl_wait();
     const int4 piece = p.pieces[blockIdx.x];
     if (piece.x == 0) return;
     constexpr int kPart = R * (D + 2), kPer = (2 + W) * kPart;  // a CTA's parts in the workspace
-    const int group = p.q_heads / p.pool.heads;
+    constexpr int kGroups = kAddThreads / D;                    // a group: a thread for each four channels of the four rows
+    __shared__ float4 sums[kGroups][D];
+    __shared__ float2 tops[kGroups][D];
+    const int head_group = p.q_heads / p.pool.heads;
     int first, count;
     kv4::rows_of(p.batch, piece.y, first, count);
     const float* mine = p.partials + static_cast<size_t>(blockIdx.x) * kPer;
     auto part = [&](int i) { return i == 0 ? mine + kPart : mine + static_cast<size_t>(i) * kPer; };
-    for (int i = threadIdx.x; i < R * (D / 4); i += 256) {
-        const int row = i / (D / 4), ch = i % (D / 4) * 4, r = piece.z * R + row;
-        if (r >= count * group) break;
-        // four parts' loads at a time, the sums on their running maximum
-        float m = -INFINITY, l = 0.0f;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k0 = 0; k0 < piece.x; k0 += 4) {
-            float2 ms[4];
-            float4 v[4];
+    const int item = threadIdx.x % D, group = threadIdx.x / D;
+    const int row = 4 * blockIdx.y + item / (D / 4), ch = item % (D / 4) * 4, r = piece.z * R + row;
+    float m = -INFINITY, l = 0.0f;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = group; k0 < piece.x; k0 += 4 * kGroups) {
+        float2 ms[4];
+        float4 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                ms[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (k0 + k < piece.x) {
-                    const float* from = part(k0 + k);
-                    ms[k] = *reinterpret_cast<const float2*>(from + R * D + 2 * row), v[k] = *reinterpret_cast<const float4*>(from + row * D + ch);
-                }
-            }
-            const float now = fmaxf(fmaxf(fmaxf(ms[0].x, ms[1].x), fmaxf(ms[2].x, ms[3].x)), m);
-            const float keep = m == -INFINITY ? 0.0f : ptx::exp2_fast(m - now);
-            a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep, l *= keep, m = now;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float w = ms[k].x == -INFINITY ? 0.0f : ptx::exp2_fast(ms[k].x - now);
-                a.x = fmaf(v[k].x, w, a.x), a.y = fmaf(v[k].y, w, a.y), a.z = fmaf(v[k].z, w, a.z), a.w = fmaf(v[k].w, w, a.w);
-                l = fmaf(ms[k].y, w, l);
+        for (int k = 0; k < 4; ++k) {
+            ms[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k0 + k * kGroups < piece.x) {
+                const float* from = part(k0 + k * kGroups);
+                ms[k] = *reinterpret_cast<const float2*>(from + R * D + 2 * row), v[k] = *reinterpret_cast<const float4*>(from + row * D + ch);
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(first + r / group) * p.q_heads + piece.w * group + r % group) * D + ch) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+        const float now = fmaxf(fmaxf(fmaxf(ms[0].x, ms[1].x), fmaxf(ms[2].x, ms[3].x)), m);
+        const float keep = m == -INFINITY ? 0.0f : ptx::exp2_fast(m - now);
+        a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep, l *= keep, m = now;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = ms[k].x == -INFINITY ? 0.0f : ptx::exp2_fast(ms[k].x - now);
+            a.x = fmaf(v[k].x, w, a.x), a.y = fmaf(v[k].y, w, a.y), a.z = fmaf(v[k].z, w, a.z), a.w = fmaf(v[k].w, w, a.w);
+            l = fmaf(ms[k].y, w, l);
+        }
     }
+    sums[group][item] = a, tops[group][item] = make_float2(m, l);
+    __syncthreads();
+    if (group != 0 || r >= count * head_group) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) top = fmaxf(top, tops[k][item].x);
+    a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const float2 ms = tops[k][item];
+        const float4 v = sums[k][item];
+        const float w = ms.x == -INFINITY ? 0.0f : ptx::exp2_fast(ms.x - top);
+        a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
+        l = fmaf(ms.y, w, l);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(first + r / head_group) * p.q_heads + piece.w * head_group + r % head_group) * D + ch) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
 // Rows of a block. Up to four rows a KV head and sequence, and two groups or more: the form in which a row has two columns.
@@ -771,7 +789,7 @@ int attend(const AttendParams& p, DeviceState* dev, cudaStream_t stream) {
     const int grid = dev->sm_count * C < kMaxGrid ? dev->sm_count * C : kMaxGrid;
     if (grid < kMinGrid) return fail(SPK_UNSUPPORTED, "kv4_attention: needs at least %d SMs, the device has %d", kMinGrid, dev->sm_count);
     SPK_CUDA(launch_chained(kernel, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, stream, p));
-    SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows, W>, dim3(grid), dim3(256), 0, stream, p));
+    SPK_CUDA(launch_chained(kv4_attend_add_kernel<D, Cfg::kRows, W>, dim3(grid, Cfg::kRows / 4), dim3(kAddThreads), 0, stream, p));
     return SPK_OK;
 }
 template <int D, int G>
