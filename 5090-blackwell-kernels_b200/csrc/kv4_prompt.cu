@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             const unsigned char* tiles_at = raw_smem + slot * Cfg::kStep + 2 * w * Cfg::kTile;
             // ---- the words, one or a few a lane: their size, and what is not finite; 0 for a key that no row sees
             constexpr int kPerLane = (Cfg::kWords + 31) / 32;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {  // not unrolled, as below: the roles share the instruction caches (684 -> 654 us)
                 float s[kPerLane], m[kPerLane];
                 uint32_t size = 0, odd = 0;
 #pragma unroll
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.s_full[i][after & 1], (after >> 1) & 1, p.status));
             if (!is_v) {
                 const int t = lane >> 1, h = lane & 1;  // a lane has half of a key's row
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < 2; ++u) {
                     const unsigned char* tile = tiles_at + u * Cfg::kTile;
                     uint2 sm[NG];
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 }
             } else {
                 const int blk = lane >> 4, g = lane >> 1 & 7, th = lane & 1;  // run g of four keys of a block of eight
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < 2; ++u) {
                     unsigned char* to = v_smem + stage * Cfg::kOperand + ((2 * w + u) * kv4::kTile + 8 * blk + 4 * th) * 128;
                     const unsigned char* at = tiles_at + u * Cfg::kTile + codes_at + kv4::v_piece_at(D, 8 * blk + 4 * th, g);
