@@ -21,7 +21,13 @@
 // warps, whatever the lengths are; every warp finds its range itself from the lengths on the device and walks it alone,
 // through a ring of its own filled by bulk copies. What a warp holds of a piece that is cut across warps is added up in
 // the CTA at its end, what crosses CTAs goes through the workspace to a second, chained launch; always in the order of the
-// units: the same bits every run.
+// units: the same bits every run. (Adding by whichever CTA is last, on counters, was slower: 43.2 -> 45.6 us at 64 x 4k.)
+//
+// Bound: instructions, then memory. A tile of 16 tokens and a head costs about 270 warp instructions (88 to build the codes'
+// fragments, 32 to centre V's, 16 MMAs, the rest words, softmax and ring), at 2.3 a cycle and SM 118 cycles for 2176 to 2560
+// bytes, which HBM delivers in 94 to 110. 32 heads over 8, d = 128, in a graph: 8 sequences of 65536 121.7 us = 4.69 TB/s (0.72 of the
+// measured copy; without the arithmetic the same copies take 100 us, without the copies the arithmetic 112); 64 sequences of up
+// to 4096 40.5 us = 3.29 TB/s; one of 200 10.5 us, of which the second launch is 2.5. Prompts: kv4_prompt.cu.
 #include <algorithm>
 
 #include "kv4_attend.cuh"
@@ -38,15 +44,17 @@ constexpr int kMinUnits = 8;  // a CTA gets at least this many units
 // a batch with short sequences waits for the warps that got many (64 x 4k, ragged: 60.1 us with 0, 56.6 / 47.7 / 43.5 / 42.0 / 43.3
 // with 1 / 3 / 6 / 10 / 16).
 constexpr int kLead = 10;
-constexpr int kMaxWarps = 11;  // consuming warps of a CTA, of any form
+constexpr int kMaxWarps = 7;  // consuming warps of a CTA, of any form
 
 constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the part, with room; fewer than any sm_100 part has
 
 // H = 2 is the form for at most four rows a KV head (NQ = 1): a row has two of the eight columns, each for half of the
 // groups, so that the scales of one group are all a column ever meets.
 //
-// W consuming warps and one that fills their rings; kCtas such blocks on an SM. The accumulators (D NQ / 4 registers) decide:
-// the more warps, the better the latencies of their long dependent chains are covered.
+// W consuming warps and one that fills their rings, C such blocks on an SM: seven and two, at 128 registers a thread; seven and one
+// where 16 rows' accumulators take more. Five and two, with nothing spilled, is as fast at 64 x 4k and 6 % slower at 8 x 64k;
+// nine and two spills in the loop and takes twice as long. 24 rows a block spills too (76 us against 45 for 16 x 5 rows on
+// 6001), and 8 rows a block instead of 16 reads the cache more often (57 us).
 template <int D, int G, int NQ, int H, int W, int C>
 struct SplitCfg {
     static constexpr int kRows = 8 * NQ / H, kGroups = D / G / H, kWords = D / 32;
@@ -794,12 +802,10 @@ int attend(const AttendParams& p, DeviceState* dev, cudaStream_t stream) {
 }
 template <int D, int G>
 int attend_rows(const AttendParams& p, int per_block, DeviceState* dev, cudaStream_t stream) {
-    // warps and blocks an SM by the accumulators: 16, 32 and 64 registers a thread
-    constexpr int kFew = D == 64 ? 7 : 7;
     if constexpr (D / G > 1) {
         if (per_block == 4) return attend<D, G, 1, 2, 7, 2>(p, dev, stream);
     }
-    if (per_block == 8) return attend<D, G, 1, 1, kFew, 2>(p, dev, stream);
+    if (per_block == 8) return attend<D, G, 1, 1, 7, 2>(p, dev, stream);
     if constexpr (D == 64) return attend<D, G, 2, 1, 7, 2>(p, dev, stream);
     else return attend<D, G, 2, 1, 7, 1>(p, dev, stream);
 }

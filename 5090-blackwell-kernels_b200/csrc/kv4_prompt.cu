@@ -3,17 +3,24 @@
 // A CTA takes 256 rows (new tokens x query heads of one KV head of a sequence) in two tiles of 128, one row a TMEM lane, and
 // walks the keys 64 at a time:
 //     S [row][key] = Q' K'^T        P = 2^(S c + b)        O [row][channel] += P V'
-// with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Eight warps turn codes
-// and words into K' and V', every value (c s + m) 2^-e rounded once to fp16 (2^-12 of it), e the exponent of
-// the 16 tokens' largest |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the
-// keys; for the values 2^e joins the softmax's exponent: with M the running maximum of score + e,
+// with tcgen05.mma on fp16 operands, P (in S's place) from TMEM, the others from shared memory. Eight warps turn codes and
+// words into K' and V', every value (c s + m) 2^-e rounded once to fp16 (2^-11 of it), e the exponent of 16 tokens' largest
+// |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the keys; for the values 2^e
+// joins the softmax's exponent: with M the running maximum of score + e,
 //     P = 2^(score + e - M),      sum += P 2^-e,      out = O / sum,
-// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread; M is the maximum of a row's first keys and moves
-// only when weights would come near fp16's end, so O (in TMEM) is rarely touched between the MMAs and the maximum rarely looked for. While one tile's row warps work on S the tensor cores
-// have the other tile.
+// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread. M is the maximum of a row's first keys and
+// moves only when weights come near fp16's end, so O (in TMEM) is rarely touched between the MMAs and the maximum
+// rarely looked for (S is then read again: its 64 scores need not stay in registers until the weights are known to fit).
 // K' rows are keys, 128 bytes = 64 channels wide (the order of the channels inside eights is the codes' own; Q' is
 // stored in the same order); V' rows are keys too, and the MMA reads them MN-major; the order of its columns is the codes',
 // put right when O is written.
+//
+// Bound: the roles' latencies, not the tensor cores (36 % active). 2 x 2048 new tokens on 6144 old ones, 32 heads over 8, d = 128:
+// 654 us = 736 TFLOP/s (0.45 of the measured cuBLAS rate); a step of 64 keys takes some 2700 cycles where its MMAs take 1084
+// and its exponentials 1024. By device clocks a row warp has about 2300 cycles of work a step (1200 for the weights, the
+// rest waits that are already over, TMEM loads and stores, exponents), a code warp 1900, an MMA warp 1600 (some hundred
+// cycles for each MMA that it issues). 256 rows a block share the conversion of the codes; 128 keys a step would halve the
+// fixed costs but leave TMEM no room for the scores to run ahead.
 #include <algorithm>
 
 #include "kv4_attend.cuh"
