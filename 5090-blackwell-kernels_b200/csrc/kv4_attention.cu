@@ -841,7 +841,7 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     if (int rc = device_state(&dev)) return rc;
     p.q = static_cast<const __nv_bfloat16*>(q), p.stride = q_stride;
     p.pool = {static_cast<unsigned char*>(const_cast<void*>(pool)), pages, page_size, kv_heads, kv4::tile_bytes(head_dim, group)};
-    p.q_heads = q_heads, p.window = window < 1 << 30 ? window : 0, p.zero_rest = zero_rest, p.scale = scale;
+    p.q_heads = q_heads, p.window = window < 1 << 30 ? window : 0, p.zero_rest = zero_rest != 0 && q_offsets != nullptr, p.scale = scale;
     p.out = static_cast<__nv_bfloat16*>(out), p.status = dev->status;
     p.pieces = static_cast<int4*>(workspace);
     p.partials = reinterpret_cast<float*>(p.pieces + kMaxGrid);

@@ -391,7 +391,7 @@ extern "C" int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool,
     if (int rc = device_state(&dev)) return rc;
     p.qkv = static_cast<const __nv_bfloat16*>(qkv), p.stride = qkv_stride;
     p.pool = {static_cast<unsigned char*>(pool), pages, page_size, kv_heads, kv4::tile_bytes(head_dim, group)};
-    p.cos_sin = cos_sin, p.positions = rot_dim > 0 ? positions : INT32_MAX, p.rot = rot_dim, p.q_heads = q_heads, p.zero_rest = zero_rest;
+    p.cos_sin = cos_sin, p.positions = rot_dim > 0 ? positions : INT32_MAX, p.rot = rot_dim, p.q_heads = q_heads, p.zero_rest = zero_rest != 0 && q_offsets != nullptr;
     p.q_out = static_cast<__nv_bfloat16*>(q_out), p.status = dev->status;
     return for_shape<Append>(head_dim, group, p, dev->sm_count, static_cast<cudaStream_t>(stream));
 }

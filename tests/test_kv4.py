@@ -464,3 +464,21 @@ def test_refusals(sk):
             call()
             raise AssertionError(f"call {i} was taken")
     assert sk._C.device_status() == 0
+
+
+def test_zeroed_rest_without_offsets(sk):
+    """The C entries asked to zero the rows behind the last sequence where every sequence has one row: there are none."""
+    g = torch.Generator().manual_seed(21)
+    cache, table = _filled(sk, g, [40, 3], 16, 2, 128, 64)
+    table, lens = table.cuda(), torch.tensor([40, 3], dtype=torch.int32).cuda()
+    q, out = _bf16(g, 2, 4, 128).cuda(), torch.full((2, 4, 128), 7.0, dtype=torch.bfloat16).cuda()
+    want = sk.kv4_attention(q, cache, table, lens)
+    nbytes = sk._C._kv4_workspace_bytes(2, 2, 4, 2, 128)
+    ws, stream = torch.empty(nbytes, dtype=torch.uint8).cuda(), torch.cuda.current_stream().cuda_stream
+    assert sk._C._spk_kv4_attention(q.data_ptr(), 512, cache.pool.data_ptr(), cache.pages, 16, 4, 2, 128, 64, table.data_ptr(), table.shape[1], lens.data_ptr(),
+                                    None, 2, 2, 128 ** -0.5, 0, out.data_ptr(), 1, ws.data_ptr(), nbytes, stream) == 0
+    assert torch.equal(out, want)
+    qkv = _bf16(g, 2, 8 * 128).cuda()
+    assert sk._C._spk_kv4_append(qkv.data_ptr(), 1024, cache.pool.data_ptr(), cache.pages, 16, 4, 2, 128, 64, table.data_ptr(), table.shape[1], lens.data_ptr(),
+                                 None, 2, 2, None, 0, 0, out.data_ptr(), 1, stream) == 0
+    assert torch.equal(out, qkv[:, :512].reshape(2, 4, 128))
