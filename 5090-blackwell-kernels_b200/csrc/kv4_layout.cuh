@@ -58,15 +58,12 @@ __device__ __forceinline__ void rows_of(const Batch& s, int b, int& first, int& 
     first = min(max(s.offsets[b], 0), s.rows);
     count = max(0, min(s.offsets[b + 1], s.rows) - first);
 }
-// Tokens of sequence b that are in the cache, at most what its table row has room for.
+// Tokens of sequence b that are in the cache; none, which makes its rows padding, where its row of the table has no room for them.
 __device__ __forceinline__ int length_of(const Batch& s, int page_size, int b, int* status) {
     const int len = s.lens[b];
-    const long long room = static_cast<long long>(s.width) * page_size;
-    if (len < 0 || len > room) {
-        atomicCAS(status, 0, SPK_BAD_INDEX);
-        return len < 0 ? 0 : static_cast<int>(room);
-    }
-    return len;
+    if (len >= 0 && len <= static_cast<long long>(s.width) * page_size) return len;
+    atomicCAS(status, 0, SPK_BAD_INDEX);
+    return 0;
 }
 __device__ __forceinline__ float word_min(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float word_scale(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }

@@ -13,8 +13,8 @@ captured CUDA graph serves growing sequences:
 Row i of n of a sequence has position lens - n + i; a row of negative position (an empty slot of a padded batch) is
 padding: it is not appended, and its q and its attention output are zeros. Pages may be shared between sequences for
 reading; two sequences of one call must not append to the same page. Indices are checked on the device: a page
-outside the pool, a length outside the table or a position outside the rotation's table is left out and makes
-`_C.device_status()` return 5. Forward only.
+outside the pool or a position outside the rotation's table is left out, the rows of a sequence whose length is past
+its row of the table are padding, and each makes `_C.device_status()` return 5. Forward only.
 """
 
 from __future__ import annotations

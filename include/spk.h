@@ -175,9 +175,9 @@ SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int3
  * [seqs][table_width] on the device, the pages of a sequence in order; q_offsets int32 [seqs + 1] on the device, the call's
  * rows of sequence b are q_offsets[b] .. q_offsets[b + 1] - 1 and they are its last tokens; NULL: one row per
  * sequence (rows == seqs). Row i of n of a sequence thus has position lens - n + i; a row of negative position is
- * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest (without q_offsets there are none). A page outside the pool, a
- * length outside the table and a position outside the rotation's table are skipped and reported as SPK_BAD_INDEX by
- * spk_device_status. seqs <= 4096, table_width * page_size <= 2^30. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
+ * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest (without q_offsets there are none). A page outside the pool and a
+ * position outside the rotation's table are skipped, the rows of a sequence whose length is negative or past its row of the table
+ * are padding, and all are reported as SPK_BAD_INDEX by spk_device_status. seqs <= 4096, table_width * page_size <= 2^30. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
 SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported pair */
 /* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
  * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16

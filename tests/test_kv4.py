@@ -482,3 +482,22 @@ def test_zeroed_rest_without_offsets(sk):
     assert sk._C._spk_kv4_append(qkv.data_ptr(), 1024, cache.pool.data_ptr(), cache.pages, 16, 4, 2, 128, 64, table.data_ptr(), table.shape[1], lens.data_ptr(),
                                  None, 2, 2, None, 0, 0, out.data_ptr(), 1, stream) == 0
     assert torch.equal(out, qkv[:, :512].reshape(2, 4, 128))
+
+
+def test_a_length_past_the_table_is_padding(sk):
+    """A sequence that has outgrown its row of the table: nothing of it is written or read, the others are served."""
+    g = torch.Generator().manual_seed(22)
+    cache, table = _filled(sk, g, [48, 20], 16, 2, 128, 64)
+    table, lens = table.cuda(), torch.tensor([49, 21], dtype=torch.int32).cuda()
+    k0, v0 = ref.unpack(cache.pool, 128, 64)
+    qkv = _bf16(g, 2, 8 * 128).cuda()
+    q = sk.kv4_append(qkv, cache, table, lens, None)
+    assert sk._C.device_status() == 5 and (q[0] == 0).all() and torch.equal(q[1], qkv[1, :512].reshape(4, 128))
+    k, v = ref.unpack(cache.pool, 128, 64)
+    full = table[0].tolist()
+    assert torch.equal(k[full], k0[full]) and torch.equal(v[full], v0[full])
+    assert not torch.equal(k[int(table[1, 1]), 4], k0[int(table[1, 1]), 4])
+    out = sk.kv4_attention(q, cache, table, lens)
+    assert sk._C.device_status() == 5 and (out[0] == 0).all()
+    want, slack = ref.attention(q[1:], k, v, table[1:].tolist(), [21], None, 128 ** -0.5, 0)
+    _check(out[1:], want, slack)
