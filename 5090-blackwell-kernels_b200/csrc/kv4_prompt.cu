@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
 #pragma unroll
                     for (int k = 0; k < NG; ++k) all |= bad[k];
                     if (is_v) {
-                        info.v_exp = static_cast<float>(e), info.v_unit = all ? -power_of_two(-e) : power_of_two(-e);
+                        const float unit = power_of_two(-e / 2) * power_of_two(-e - -e / 2);  // e up to 128: below the normal numbers, still exact
+                        info.v_exp = static_cast<float>(e), info.v_unit = all ? -unit : unit;
 #pragma unroll
                         for (int k = 0; k < NG; ++k) info.bad_v[k] = bad[k];
                     } else {

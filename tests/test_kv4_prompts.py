@@ -147,3 +147,22 @@ def test_same_bits_captured_and_with_other_streams(sk):
     lens.copy_(torch.tensor([17, 900], dtype=torch.int32)), off.copy_(torch.tensor([0, 1, 601], dtype=torch.int32))
     graph.replay()
     assert torch.equal(got.view(torch.int16), sk.kv4_attention(q, cache, t, lens, off).view(torch.int16))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 125, 2.0 ** 126, 2.0 ** 127, 2.0 ** -100, 2.0 ** -126])
+def test_values_at_the_ends_of_the_range(sk, size):
+    """Values between one and one and a half times `size` (of the least, groups have no scale left and are their minimum) in a
+    prompt: as near to 64 bits as others, relative to the values."""
+    g = torch.Generator().manual_seed(12)
+    d, hkv, n = 128, 16, 150
+    cache = sk.KV4Cache(3, hkv, d, 64, 64)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    x = _bf16(g, n, 2 * hkv * d)
+    x[:, hkv * d:] = ((1 + 0.5 * torch.rand(n, hkv * d, generator=g)).double() * size).to(torch.bfloat16)
+    lens, off = torch.tensor([n], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda()
+    sk.kv4_append(x.cuda(), cache, table.cuda(), lens, None, off)
+    q = _bf16(g, n, 2 * hkv, d)
+    got = sk.kv4_attention(q.cuda(), cache, table.cuda(), lens, off).double().cpu() / size
+    k, v = ref.unpack(cache.pool, d, 64)
+    want, slack = ref.attention(q, k, v / size, table.tolist(), [n], [0, n], d ** -0.5, 0)
+    assert ((got - want).abs() <= want * 2 ** -8 + (2 ** -10 + 2.2e-2) * slack).all()
