@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         if (lane >= o) run += up;
     }
     if (lane == 31) warp_blocks[warp] = run;
+    if (threadIdx.x == 0) s_seq = s_block = 0;  // stays so only if offsets that overlap add up past 32 bits
     __syncthreads();
     int before = run - n, total = 0;
     for (int w = 0; w < kThreadsP / 32; ++w) {
