@@ -84,7 +84,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
     window > 0 the last `window` of them; softmax of scale * q.k (default head_dim ** -0.5) in fp32, bf16 out
     [rows, Hq, head_dim]. Hq is a multiple of the cache's heads, query head h reading head h // (Hq // Hkv). A row that
     sees nothing gets zeros. Rows of a given `out` behind the last sequence are left as they were (zeros in one that
-    the call allocates)."""
+    the call allocates); `out` must not lie in q's memory. The weighted values are summed in fp32 before they are
+    divided by the weights' sum: values of up to 1e27 are safe at every length."""
     return _C.kv4_attention(q, cache.pool, page_table, lens, q_offsets, cache.head_dim, cache.group,
                             cache.head_dim ** -0.5 if scale is None else scale, window, out)
 

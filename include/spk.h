@@ -182,7 +182,8 @@ SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported
 /* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
  * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16
  * [rows][q_heads][head_dim] (zeros for padding) and quantizes k and v into the pool: per group m = bf16(min), s = bf16((max - m) * fp32(1 / 15)),
- * c = clamp(rint((x - m) / s), 0, 15); a group with an infinity or a NaN reads back as NaN. */
+ * c = clamp(rint((x - m) / s), 0, 15); a group with an infinity or a NaN reads back as NaN. q_out must not lie in what
+ * qkv's rows span. */
 SPK_API int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool, int pages, int page_size, int q_heads, int kv_heads,
                            int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,
                            const int32_t* q_offsets, int seqs, int rows, const float* cos_sin, int positions, int rot_dim,
@@ -193,7 +194,7 @@ SPK_API int spk_kv4_read(const void* pool, int pages, int page_size, int kv_head
                          void* k, void* v, void* stream);
 /* out bf16 [rows][q_heads][head_dim] = softmax(scale q k^T) v over the tokens at positions <= the row's own (window > 0:
  * only the last `window` of them), fp32 sums; zeros where there are none. q bf16, rows q_stride elements apart; q_heads a
- * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads); out must not be q's memory. workspace: spk_kv4_attention_workspace(...) bytes of
+ * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads); out must not lie in what q's rows span. workspace: spk_kv4_attention_workspace(...) bytes of
  * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter. */
 SPK_API long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim);
 SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,

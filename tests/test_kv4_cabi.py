@@ -86,3 +86,16 @@ def test_norm(lib, at):
                      (dict(x=at(0) + 2), "aligned"), (dict(xs=68), "strides"), (dict(gs=-8), "strides")):
         _refused(lib, call(**kw), word)
     assert call(rows=0) == 0
+
+
+def test_outputs_in_the_inputs_memory(lib, at):
+    """An output that begins, ends or lies inside what the input's rows span."""
+    buf = ctypes.create_string_buffer(16384)
+    base = ctypes.addressof(buf)
+    base += -base % 16
+    for out in (base + 16, base + 1024 - 16, base + 2032):  # q: two rows of 1 KiB at base + 1024
+        rc = lib.spk_kv4_attention(base + 1024, 512, at(1), 4, 16, 4, 2, 128, 64, at(2), 2, at(3), None, 2, 2, 0.1, 0, out, 0, at(5), 1 << 40, None)
+        _refused(lib, rc, "out must not be in q's memory")
+    for out in (base + 16, base + 2048 + 16, base + 2048 + 4080):  # qkv: two rows of 2 KiB at base + 2048
+        rc = lib.spk_kv4_append(base + 2048, 1024, at(1), 4, 16, 4, 2, 128, 64, at(2), 2, at(3), None, 2, 2, at(6), 8, 128, out, 0, None)
+        _refused(lib, rc, "q_out must not be in qkv's memory")
