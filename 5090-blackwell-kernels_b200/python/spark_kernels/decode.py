@@ -176,14 +176,15 @@ class QuantizedDecoder:
 
     def extend(self, x: torch.Tensor, lens: torch.Tensor, q_offsets: torch.Tensor | None = None) -> torch.Tensor:
         """kv="int4" only: the hidden states after the last layer for the new tokens x [rows, hidden] of the sequences.
-        lens int32 [batch]: tokens of every sequence after this call (0: an empty slot); q_offsets int32 [batch + 1]: rows
-        q_offsets[b] .. q_offsets[b + 1] - 1 are the new tokens of sequence b, its last ones; None: one each."""
+        lens int32 [n], n at most `batch`: tokens of the first n sequences after this call (0: an empty slot); q_offsets int32
+        [n + 1]: rows q_offsets[b] .. q_offsets[b + 1] - 1 are the new tokens of sequence b, its last ones; None: one each."""
         if self.kv != "int4":
             raise ValueError("extend needs kv='int4'")
+        table = self.page_table[: lens.shape[0]]
         r, h = sk.add_rmsnorm(x, gain=self.norms[0][0], eps=self.cfg.eps)
         for li, lay in enumerate(self.layers):
-            q = kv4.kv4_append(lay.qkv(h), self.cache[li], self.page_table, lens, self.cos_sin, q_offsets)
-            att = kv4.kv4_attention(q, self.cache[li], self.page_table, lens, q_offsets)
+            q = kv4.kv4_append(lay.qkv(h), self.cache[li], table, lens, self.cos_sin, q_offsets)
+            att = kv4.kv4_attention(q, self.cache[li], table, lens, q_offsets)
             r, h = sk.add_rmsnorm(r, lay.o(att.reshape(x.shape[0], -1)), gain=self.norms[li][1], eps=self.cfg.eps)
             nxt = self.norms[li + 1][0] if li + 1 < len(self.layers) else None
             r, h = sk.add_rmsnorm(r, lay.down(lay.mlp_in(h)), gain=nxt, eps=self.cfg.eps)

@@ -141,3 +141,23 @@ def test_cache_formats_are_checked(sk):
         decode.QuantizedDecoder(cfg, w, kv="int8")
     with pytest.raises(ValueError):
         decode.QuantizedDecoder(cfg, w, batch=1).extend(torch.zeros(1, cfg.hidden, dtype=torch.bfloat16).cuda(), torch.ones(1, dtype=torch.int32).cuda())
+
+
+def test_four_bit_cache_fewer_sequences_than_slots(sk):
+    """A step of the first of three sequences, eager and captured, is the first row's step of a decoder for one."""
+    from spark_kernels import decode
+
+    cfg = _cfg(sk)
+    w = decode.random_weights(cfg, "cuda", seed=19)
+    one = decode.QuantizedDecoder(cfg, w, fmt="fp8-tok", batch=1, max_len=40, kv="int4")
+    three = decode.QuantizedDecoder(cfg, w, fmt="fp8-tok", batch=3, max_len=40, kv="int4")
+    captured = decode.QuantizedDecoder(cfg, w, fmt="fp8-tok", batch=3, max_len=40, kv="int4")
+    captured.capture(1)
+    g = torch.Generator(device="cuda").manual_seed(20)
+    for t in range(3):
+        x, pos = torch.randn(1, cfg.hidden, device="cuda", generator=g).to(torch.bfloat16), torch.tensor([t], device="cuda")
+        want = one.decode(x, pos)
+        assert torch.equal(three.decode(x, pos), want) and torch.equal(captured.replay(x, pos), want), t
+    with pytest.raises(RuntimeError):
+        one.extend(torch.randn(2, cfg.hidden, device="cuda").to(torch.bfloat16), torch.ones(2, dtype=torch.int32).cuda())
+    assert sk._C.device_status() == 0
