@@ -49,7 +49,9 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const Four& x) {
 }
 
 // A head vector belongs to L = D / 8 neighbouring lanes; lane l holds channels 4 l .. + 3 and, half a vector on, D / 2 + 4 l .. + 3.
-// With all channels rotated these are each other's partners; with fewer the partner's channels are loaded beside them.
+// With all channels rotated these are each other's partners; with half of them or fewer the partner is another lane's first
+// four channels, which come by shuffles; with a number between the two the partner's channels are loaded again.
+enum class Rot { kAll, kHalf, kMost };
 struct Pair {
     Four a, b;
 };
@@ -93,11 +95,18 @@ __device__ __forceinline__ Four turned(const Four& x, const Four& partner, const
     return y;
 }
 
-template <int D, bool Whole>
+// With R = kHalf all lanes of the warp call it.
+template <int D, Rot R>
 __device__ __forceinline__ Pair rotated(uint2 ra, uint2 rb, const __nv_bfloat16* vec, const Turn& t) {
     Pair x{unpack4(ra), unpack4(rb)};
-    if constexpr (Whole) {
+    if constexpr (R == Rot::kAll) {
         return {turned(x.a, x.b, t.ca, t.sa, true), turned(x.b, x.a, t.ca, t.sa, false)};
+    } else if constexpr (R == Rot::kHalf) {
+        constexpr int L = D / 8;
+        const int from = max(t.pa, 0) / 4;
+        const uint2 partner = make_uint2(__shfl_sync(0xffffffffu, ra.x, from, L), __shfl_sync(0xffffffffu, ra.y, from, L));
+        if (t.pa >= 0) x.a = turned(x.a, unpack4(partner), t.ca, t.sa, t.fa);
+        return x;
     } else {
         if (t.pa >= 0) x.a = turned(x.a, unpack4(load4(vec + t.pa)), t.ca, t.sa, t.fa);
         if (t.pb >= 0) x.b = turned(x.b, unpack4(load4(vec + t.pb)), t.cb, t.sb, t.fb);
@@ -167,9 +176,11 @@ __device__ __forceinline__ uint32_t codes4(const Four& x, const Scale& g) {
 }
 
 // Block: eight tokens, one per warp, and the head vectors of slice blockIdx.y, kPer of them at a time. Neighbouring tokens
-// of a sequence share V blocks, so their pieces leave the SM close together.
-template <int D, int G, bool Whole>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
+// of a sequence share V blocks, so their pieces leave the SM close together. Four blocks on an SM: with the registers that a half
+// rotated head likes (71) there are three, and 5015 tokens of 20 + 2 x 20 heads of 64 with their read take 41.4 us, not 38.4; with loads
+// in place of the shuffles 39.6. (Where all channels rotate 64 registers do anyway; five blocks spill and gain nothing.)
+template <int D, int G, Rot R>
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const AppendParams p) {
     constexpr int L = D / 8, kPer = 32 / L, kAhead = 4;  // lanes of a head vector, head vectors of a warp, loads in flight
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
     pdl_release();
@@ -239,7 +250,10 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
             const int h = (i0 + j) * kPer + sub;
             const bool is_k = h < p.pool.heads;
             Pair x{unpack4(ra[j]), unpack4(rb[j])};
-            if (is_k) x = rotated<D, Whole>(ra[j], rb[j], kv_row + h * D, turn);
+            if (R == Rot::kHalf || is_k) {
+                const Pair y = rotated<D, R>(ra[j], rb[j], kv_row + h * D, turn);
+                if (is_k) x = y;
+            }
             uint32_t ca, cb, wa, wb;
             if constexpr (G == D) {
                 const Scale g = scale_of<L>(min_nan(low4(x.a), low4(x.b)), max_nan(high4(x.a), high4(x.b)));
@@ -281,8 +295,9 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int h = (i0 + j) * kPer + sub;
-            if (i0 + j >= q_to || h >= p.q_heads) continue;
-            const Pair y = rotated<D, Whole>(ra[j], rb[j], row + h * D, turn);
+            if (i0 + j >= q_to || (R != Rot::kHalf && h >= p.q_heads)) continue;
+            const Pair y = rotated<D, R>(ra[j], rb[j], row + h * D, turn);
+            if (h >= p.q_heads) continue;
             __nv_bfloat16* q = p.q_out + (static_cast<size_t>(t) * p.q_heads + h) * D + 4 * l;
             store4(q, y.a), store4(q + D / 2, y.b);
         }
@@ -350,7 +365,7 @@ struct Append {
         const int blocks = cdiv(p.batch.rows, 8), steps = cdiv(p.q_heads, kPer) + cdiv(2 * p.pool.heads, kPer);
         // the heads are sliced over blocks until there are several rounds of them (four live on an SM), or one step each
         const int slices = std::max(1, std::min(steps, 16 * sms / blocks));
-        auto kernel = p.rot == D ? kv4_append_kernel<D, G, true> : kv4_append_kernel<D, G, false>;
+        auto kernel = p.rot == D ? kv4_append_kernel<D, G, Rot::kAll> : p.rot <= D / 2 ? kv4_append_kernel<D, G, Rot::kHalf> : kv4_append_kernel<D, G, Rot::kMost>;
         SPK_CUDA(launch_chained(kernel, dim3(blocks, slices), dim3(256), 0, stream, p));
         return SPK_OK;
     }

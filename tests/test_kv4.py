@@ -501,3 +501,26 @@ def test_a_length_past_the_table_is_padding(sk):
     assert sk._C.device_status() == 5 and (out[0] == 0).all()
     want, slack = ref.attention(q[1:], k, v, table[1:].tolist(), [21], None, 128 ** -0.5, 0)
     _check(out[1:], want, slack)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("more", [-24, -8, 8, -1])
+def test_numbers_of_rotated_channels(sk, d, more):
+    """Rotated channels just below half a head, above it, and one step short of all: q and the keys, to the roundings of a rotation
+    in fp32 (2^-22 of the largest input) and, for the keys, of a code."""
+    g = torch.Generator().manual_seed(d + more)
+    hq, hkv, rows = 3, 2, 20
+    rot = d - 8 if more == -1 else d // 2 + more
+    cs = sk.kv4.rotation_table(64, rot, device="cpu")
+    cache, table = sk.KV4Cache(3, hkv, d, 16, 32), torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda()
+    qkv = _bf16(g, rows, (hq + 2 * hkv) * d)
+    lens, off = torch.tensor([37], dtype=torch.int32).cuda(), torch.tensor([0, rows], dtype=torch.int32).cuda()
+    q = sk.kv4_append(qkv.cuda(), cache, table, lens, cs.cuda(), off).cpu().double()
+    x = qkv.double().reshape(rows, -1, d)
+    want = ref.rotate(x[:, : hq + hkv], cs[17:37])
+    assert ((q - want[:, :hq]).abs() <= want[:, :hq].abs() * 2 ** -8 + 2.0 ** -22 * x.abs().amax()).all()
+    pos = torch.arange(17, 37)
+    k, v = (t.cpu().double() for t in sk.kv4_read(cache, (torch.tensor([2, 0, 1])[pos // 16] * 16 + pos % 16).cuda()))
+    want_k, s, _ = ref.quantize(want[:, hq:], 32)
+    assert ((k - want_k).abs() <= want_k.abs() * 2 ** -8 + s * (1 + 2 ** -7) + 15 * s * 2 ** -7).all()
+    assert torch.equal(v, ref.quantize(x[:, hq + hkv:], 32)[0].to(torch.bfloat16).double())
