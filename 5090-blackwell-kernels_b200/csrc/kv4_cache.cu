@@ -12,7 +12,7 @@
 //
 // Both are bound by memory first: a token of Hq = 32, Hkv = 8, d = 128 is 12 KiB of qkv in, 8 KiB of q and 1.1 KiB of cache out.
 // 8192 such tokens: the append 42 us (4.3 TB/s, 0.66 of the measured copy; 29 M warp instructions at 2.7 a cycle and SM are
-// what is above it), reading them back 16 us. 16 tokens: 4.9 us for the two in a graph.
+// what is above it), reading them back 11 us. 16 tokens: 4.7 us for the two in a graph.
 #include <algorithm>
 #include <cfloat>
 
@@ -177,8 +177,8 @@ __device__ __forceinline__ uint32_t codes4(const Four& x, const Scale& g) {
 
 // Block: eight tokens, one per warp, and the head vectors of slice blockIdx.y, kPer of them at a time. Neighbouring tokens
 // of a sequence share V blocks, so their pieces leave the SM close together. Four blocks on an SM: with the registers that a half
-// rotated head likes (71) there are three, and 5015 tokens of 20 + 2 x 20 heads of 64 with their read take 41.4 us, not 38.4; with loads
-// in place of the shuffles 39.6. (Where all channels rotate 64 registers do anyway; five blocks spill and gain nothing.)
+// rotated head likes (71) there are three, and 5015 tokens of 20 + 2 x 20 heads of 64 take 2.9 us more of 25; with loads in
+// place of the shuffles 1.1 more. (Where all channels rotate 64 registers do anyway; five blocks spill and gain nothing.)
 template <int D, int G, Rot R>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const AppendParams p) {
     constexpr int L = D / 8, kPer = 32 / L, kAhead = 4;  // lanes of a head vector, head vectors of a warp, loads in flight
@@ -312,7 +312,8 @@ struct ReadParams {
     int* status;
 };
 
-// A warp reads a token: D / 8 lanes a head vector, eight channels each, the vectors of slice blockIdx.y.
+// A warp reads a token: D / 8 lanes a head's keys and values, eight channels each, the heads of slice blockIdx.y. What hides
+// the loads is other warps: with two or four heads' loads in flight, and the registers for them, 8192 tokens take 1.7 and 2.0 us more.
 template <int D, int G>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadParams p) {
     constexpr int L = D / 8, kPer = 32 / L;
@@ -328,27 +329,29 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadParams p) {
     const unsigned char* tile = p.pool.data + (static_cast<size_t>(page) * p.pool.heads * tiles + in_page / kv4::kTile) * p.pool.tile_bytes;
     const int k_at = kv4::k_word_at(D, t, ch), v_at = kv4::v_codes_at(D) + kv4::v_piece_at(D, t, ch % 32 / 4) + ch / 32 * 2;
     const int word = (t * (D / G) + ch / G) * 4;
-#pragma unroll 4
-    for (int i = blockIdx.y * kPer + sub; i < 2 * p.pool.heads; i += gridDim.y * kPer) {
-        const bool is_v = i >= p.pool.heads;
-        const int head = is_v ? i - p.pool.heads : i;
-        uint32_t out[4] = {};
+    auto write = [&](__nv_bfloat16* to, uint32_t codes, uint32_t w) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(__uint_as_float((codes >> (4 * j) & 15u) | 0x4b000000u) - 8388608.0f, kv4::word_scale(w), kv4::word_min(w));
+        uint32_t out[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+            out[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        *reinterpret_cast<uint4*>(to) = make_uint4(out[0], out[1], out[2], out[3]);
+    };
+#pragma unroll 1
+    for (int head = blockIdx.y * kPer + sub; head < p.pool.heads; head += gridDim.y * kPer) {
+        uint32_t kc = 0, vc = 0, kw = 0, vw = 0;
         if (there) {
             const unsigned char* at = tile + static_cast<size_t>(head) * tiles * p.pool.tile_bytes;
-            uint32_t codes;
-            if (is_v) codes = *reinterpret_cast<const uint16_t*>(at + v_at) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + v_at + D / 2)) << 16;
-            else codes = *reinterpret_cast<const uint32_t*>(at + k_at);
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + (is_v ? kv4::v_words_at(D, G) : kv4::k_words_at(D)) + word);
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = fmaf(__uint_as_float((codes >> (4 * j) & 15u) | 0x4b000000u) - 8388608.0f, kv4::word_scale(w), kv4::word_min(w));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-                out[j] = *reinterpret_cast<const uint32_t*>(&v);
-            }
+            kc = *reinterpret_cast<const uint32_t*>(at + k_at);
+            vc = *reinterpret_cast<const uint16_t*>(at + v_at) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + v_at + D / 2)) << 16;
+            kw = *reinterpret_cast<const uint32_t*>(at + kv4::k_words_at(D) + word), vw = *reinterpret_cast<const uint32_t*>(at + kv4::v_words_at(D, G) + word);
         }
-        *reinterpret_cast<uint4*>((is_v ? p.v : p.k) + (static_cast<size_t>(n) * p.pool.heads + head) * D + ch) = make_uint4(out[0], out[1], out[2], out[3]);
+        const size_t to = (static_cast<size_t>(n) * p.pool.heads + head) * D + ch;
+        write(p.k + to, kc, kw), write(p.v + to, vc, vw);
     }
 }
 
@@ -373,7 +376,7 @@ struct Append {
 template <int D, int G>
 struct Read {
     static int run(const ReadParams& p, int sms, cudaStream_t stream) {
-        const int blocks = cdiv(p.n, 8), steps = cdiv(2 * p.pool.heads, 256 / D);
+        const int blocks = cdiv(p.n, 8), steps = cdiv(p.pool.heads, 256 / D);
         const int slices = std::max(1, std::min(steps, 16 * sms / blocks));
         SPK_CUDA(launch_chained(kv4_read_kernel<D, G>, dim3(blocks, slices), dim3(256), 0, stream, p));
         return SPK_OK;
