@@ -152,6 +152,7 @@ extern "C" int spk_add_rmsnorm(const void* x, long long x_stride, const void* y,
                 "add_rmsnorm: pointers must be 16-byte aligned");
     SPK_REQUIRE(x_stride % 8 == 0 && y_stride % 8 == 0 && gate_stride % 8 == 0 && x_stride >= 0 && y_stride >= 0 && gate_stride >= 0,
                 "add_rmsnorm: row strides must be multiples of 8");
+    SPK_REQUIRE(r == nullptr || r != x || x_stride == hidden || rows == 1, "add_rmsnorm: r may be x where its rows are contiguous, got a stride of %lld", x_stride);
     DeviceState* dev = nullptr;
     if (int rc = device_state(&dev)) return rc;
     NormParams p{};

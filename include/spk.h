@@ -165,19 +165,20 @@ SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int3
                                         int K, const float* scale_a, const float* scale_b, void* stream);
 
 /* ---- 4-bit KV cache and the row operations of a decode step ------------------------------------
- * No counterpart in the reference for the 4-bit cache (its own is bf16). A pool is bytes
- * [pages][kv_heads][page_size / 16][spk_kv4_tile_bytes(head_dim, group)], 16-byte aligned; a tile is 16 tokens of
- * one head: K codes, V codes, then per token and group of `group` channels a word (minimum in the low
- * half, scale in the high half, bf16), K's and V's. A code c stands for c * scale + minimum; the order of the codes
- * inside a tile is the kernels' (csrc/kv4_layout.cuh). head_dim 64 or 128; group 32, 64 or 128, at most
- * head_dim; page_size a multiple of 16 up to 1024.
+ * No counterpart in the reference for the 4-bit cache (its own is bf16). A pool is bytes [pages][kv_heads][page_size /
+ * 16][spk_kv4_tile_bytes(head_dim, group)], 16-byte aligned; a tile is 16 tokens of one head: K codes, V codes, then per
+ * token and group of `group` channels a word (minimum in the low half, scale in the high half, bf16), K's and V's. A
+ * code c stands for c * scale + minimum; the order of the codes inside a tile is the kernels' (csrc/kv4_layout.cuh).
+ * head_dim 64 or 128; group 32, 64 or 128, at most head_dim; page_size a multiple of 16 up to 1024.
  * A call's sequences: lens int32 [seqs] on the device, tokens in the cache INCLUDING this call's; page_table int32
- * [seqs][table_width] on the device, the pages of a sequence in order; q_offsets int32 [seqs + 1] on the device, the call's
- * rows of sequence b are q_offsets[b] .. q_offsets[b + 1] - 1 and they are its last tokens; NULL: one row per
+ * [seqs][table_width] on the device, the pages of a sequence in order; q_offsets int32 [seqs + 1] on the device, the
+ * call's rows of sequence b are q_offsets[b] .. q_offsets[b + 1] - 1 and they are its last tokens; NULL: one row per
  * sequence (rows == seqs). Row i of n of a sequence thus has position lens - n + i; a row of negative position is
- * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest (without q_offsets there are none). A page outside the pool and a
- * position outside the rotation's table are skipped, the rows of a sequence whose length is negative or past its row of the table
- * are padding, and all are reported as SPK_BAD_INDEX by spk_device_status. seqs <= 4096, table_width * page_size <= 2^30. Nothing here uses the shared split-K scratch: calls on different streams may overlap. */
+ * padding. Rows behind the last sequence are left as they were, or set to zero with zero_rest (without q_offsets there
+ * are none). A page outside the pool and a position outside the rotation's table are skipped, the rows of a sequence
+ * whose length is negative or past its row of the table are padding, and all are reported as SPK_BAD_INDEX by
+ * spk_device_status. seqs <= 4096, table_width * page_size <= 2^30. Nothing here uses the shared split-K scratch: calls
+ * on different streams may overlap. */
 SPK_API int spk_kv4_tile_bytes(int head_dim, int group); /* 0 for an unsupported pair */
 /* qkv bf16 [rows], rows qkv_stride elements apart, each q_heads + 2 kv_heads vectors of head_dim: rotates the first
  * rot_dim channels of q and k (halves; cos_sin fp32 [positions][rot_dim]: cosines, then sines), writes q_out bf16
@@ -205,7 +206,7 @@ SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* poo
  * forms that other blocks have. z = y, or with post_gain rmsnorm(y) * post_gain; r = bf16(residual_scale * x + gate * z);
  * h = bf16(rmsnorm(r) * gain), rmsnorm(v) = v / sqrt(mean(v^2) + eps), all in fp32. y NULL: r is x (and not written).
  * gain NULL: no h. gate bf16, rows gate_stride elements apart (0: one row for all). x, y, r, h bf16 [rows][hidden], x and y with row
- * strides; r may be x. hidden a multiple of 8, at most 65536; 16-byte aligned pointers, strides multiples of 8. */
+ * strides; r may be x if x_stride is hidden. hidden a multiple of 8, at most 65536; 16-byte aligned pointers, strides multiples of 8. */
 SPK_API int spk_add_rmsnorm(const void* x, long long x_stride, const void* y, long long y_stride, const void* gain, const void* post_gain,
                             const void* gate, long long gate_stride, float residual_scale, float eps, void* r, void* h, int rows,
                             int hidden, void* stream);

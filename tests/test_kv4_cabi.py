@@ -99,3 +99,8 @@ def test_outputs_in_the_inputs_memory(lib, at):
     for out in (base + 16, base + 2048 + 16, base + 2048 + 4080):  # qkv: two rows of 2 KiB at base + 2048
         rc = lib.spk_kv4_append(base + 2048, 1024, at(1), 4, 16, 4, 2, 128, 64, at(2), 2, at(3), None, 2, 2, at(6), 8, 128, out, 0, None)
         _refused(lib, rc, "q_out must not be in qkv's memory")
+
+
+def test_norm_in_place_needs_contiguous_rows(lib, at):
+    rc = lib.spk_add_rmsnorm(at(0), 72, at(1), 64, at(2), None, None, 0, 1.0, 1e-5, at(0), at(4), 2, 64, None)
+    _refused(lib, rc, "r may be x")
