@@ -344,10 +344,10 @@ __device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq
         most = max(most >> 16, most & 0xffffu);
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = static_cast<int>(most >> 7);  // biased exponent of the row's largest |q|
+        const int e = max(1, static_cast<int>(most >> 7));  // biased exponent of the row's largest |q|; below the normal numbers as theirs
         const bool finite = e < 255;
-        float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23) : 0.0f;
-        const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
+        float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(254 - e) << 23) : 0.0f;  // down x up = 1
+        const float up = finite ? __uint_as_float(static_cast<uint32_t>(e) << 23) : __uint_as_float(0x7fc00000u);
         if (p.scale < 0.0f) down = -down;
         uint4 q[NW];
 #pragma unroll

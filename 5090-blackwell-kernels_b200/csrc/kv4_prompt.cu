@@ -186,11 +186,11 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(q) + i) : uint4{};
             most = __vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
         }
-        const int e = static_cast<int>(max(most >> 16, most & 0xffffu) >> 7);  // biased exponent of the row's largest |q|
+        const int e = max(1, static_cast<int>(max(most >> 16, most & 0xffffu) >> 7));  // biased exponent of the row's largest |q|; below the normal numbers as theirs
         const bool finite = e < 255;
-        float down = __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(max(1, 254 - e)) << 23);
+        float down = __uint_as_float(e >= 254 ? 0x00400000u : static_cast<uint32_t>(254 - e) << 23);  // down x up = 1
         if (p.scale < 0.0f) down = -down;
-        const float up = finite ? __uint_as_float(static_cast<uint32_t>(max(1, e)) << 23) : __uint_as_float(0x7fc00000u);
+        const float up = finite ? __uint_as_float(static_cast<uint32_t>(e) << 23) : __uint_as_float(0x7fc00000u);
         const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
         const bool work = tile < tiles && steps > 0;
         if (work) {
