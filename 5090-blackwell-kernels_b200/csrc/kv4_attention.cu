@@ -185,7 +185,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                 for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
             }
 #pragma unroll
-            for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k]);
+            for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k] & 0x7fffffffu);  // s may be negative in a pool of the caller's
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {

@@ -168,7 +168,8 @@ SPK_API int spk_grouped_gemm_swiglu_fp8(const void* A, const void* W, const int3
  * No counterpart in the reference for the 4-bit cache (its own is bf16). A pool is bytes [pages][kv_heads][page_size /
  * 16][spk_kv4_tile_bytes(head_dim, group)], 16-byte aligned; a tile is 16 tokens of one head: K codes, V codes, then per
  * token and group of `group` channels a word (minimum in the low half, scale in the high half, bf16), K's and V's. A
- * code c stands for c * scale + minimum; the order of the codes inside a tile is the kernels' (csrc/kv4_layout.cuh).
+ * code c stands for c * scale + minimum, whatever the scale's sign (spk_kv4_append writes none below 0); the order of the
+ * codes inside a tile is the kernels' (csrc/kv4_layout.cuh).
  * head_dim 64 or 128; group 32, 64 or 128, at most head_dim; page_size a multiple of 16 up to 1024.
  * A call's sequences: lens int32 [seqs] on the device, tokens in the cache INCLUDING this call's; page_table int32
  * [seqs][table_width] on the device, the pages of a sequence in order; q_offsets int32 [seqs + 1] on the device, the

@@ -26,3 +26,43 @@ def test_queries_at_the_ends_of_the_range(sk, lens, news, hq, hkv, power):
     assert torch.equal(q.double(), n.double() * 2.0 ** power)
     got, want, slack = _attend(sk, g, lens, news, 16, hq, hkv, 128, 64, scale=2.0 ** -power / 40 * 128 ** -0.5, q=q)
     _check(got, want, slack, f"2^{power}")
+
+
+def _cache(sk, g, n, hkv, d, group, spoil, page=64):
+    """One sequence of n tokens appended to a cache; spoil(x [n, 2, hkv, d]) changes its keys and values before."""
+    pages = -(-n // page)
+    cache = sk.KV4Cache(pages + 2, hkv, d, page, group)
+    table = torch.randperm(pages + 2, generator=g)[:pages].reshape(1, pages).to(torch.int32)
+    x = torch.randn(n, 2, hkv, d, generator=g)
+    spoil(x)
+    off = torch.tensor([0, n], dtype=torch.int32).cuda()
+    sk.kv4_append(x.to(torch.bfloat16).reshape(n, -1).cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), None, off)
+    return cache, table
+
+
+def _attend_last(sk, cache, table, n, q, scale, rows):
+    """q [new tokens, heads, d], the sequence's last ones -> (got, want, slack) of the named rows."""
+    news = q.shape[0]
+    off = None if news == 1 else torch.tensor([0, news], dtype=torch.int32).cuda()
+    got = sk.kv4_attention(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), off, scale=scale)
+    k, v = ref.unpack(cache.pool, cache.head_dim, cache.group)
+    parts = [ref.attention(q[r: r + 1], k, v, table.tolist(), [n - news + r + 1], None, scale, 0) for r in rows]
+    return got[rows], torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+
+
+@pytest.mark.parametrize("n,news,hq,hkv", [(200, 1, 4, 2), (60000, 1, 4, 2), (400, 150, 32, 16)])
+@pytest.mark.parametrize("which", ["keys", "values"])
+def test_scales_below_zero(sk, n, news, hq, hkv, which):
+    """A pool of the caller's whose scales are negative or -0 in a third of the tiles each: c * scale + minimum all the same. The
+    keys are then up to three times as large: a quarter of the usual scale keeps the scores' error below its bound."""
+    g = torch.Generator().manual_seed(31)
+    d, group = 128, 64
+    cache, table = _cache(sk, g, n, hkv, d, group, lambda x: None)
+    at = 16 * d + (64 * (d // group) if which == "values" else 0)
+    words = cache.pool[..., at: at + 64 * (d // group)].contiguous().view(torch.bfloat16)  # ..., minimum, scale, ...
+    s = words[..., 1::2]
+    kind = torch.randint(0, 3, (*s.shape[:3], 1), generator=g).cuda()
+    words[..., 1::2] = torch.where(kind == 0, s, torch.where(kind == 1, -s, torch.full_like(s, -0.0)))
+    cache.pool[..., at: at + 64 * (d // group)] = words.view(torch.uint8)
+    got, want, slack = _attend_last(sk, cache, table, n, _bf16(g, news, hq, d), 0.25 * d ** -0.5, list(range(0, news, 7)))
+    _check(got, want, slack, which)
