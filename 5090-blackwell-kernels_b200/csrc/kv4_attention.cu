@@ -292,7 +292,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                 for (int x = 0; x < 4; ++x) {
                     const uint32_t w = vw[t][x >> 1][k];
                     float sv = kv4::word_scale(w), mid = fmaf(8.0f, sv, kv4::word_min(w));
-                    if (Masked && pr[x] == 0.0f) sv = mid = 0.0f;  // a row that does not see the token: it may be a NaN
+                    if (Masked && sc[n][t][x] == -INFINITY) sv = mid = 0.0f;  // a row that does not see the token: it may be a NaN
                     ps[x] = pr[x] * (sv * scale_s);
                     st.z[n][k][x & 1] = fmaf(pr[x], mid, st.z[n][k][x & 1]);
                 }

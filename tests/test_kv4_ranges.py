@@ -66,3 +66,21 @@ def test_scales_below_zero(sk, n, news, hq, hkv, which):
     cache.pool[..., at: at + 64 * (d // group)] = words.view(torch.uint8)
     got, want, slack = _attend_last(sk, cache, table, n, _bf16(g, news, hq, d), 0.25 * d ** -0.5, list(range(0, news, 7)))
     _check(got, want, slack, which)
+
+
+@pytest.mark.parametrize("n", [20, 64, 60000])
+def test_values_that_are_no_numbers_under_weights_that_vanish(sk, n):
+    """A value that is a NaN spoils the rows that see it whatever its weight: 0 x NaN is no number. The first two lengths are read in
+    steps with tokens out of sight; the last is cut over all CTAs, most of them without the token."""
+    g = torch.Generator().manual_seed(33)
+
+    def spoil(x):
+        x[5, 0] = -30  # scores below -300: a weight that fp32 does not hold
+        x[5, 1, 0, 3] = float("nan")
+
+    cache, table = _cache(sk, g, n, 2, 128, 64, spoil)
+    q = 1 + _bf16(g, 1, 4, 128).abs()
+    out = torch.isnan(sk.kv4_attention(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda()).cpu())
+    want = torch.zeros_like(out)
+    want[:, :2, :64] = True
+    assert torch.equal(out, want)
