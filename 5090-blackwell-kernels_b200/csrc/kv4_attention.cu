@@ -12,9 +12,11 @@
 //        q' = q 2^-e fits fp16 exactly (bf16 has fewer bits; e the exponent of the row's largest |q|), the products are exact
 //        in fp32, and four to eight MMAs a group leave the offset no room to cost precision
 //     V  sum p v = sum (p s)(c - 8) + sum p (8 s + m): here the offsets are taken out before the MMA (a sum over the whole
-//        sequence of values with a large common offset would drift), p s is rounded to fp16 against a power of two
-//        that follows the largest s so far (2^-11 each, unbiased; bf16 would lose another half step of the output), and the
-//        second sum is fp32.
+//        sequence of values with a large common offset would drift), and the second sum is fp32. p s is rounded to fp16
+//        (2^-11 of it, unbiased; bf16 would lose another half step of the output) times a power of two of its row's and
+//        group's own, which puts the largest p s so far at 2^3 to 2^4: rounded in full down to 2^-17 of that, gone below
+//        2^-28, so that a group loses at most keys x 2^-28 of its largest p s, however loud other groups, or tokens without
+//        weight, may be. (One power for a warp, after its largest s, was 2 % faster and lost the groups 2^20 below it.)
 // P^T comes out of S^T's accumulator layout by movmatrix (one 8 x 8 transpose per register).
 //
 // Work is cut into equal contiguous ranges of (sequence, block of rows, KV head, 16-token tile) units over the resident
@@ -158,8 +160,20 @@ struct State {
     float start[NQ][kGroups][2], q_sum[NQ][kGroups][2], mult[NQ][2];
     // the running softmax: maxima (in powers of two), sums, values (channels 32 u + 4 g + {0, 2} in o[2 u], {1, 3} in o[2 u + 1]), sum p (8 s + m)
     float top[NQ][2], sum[NQ][2], o[NQ][D / 16][4], z[NQ][kGroups][2];
-    int ref;  // biased exponent of the largest s so far: what p s is scaled against
+    // by column and group, the power of two that p s is multiplied by before fp16 and that o carries; and, of what this lane
+    // reads, the largest |s| with which no p up to 2^kSlack makes p s too large for fp16
+    float lift[NQ][kGroups][2], safe[kGroups];
 };
+
+// The running maximum lags behind by up to kSlack; the largest p s of a column and group, seen from there, is lifted to 2^(kLift - 1)
+// to 2^kLift, and p s may reach 2^15.
+constexpr float kSlack = 6.0f;
+constexpr int kLift = 4;
+__device__ __forceinline__ float lift_of(float largest) {  // 2^126 for none
+    const int e = static_cast<int>((__float_as_uint(largest) + 0x7fffffu) >> 23);
+    return __uint_as_float(static_cast<uint32_t>(min(254 + kLift - e, 253)) << 23);
+}
+__device__ __forceinline__ float inverse_of(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 
 // kSteps tiles of 16 tokens. Masked: some token is out of some row's sight, or a tile is missing (ok: the tiles that are there).
 template <int D, int G, int NQ, int H, bool Masked>
@@ -167,8 +181,10 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
     constexpr int NG = D / G / H, NW = D / 32, kTileBytes = kv4::tile_bytes(D, G);
     const int g = lane >> 2, c = lane & 3;
     const int my_words = H == 2 ? (c >> 1) * NG * 4 : 0;  // where the words of this lane's columns begin in a token's
-    float sc[NQ][kSteps][4];
-    uint32_t vw[kSteps][2][NG], most = 0;
+    float sc[NQ][kSteps][4], most[NG];
+    uint32_t vw[kSteps][2][NG];
+#pragma unroll
+    for (int k = 0; k < NG; ++k) most[k] = 0.0f;
 #pragma unroll
     for (int t = 0; t < kSteps; ++t) {
         const unsigned char* tile = tiles + t * kTileBytes;
@@ -185,7 +201,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                 for (int k = 0; k < NG; ++k) kw[x][k] = seen ? kw[x][k] : 0, vw[t][x][k] = seen ? vw[t][x][k] : 0;
             }
 #pragma unroll
-            for (int k = 0; k < NG; ++k) most = max(most, vw[t][x][k] & 0x7fffffffu);  // s may be negative in a pool of the caller's
+            for (int k = 0; k < NG; ++k) most[k] = fmaxf(most[k], fabsf(__uint_as_float(vw[t][x][k])));  // m in the low bits does not matter
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
@@ -233,11 +249,12 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                 }
         }
     }
-    // ---- running maximum, reference exponent: moved only when some score is 2^kSlack over the maximum or some s over
-    // the reference (p is then at most 2^kSlack, p s scale_s below 2^(8 + kSlack)), so most steps need no shuffle
-    constexpr float kSlack = 6.0f;
+    // ---- running maximum and lifts: moved only when some score is 2^kSlack over the maximum or some s too large for the
+    // lifts, so most steps need no shuffle
     float high[NQ][2];
-    bool over = static_cast<int>(most >> 23) > st.ref;
+    bool over = false;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) over |= most[k] > st.safe[k];
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -249,9 +266,9 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
             over |= high[n][x] > st.top[n][x] + kSlack;
         }
     if (__any_sync(0xffffffffu, over)) {
-        const int ref = max(st.ref, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 23));
-        const float fall = ref - st.ref > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - ref + st.ref) << 23);
-        st.ref = ref;
+        float widest[NG];
+#pragma unroll
+        for (int k = 0; k < NG; ++k) widest[k] = INFINITY;
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -261,16 +278,41 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                 m = fmaxf(m, st.top[n][x]);
-                const float keep = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m), both = keep * fall;
+                const float keep = st.top[n][x] == -INFINITY ? 0.0f : ptx::exp2_fast(st.top[n][x] - m);
                 st.sum[n][x] *= keep;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) st.z[n][k][x] *= keep;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) st.o[n][i][x] *= both, st.o[n][i][x + 2] *= both;
                 st.top[n][x] = m;
+                const float shift = m == -INFINITY ? 0.0f : m;
+                float p[kSteps][2];
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) p[t][y] = ptx::exp2_fast(fmaf(sc[n][t][x + 2 * y], st.mult[n][x], -shift));
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    st.z[n][k][x] *= keep;
+                    // the largest p s: of the tokens before, of these (0 x infinity is passed over)
+                    float largest = keep * 0x1p4f * inverse_of(st.lift[n][k][x]);
+#pragma unroll
+                    for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) largest = fmaxf(largest, p[t][y] * fabsf(kv4::word_scale(vw[t][y][k])));
+                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 4));
+                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 8));
+                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 16));
+                    const float lift = lift_of(largest), both = keep == 0.0f ? 0.0f : keep * (lift * inverse_of(st.lift[n][k][x]));
+                    st.lift[n][k][x] = lift;
+                    if (m != -INFINITY) widest[k] = fminf(widest[k], inverse_of(lift));
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) {
+                        if (32 * i / G % NG != k) continue;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) st.o[n][2 * i + (y >> 1)][x + 2 * (y & 1)] *= both;
+                    }
+                }
             }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) st.safe[k] = 512.0f * widest[k];
     }
-    const float scale_s = __uint_as_float(static_cast<uint32_t>(261 - st.ref) << 23);  // s scale_s < 2^8
     // ---- weights and values
 #pragma unroll
     for (int t = 0; t < kSteps; ++t) {
@@ -293,7 +335,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
                     const uint32_t w = vw[t][x >> 1][k];
                     float sv = kv4::word_scale(w), mid = fmaf(8.0f, sv, kv4::word_min(w));
                     if (Masked && sc[n][t][x] == -INFINITY) sv = mid = 0.0f;  // a row that does not see the token: it may be a NaN
-                    ps[x] = pr[x] * (sv * scale_s);
+                    ps[x] = pr[x] * (sv * st.lift[n][k][x & 1]);
                     st.z[n][k][x & 1] = fmaf(pr[x], mid, st.z[n][k][x & 1]);
                 }
                 pf[n][k][0] = ptx::transpose_8x8(ptx::f16x2_pack(ps[0], ps[1]));
@@ -598,12 +640,13 @@ kv4_attend_split_kernel(const AttendParams p) {
 #pragma unroll
                     for (int k = 0; k < NG; ++k) {
                         st.start[n][k][x] = task.start[n][k][2 * c + x], st.q_sum[n][k][x] = task.q_sum[n][k][2 * c + x];
-                        st.z[n][k][x] = 0.0f;
+                        st.z[n][k][x] = 0.0f, st.lift[n][k][x] = lift_of(0.0f);
                     }
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) st.o[n][i][x] = st.o[n][i][x + 2] = 0.0f;
                 }
-            st.ref = 8;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) st.safe[k] = INFINITY;  // the first score that any row sees is over its maximum
             int base = s.tile0 * kv4::kTile;
             for (int left = s.tiles; left > 0; left -= kSteps, base += kSteps * kv4::kTile) {
                 if (alive) alive = __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, p.status));
@@ -621,7 +664,6 @@ kv4_attend_split_kernel(const AttendParams p) {
             // ---- what the warp has of the piece: to the output if that is all of it, else kept for the CTA's end
             const bool whole = s.begins && s.ends, last = u >= end;
             float* part = last ? reinterpret_cast<float*>(ring) : parts + (2 + warp) * Cfg::kPart;
-            const float unscale = __uint_as_float(static_cast<uint32_t>(st.ref - 7) << 23);
             const int first = task.first, count = task.count, block = s.block, head = s.head;
             if (last) __syncwarp();  // every lane is past the ring
 #pragma unroll
@@ -636,7 +678,7 @@ kv4_attend_split_kernel(const AttendParams p) {
                     }
                     const bool second = H == 2 && c >= 2;  // H = 2: a lane's columns hold one half of the channels
                     const int row = 8 * n + (H == 2 ? (2 * c + x) & 3 : 2 * c + x), r = block * R + row;
-                    const float l = st.sum[n][x], k = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l, ku = k * unscale;
+                    const float l = st.sum[n][x], k = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
                     __nv_bfloat16* to = p.out + (static_cast<size_t>(first + r / group) * p.q_heads + head * group + r % group) * D + 4 * g;
 #pragma unroll
                     for (int i = 0; i < NW / H; ++i) {
@@ -645,7 +687,7 @@ kv4_attend_split_kernel(const AttendParams p) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const float a = st.o[n][2 * i + (j & 1)][x + (j & 2)], b = st.o[n][(2 * i + (j & 1) + (H - 1) * NW) % (D / 16)][x + (j & 2)];
-                            f[j] = whole ? fmaf(second ? b : a, ku, st.z[n][32 * i / G % NG][x] * k) : fmaf(second ? b : a, unscale, st.z[n][32 * i / G % NG][x]);
+                            f[j] = fmaf((second ? b : a) * k, inverse_of(st.lift[n][32 * i / G % NG][x]), st.z[n][32 * i / G % NG][x] * k);
                         }
                         if (!whole) {
                             *reinterpret_cast<float4*>(part + row * D + ch + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);

@@ -50,6 +50,11 @@ def _attend_last(sk, cache, table, n, q, scale, rows):
     return got[rows], torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
 
 
+def _check_groups(got, want, slack, group, what):
+    for at in range(0, got.shape[-1], group):
+        _check(got[..., at: at + group], want[..., at: at + group], slack[..., at: at + group], f"{what}, channels {at}..")
+
+
 @pytest.mark.parametrize("n,news,hq,hkv", [(200, 1, 4, 2), (60000, 1, 4, 2), (400, 150, 32, 16)])
 @pytest.mark.parametrize("which", ["keys", "values"])
 def test_scales_below_zero(sk, n, news, hq, hkv, which):
@@ -66,6 +71,58 @@ def test_scales_below_zero(sk, n, news, hq, hkv, which):
     cache.pool[..., at: at + 64 * (d // group)] = words.view(torch.uint8)
     got, want, slack = _attend_last(sk, cache, table, n, _bf16(g, news, hq, d), 0.25 * d ** -0.5, list(range(0, news, 7)))
     _check(got, want, slack, which)
+
+
+def _opposed(x, at):
+    """Token `at` gets keys that every query of positive channels scores far below the others: its weight is nothing."""
+    x[at, 0] = -3
+
+
+@pytest.mark.parametrize("n", [150, 30000])
+@pytest.mark.parametrize("power", [8, 12, 16, 20, 40])
+@pytest.mark.parametrize("hq,hkv,d,group", [(4, 1, 128, 64), (8, 1, 128, 32), (16, 1, 64, 32), (2, 1, 64, 64), (16, 1, 128, 128)])
+def test_quiet_values_beside_loud_ones(sk, hq, hkv, d, group, power, n):
+    """Values of the first 32 channels (all of them where they are one group) 2^power louder: of the whole sequence, of one token with
+    an ordinary weight, of one token with next to none. Every group of channels is as near to 64 bits as it would be alone."""
+    def every(x):
+        x[:, 1, :, :32] *= 2.0 ** power
+
+    def one(x):
+        x[3, 1, :, :32] *= 2.0 ** power
+
+    def weightless(x):
+        x[3, 1, :, :32] *= 2.0 ** power
+        _opposed(x, 3)
+
+    g = torch.Generator().manual_seed(power + n)
+    for spoil in (every, one, weightless):
+        cache, table = _cache(sk, g, n, hkv, d, group, spoil)
+        q = _bf16(g, 1, hq, d).abs()
+        got, want, slack = _attend_last(sk, cache, table, n, q, d ** -0.5, [0])
+        _check_groups(got, want, slack, group, spoil.__name__)
+
+
+@pytest.mark.parametrize("power", [12, 18, 30])
+@pytest.mark.parametrize("hq,d,group", [(64, 128, 64), (160, 64, 32), (320, 128, 64)])
+def test_quiet_values_beside_loud_ones_in_long_ranges(sk, hq, d, group, power):
+    """The same where a warp reads some 250 tokens of a head on its own: loud groups, and every 50th token loud and nearly without weight."""
+    n, hkv = 16000, 32
+
+    def every(x):
+        x[:, 1, :, :32] *= 2.0 ** power
+
+    def weightless(x):
+        x[::50, 1, :, :32] *= 2.0 ** power
+        _opposed(x, slice(None, None, 50))
+
+    g = torch.Generator().manual_seed(power)
+    for spoil in (every, weightless):
+        cache, table = _cache(sk, g, n, hkv, d, group, spoil)
+        q = _bf16(g, 1, hq, d).abs()
+        got = sk.kv4_attention(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())[:, : hq // hkv]
+        k, v = ref.unpack(cache.pool[:, :1], d, group)
+        want, slack = ref.attention(q[:, : hq // hkv], k, v, table.tolist(), [n], None, d ** -0.5, 0)
+        _check_groups(got, want, slack, group, spoil.__name__)
 
 
 @pytest.mark.parametrize("n", [20, 64, 60000])
