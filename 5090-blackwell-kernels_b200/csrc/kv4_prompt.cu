@@ -7,16 +7,20 @@
 // words into K' and V', every value (c s + m) 2^-e rounded once to fp16 (2^-11 of it), e the exponent of 16 tokens' largest
 // |m| + 15 s, so that nothing overflows or vanishes whatever the scale. S is put right by 2^e of the keys; for the values 2^e
 // joins the softmax's exponent: with M the running maximum of score + e,
-//     P = 2^(score + e - M),      sum += P 2^-e,      out = O / sum,
-// fp32 but for P's rounding to fp16. Eight warps hold the softmax, a row a thread. M is the maximum of a row's first keys and
-// moves only when weights come near fp16's end, so O (in TMEM) is rarely touched between the MMAs and the maximum
-// rarely looked for (S is then read again: its 64 scores need not stay in registers until the weights are known to fit).
+//     P = 2^(score + e - M + 4),      sum += P 2^-e,      out = O / sum,
+// fp32 but for P's rounding to fp16. Values quieter than the loudest so far take the loudest's e, or one 16 above their own if that
+// is less: V' has the room, and P would run out of it. So a value is held to 2^-11 of itself and 2^-32 of the largest so far, in
+// whatever group, and a weight to 2^-11 and, while tokens are within 2^16 of each other, 2^-29 of the largest weight (one bit
+// less for each past that). The tensor core's sums are fp32. Eight warps hold the softmax, a row a thread. M is the maximum
+// of a row's first keys and moves only when weights come near fp16's end, so O (in TMEM) is rarely touched between the MMAs
+// and the maximum rarely looked for (S is then read again: its 64 scores need not stay in registers until the weights are
+// known to fit).
 // K' rows are keys, 128 bytes = 64 channels wide (the order of the channels inside eights is the codes' own; Q' is
 // stored in the same order); V' rows are keys too, and the MMA reads them MN-major; the order of its columns is the codes',
 // put right when O is written.
 //
 // Bound: the roles' latencies, not the tensor cores (36 % active). 2 x 2048 new tokens on 6144 old ones, 32 heads over 8, d = 128:
-// 654 us = 736 TFLOP/s (0.45 of the measured cuBLAS rate); a step of 64 keys takes some 2700 cycles where its MMAs take 1084
+// 674 us = 714 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2700 cycles where its MMAs take 1084
 // and its exponentials 1024. By device clocks a row warp has about 2300 cycles of work a step (1200 for the weights, the
 // rest waits that are already over, TMEM loads and stores, exponents), a code warp 1900, an MMA warp 1600 (some hundred
 // cycles for each MMA that it issues). 256 rows a block share the conversion of the codes; 128 keys a step would halve the
@@ -36,8 +40,12 @@ using kv4::AttendParams;
 constexpr int kKeys = 64, kRowWarps = 8, kKWarp = 8, kVWarp = 12, kMmaWarp = 16, kThreadsP = 640;
 constexpr int kRowRegs = 144, kCodeRegs = 72, kMmaRegs = 48;
 constexpr int kInfos = 8;       // steps whose exponents are kept: the code warps are at most four ahead of a row warp
-constexpr float kMost = 32768.0f;  // what 16 weights may add up to before the maximum moves: then none overflows fp16
+// A weight at the maximum is 2^4, so that fp16 holds weights down to 2^-29 of it (2 x 2048 rows on 8192: 658 us with 2^0, 668 with 2^4,
+// 678 with 2^6, 686 with 2^8: the higher, the more often the maximum moves).
+constexpr int kLevel = 4;
+constexpr float kMost = 60000.0f;  // what 16 weights may add up to before the maximum moves: then none overflows fp16
 constexpr int kFit = 14;        // |K'|, |V'| < 2^14
+constexpr int kSpare = 16;      // V' of tokens quieter than the loudest so far stays that many bits lower, at most
 
 // What the code warps say of 16 keys: of the keys 2^(e - 14), and which are not finite; of the values e and 2^-e (negative if any
 // is not finite), and then which, by group.
@@ -96,6 +104,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
     unsigned char *q_smem = smem, *k_smem = q_smem + 2 * Cfg::kRows, *v_smem = k_smem + 2 * Cfg::kOperand, *raw_smem = v_smem + 2 * Cfg::kOperand;
     __shared__ PromptBars bars;
     __shared__ TileInfo infos[kInfos][4];
+    __shared__ int loudest[kInfos];  // the exponent above the values of a step and of all before it
     __shared__ uint32_t raw_there[Cfg::kRaw];  // which tiles of a slot were copied
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_block;
@@ -268,7 +277,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         float m = x[16 * t];
 #pragma unroll
                         for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
-                        most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
+                        most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t] - kLevel));
                     }
                     keep = top == -INFINITY ? 0.0f : exp2f(top - fmaxf(top, most_here));
                     top = fmaxf(top, most_here);
@@ -367,6 +376,27 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             const unsigned char* tiles_at = raw_smem + slot * Cfg::kStep + 2 * w * Cfg::kTile;
             // ---- the words, one or a few a lane: their size, and what is not finite; 0 for a key that no row sees
             constexpr int kPerLane = (Cfg::kWords + 31) / 32;
+            int loud = 0;
+            if (is_v) {  // the exponent above all values so far, two keys a lane; the step's two warps find the same
+                const uint2* at = reinterpret_cast<const uint2*>(raw_smem + slot * Cfg::kStep + (lane >> 3) * Cfg::kTile + words_at + (lane & 7) * 8 * NG);
+                const int key = key0 + j * kKeys + 2 * lane;
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const uint2 two = at[i];
+                    const uint32_t x = two.x & 0x7fff7fffu, y = two.y & 0x7fff7fffu;
+                    const int kx = key + 2 * i / NG, ky = key + (2 * i + 1) / NG;
+                    if (kx >= any_lo && kx < any_hi && !__vcmpgeu2(x, 0x7f807f80u)) most = __vmaxu2(most, x);
+                    if (ky >= any_lo && ky < any_hi && !__vcmpgeu2(y, 0x7f807f80u)) most = __vmaxu2(most, y);
+                }
+                if (!(raw_there[slot] >> (lane >> 3) & 1)) most = 0;
+                loud = exponent_of(__float_as_uint(fminf(fmaf(15.0f, kv4::word_scale(most), kv4::word_min(most)), 3.4e38f)));
+                if (j > 0) {
+                    if (alive) alive = __all_sync(kAll, ptx::mbar_wait(&bars.info[(j - 1) % kInfos], ((j - 1) / kInfos) & 1, p.status));
+                    loud = max(loud, loudest[(j - 1) % kInfos]);
+                }
+                if (w == 0 && lane == 0) loudest[j % kInfos] = loud;
+            }
 #pragma unroll 1
             for (int u = 0; u < 2; ++u) {  // not unrolled, as below: the roles share the instruction caches (684 -> 654 us)
                 float s[kPerLane], m[kPerLane];
@@ -380,7 +410,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                     s[i] = kv4::word_scale(x), m[i] = kv4::word_min(x);
                     size = max(size, __float_as_uint(fminf(fmaf(15.0f, fabsf(s[i]), fabsf(m[i])), 3.4e38f)));
                 }
-                const int e = exponent_of(size);
+                int e = exponent_of(size);
+                if (is_v) e = min(loud, e + kSpare);
                 const float fit = power_of_two(kFit - e);
 #pragma unroll
                 for (int i = 0; i < kPerLane; ++i)

@@ -197,7 +197,10 @@ SPK_API int spk_kv4_read(const void* pool, int pages, int page_size, int kv_head
 /* out bf16 [rows][q_heads][head_dim] = softmax(scale q k^T) v over the tokens at positions <= the row's own (window > 0:
  * only the last `window` of them), fp32 sums; zeros where there are none. q bf16, rows q_stride elements apart; q_heads a
  * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads); out must not lie in what q's rows span. workspace: spk_kv4_attention_workspace(...) bytes of
- * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter. */
+ * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter.
+ * Weights enter the products in fp16, each off by 2^-11 of itself, and by 2^-28 of the row's largest (with few rows a
+ * sequence: largest weight x scale of the group; in prompts, where values do as well, off by 2^-11 of themselves and 2^-32
+ * of the largest value up to there, in any group: a weight 2^-29, one bit less for each past 2^16 between tokens' values). */
 SPK_API long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim);
 SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
                               int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,

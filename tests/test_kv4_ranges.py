@@ -50,9 +50,16 @@ def _attend_last(sk, cache, table, n, q, scale, rows):
     return got[rows], torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
 
 
-def _check_groups(got, want, slack, group, what):
+def _check_groups(got, want, slack, group, what, held=0.0):
+    """_check of every group by itself; held: what an output may be off by besides."""
     for at in range(0, got.shape[-1], group):
-        _check(got[..., at: at + group], want[..., at: at + group], slack[..., at: at + group], f"{what}, channels {at}..")
+        g, w, s = (t[..., at: at + group] for t in (got, want, slack))
+        if held == 0.0:
+            _check(g, w, s, f"{what}, channels {at}..")
+            continue
+        off = (g.double().cpu() - w).abs()
+        assert torch.isfinite(g).all() and (off <= w.abs() * 2 ** -8 + (2 ** -11 + 2.2e-2) * s + held).all(), f"{what}, channels {at}.."
+        assert off.norm() <= 1.5 * 2 ** -8 * w.norm() + held * w.numel() ** 0.5, f"{what}, channels {at}.."
 
 
 @pytest.mark.parametrize("n,news,hq,hkv", [(200, 1, 4, 2), (60000, 1, 4, 2), (400, 150, 32, 16)])
@@ -125,6 +132,32 @@ def test_quiet_values_beside_loud_ones_in_long_ranges(sk, hq, d, group, power):
         _check_groups(got, want, slack, group, spoil.__name__)
 
 
+@pytest.mark.parametrize("n", [150, 4000])
+@pytest.mark.parametrize("power", [8, 12, 16, 20, 28])
+@pytest.mark.parametrize("d,group", [(128, 64), (64, 32), (128, 128)])
+def test_quiet_values_beside_loud_ones_in_prompts(sk, d, group, power, n):
+    """In prompts a value is c s' + m' in fp16, s' and m' being the group's times 2^(14 - e), 2^e the power above the largest |m| + 15 s of its
+    16 tokens. Where s' and m' are below fp16's normal numbers each is off by up to 2^-25, and so is the result: 17 x 2^-25 x 2^(e - 14) of
+    the value. |m| is at most the largest |v|, 15 s at most twice that and a rounding: 2^e is at most 2 x 3.03 of it and the
+    value off by at most 2^-32 of the largest value."""
+    def every(x):
+        x[:, 1, :, :32] *= 2.0 ** power
+
+    def one(x):
+        x[3, 1, :, :32] *= 2.0 ** power
+
+    def weightless(x):
+        x[3, 1, :, :32] *= 2.0 ** power
+        _opposed(x, 3)
+
+    g = torch.Generator().manual_seed(power + n)
+    for spoil in (every, one, weightless):
+        cache, table = _cache(sk, g, n, 16, d, group, spoil)
+        q = _bf16(g, 150, 32, d).abs()
+        got, want, slack = _attend_last(sk, cache, table, n, q, d ** -0.5, [20, 149])
+        _check_groups(got, want, slack, group, spoil.__name__, held=2.0 ** -32 * slack.amax().item())
+
+
 @pytest.mark.parametrize("n", [20, 64, 60000])
 def test_values_that_are_no_numbers_under_weights_that_vanish(sk, n):
     """A value that is a NaN spoils the rows that see it whatever its weight: 0 x NaN is no number. The first two lengths are read in
@@ -141,3 +174,27 @@ def test_values_that_are_no_numbers_under_weights_that_vanish(sk, n):
     want = torch.zeros_like(out)
     want[:, :2, :64] = True
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("first", [1.0, 0.0])
+def test_many_small_weights_beside_a_large_one_in_prompts(sk, first):
+    """A key at 2^25.1 times the weight of each of 2^18 others, which together have 1 % of the sum. Its value is 1 or 0, theirs 1: the
+    output is 1 or that percent. Keys and values are exact in fp16 here; the large weight is 2^4, the others 2^-21.1 in steps of 2^-24:
+    off by up to 2^-25, 2^-3.8 of them. The values' products are 2^13 times that, summed in fp32. A sum of 2^17, which the large one
+    makes, ends at 2^-6 and may drop each of the others, 2^-8.1, whole; without it the sum ends below 2^10, its last bit is 2^-14
+    and may be cut off each, 2^-5.8 of it."""
+    d, hkv, page, n = 128, 16, 1024, 1 << 18
+    cache = sk.KV4Cache(4, hkv, d, page, 64)
+    x = torch.ones(2 * page, 2, hkv, d)
+    x[:, 0] = 0
+    x[0, 0] = 1.5390625  # its score is 128 x that x 128^-1/2 = 25.12 ln 2
+    x[0, 1] = first
+    off, lens = torch.tensor([0, 2 * page], dtype=torch.int32).cuda(), torch.tensor([2 * page], dtype=torch.int32).cuda()
+    sk.kv4_append(x.reshape(2 * page, -1).to(torch.bfloat16).cuda(), cache, torch.tensor([[3, 1]], dtype=torch.int32).cuda(), lens, None, off)
+    table = torch.tensor([[3] + (n // page - 1) * [1]], dtype=torch.int32).cuda()  # pages may be shared for reading
+    q = torch.ones(150, 2 * hkv, d, dtype=torch.bfloat16).cuda()
+    got = sk.kv4_attention(q, cache, table, torch.tensor([n], dtype=torch.int32).cuda(), torch.tensor([0, 150], dtype=torch.int32).cuda()).double().cpu()
+    small = (n - 150 + torch.arange(150, dtype=torch.float64)) * 2.718281828459045 ** (-1.5390625 * 128 ** 0.5)
+    want = ((first + small) / (1 + small))[:, None, None]
+    tol = 2 ** -9 + 2 ** -11 + small / (1 + small) if first else want.flatten() * (2 ** -8 + 2 ** -3.8 + 2 ** -5.8)
+    assert ((got - want).abs() <= tol[:, None, None]).all(), got.aminmax()
