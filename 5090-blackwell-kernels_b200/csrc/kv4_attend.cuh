@@ -26,6 +26,17 @@ constexpr int kPromptRows = 128, kBlockRows = 256, kPromptBlocks = 32;
 
 __host__ __device__ inline long long prompt_blocks(long long rows) { return rows >= kPromptRows ? (rows + kBlockRows - 1) / kBlockRows : 0; }
 
+#ifdef __CUDACC__
+// A row's queries go into the products in fp16, times a power of two that puts the largest of them, of biased exponent e, at 2^13 to
+// 2^14 (as near as a power of two comes to that where e is below 13). And its inverse, by which the scores are put right.
+__device__ __forceinline__ float query_scale(int e) { return __uint_as_float(static_cast<uint32_t>(min(267 - e, 254)) << 23); }
+__device__ __forceinline__ float query_unscale(float by) {
+    const uint32_t bits = (254u << 23) - __float_as_uint(by);
+    return __uint_as_float(bits == 0 ? 0x00400000u : bits);
+}
+constexpr float kLeast = 1.4e-45f;  // above 0
+#endif
+
 // kv4_prompt.cu: the call's prompts; nothing if they are too few.
 int attend_prompts(const AttendParams& p, int head_dim, int group, DeviceState* dev, cudaStream_t stream);
 

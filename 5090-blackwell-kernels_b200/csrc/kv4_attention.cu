@@ -9,8 +9,8 @@
 // The codes go into the MMA as small integers in fp16, built by one LOP3 per pair (a nibble or-ed into the mantissa of
 // 1024 reads 1024 + c, one nibble higher into that of 64 reads 64 + c); the words are applied outside it:
 //     K  q . k = sum over groups of s (sum (c + o) q' - sum o q') + m sum q'   with the o-sums of q as the accumulator's start;
-//        q' = q 2^-e fits fp16 exactly (bf16 has fewer bits; e the exponent of the row's largest |q|), the products are exact
-//        in fp32, and four to eight MMAs a group leave the offset no room to cost precision
+//        q' = q 2^(13 - e) (e the exponent of the row's largest |q|) fits fp16 exactly, but for channels below 2^-30 of the
+//        largest; the products are exact in fp32, and four to eight MMAs a group leave the offset no room to cost precision
 //     V  sum p v = sum (p s)(c - 8) + sum p (8 s + m): here the offsets are taken out before the MMA (a sum over the whole
 //        sequence of values with a large common offset would drift), and the second sum is fp32. p s is rounded to fp16
 //        (2^-11 of it, unbiased; bf16 would lose another half step of the output) times a power of two of its row's and
@@ -386,10 +386,11 @@ __device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq
         most = max(most >> 16, most & 0xffffu);
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = max(1, static_cast<int>(most >> 7));  // biased exponent of the row's largest |q|; below the normal numbers as theirs
+        const int e = static_cast<int>(most >> 7);  // biased exponent of the row's largest |q|
         const bool finite = e < 255;
-        float down = finite ? __uint_as_float(e == 254 ? 0x00400000u : static_cast<uint32_t>(254 - e) << 23) : 0.0f;  // down x up = 1
-        const float up = finite ? __uint_as_float(static_cast<uint32_t>(e) << 23) : __uint_as_float(0x7fc00000u);
+        const float to_fp16 = kv4::query_scale(e);
+        float down = finite ? to_fp16 : 0.0f;
+        const float up = finite ? kv4::query_unscale(to_fp16) : __uint_as_float(0x7fc00000u);
         if (p.scale < 0.0f) down = -down;
         uint4 q[NW];
 #pragma unroll
@@ -408,7 +409,7 @@ __device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq
         const int hi = there ? max(0, pos + 1) : 0, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         if (c == 0) {
             // never 0: masked scores are -inf times it
-            task.mult[n][g] = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);
+            task.mult[n][g] = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, kv4::kLeast) + (up - up);
             task.lo[n][g] = lo, task.hi[n][g] = hi;
         }
         // the sums over a group of what the codes' offsets multiply: 1024 the even channels, 64 the odd ones

@@ -195,12 +195,12 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             const uint4 w = there ? __ldg(reinterpret_cast<const uint4*>(q) + i) : uint4{};
             most = __vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
         }
-        const int e = max(1, static_cast<int>(max(most >> 16, most & 0xffffu) >> 7));  // biased exponent of the row's largest |q|; below the normal numbers as theirs
+        const int e = static_cast<int>(max(most >> 16, most & 0xffffu) >> 7);  // biased exponent of the row's largest |q|
         const bool finite = e < 255;
-        float down = __uint_as_float(e >= 254 ? 0x00400000u : static_cast<uint32_t>(254 - e) << 23);  // down x up = 1
+        float down = kv4::query_scale(e);
+        const float up = finite ? kv4::query_unscale(down) : __uint_as_float(0x7fc00000u);
         if (p.scale < 0.0f) down = -down;
-        const float up = finite ? __uint_as_float(static_cast<uint32_t>(e) << 23) : __uint_as_float(0x7fc00000u);
-        const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, 1.2e-38f) + (up - up);  // never 0: masked scores are -inf times it
+        const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, kv4::kLeast) + (up - up);  // never 0: masked scores are -inf times it
         const bool work = tile < tiles && steps > 0;
         if (work) {
             const int r = (warp & 3) * 32 + lane;
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const float4 of = *reinterpret_cast<const float4*>(&info[t]);
-                unit[t] = fmaxf(of.x * mult, 1.2e-38f), v_exp[t] = of.z, v_unit[t] = fabsf(of.w);
+                unit[t] = fmaxf(of.x * mult, kv4::kLeast), v_exp[t] = of.z, v_unit[t] = fabsf(of.w);
                 bad |= __float_as_uint(of.y) | __float_as_uint(of.w) >> 31;
             }
             if (bad) {

@@ -198,3 +198,18 @@ def test_many_small_weights_beside_a_large_one_in_prompts(sk, first):
     want = ((first + small) / (1 + small))[:, None, None]
     tol = 2 ** -9 + 2 ** -11 + small / (1 + small) if first else want.flatten() * (2 ** -8 + 2 ** -3.8 + 2 ** -5.8)
     assert ((got - want).abs() <= tol[:, None, None]).all(), got.aminmax()
+
+
+@pytest.mark.parametrize("n,news,hq,hkv,power", [(200, 1, 4, 2, p) for p in (12, 16, 20, 24, 28)] + [(300, 1, 20, 2, 28)] + [(200, 150, 32, 16, p) for p in (12, 16, 20)])
+def test_quiet_queries_of_loud_keys(sk, n, news, hq, hkv, power):
+    """The second group's queries 2^power quieter than the first's and its keys as much louder: both have their part in the scores. In prompts
+    a key is held to 2^-32 of the largest of its 16 tokens' (see the values below), which times 2^20 and a sum of |q| is nothing."""
+    def spoil(x):
+        x[:, 0, :, 64:] *= 2.0 ** power
+
+    g = torch.Generator().manual_seed(power)
+    cache, table = _cache(sk, g, n, hkv, 128, 64, spoil)
+    q = torch.randn(news, hq, 128, generator=g)
+    q[..., 64:] *= 2.0 ** -power
+    q = q.to(torch.bfloat16)
+    _check(*_attend_last(sk, cache, table, n, q, 128 ** -0.5, list(range(0, news, 31))), f"2^{power}")
