@@ -409,7 +409,7 @@ __device__ __forceinline__ void write_task(const AttendParams& p, const Seq& seq
         const int hi = there ? max(0, pos + 1) : 0, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         if (c == 0) {
             // never 0: masked scores are -inf times it
-            task.mult[n][g] = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, kv4::kLeast) + (up - up);
+            task.mult[n][g] = fmaxf(fabsf(p.scale) * (1.4426950408889634f * up), kv4::kLeast) + (up - up);
             task.lo[n][g] = lo, task.hi[n][g] = hi;
         }
         // the sums over a group of what the codes' offsets multiply: 1024 the even channels, 64 the odd ones

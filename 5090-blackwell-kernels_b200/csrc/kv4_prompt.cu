@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         float down = kv4::query_scale(e);
         const float up = finite ? kv4::query_unscale(down) : __uint_as_float(0x7fc00000u);
         if (p.scale < 0.0f) down = -down;
-        const float mult = fmaxf(fabsf(p.scale) * 1.4426950408889634f * up, kv4::kLeast) + (up - up);  // never 0: masked scores are -inf times it
+        const float mult = fmaxf(fabsf(p.scale) * (1.4426950408889634f * up), kv4::kLeast) + (up - up);  // never 0: masked scores are -inf times it
         const bool work = tile < tiles && steps > 0;
         if (work) {
             const int r = (warp & 3) * 32 + lane;

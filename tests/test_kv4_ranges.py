@@ -213,3 +213,14 @@ def test_quiet_queries_of_loud_keys(sk, n, news, hq, hkv, power):
     q[..., 64:] *= 2.0 ** -power
     q = q.to(torch.bfloat16)
     _check(*_attend_last(sk, cache, table, n, q, 128 ** -0.5, list(range(0, news, 31))), f"2^{power}")
+
+
+@pytest.mark.parametrize("lens,news,hq,hkv", [FEW, PROMPT])
+@pytest.mark.parametrize("scale", [2.5e38, 3e38, -3e38])
+def test_scales_of_the_scores_at_the_end_of_the_range(sk, lens, news, hq, hkv, scale):
+    """As large as the entry takes, with queries below the normal numbers: n 2^-133 x 3e38 is n / 36, and n is some three in size."""
+    g = torch.Generator().manual_seed(41)
+    rows = len(lens) if news is None else sum(news)
+    q = ((3 * torch.randn(rows, hq, 128, generator=g)).round().double() * 2.0 ** -133).to(torch.bfloat16)
+    got, want, slack = _attend(sk, g, lens, news, 16, hq, hkv, 128, 64, scale=scale, q=q)
+    _check(got, want, slack, f"{scale}")
