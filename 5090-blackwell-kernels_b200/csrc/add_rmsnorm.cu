@@ -5,6 +5,8 @@
 // rmsnorm(v) = v / sqrt(mean(v^2) + eps). All sums in fp32; the unfused order (python/spark_kernels/engine.py:441-456 of
 // the reference) writes and re-reads the residual between the two kernels. Bound by memory: x and y in, r and h out, 8
 // bytes an element.
+#include <initializer_list>
+
 #include "spk_common.cuh"
 
 namespace spk {
@@ -21,7 +23,7 @@ struct NormParams {
 struct Eight {
     float v[8];
 };
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }  // not __ldg: r or h may take its place
 __device__ __forceinline__ Eight unpack8(const uint4& w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     Eight e;
@@ -153,6 +155,23 @@ extern "C" int spk_add_rmsnorm(const void* x, long long x_stride, const void* y,
     SPK_REQUIRE(x_stride % 8 == 0 && y_stride % 8 == 0 && gate_stride % 8 == 0 && x_stride >= 0 && y_stride >= 0 && gate_stride >= 0,
                 "add_rmsnorm: row strides must be multiples of 8");
     SPK_REQUIRE(r == nullptr || r != x || x_stride == hidden || rows == 1, "add_rmsnorm: r may be x where its rows are contiguous, got a stride of %lld", x_stride);
+    // a block reads its row of x, y and the gate before it writes it, so an output may take the place of one of them row by row
+    const struct {
+        const char* name;
+        const void* at;
+        long long stride;
+        bool vector;
+    } inputs[] = {{"x", x, x_stride, false}, {"y", y, y_stride, false}, {"the gate", gate, gate_stride, false}, {"the gain", gain, 0, true}, {"post_gain", post_gain, 0, true}};
+    const long long bytes = 2ll * rows * hidden;
+    for (const auto& in : inputs) {
+        if (in.at == nullptr) continue;
+        for (const void* out : {r, h}) {
+            if (out == nullptr || !overlap(out, bytes, in.at, in.vector ? 1 : rows, in.stride, hidden)) continue;
+            SPK_REQUIRE(out == in.at && !in.vector && (in.stride == hidden || rows == 1), "add_rmsnorm: %s must not lie in the memory of %s, except in its place where its rows are contiguous",
+                        out == r ? "r" : "h", in.name);
+        }
+    }
+    SPK_REQUIRE(r == nullptr || h == nullptr || !overlap(r, bytes, h, rows, hidden, hidden), "add_rmsnorm: r and h must not share memory");
     DeviceState* dev = nullptr;
     if (int rc = device_state(&dev)) return rc;
     NormParams p{};

@@ -880,7 +880,7 @@ extern "C" int spk_kv4_attention(const void* q, long long q_stride, const void* 
     SPK_REQUIRE(static_cast<long long>(rows) * (q_heads / kv_heads) <= INT32_MAX / 2, "kv4_attention: rows x query heads per KV head must stay below 2^30");
     SPK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= spk_kv4_attention_workspace(rows, seqs, q_heads, kv_heads, head_dim),
                 "kv4_attention: the workspace must be 16-byte aligned and hold spk_kv4_attention_workspace() bytes, got %lld", workspace_bytes);
-    SPK_REQUIRE(!kv4::overlap(out, 2ll * rows * q_heads * head_dim, q, rows, q_stride, static_cast<long long>(q_heads) * head_dim), "kv4_attention: out must not be in q's memory");
+    SPK_REQUIRE(!overlap(out, 2ll * rows * q_heads * head_dim, q, rows, q_stride, static_cast<long long>(q_heads) * head_dim), "kv4_attention: out must not be in q's memory");
     DeviceState* dev = nullptr;
     if (int rc = device_state(&dev)) return rc;
     p.q = static_cast<const __nv_bfloat16*>(q), p.stride = q_stride;

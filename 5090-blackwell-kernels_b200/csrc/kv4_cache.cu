@@ -405,7 +405,7 @@ extern "C" int spk_kv4_append(const void* qkv, long long qkv_stride, void* pool,
     SPK_REQUIRE(aligned16(qkv) && aligned16(q_out) && aligned16(cos_sin), "kv4_append: qkv, q_out and cos_sin must be 16-byte aligned");
     SPK_REQUIRE(qkv_stride >= static_cast<long long>(q_heads + 2 * kv_heads) * head_dim && qkv_stride % 8 == 0,
                 "kv4_append: rows of qkv must be at least (q_heads + 2 kv_heads) head_dim apart and a multiple of 8, got %lld", qkv_stride);
-    SPK_REQUIRE(!kv4::overlap(q_out, 2ll * rows * q_heads * head_dim, qkv, rows, qkv_stride, static_cast<long long>(q_heads + 2 * kv_heads) * head_dim),
+    SPK_REQUIRE(!overlap(q_out, 2ll * rows * q_heads * head_dim, qkv, rows, qkv_stride, static_cast<long long>(q_heads + 2 * kv_heads) * head_dim),
                 "kv4_append: q_out must not be in qkv's memory");
     DeviceState* dev = nullptr;
     if (int rc = device_state(&dev)) return rc;

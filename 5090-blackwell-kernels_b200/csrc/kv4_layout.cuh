@@ -87,10 +87,4 @@ inline int check_batch(const char* what, const Batch& s, int page_size) {
     return SPK_OK;
 }
 
-// Whether an output of `bytes` lies in memory that `rows` rows of `row` elements span, `stride` apart, all bf16.
-inline bool overlap(const void* out, long long bytes, const void* in, long long rows, long long stride, long long row) {
-    const char *a = static_cast<const char*>(out), *b = static_cast<const char*>(in);
-    return a < b + 2 * ((rows - 1) * stride + row) && b < a + bytes;
-}
-
 }  // namespace spk::kv4

@@ -43,6 +43,12 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether an output of `bytes` lies in memory that `rows` rows of `row` elements span, `stride` apart, all bf16.
+inline bool overlap(const void* out, long long bytes, const void* in, long long rows, long long stride, long long row) {
+    const char *a = static_cast<const char*>(out), *b = static_cast<const char*>(in);
+    return a < b + 2 * ((rows - 1) * stride + row) && b < a + bytes;
+}
+
 // Scratch every split-K kernel shares on one device. Allocated once per device on first use
 // (or by spk_init), never moved or freed, so pointers baked into captured CUDA graphs stay
 // valid. The kernels leave partials and counters zeroed when they finish.

@@ -210,7 +210,9 @@ SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* poo
  * forms that other blocks have. z = y, or with post_gain rmsnorm(y) * post_gain; r = bf16(residual_scale * x + gate * z);
  * h = bf16(rmsnorm(r) * gain), rmsnorm(v) = v / sqrt(mean(v^2) + eps), all in fp32. y NULL: r is x (and not written).
  * gain NULL: no h. gate bf16, rows gate_stride elements apart (0: one row for all). x, y, r, h bf16 [rows][hidden], x and y with row
- * strides; r may be x if x_stride is hidden. hidden a multiple of 8, at most 65536; 16-byte aligned pointers, strides multiples of 8. */
+ * strides. r and h may each take the place of x, y or the gate, where its rows are `hidden` apart; otherwise neither may lie
+ * in an input's memory, nor in each other's. hidden a multiple of 8, at most 65536; 16-byte aligned pointers, strides
+ * multiples of 8. */
 SPK_API int spk_add_rmsnorm(const void* x, long long x_stride, const void* y, long long y_stride, const void* gain, const void* post_gain,
                             const void* gate, long long gate_stride, float residual_scale, float eps, void* r, void* h, int rows,
                             int hidden, void* stream);

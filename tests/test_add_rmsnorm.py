@@ -113,3 +113,18 @@ def test_refusals(sk):
     ):
         with pytest.raises((RuntimeError, ValueError)):
             call()
+
+
+@pytest.mark.parametrize("rows,hidden", [(3, 4096), (700, 264), (400, 8200), (3, 40000)])
+def test_outputs_in_the_place_of_inputs(sk, rows, hidden):
+    """The C entry with r and h in the place of x, y or a gate with rows: the same bits as beside them."""
+    g = torch.Generator().manual_seed(4)
+    x, y, gate, gain, post = _bf16(g, rows, hidden), _bf16(g, rows, hidden), _bf16(g, rows, hidden), _bf16(g, hidden), _bf16(g, hidden)
+    want = sk.add_rmsnorm(x, y, gain, post_gain=post, gate=gate, residual_scale=0.5)
+    stream = torch.cuda.current_stream().cuda_stream
+    for r_in, h_in in (("x", None), ("y", "x"), ("gate", "y"), (None, "gate")):
+        t = {"x": x.clone(), "y": y.clone(), "gate": gate.clone(), None: None}
+        r, h = (torch.empty_like(x) if name is None else t[name] for name in (r_in, h_in))
+        assert sk._C._spk_add_rmsnorm(t["x"].data_ptr(), hidden, t["y"].data_ptr(), hidden, gain.data_ptr(), post.data_ptr(), t["gate"].data_ptr(), hidden,
+                                      0.5, 1e-5, r.data_ptr(), h.data_ptr(), rows, hidden, stream) == 0
+        assert torch.equal(r, want[0]) and torch.equal(h, want[1]), (r_in, h_in)

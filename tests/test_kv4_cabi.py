@@ -104,3 +104,34 @@ def test_outputs_in_the_inputs_memory(lib, at):
 def test_norm_in_place_needs_contiguous_rows(lib, at):
     rc = lib.spk_add_rmsnorm(at(0), 72, at(1), 64, at(2), None, None, 0, 1.0, 1e-5, at(0), at(4), 2, 64, None)
     _refused(lib, rc, "r may be x")
+
+
+def test_norm_outputs_in_the_inputs_memory(lib, at):
+    """r or h anywhere in what x, y, a gate or the gains span, or in each other; in the place of one with contiguous rows they
+    are not refused (without a GPU the call then ends at the device)."""
+    buf = ctypes.create_string_buffer(16384)
+    base = ctypes.addressof(buf)
+    base += -base % 16
+    place = dict(x=base, y=base + 1024, gain=base + 2048, post=base + 3072, gate=base + 4096, r=base + 5120, h=base + 6144)
+
+    def call(xs=64, ys=64, gs=64, rows=2, **kw):
+        a = place | kw
+        return lib.spk_add_rmsnorm(a["x"], xs, a["y"], ys, a["gain"], a["post"], a["gate"], gs, 1.0, 1e-5, a["r"], a["h"], rows, 64, None)
+
+    for out in ("r", "h"):
+        for name, word in (("x", "of x"), ("y", "of y"), ("gain", "of the gain"), ("post", "of post_gain"), ("gate", "of the gate")):
+            size = 128 if name in ("gain", "post") else 256
+            for shift in (16 - 256, -128, 16, size - 16):
+                _refused(lib, call(**{out: place[name] + shift}), word)
+        _refused(lib, call(**{out: place["gain"]}), "of the gain")
+        _refused(lib, call(**{out: place["y"]}, ys=72), "of y")
+        _refused(lib, call(**{out: place["y"]}, ys=0), "of y")
+        _refused(lib, call(**{out: place["gate"]}, gs=0), "of the gate")
+        _refused(lib, call(**{out: place["gate"] + 112}, gs=0), "of the gate")
+        for name in ("x", "y", "gate"):
+            assert call(**{out: place[name]}) != 1, (out, name, lib.spk_last_error())
+        assert call(**{out: place["y"]}, ys=72, rows=1) != 1
+        assert call(**{out: place["gate"] + 128}, gs=0) != 1  # behind the one row that there is
+    _refused(lib, call(h=place["x"], xs=72), "of x")
+    _refused(lib, call(h=place["r"]), "share")
+    _refused(lib, call(h=place["r"] + 240), "share")
