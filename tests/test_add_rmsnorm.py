@@ -128,3 +128,26 @@ def test_outputs_in_the_place_of_inputs(sk, rows, hidden):
         assert sk._C._spk_add_rmsnorm(t["x"].data_ptr(), hidden, t["y"].data_ptr(), hidden, gain.data_ptr(), post.data_ptr(), t["gate"].data_ptr(), hidden,
                                       0.5, 1e-5, r.data_ptr(), h.data_ptr(), rows, hidden, stream) == 0
         assert torch.equal(r, want[0]) and torch.equal(h, want[1]), (r_in, h_in)
+
+
+@pytest.mark.parametrize("hidden", [8, 1024, 1032, 2040, 2048, 2056, 5120, 8184, 8192, 8200, 20000, 32768, 32776, 65536])
+@pytest.mark.parametrize("more", [0, 1, 400])
+@pytest.mark.parametrize("form", ["plain", "all", "partial"])
+def test_many_rows_against_64_bits(sk, hidden, more, form):
+    """From two rows an SM up other blocks are launched, by the number of channels: every one at a full size, the next larger and a last
+    piece that is not full, with the last count of rows of the other launch and the first of this."""
+    rows = 2 * torch.cuda.get_device_properties(0).multi_processor_count + more
+    g = torch.Generator().manual_seed(hidden + rows)
+    x, y, gain = 4 * _bf16(g, rows, hidden), _bf16(g, rows, hidden), _bf16(g, hidden)
+    if form == "partial":
+        r, h = sk.add_rmsnorm(x, gain=gain, eps=1e-6)
+        assert r is x
+        _check(x, None, gain, 1e-6, None, None, 1.0, x, h)
+        r, h = sk.add_rmsnorm(x, y, post_gain=gain)
+        assert h is None
+        return _check(x, y, None, 1e-5, gain, None, 1.0, r, None)
+    post = _bf16(g, hidden) if form == "all" else None
+    gate = _bf16(g, rows, hidden) if form == "all" else None
+    scale = 0.7071 if form == "all" else 1.0
+    r, h = sk.add_rmsnorm(x, y, gain, eps=1e-6, post_gain=post, gate=gate, residual_scale=scale)
+    _check(x, y, gain, 1e-6, post, gate, scale, r, h)
