@@ -76,7 +76,7 @@ struct PromptCfg {
 
 struct PromptBars {
     // by stage; by tile of rows and buffer (a step's parity); by tile; by step; by slot
-    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], info[kInfos], raw_full[4], raw_empty[4];
+    uint64_t q_ready, k_full[2], v_full[2], s_full[2][2], p_full[2][2], before_last[2], o_full[2], drained[2], info[kInfos], raw_full[4], raw_empty[4];
 };
 
 // Eight codes (nibble n of w), four fp16 pairs (n, n + 4) of (c s + m).
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&bars.k_full[i], 2), ptx::mbar_init(&bars.v_full[i], 2);
             for (int k = 0; k < 2; ++k) ptx::mbar_init(&bars.s_full[i][k], 1), ptx::mbar_init(&bars.p_full[i][k], 4);
-            ptx::mbar_init(&bars.before_last[i], 1), ptx::mbar_init(&bars.o_full[i], 1);
+            ptx::mbar_init(&bars.before_last[i], 1), ptx::mbar_init(&bars.o_full[i], 1), ptx::mbar_init(&bars.drained[i], 1);
         }
         for (int i = 0; i < kInfos; ++i) ptx::mbar_init(&bars.info[i], 4);
         for (int i = 0; i < Cfg::kRaw; ++i) ptx::mbar_init(&bars.raw_full[i], 1), ptx::mbar_init(&bars.raw_empty[i], 4);
@@ -506,7 +506,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             }
             ptx::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]), ptx::mbar_arrive(&bars.raw_empty[slot]);
+            if (lane == 0) {
+                ptx::mbar_arrive(is_v ? &bars.v_full[stage] : &bars.k_full[stage]);
+                if (alive) ptx::mbar_arrive(&bars.raw_empty[slot]);  // a copy that was given up on may still write to the slot
+            }
         }
     } else {
         registers_down<kMmaRegs>();
@@ -518,10 +521,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
             const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTile;
             int key = key0 + (lane & 3) * kv4::kTile, at = key / kv4::kTile / tiles_per_page, in_page = key / kv4::kTile % tiles_per_page, page = -1;
             if (key < any_hi) page = __ldg(table + at);
-            bool ok = true;
-            for (int j = 0; ok && j < steps; ++j) {
+            int j = 0;
+            for (; j < steps; ++j) {
                 const int slot = j % Cfg::kRaw;
-                if (j >= Cfg::kRaw) ok = __all_sync(kAll, ptx::mbar_wait(&bars.raw_empty[slot], (j / Cfg::kRaw - 1) & 1, p.status));
+                if (j >= Cfg::kRaw && !__all_sync(kAll, ptx::mbar_wait(&bars.raw_empty[slot], (j / Cfg::kRaw - 1) & 1, p.status))) break;
                 const bool good = key < any_hi && page >= 0 && page < p.pool.pages;
                 if (key < any_hi && !good && lane < 4) atomicCAS(p.status, 0, SPK_BAD_INDEX);
                 const uint32_t there = __ballot_sync(kAll, good) & 15u;
@@ -543,6 +546,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 while (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
                 if (key < any_hi) page = __ldg(table + at);
             }
+            // no copy is on its way when the block ends, whoever gave up on what: the last one into each slot has landed
+            for (int k = max(0, j - Cfg::kRaw); k < j; ++k) ptx::mbar_wait(&bars.raw_full[k % Cfg::kRaw], (k / Cfg::kRaw) & 1, p.status);
         } else if (i < tiles && steps > 0) {
             // ---- the MMAs of a tile of rows, a warp for each (a warp's waits and commits alone take longer than a step's MMAs). The
             // scores run two steps ahead of the values, into the buffer whose P the values have just taken: the MMAs of a
@@ -579,6 +584,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 }
                 __syncwarp();
             }
+            // nor an MMA, which may be on its way still if this warp or a row warp gave up
+            if (umma::elect_one()) umma::mma_commit(&bars.drained[i]);
+            __syncwarp();
+            ptx::mbar_wait(&bars.drained[i], 0, p.status);
         }
     }
     umma::fence_before_sync();
