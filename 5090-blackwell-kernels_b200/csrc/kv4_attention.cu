@@ -567,6 +567,7 @@ kv4_attend_split_kernel(const AttendParams p) {
         const unsigned char* base = nullptr;
         const long long page_bytes = static_cast<long long>(p.pool.heads) * tiles_per_page * Cfg::kTileBytes;
         unsigned phase = 1;  // the first round of a ring is free
+        int filled = 0;
         auto settle = [&]() {  // to this lane's next step; false at the end of the range
             while (left <= 0) {
                 if (u >= end) return false;
@@ -607,18 +608,21 @@ kv4_attend_split_kernel(const AttendParams p) {
                 in_page += kSteps;
                 while (in_page >= tiles_per_page) in_page -= tiles_per_page, ++at;
                 if (++slot == S) slot = 0, phase ^= 1u;
+                ++filled;
                 filling = settle();
             }
             if (__any_sync(0xffffffffu, went)) {
                 since = clock64();
             } else {
-                if (clock64() - since > 2 * ptx::kWaitCycles) {  // the consumers gave up; what is in flight has long landed
+                if (__any_sync(0xffffffffu, clock64() - since > 2 * ptx::kWaitCycles)) {  // the consumers gave up
                     if (lane == 0) atomicCAS(p.status, 0, SPK_TIMEOUT);
                     break;
                 }
                 __nanosleep(20);
             }
         }
+        // no copy is on its way when the block ends, even if its consumer gave up on it: the last one into each slot has landed
+        for (int k = max(0, filled - S); k < filled; ++k) ptx::mbar_wait(&full[k % S], (k / S) & 1, p.status);
     } else {
         // ---- a consuming warp -----------------------------------------------------------------------------------------
         Task_& task = *reinterpret_cast<Task_*>(smem + Cfg::kRing + warp * Cfg::kTask);
@@ -658,7 +662,7 @@ kv4_attend_split_kernel(const AttendParams p) {
                 else
                     attend_step<D, G, NQ, H, false>(st, task, tiles, lane, ok, base);
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&empty[slot]);
+                if (lane == 0 && alive) ptx::mbar_arrive(&empty[slot]);  // a copy that was given up on may still write to the slot
                 if (++slot == S) slot = 0, phase ^= 1u;
             }
 

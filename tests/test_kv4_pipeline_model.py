@@ -1,5 +1,6 @@
-"""A CPU model of the hand-offs inside the attention kernel for prompts over the 4-bit cache (csrc/kv4_prompt.cu): its roles run as coroutines under a random scheduler, copies and MMAs complete at random later times (MMAs of one warp in their
-order), mbarriers count phases and are waited for by parity. The index arithmetic is the kernel's.
+"""A CPU model of the hand-offs inside the two attention kernels over the 4-bit cache (csrc/kv4_prompt.cu, csrc/kv4_attention.cu):
+their roles run as coroutines under a random scheduler, copies and MMAs complete at random later times (MMAs of one warp in their
+order), mbarriers count phases and are waited for by parity. The index arithmetic is the kernels'.
 
 Every wait names the completion it means, and fails if it passes before that; every buffer knows whose content it holds, and a
 read of another's fails. A wait may also give up, one chosen at random, and then whichever can no longer be met: the role goes
@@ -199,11 +200,57 @@ def prompt_block(steps, tiles, seed, give_up=None, drains=True):
     return b.waits
 
 
+def split_block(stages, fills, seed, give_up=None, drains=True):
+    """One consuming warp's ring; a warp that gave up reads on without waiting and hands nothing back, and the filler gives up on it."""
+    b = Block(seed, give_up)
+    full, empty = [Barrier(1) for _ in range(stages)], [Barrier(1) for _ in range(stages)]
+    ring = [None] * stages
+
+    def filler():
+        n = 0
+        while n < fills:
+            slot = n % stages
+            if n >= stages and not (yield from b.wait(empty[slot], n // stages - 1)):
+                break
+
+            def land(n=n, slot=slot):
+                ring[slot] = n
+                full[slot].arrive()
+
+            b.copies.append(land)
+            n += 1
+            yield
+        if drains:
+            for k in range(max(0, n - stages), n):
+                yield from b.wait(full[k % stages], k // stages, hardware=True)
+
+    def consumer():
+        alive = True
+        for n in range(fills):
+            alive = alive and (yield from b.wait(full[n % stages], n // stages))
+            b.hold(ring[n % stages], n, "ring")
+            yield
+            b.hold(ring[n % stages], n, "ring")
+            if alive:
+                empty[n % stages].arrive()
+
+    b.roles = [filler(), consumer()]
+    b.run()
+    return b.waits
+
+
 @pytest.mark.parametrize("tiles", [1, 2])
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 9, 20, 33])
 def test_prompt_block(steps, tiles):
     for seed in range(20):
         prompt_block(steps, tiles, seed)
+
+
+@pytest.mark.parametrize("fills", [1, 2, 5, 6, 7, 31])
+@pytest.mark.parametrize("stages", [2, 3, 6])
+def test_split_block(stages, fills):
+    for seed in range(20):
+        split_block(stages, fills, seed)
 
 
 def _ended_early(block, waits, **kw):
@@ -221,3 +268,10 @@ def test_prompt_block_whose_waits_give_up(steps, tiles):
     waits = prompt_block(steps, tiles, 0)
     assert _ended_early(prompt_block, waits, steps=steps, tiles=tiles) == 0
     assert _ended_early(prompt_block, waits, steps=steps, tiles=tiles, drains=False) > 0  # what the waits at the end are for
+
+
+@pytest.mark.parametrize("stages,fills", [(2, 9), (6, 20)])
+def test_split_block_whose_waits_give_up(stages, fills):
+    waits = split_block(stages, fills, 0)
+    assert _ended_early(split_block, waits, stages=stages, fills=fills) == 0
+    assert _ended_early(split_block, waits, stages=stages, fills=fills, drains=False) > 0
