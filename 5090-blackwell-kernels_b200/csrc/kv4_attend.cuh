@@ -28,12 +28,10 @@ __host__ __device__ inline long long prompt_blocks(long long rows) { return rows
 
 #ifdef __CUDACC__
 // A row's queries go into the products in fp16, times a power of two that puts the largest of them, of biased exponent e, at 2^13 to
-// 2^14 (as near as a power of two comes to that where e is below 13). And its inverse, by which the scores are put right.
-__device__ __forceinline__ float query_scale(int e) { return __uint_as_float(static_cast<uint32_t>(min(267 - e, 254)) << 23); }
-__device__ __forceinline__ float query_unscale(float by) {
-    const uint32_t bits = (254u << 23) - __float_as_uint(by);
-    return __uint_as_float(bits == 0 ? 0x00400000u : bits);
-}
+// 2^14; lower, down to 1, where it is below 2^-50: keys that give such queries their scores are large, and the sums stay inside
+// fp32. And its inverse, by which the scores are put right.
+__device__ __forceinline__ float query_scale(int e) { return __uint_as_float(static_cast<uint32_t>(254 - max(e, 1) + min(max(e - 64, 0), 13)) << 23); }
+__device__ __forceinline__ float query_unscale(float by) { return __uint_as_float((254u << 23) - __float_as_uint(by)); }
 constexpr float kLeast = 1.4e-45f;  // above 0
 #endif
 

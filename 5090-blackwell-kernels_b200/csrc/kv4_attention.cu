@@ -9,8 +9,8 @@
 // The codes go into the MMA as small integers in fp16, built by one LOP3 per pair (a nibble or-ed into the mantissa of
 // 1024 reads 1024 + c, one nibble higher into that of 64 reads 64 + c); the words are applied outside it:
 //     K  q . k = sum over groups of s (sum (c + o) q' - sum o q') + m sum q'   with the o-sums of q as the accumulator's start;
-//        q' = q 2^(13 - e) (e the exponent of the row's largest |q|) fits fp16 exactly, but for channels below 2^-30 of the
-//        largest; the products are exact in fp32, and four to eight MMAs a group leave the offset no room to cost precision
+//        q' = q 2^(13 - e) (e the exponent of the row's largest |q|; kv4_attend.cuh) fits fp16 exactly, but for channels below
+//        2^-30 of the largest; the products are exact in fp32, and four to eight MMAs a group leave the offset no room to cost precision
 //     V  sum p v = sum (p s)(c - 8) + sum p (8 s + m): here the offsets are taken out before the MMA (a sum over the whole
 //        sequence of values with a large common offset would drift), and the second sum is fp32. p s is rounded to fp16
 //        (2^-11 of it, unbiased; bf16 would lose another half step of the output) times a power of two of its row's and

@@ -224,3 +224,17 @@ def test_scales_of_the_scores_at_the_end_of_the_range(sk, lens, news, hq, hkv, s
     q = ((3 * torch.randn(rows, hq, 128, generator=g)).round().double() * 2.0 ** -133).to(torch.bfloat16)
     got, want, slack = _attend(sk, g, lens, news, 16, hq, hkv, 128, 64, scale=scale, q=q)
     _check(got, want, slack, f"{scale}")
+
+
+
+@pytest.mark.parametrize("n,news,hq,hkv", [(200, 1, 4, 2), (300, 1, 20, 2), (200, 150, 32, 16)])
+@pytest.mark.parametrize("power", [60, 100, 112])
+def test_huge_keys_of_tiny_queries(sk, n, news, hq, hkv, power):
+    """Keys 2^power and queries 2^-power times the usual: ordinary scores, through sums that stay inside fp32."""
+    def spoil(x):
+        x[:, 0] *= 2.0 ** power
+
+    g = torch.Generator().manual_seed(power)
+    cache, table = _cache(sk, g, n, hkv, 128, 64, spoil)
+    q = (torch.randn(news, hq, 128, generator=g) * 2.0 ** -power).to(torch.bfloat16)
+    _check(*_attend_last(sk, cache, table, n, q, 128 ** -0.5, list(range(0, news, 31))), f"2^{power}")
