@@ -165,13 +165,13 @@ extern "C" int spk_add_rmsnorm(const void* x, long long x_stride, const void* y,
     const long long bytes = 2ll * rows * hidden;
     for (const auto& in : inputs) {
         if (in.at == nullptr) continue;
-        for (const void* out : {r, h}) {
+        for (const void* out : {y == nullptr ? nullptr : r, h}) {  // r is not written without y
             if (out == nullptr || !overlap(out, bytes, in.at, in.vector ? 1 : rows, in.stride, hidden)) continue;
             SPK_REQUIRE(out == in.at && !in.vector && (in.stride == hidden || rows == 1), "add_rmsnorm: %s must not lie in the memory of %s, except in its place where its rows are contiguous",
                         out == r ? "r" : "h", in.name);
         }
     }
-    SPK_REQUIRE(r == nullptr || h == nullptr || !overlap(r, bytes, h, rows, hidden, hidden), "add_rmsnorm: r and h must not share memory");
+    SPK_REQUIRE(r == nullptr || h == nullptr || y == nullptr || !overlap(r, bytes, h, rows, hidden, hidden), "add_rmsnorm: r and h must not share memory");
     DeviceState* dev = nullptr;
     if (int rc = device_state(&dev)) return rc;
     NormParams p{};

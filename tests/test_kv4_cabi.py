@@ -135,3 +135,12 @@ def test_norm_outputs_in_the_inputs_memory(lib, at):
     _refused(lib, call(h=place["x"], xs=72), "of x")
     _refused(lib, call(h=place["r"]), "share")
     _refused(lib, call(h=place["r"] + 240), "share")
+
+
+def test_norm_without_y_does_not_look_at_r(lib, at):
+    """r is not written then, wherever it points."""
+    buf = ctypes.create_string_buffer(4096)
+    base = ctypes.addressof(buf)
+    base += -base % 16
+    for r in (base, base + 16, base + 1024, base + 2048 + 16):
+        assert lib.spk_add_rmsnorm(base, 64, None, 0, base + 1024, None, None, 0, 1.0, 1e-5, r, base + 2048, 2, 64, None) != 1, r - base
