@@ -106,7 +106,9 @@ class _Dense:
 class QuantizedDecoder:
     """Decoder whose projections run on this library. `decode(x, pos)` advances every sequence of the batch by
     one token: x [B, hidden] bf16 are the embedded tokens, pos [B] int64 their positions; the KV cache holds
-    `max_len` positions per sequence, in bf16, or with kv="int4" in 4 bits (head_dim 64 or 128)."""
+    `max_len` positions per sequence, in bf16, or with kv="int4" in 4 bits (head_dim 64 or 128). A position at or past max_len is
+    an error: the bf16 cache fails at the index; the 4-bit one leaves the token out of the cache, so that row's result means
+    nothing, and `_C.device_status()` returns 5 (a captured step cannot raise: ask after the steps whose lengths may have ended)."""
 
     def __init__(self, cfg: DecoderConfig, weights: list[dict], fmt: str = "int4", fuse_swiglu: bool = True,
                  batch: int = 1, max_len: int = 64, kv: str = "bf16"):

@@ -161,3 +161,22 @@ def test_four_bit_cache_fewer_sequences_than_slots(sk):
     with pytest.raises(RuntimeError):
         one.extend(torch.randn(2, cfg.hidden, device="cuda").to(torch.bfloat16), torch.ones(2, dtype=torch.int32).cuda())
     assert sk._C.device_status() == 0
+
+
+@pytest.mark.parametrize("pos", [40, 63, 64, 1000])
+def test_four_bit_cache_past_its_length(sk, pos):
+    """A position past max_len, inside the sequence's last page and behind it: reported, not written, the other sequence served."""
+    from spark_kernels import decode
+
+    cfg = _cfg(sk)
+    w = decode.random_weights(cfg, "cuda", seed=21)
+    one, two = (decode.QuantizedDecoder(cfg, w, fmt="fp8-tok", batch=n, max_len=40, kv="int4") for n in (1, 2))
+    g = torch.Generator(device="cuda").manual_seed(22)
+    x = torch.randn(2, cfg.hidden, device="cuda", generator=g).to(torch.bfloat16)
+    before = [c.pool.clone() for c in two.cache]
+    got = two.decode(x, torch.tensor([pos, 0], device="cuda"))
+    assert sk._C.device_status() == 5 and sk._C.device_status() == 0
+    assert torch.equal(got[1:], one.decode(x[1:], torch.tensor([0], device="cuda")))
+    for c, old, alone in zip(two.cache, before, one.cache):
+        assert torch.equal(c.pool[0], old[0]) and torch.equal(c.pool[1], alone.pool[0])
+    assert sk._C.device_status() == 0
