@@ -181,9 +181,13 @@ extern "C" int spk_add_rmsnorm(const void* x, long long x_stride, const void* y,
     p.r = static_cast<__nv_bfloat16*>(r), p.h = static_cast<__nv_bfloat16*>(h), p.rows = rows, p.hidden = hidden;
     auto stream = static_cast<cudaStream_t>(stream_);
     const int pieces = hidden >> 3;
-    // Few rows: as many threads as a block holds, for the shortest chain from load to store (1 x 4096: 2.2 us in a graph).
+    // Few rows: as many threads as a block holds, for the shortest chain from load to store (1 x 4096: 2.1 us in a graph).
     // Many: four pieces a thread, so that an SM has several rows' loads in flight: 16384 x 4096 with both norms and a gate per
-    // row 99.6 us (6.74 TB/s, 1.03 of the measured copy) against 107.5 / 101.9 / 117.8 with three, two and one piece.
+    // row 99 us (6.78 TB/s, 1.04 of the measured copy) against 107.5 / 101.9 / 117.8 with three, two and one piece. Sum and norm
+    // alone, the blocks for few and for many: 1000 rows of 4096 5.7 and 4.9 us, 400 rows 3.6 and 3.7, 296 rows 2.7 and 2.8; of 8192 12.8
+    // and 8.1, 6.4 and 4.1, 4.5 and 4.0; of 16384 28.3 and 23.4, 9.4 and 7.9, 6.8 and 5.4; of 1024 the same.
+    // From 32776 channels up a thread holds eight pieces and a block 1024 threads, whose registers do not hold them (1352 bytes
+    // stored, 1444 loaded); no block holds more threads.
     if (rows > 2 * dev->sm_count) {
         if (pieces <= 128) return launch<1, 128>(p, stream);
         if (pieces <= 256) return launch<2, 128>(p, stream);

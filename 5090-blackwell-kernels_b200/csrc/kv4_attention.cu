@@ -25,11 +25,11 @@
 // the CTA at its end, what crosses CTAs goes through the workspace to a second, chained launch; always in the order of the
 // units: the same bits every run. (Adding by whichever CTA is last, on counters, was slower: 43.2 -> 45.6 us at 64 x 4k.)
 //
-// Bound: instructions, then memory. A tile of 16 tokens and a head costs about 270 warp instructions (88 to build the codes'
-// fragments, 32 to centre V's, 16 MMAs, the rest words, softmax and ring), at 2.3 a cycle and SM 118 cycles for 2176 to 2560
-// bytes, which HBM delivers in 94 to 110. 32 heads over 8, d = 128, in a graph: 8 sequences of 65536 121.7 us = 4.69 TB/s (0.72 of the
-// measured copy; without the arithmetic the same copies take 100 us, without the copies the arithmetic 112); 64 sequences of up
-// to 4096 40.5 us = 3.29 TB/s; one of 200 10.5 us, of which the second launch is 2.5. Prompts: kv4_prompt.cu.
+// Bound: instructions, then memory. A tile of 16 tokens and a head costs about 280 warp instructions (88 to build the codes'
+// fragments, 32 to centre V's, 16 MMAs, the rest words, softmax and ring), at 2.3 a cycle and SM 122 cycles for 2176 to 2560
+// bytes, which HBM delivers in 94 to 110. 32 heads over 8, d = 128, in a graph: 8 sequences of 65536 124.8 us = 4.57 TB/s (0.70 of the
+// measured copy; the same copies without the arithmetic take 100 us); 64 sequences of up to 4096 41.2 us = 3.23 TB/s; one of
+// 200 10.5 us, of which the second launch is 2.5. Prompts: kv4_prompt.cu.
 #include <algorithm>
 
 #include "kv4_attend.cuh"
@@ -44,7 +44,8 @@ constexpr int kSteps = 2;     // 16-token tiles of a ring stage
 constexpr int kMinUnits = 8;  // a CTA gets at least this many units
 // Units that stand in front of a piece's tiles for what its beginning costs (q, the lengths, the end's sums). Without them
 // a batch with short sequences waits for the warps that got many (64 x 4k, ragged: 60.1 us with 0, 56.6 / 47.7 / 43.5 / 42.0 / 43.3
-// with 1 / 3 / 6 / 10 / 16).
+// with 1 / 3 / 6 / 10 / 16). With 0 / 5 / 10 / 20: 16 x 4097 29.5 / 26.4 / 27.7 / 28.0, 64 x 1000 31.5 / 29.4 / 28.7 / 31.7, 256 x 300 40
+// with all, 8 x 65536 125 with all, 32 x 8000 with a window of 1024 24.1 / 22.2 / 22.3 / 23.7.
 constexpr int kLead = 10;
 constexpr int kMaxWarps = 7;  // consuming warps of a CTA, of any form
 
@@ -56,7 +57,9 @@ constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the
 // W consuming warps and one that fills their rings, C such blocks on an SM: seven and two, at 128 registers a thread; seven and one
 // where 16 rows' accumulators take more. Five and two, with nothing spilled, is as fast at 64 x 4k and 6 % slower at 8 x 64k;
 // nine and two spills in the loop and takes twice as long. 24 rows a block spills too (76 us against 45 for 16 x 5 rows on
-// 6001), and 8 rows a block instead of 16 reads the cache more often (57 us).
+// 6001), and 8 rows a block instead of 16 reads the cache more often (57 us). Two of the forms spill as they are, with groups of
+// 32: d = 64 with 16 rows (542 bytes stored, 708 loaded) and d = 128 with 8 (470, 588). With one block on an SM they are
+// faster: 64 sequences of 4096 with 16 query heads a KV head 88 us for 115, with 8 heads of 128 98 for 115.
 template <int D, int G, int NQ, int H, int W, int C>
 struct SplitCfg {
     static constexpr int kRows = 8 * NQ / H, kGroups = D / G / H, kWords = D / 32;

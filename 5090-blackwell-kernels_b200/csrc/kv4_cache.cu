@@ -153,10 +153,11 @@ __device__ __forceinline__ Scale scale_of(float lo, float hi) {
 }
 
 // rint((x - m) / s) clamped to a code, four of them in the low 16 bits. The quotient has to be the correctly rounded one: bf16
-// values often lie exactly on the border between two codes. q + (d - q s) / s from a first q = d (1 / s) is that: d - q s is
-// exact, what the last product leaves is 2^-45 of the quotient, and a quotient of 24 bits by s's 8 is never closer than
-// 2^-33 to where the rounding turns. (Below 2^-100 the remainder falls out of fp32's range; there the division is
-// made.) The rounding to an integer is an addition of 1.5 x 2^23, which leaves it in the low bits.
+// values often lie exactly on the border between two codes. It is had by Markstein's method (IBM Journal of Research and
+// Development 34, 1990), an estimate from the reciprocal put right by its exact remainder: q + (d - q s) (1 / s) from a first
+// q = d (1 / s) is that: d - q s is exact, what the last product leaves is 2^-45 of the quotient, and a quotient of 24 bits by
+// s's 8 is never closer than 2^-33 to where the rounding turns. (Below 2^-100 the remainder falls out of fp32's range; there
+// the division is made.) The rounding to an integer is an addition of 1.5 x 2^23, which leaves it in the low bits.
 __device__ __forceinline__ uint32_t codes4(const Four& x, const Scale& g) {
     constexpr float kRound = 12582912.0f;
     int k[4];

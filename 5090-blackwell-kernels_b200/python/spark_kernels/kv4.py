@@ -85,7 +85,9 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
     [rows, Hq, head_dim]. Hq is a multiple of the cache's heads, query head h reading head h // (Hq // Hkv). A row that
     sees nothing gets zeros. Rows of a given `out` behind the last sequence are left as they were (zeros in one that
     the call allocates); `out` must not lie in q's memory. The weighted values are summed in fp32 before they are
-    divided by the weights' sum: values of up to 1e27 are safe at every length."""
+    divided by the weights' sum: values of up to 1e27 are safe at every length. Weights are rounded to fp16, 2^-11 of each and
+    2^-28 of the row's largest (times its group's scale); in prompts values are too, to 2^-11 and 2^-32 of the largest before
+    them in any group, and a weight of a token whose values are more than 2^16 below the loudest loses a bit for each 2 past that."""
     return _C.kv4_attention(q, cache.pool, page_table, lens, q_offsets, cache.head_dim, cache.group,
                             cache.head_dim ** -0.5 if scale is None else scale, window, out)
 
