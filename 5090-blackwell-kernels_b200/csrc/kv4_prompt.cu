@@ -20,11 +20,12 @@
 // put right when O is written.
 //
 // Bound: the roles' latencies, not the tensor cores (37 % active). 2 x 2048 new tokens on 6144 old ones, 32 heads over 8, d = 128:
-// 674 us = 714 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2700 cycles where its MMAs take 1084
+// 674 us = 714 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2800 cycles where its MMAs take 1084
 // and its exponentials 1024. By device clocks (taken at 654 us, before V's warps looked for the loudest values) a row warp has
 // about 2300 cycles of work a step (1200 for the weights, the rest waits that are already over, TMEM loads and stores,
-// exponents), a code warp 1900 every other step, an MMA warp 1600 (some hundred cycles for each MMA that it issues). 256 rows a block share the conversion of the codes; 128 keys a step would halve the
-// fixed costs but leave TMEM no room for the scores to run ahead.
+// exponents), a code warp 1900 every other step, an MMA warp 1600 (some hundred cycles for each MMA that it issues). 256 rows
+// a block share the conversion of the codes; 128 keys a step would halve the fixed costs but leave TMEM no room for the
+// scores to run ahead.
 #include <algorithm>
 
 #include "kv4_attend.cuh"

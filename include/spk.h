@@ -198,9 +198,11 @@ SPK_API int spk_kv4_read(const void* pool, int pages, int page_size, int kv_head
  * only the last `window` of them), fp32 sums; zeros where there are none. q bf16, rows q_stride elements apart; q_heads a
  * multiple of kv_heads, head h reads KV head h / (q_heads / kv_heads); out must not lie in what q's rows span. workspace: spk_kv4_attention_workspace(...) bytes of
  * device memory, 16-byte aligned, that no other call uses until this one has finished; its content does not matter.
- * Weights enter the products in fp16, each off by 2^-11 of itself, and by 2^-28 of the row's largest (with few rows a
- * sequence: largest weight x scale of the group; in prompts, where values do as well, off by 2^-11 of themselves and 2^-32
- * of the largest value up to there, in any group: a weight 2^-29, one bit less for each past 2^16 between tokens' values). */
+ * Precision: weights enter the products in fp16, each off by 2^-11 of itself. With few rows a sequence it is further off by
+ * 2^-28 of the row's largest weight x scale in the channel's group. In prompts (128 rows a KV head and more, where the call
+ * has enough of them) by 2^-29 of the row's largest weight, and values are in fp16 too, off by 2^-11 of themselves and
+ * 2^-32 of the largest value before them in any group; a token whose values are more than 2^16 below that largest loses a
+ * bit of its weight for each 2 past it. */
 SPK_API long long spk_kv4_attention_workspace(int rows, int seqs, int q_heads, int kv_heads, int head_dim);
 SPK_API int spk_kv4_attention(const void* q, long long q_stride, const void* pool, int pages, int page_size, int q_heads, int kv_heads,
                               int head_dim, int group, const int32_t* page_table, int table_width, const int32_t* lens,
