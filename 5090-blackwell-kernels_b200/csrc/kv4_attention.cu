@@ -241,6 +241,11 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
 #pragma unroll
                 for (int x = 0; x < 4; ++x) sc[n][t][x] += __shfl_xor_sync(0xffffffffu, sc[n][t][x], 2);
         }
+        // the scores as the softmax has them, rounded once: the largest minus the maximum is then 0 however large both are
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[n][t][x] = __fmul_rn(sc[n][t][x], st.mult[n][x & 1]);
         if (Masked) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
@@ -265,7 +270,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
             float m = fmaxf(sc[n][0][x], sc[n][0][x + 2]);
 #pragma unroll
             for (int t = 1; t < kSteps; ++t) m = fmaxf(m, fmaxf(sc[n][t][x], sc[n][t][x + 2]));
-            high[n][x] = m * st.mult[n][x];
+            high[n][x] = m;
             over |= high[n][x] > st.top[n][x] + kSlack;
         }
     if (__any_sync(0xffffffffu, over)) {
@@ -289,7 +294,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
 #pragma unroll
                 for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) p[t][y] = ptx::exp2_fast(fmaf(sc[n][t][x + 2 * y], st.mult[n][x], -shift));
+                    for (int y = 0; y < 2; ++y) p[t][y] = ptx::exp2_fast(sc[n][t][x + 2 * y] - shift);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     st.z[n][k][x] *= keep;
@@ -327,7 +332,7 @@ __device__ __forceinline__ void attend_step(State<D, G, NQ, H>& st, const Task<D
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float m = Masked && st.top[n][x & 1] == -INFINITY ? 0.0f : st.top[n][x & 1];
-                pr[x] = ptx::exp2_fast(fmaf(sc[n][t][x], st.mult[n][x & 1], -m));
+                pr[x] = ptx::exp2_fast(sc[n][t][x] - m);
                 st.sum[n][x & 1] += pr[x];
             }
 #pragma unroll

@@ -20,7 +20,7 @@
 // put right when O is written.
 //
 // Bound: the roles' latencies, not the tensor cores (37 % active). 2 x 2048 new tokens on 6144 old ones, 32 heads over 8, d = 128:
-// 674 us = 714 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2800 cycles where its MMAs take 1084
+// 682 us = 706 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2800 cycles where its MMAs take 1084
 // and its exponentials 1024. By device clocks (taken at 654 us, before V's warps looked for the loudest values) a row warp has
 // about 2300 cycles of work a step (1200 for the weights, the rest waits that are already over, TMEM loads and stores,
 // exponents), a code warp 1900 every other step, an MMA warp 1600 (some hundred cycles for each MMA that it issues). 256 rows
@@ -278,19 +278,22 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                         float m = x[16 * t];
 #pragma unroll
                         for (int i = 1; i < 16; ++i) m = fmaxf(m, x[16 * t + i]);
-                        most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t] - kLevel));
+                        most_here = fmaxf(most_here, fmaf(m, unit[t], v_exp[t]));
                     }
+                    most_here -= kLevel;
                     keep = top == -INFINITY ? 0.0f : exp2f(top - fmaxf(top, most_here));
                     top = fmaxf(top, most_here);
                 }
+                // score + e is rounded as the maximum's was before the maximum leaves it: their difference is then 0 however large they are
+                // (in one rounding what the maximum's lost would be a weight: 2^64 at a score of 10^9; 677 us for 682)
                 const float shift = top == -INFINITY ? 0.0f : top;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const float2 by = make_float2(unit[t], unit[t]), add = make_float2(v_exp[t] - shift, v_exp[t] - shift);
+                    const float2 by = make_float2(unit[t], unit[t]), add = make_float2(v_exp[t], v_exp[t]), less = make_float2(-shift, -shift);
                     float2 all = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        float2 e = ptx::fma2(make_float2(x[16 * t + i], x[16 * t + i + 1]), by, add);
+                        float2 e = ptx::add2(ptx::fma2(make_float2(x[16 * t + i], x[16 * t + i + 1]), by, add), less);
                         e.x = ptx::exp2_fast(e.x), e.y = ptx::exp2_fast(e.y);
                         all = ptx::add2(all, e);
                         pr[8 * t + i / 2] = ptx::f16x2_pack(e.x, e.y);

@@ -238,3 +238,31 @@ def test_huge_keys_of_tiny_queries(sk, n, news, hq, hkv, power):
     cache, table = _cache(sk, g, n, hkv, 128, 64, spoil)
     q = (torch.randn(news, hq, 128, generator=g) * 2.0 ** -power).to(torch.bfloat16)
     _check(*_attend_last(sk, cache, table, n, q, 128 ** -0.5, list(range(0, news, 31))), f"2^{power}")
+
+
+@pytest.mark.parametrize("n,news,hq,hkv", [(3000, 1, 4, 2), (3000, 1, 20, 2), (9000, 3, 8, 1), (3000, 150, 32, 16)])
+@pytest.mark.parametrize("scale", [1e4, 1e6, 1e7, 1e9, 1e20, -1e12, 1e36])
+def test_scores_so_large_that_one_token_has_all_the_weight(sk, n, news, hq, hkv, scale):
+    """Where a row's largest q . k stands out by 2, more than the sums' errors (|q . k| is some 50, a sum of 128 |q k| some 80, off by
+    at most 2^-11 of that), its output is that token's value: rounded to bf16, behind a weight times scale and a value in fp16 (2^-11
+    each of c s + 8 s + m or so: 2^-9 of the largest value). Where none does it is a mean of values."""
+    g = torch.Generator().manual_seed(51)
+    d = 128
+    cache, table = _cache(sk, g, n, hkv, d, 64, lambda x: None)
+    q = _bf16(g, news, hq, d)
+    off = None if news == 1 else torch.tensor([0, news], dtype=torch.int32).cuda()
+    got = sk.kv4_attention(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), off, scale=scale).double().cpu()
+    k, v = (t[table[0].long()].flatten(0, 1)[:n] for t in ref.unpack(cache.pool, d, 64))
+    assert torch.isfinite(got).all()
+    sure = 0
+    for r in range(0, news, 17):
+        for h in range(hq):
+            s = k[: n - news + r + 1, h * hkv // hq] @ q[r, h].double() * (1 if scale > 0 else -1)
+            best = s.topk(2)
+            vv = v[: len(s), h * hkv // hq]
+            assert (got[r, h].abs() <= vv.abs().amax(0) * (1 + 2 ** -7)).all()
+            if best.values[0] - best.values[1] > 2:
+                sure += 1
+                want = vv[best.indices[0]]
+                assert ((got[r, h] - want).abs() <= want.abs() * 2 ** -8 + 2 ** -9 * vv.abs().amax(0)).all(), (r, h)
+    assert sure > 0
