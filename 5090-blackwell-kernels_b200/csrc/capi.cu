@@ -74,18 +74,21 @@ extern "C" int spk_device_status(void* stream, int* code) {
     DeviceState* d = nullptr;
     if (int rc = device_state(&d)) return rc;
     auto st = static_cast<cudaStream_t>(stream);
-    int host = 0;
-    SPK_CUDA(cudaMemcpyAsync(&host, d->status, sizeof(int), cudaMemcpyDeviceToHost, st));
+    int host[kIndexWord + 1] = {};
+    SPK_CUDA(cudaMemcpyAsync(host, d->status, sizeof(host), cudaMemcpyDeviceToHost, st));
     SPK_CUDA(cudaStreamSynchronize(st));
-    if (host != 0) {
+    if (host[0] != 0) {
         // A kernel that gave up on a wait returned without its completion step: partial sums and strip
         // counters may be left behind, and every later split-K launch assumes they are zero. Put the
         // scratch back into its clean state together with the status word.
         SPK_CUDA(cudaMemsetAsync(d->partials, 0, kPartialFloats * sizeof(float), st));
         SPK_CUDA(cudaMemsetAsync(d->counters, 0, kCounters * sizeof(unsigned), st));
         SPK_CUDA(cudaMemsetAsync(d->status, 0, sizeof(int), st));
+    } else if (host[kIndexWord] != 0) {
+        // The scratch is as it should be, and kernels on other streams may be at work in it.
+        SPK_CUDA(cudaMemsetAsync(d->status + kIndexWord, 0, sizeof(int), st));
     }
-    *code = host;
+    *code = host[0] != 0 ? host[0] : host[kIndexWord];
     return SPK_OK;
 }
 

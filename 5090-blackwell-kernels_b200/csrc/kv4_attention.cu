@@ -599,7 +599,7 @@ kv4_attend_split_kernel(const AttendParams p) {
                 went = true;
                 const int n = min(left, kSteps);
                 int ok = (page >= 0 && page < p.pool.pages ? 1 : 0) | (next_page >= 0 && next_page < p.pool.pages ? 2 : 0);
-                if (ok != 3) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                if (ok != 3) kv4::bad_index(p.status);
                 ok &= (1 << n) - 1;
                 valid[slot] = ok;
                 unsigned char* to = ring + slot * Cfg::kStageBytes;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const AppendParams p
     }
     if (!known && !p.zero_rest) return;
     if (known && pos >= p.positions) {
-        if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+        if (lane == 0) kv4::bad_index(p.status);
         pos = -1;
     }
     const bool placed = known && pos >= 0;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const AppendParams p
     if (from < kv_to) {
         const int page = p.batch.table[static_cast<size_t>(b) * p.batch.width + pos / p.pool.page_size];
         if (page < 0 || page >= p.pool.pages) {
-            if (lane == 0) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+            if (lane == 0) kv4::bad_index(p.status);
         } else {
             tile = p.pool.data + (static_cast<size_t>(page) * p.pool.heads * tiles + pos % p.pool.page_size / kv4::kTile) * p.pool.tile_bytes;
         }
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadParams p) {
     if (n >= p.n) return;
     const long long slot = p.slots[n];
     const bool there = slot >= 0 && slot < static_cast<long long>(p.pool.pages) * p.pool.page_size;
-    if (slot >= 0 && !there) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+    if (slot >= 0 && !there) kv4::bad_index(p.status);
     const long long page = there ? slot / p.pool.page_size : 0;
     const int tiles = p.pool.page_size / kv4::kTile, in_page = there ? static_cast<int>(slot - page * p.pool.page_size) : 0, t = in_page % kv4::kTile;
     const unsigned char* tile = p.pool.data + (static_cast<size_t>(page) * p.pool.heads * tiles + in_page / kv4::kTile) * p.pool.tile_bytes;

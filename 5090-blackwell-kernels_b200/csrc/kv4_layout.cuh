@@ -49,6 +49,7 @@ struct Pool {
 };
 
 #ifdef __CUDACC__
+__device__ __forceinline__ void bad_index(int* status) { status[kIndexWord] = SPK_BAD_INDEX; }
 // First row and number of rows of sequence b, inside the call's tensors whatever the offsets say.
 __device__ __forceinline__ void rows_of(const Batch& s, int b, int& first, int& count) {
     if (s.offsets == nullptr) {
@@ -62,7 +63,7 @@ __device__ __forceinline__ void rows_of(const Batch& s, int b, int& first, int& 
 __device__ __forceinline__ int length_of(const Batch& s, int page_size, int b, int* status) {
     const int len = s.lens[b];
     if (len >= 0 && len <= static_cast<long long>(s.width) * page_size) return len;
-    atomicCAS(status, 0, SPK_BAD_INDEX);
+    bad_index(status);
     return 0;
 }
 __device__ __forceinline__ float word_min(uint32_t w) { return __uint_as_float(w << 16); }

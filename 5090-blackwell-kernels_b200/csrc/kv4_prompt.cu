@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv4_attend_prompt_kernel(const A
                 const int slot = j % Cfg::kRaw;
                 if (j >= Cfg::kRaw && !__all_sync(kAll, ptx::mbar_wait(&bars.raw_empty[slot], (j / Cfg::kRaw - 1) & 1, p.status))) break;
                 const bool good = key < any_hi && page >= 0 && page < p.pool.pages;
-                if (key < any_hi && !good && lane < 4) atomicCAS(p.status, 0, SPK_BAD_INDEX);
+                if (key < any_hi && !good && lane < 4) kv4::bad_index(p.status);
                 const uint32_t there = __ballot_sync(kAll, good) & 15u;
                 const int first_page = __shfl_sync(kAll, page, 0);
                 const bool one = __ballot_sync(kAll, good && page == first_page) == kAll && __shfl_sync(kAll, in_page, 0) + 3 < tiles_per_page;

@@ -61,7 +61,7 @@ struct DeviceState {
     int max_smem_optin = 0;
     float* partials = nullptr;      // kPartialFloats fp32, zero between launches
     unsigned* counters = nullptr;   // kCounters, zero between launches
-    int* status = nullptr;          // kStatusWords device ints: [0] first error code of a kernel
+    int* status = nullptr;          // kStatusWords device ints: [0] first error code of a kernel, [kIndexWord] SPK_BAD_INDEX
     unsigned char* act_scratch = nullptr;  // kActScratchBytes: re-ordered activations of one GEMM
     bool ready = false;
 };
@@ -72,7 +72,7 @@ constexpr int kMaxDevices = 16;
 
 constexpr int64_t kPartialFloats = int64_t{64} * 65536;  // 64 tokens x 65536 columns, 16 MiB
 constexpr int kCounters = 1 << 16;
-constexpr int kStatusWords = 8;
+constexpr int kStatusWords = 8, kIndexWord = 1;  // a bad index must not hide a wait that gave up
 constexpr int64_t kActScratchBytes = int64_t{64} * 32768 * 2;  // 64 tokens x 32768 k of bf16, 4 MiB
 
 // Programmatic dependent launch. A kernel launched through launch_chained() may begin while the

@@ -118,7 +118,7 @@ def init(device=None) -> None:
 
 def device_status(device=None) -> int:
     """Synchronize and return the device status word (0, 3 after a bounded wait timed out, 5 after a kernel over the 4-bit
-    KV cache met a page, slot, length or position outside its table)."""
+    KV cache met a page, slot, length or position outside its table; where both have happened 3 first and 5 from the next call)."""
     code = _i(0)
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):

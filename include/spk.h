@@ -47,9 +47,9 @@ SPK_API int spk_init(void);
  * the outputs of the GEMMs launched since the last clean status are not to be trusted: run them
  * again. Does not cover spk_w4gemm_bf16_noalloc, which has its own status call below. */
 SPK_API int spk_device_status(void* stream, int* code);
-/* The same word also reports SPK_BAD_INDEX, from the kernels over the 4-bit KV cache: they never follow a
- * bad index (the token is left out), so the scratch needs no repair then, but the call's output is not what
- * was asked for. */
+/* The same call also reports SPK_BAD_INDEX, from the kernels over the 4-bit KV cache: they never follow a
+ * bad index (the token is left out), so the scratch needs no repair then and gets none, but the call's output
+ * is not what was asked for. Where both have happened SPK_TIMEOUT is reported first, SPK_BAD_INDEX by the next call. */
 /* Test hook, no counterpart in the reference: launches a one-block kernel that leaves `dirty` words of
  * the split-K scratch non-zero, waits a tenth of a millisecond for a barrier phase nothing completes and
  * records SPK_TIMEOUT, i.e. the state a broken pipeline would leave. No fault, no trap; the context

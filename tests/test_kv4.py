@@ -524,3 +524,22 @@ def test_numbers_of_rotated_channels(sk, d, more):
     want_k, s, _ = ref.quantize(want[:, hq:], 32)
     assert ((k - want_k).abs() <= want_k.abs() * 2 ** -8 + s * (1 + 2 ** -7) + 15 * s * 2 ** -7).all()
     assert torch.equal(v, ref.quantize(x[:, hq + hkv:], 32)[0].to(torch.bfloat16).double())
+
+
+def test_a_bad_index_does_not_hide_a_wait_that_gave_up(sk):
+    """Both are reported, the wait first, whichever came first; and a split-K GEMM after them is right."""
+    g = torch.Generator().manual_seed(23)
+    cache, table = _filled(sk, g, [20], 16, 2, 128, 64)
+    q, past = _bf16(g, 1, 4, 128).cuda(), torch.tensor([1 << 20], dtype=torch.int32).cuda()
+    w = sk.W4Weight.quantize((torch.randn(4096, 256, generator=g) / 64).to(torch.bfloat16).cuda())
+    a = _bf16(g, 1, 4096).cuda()
+    want = sk.w4gemm(a, w)
+    assert sk._C.device_status() == 0
+    for first in (True, False):
+        if first:
+            sk.kv4_attention(q, cache, table.cuda(), past)
+        sk._C.debug_expire_wait(4096)
+        if not first:
+            sk.kv4_attention(q, cache, table.cuda(), past)
+        assert [sk._C.device_status() for _ in range(3)] == [3, 5, 0]
+        assert torch.equal(sk.w4gemm(a, w), want)
