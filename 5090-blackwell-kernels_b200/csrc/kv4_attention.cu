@@ -27,9 +27,9 @@
 //
 // Bound: instructions, then memory. A tile of 16 tokens and a head costs about 280 warp instructions (88 to build the codes'
 // fragments, 32 to centre V's, 16 MMAs, the rest words, softmax and ring), at 2.3 a cycle and SM 122 cycles for 2176 to 2560
-// bytes, which HBM delivers in 94 to 110. 32 heads over 8, d = 128, in a graph: 8 sequences of 65536 124.8 us = 4.57 TB/s (0.70 of the
-// measured copy; the same copies without the arithmetic take 100 us); 64 sequences of up to 4096 41.2 us = 3.23 TB/s; one of
-// 200 10.5 us, of which the second launch is 2.5. Prompts: kv4_prompt.cu.
+// bytes, which HBM delivers in 94 to 110. 32 heads over 8, d = 128, in a graph: 8 sequences of 65536 125.4 us = 4.55 TB/s (0.70 of the
+// measured copy; the same copies without the arithmetic take 100 us); 64 sequences of up to 4096 41.7 us = 3.19 TB/s; one of
+// 200 10.2 us, of which the second launch is 2.5. Prompts: kv4_prompt.cu.
 #include <algorithm>
 
 #include "kv4_attend.cuh"
@@ -58,7 +58,7 @@ constexpr int kMaxGrid = 2 * 160, kMinGrid = 64;  // two CTAs on every SM of the
 // where 16 rows' accumulators take more. Five and two, with nothing spilled, is as fast at 64 x 4k and 6 % slower at 8 x 64k;
 // nine and two spills in the loop and takes twice as long. 24 rows a block spills too (76 us against 45 for 16 x 5 rows on
 // 6001), and 8 rows a block instead of 16 reads the cache more often (57 us). Two of the forms spill as they are, with groups of
-// 32: d = 64 with 16 rows (542 bytes stored, 708 loaded) and d = 128 with 8 (470, 588). With one block on an SM they are
+// 32: d = 64 with 16 rows (542 bytes stored, 704 loaded) and d = 128 with 8 (458, 572). With one block on an SM they are
 // faster: 64 sequences of 4096 with 16 query heads a KV head 88 us for 115, with 8 heads of 128 98 for 115.
 template <int D, int G, int NQ, int H, int W, int C>
 struct SplitCfg {

@@ -20,7 +20,7 @@
 // put right when O is written.
 //
 // Bound: the roles' latencies, not the tensor cores (37 % active). 2 x 2048 new tokens on 6144 old ones, 32 heads over 8, d = 128:
-// 682 us = 706 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2800 cycles where its MMAs take 1084
+// 680 us = 707 TFLOP/s (0.43 of the measured cuBLAS rate); a step of 64 keys takes some 2800 cycles where its MMAs take 1084
 // and its exponentials 1024. By device clocks (taken at 654 us, before V's warps looked for the loudest values) a row warp has
 // about 2300 cycles of work a step (1200 for the weights, the rest waits that are already over, TMEM loads and stores,
 // exponents), a code warp 1900 every other step, an MMA warp 1600 (some hundred cycles for each MMA that it issues). 256 rows
