@@ -112,7 +112,7 @@ def test_norm_outputs_in_the_inputs_memory(lib, at):
     buf = ctypes.create_string_buffer(16384)
     base = ctypes.addressof(buf)
     base += -base % 16
-    place = dict(x=base, y=base + 1024, gain=base + 2048, post=base + 3072, gate=base + 4096, r=base + 5120, h=base + 6144)
+    place = {name: base + 1200 * i for i, name in enumerate(("x", "y", "gain", "post", "gate", "r", "h"), 1)}
 
     def call(xs=64, ys=64, gs=64, rows=2, **kw):
         a = place | kw
